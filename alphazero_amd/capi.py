@@ -15,6 +15,8 @@ LIB_PATH = os.environ.get("AZ_HIP_LIB") or os.path.join(_HERE, "libazhip.so")   
 AZ_EVAL_TOWER, AZ_EVAL_HASH, AZ_EVAL_EXTERNAL = 0, 1, 2
 AZ_NOISE_EXPLICIT, AZ_NOISE_DEVICE = 0, 1
 AZ_PREC_FP16, AZ_PREC_BF16, AZ_PREC_FP16X3 = 0, 1, 2   # fp16 operands are the default; FP16X3 = compensated three-pass parity mode
+AZ_F32, AZ_F16, AZ_BF16 = 0, 1, 2                      # element types of the learner's tensors
+AZ_CHANNELS_FIRST, AZ_CHANNELS_LAST = 0, 1
 AZ_MAX_LAYERS = 64
 AZ_OK, AZ_E_ARG, AZ_E_HIP, AZ_E_CAPACITY, AZ_E_STATE, AZ_E_NOWEIGHTS = 0, -1, -2, -3, -4, -5
 
@@ -37,6 +39,8 @@ EXPORTS = [
     "az_search", "az_search_begin", "az_search_select", "az_search_apply", "az_search_result",
     "az_tree_clear", "az_tree_dump", "az_selfplay_begin", "az_selfplay_run", "az_selfplay_run_pair", "az_pair_read", "az_selfplay_chain", "az_tree_timing", "az_tree_timing_read", "az_replay_drain",
     "az_get_stats", "az_replay_symmetries", "az_profile_enable", "az_profile_read", "az_profile_overhead", "az_tower_is_fused", "az_host_env_step", "az_selfplay_batch",
+    "az_policy_loss_workspace", "az_policy_loss_dev", "az_orthogonalize_workspace", "az_orthogonalize_dev",
+    "az_muon_step_workspace", "az_muon_step_dev",
 ]
 
 
@@ -68,6 +72,35 @@ class AzStats(C.Structure):
         ("max_nodes", C.c_int32), ("max_edges", C.c_int32), ("error_games", C.c_int32), ("tree_restarts", C.c_int32),
         ("sims_backed_up", C.c_int64), ("descents", C.c_int64), ("tree_levels", C.c_int64),
         ("children_scanned", C.c_int64), ("children_expanded", C.c_int64), ("saturated", C.c_int64),
+    ]
+
+
+class AzPolicyLossArgs(C.Structure):
+    _fields_ = [
+        ("device", C.c_int), ("B", C.c_int), ("N", C.c_int), ("C", C.c_int), ("c_out", C.c_int), ("dtype", C.c_int), ("layout", C.c_int),
+        ("features", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("target", C.c_void_p), ("counts", C.c_void_p),
+        ("actions", C.c_void_p), ("probs", C.c_void_p), ("cap", C.c_int), ("legal", C.c_void_p), ("scale", C.c_float),
+        ("row_scale", C.c_void_p), ("loss", C.c_void_p), ("stats", C.c_void_p), ("stats_given", C.c_int),
+        ("d_features", C.c_void_p), ("d_weight", C.c_void_p), ("d_bias", C.c_void_p),
+    ]
+
+
+class AzOrthogonalizeArgs(C.Structure):
+    _fields_ = [
+        ("device", C.c_int), ("n", C.c_int), ("rows", C.c_int), ("cols", C.c_int), ("dtype", C.c_int), ("steps", C.c_int),
+        ("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("eps", C.c_float), ("scale", C.c_float),
+        ("update", C.c_void_p), ("update_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64),
+    ]
+
+
+class AzMuonStepArgs(C.Structure):
+    _fields_ = [
+        ("device", C.c_int), ("n", C.c_int), ("rows", C.c_int), ("cols", C.c_int), ("grad_dtype", C.c_int), ("steps", C.c_int),
+        ("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("eps", C.c_float), ("scale", C.c_float),
+        ("lr", C.c_float), ("beta", C.c_float), ("weight_decay", C.c_float), ("nesterov", C.c_int),
+        ("grad", C.c_void_p), ("grad_stride", C.c_int64), ("weight", C.c_void_p), ("weight_stride", C.c_int64),
+        ("momentum", C.c_void_p), ("momentum_stride", C.c_int64), ("weight_out", C.c_void_p), ("weight_out_stride", C.c_int64),
+        ("momentum_out", C.c_void_p), ("momentum_out_stride", C.c_int64),
     ]
 
 
@@ -134,6 +167,10 @@ def load():
         L.az_blokus_host_state_size.restype = C.c_size_t
         L.az_blokus_stream.restype = C.c_void_p
         L.az_blokus_search_config.argtypes = [C.c_void_p, C.c_float, C.c_float, C.c_int, C.c_int]
+        for name in ("policy_loss", "orthogonalize", "muon_step"):
+            ws, run = getattr(L, "az_%s_workspace" % name), getattr(L, "az_%s_dev" % name)
+            ws.restype, ws.argtypes = C.c_size_t, [C.c_void_p]
+            run.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
         _lib = L
     return _lib
 

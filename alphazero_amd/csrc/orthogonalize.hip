@@ -1,0 +1,586 @@
+// orthogonalize.hip -- an update matrix orthogonalised by Newton-Schulz products, and the optimiser step around it.
+//
+//   X0 = U / (|U|_F + eps);   X <- a X + (b A + c A^2) X,  A = X X^T,  a number of times;   result s X
+//
+// The singular vectors stay what they are and every singular value x goes to a x + b x^3 + c x^5.  With X r x k, r <= k
+// (a taller matrix is read transposed), every iterate is Q X0 with Q a polynomial of A0 = X0 X0^T, and A, Q and
+// P = a + b A + c A^2 all commute and are symmetric:
+//   P = a I + b A + c A A,   Q <- Q P,   A <- P A P
+// so the long dimension is touched twice, for A0 and for Q X0, and what lies between are r x r products: 4 r^3 k-free
+// products a step instead of 2 r^2 k + r^3.  The price is that a singular value is carried as its square: one that is
+// small against the largest keeps the absolute precision of A's arithmetic, and the steps enlarge that error as they
+// enlarge the value (a^2 each).  So the products run on pairs of fp16 values, x = hi + lo / 2048 (22 bits; three MFMA a
+// product, fp32 sums), and for fp32 results X is formed anew after `stage` steps and A from it.
+#include "../../include/az_hip.h"
+#include "az_learn.h"
+
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+namespace {
+
+int ofail(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap; va_start(ap, fmt); vsnprintf(buf, sizeof buf, fmt, ap); va_end(ap);
+    return az_internal_fail(code, buf);
+}
+
+constexpr float LO = 2048.f;                  // scale of a pair's second value
+constexpr int KSTEP = 32;                     // contraction of one step of a tile product
+constexpr int MAX_SLICES = 64;                // pieces of a matrix whose squares are summed apart
+constexpr int SRC_PAIR = 3;                   // operand kinds: AZ_F32, AZ_F16, AZ_BF16, or pairs
+
+enum { GRAM_WIDE, GRAM_TALL, APPLY_WIDE, APPLY_TALL, SYM };          // what a tile product computes
+enum { EPI_PAIR, EPI_PARTIAL, EPI_POLY };                             // what SYM / GRAM leave
+
+struct OrthoDev {
+    const void* x;            // operand X: the update or a formed iterate
+    size_t x_stride;          // elements from matrix to matrix
+    int rows, cols, r, k, rp; // as stored; r = min, k = max; rp = r padded to the tile
+    int slices;
+    const double* sq;         // [n][slices] sums of squares, or null: X is an iterate, scale_exp its power of two
+    int scale_exp;
+    float eps, a, b, c;
+    short *A, *P, *T, *Q, *Q2;// [n][2][rp][rp]: hi plane, lo plane
+    float* partial;           // [n][split][rp][rp]
+    int split;
+    // result
+    void* out;
+    size_t out_stride;
+    int out_dtype;
+    float scale;
+    const float* w;           // optimiser step: out = keep * w + scale * X
+    size_t w_stride;
+    float keep;
+};
+
+// |U|_F of matrix z, and the power of two under which its elements are split into pairs (root mean square near 1)
+__device__ __forceinline__ void norm_of(const OrthoDev& d, int z, int& e, float& back) {
+    if (!d.sq) { e = d.scale_exp; back = ldexpf(1.f, -e); return; }
+    double s = 0.0;
+    for (int i = 0; i < d.slices; ++i) s += d.sq[(size_t)z * d.slices + i];
+    const double norm = sqrt(s);
+    e = 0;
+    if (norm > 0.0 && norm < 1e300) e = min(max(ilogb(sqrt((double)d.r * d.k) / norm), -120), 120);
+    back = (float)ldexp(1.0 / (norm + (double)d.eps), -e);
+}
+
+// sums of squares of a matrix's slices; with mom the update itself: m' = beta m + g, u = nesterov ? g + beta m' : m'
+template <int DT> __global__ void __launch_bounds__(256) az_ortho_norm_kernel(const void* g, size_t g_stride, int count, int slices, double* sq,
+                                                                          const float* mom, size_t m_stride, float* mom_out, size_t mo_stride, float* u, float beta, int nesterov) {
+    __shared__ double red[4];
+    const int z = blockIdx.y, sl = blockIdx.x;
+    const long long lo = (long long)count * sl / slices, hi = (long long)count * (sl + 1) / slices;
+    double s = 0.0;
+    for (long long i = lo + threadIdx.x; i < hi; i += 256) {
+        float v = az_load<DT>(g, z * g_stride + i);
+        if (mom) {
+            const float m = beta * mom[z * m_stride + i] + v;
+            v = nesterov ? v + beta * m : m;
+            mom_out[z * mo_stride + i] = m;
+            u[(size_t)z * count + i] = v;
+        }
+        s += (double)v * v;
+    }
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) sq[(size_t)z * slices + sl] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// 8 elements of a line: hi (and lo) halves.  Lines and positions beyond the matrix are zero.
+template <int SRC> __device__ __forceinline__ void load8(const void* p, const void* plo, size_t ld, int line, int pos, int nlines, int npos, float up, az_s8& hi, az_s8& lo) {
+    if constexpr (SRC == SRC_PAIR) {
+        hi = *(const az_s8*)((const short*)p + (size_t)line * ld + pos);
+        lo = *(const az_s8*)((const short*)plo + (size_t)line * ld + pos);
+    } else {
+        float v[8];
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+        if (line < nlines && pos < npos) {
+            const size_t at = (size_t)line * ld + pos;
+            if (pos + 8 <= npos) {
+                if constexpr (SRC == 0) {
+                    const az_f4 x = *(const az_f4_u*)((const float*)p + at), y = *(const az_f4_u*)((const float*)p + at + 4);
+                    for (int j = 0; j < 4; ++j) { v[j] = x[j]; v[4 + j] = y[j]; }
+                } else {
+                    const az_s8 x = *(const az_s8_u*)((const short*)p + at);
+                    #pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = az_from16<SRC>(x[j]);
+                }
+            } else {
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) if (pos + j < npos) v[j] = az_load<SRC>(p, at + j);
+            }
+        }
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = v[j] * up;
+            hi[j] = az_to16<1>(x);
+            if constexpr (SRC == 0) lo[j] = az_to16<1>((x - az_from16<1>(hi[j])) * LO);
+        }
+    }
+}
+
+// One operand of a tile product: TILE lines-or-columns by KSTEP.  Along: the contraction runs along a line (LDS rows are
+// the tile's rows); otherwise lines are the contraction (LDS rows are its steps, read transposed).
+template <int TILE, int SRC, bool ALONG> struct Operand {
+    static constexpr int PARTS = SRC == 0 || SRC == SRC_PAIR ? 2 : 1;
+    static constexpr int LD = ALONG ? KSTEP + 8 : TILE + 16;
+    static constexpr int LINES = ALONG ? TILE : KSTEP, PER = (ALONG ? KSTEP : TILE) / 8;
+    static constexpr int NP = LINES * PER / 256;                     // pieces a thread
+    static constexpr int HALVES = LINES * LD;                        // of one part
+    az_s8 hi[NP], lo[NP];
+    __device__ __forceinline__ void load(const void* p, const void* plo, size_t ld, int t0, int k0, int nlines, int npos, float up, int tid) {
+        #pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int w = tid + i * 256, line = w / PER, pos = w % PER * 8;
+            load8<SRC>(p, plo, ld, (ALONG ? t0 : k0) + line, (ALONG ? k0 : t0) + pos, nlines, npos, up, hi[i], lo[i]);
+        }
+    }
+    __device__ __forceinline__ void store(short* s, int tid) const {
+        #pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int w = tid + i * 256, at = w / PER * LD + w % PER * 8;
+            *(az_s8*)(s + at) = hi[i];
+            if constexpr (PARTS == 2) *(az_s8*)(s + HALVES + at) = lo[i];
+        }
+    }
+    static __device__ __forceinline__ az_i4 frag(const short* s, int part, int t, int lane) {
+        if constexpr (ALONG) return az_row_frag<1>(s + part * HALVES, LD, t, 0, lane);
+        else return az_col_frag<1>(s + part * HALVES, LD, 0, t, lane);
+    }
+};
+
+// tile (ti, tj) of the lower triangle, ti >= tj, from a running number
+__device__ __forceinline__ void lower_tile(int i, int& ti, int& tj) {
+    ti = (int)((sqrtf(8.f * i + 1.f) - 1.f) * 0.5f);
+    while ((ti + 1) * (ti + 2) / 2 <= i) ++ti;
+    while (ti * (ti + 1) / 2 > i) --ti;
+    tj = i - ti * (ti + 1) / 2;
+}
+
+// D[m][n] = sum over the contraction, 4 waves of TILE/2 x TILE/2.  Lane l of a 16 x 16 tile holds rows 4 (l / 16) .. + 3 of
+// column l % 16, so M is the side along which the result is contiguous in memory.
+//   SYM         M = rows of a symmetric matrix, N = rows of another that commutes with it: their product, lower triangle
+//   GRAM_*      M = N = rows of X: lower triangle
+//   APPLY_WIDE  M = columns of X, N = rows of Q;   APPLY_TALL  M = rows of Q, N = rows of X as stored (columns of X)
+template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256) az_ortho_product_kernel(OrthoDev d, const short* ma, const short* na, short* res,
+                                                                                                 const short* ma2, const short* na2, short* res2, int epi, int n) {
+    constexpr bool GRAM = MODE == GRAM_WIDE || MODE == GRAM_TALL;
+    constexpr int MS = MODE == SYM || MODE == APPLY_TALL ? SRC_PAIR : DT, NS = MODE == SYM || MODE == APPLY_WIDE ? SRC_PAIR : DT;
+    constexpr bool MA = !(MODE == GRAM_TALL || MODE == APPLY_WIDE), NA = MODE != GRAM_TALL;
+    typedef Operand<TILE, MS, MA> OM;
+    typedef Operand<TILE, NS, NA> ON;
+    constexpr int WT = TILE / 2 / 16;                                // 16 x 16 tiles of a wave, each way
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    constexpr int STAGE = OM::PARTS * OM::HALVES + ON::PARTS * ON::HALVES;
+    short* lds = (short*)smem;                                       // two stages
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
+    int z = blockIdx.z, m0, n0, k_lo = 0, k_hi, sp = 0;
+    const size_t plane = (size_t)d.rp * d.rp;
+    if constexpr (MODE == SYM || GRAM) {
+        int ti, tj;
+        lower_tile(blockIdx.x, ti, tj);
+        m0 = tj * TILE; n0 = ti * TILE;
+        if constexpr (GRAM) {
+            sp = blockIdx.y;
+            const int steps = (d.k + KSTEP - 1) / KSTEP;
+            k_lo = steps * sp / d.split * KSTEP;
+            k_hi = steps * (sp + 1) / d.split * KSTEP;
+        } else {
+            if (blockIdx.y) { ma = ma2; na = na2; res = res2; epi = EPI_PAIR; }   // a second product of the same launch
+            k_hi = d.rp;
+        }
+    } else {
+        // APPLY: x runs over the long side
+        m0 = (MODE == APPLY_WIDE ? blockIdx.x : blockIdx.y) * TILE;
+        n0 = (MODE == APPLY_WIDE ? blockIdx.y : blockIdx.x) * TILE;
+        k_hi = (d.r + KSTEP - 1) / KSTEP * KSTEP;
+    }
+    int e = 0;
+    float back = 1.f, up = 1.f;
+    if constexpr (MODE != SYM) { norm_of(d, z, e, back); up = ldexpf(1.f, e); }
+    const void *mp, *mlo = nullptr, *np, *nlo = nullptr;
+    size_t mld, nld;
+    const size_t esz = DT == 0 ? 4 : 2;
+    if constexpr (MS == SRC_PAIR) { mp = ma + (size_t)z * 2 * plane; mlo = ma + (size_t)z * 2 * plane + plane; mld = d.rp; }
+    else { mp = (const char*)d.x + z * d.x_stride * esz; mld = d.cols; }
+    if constexpr (NS == SRC_PAIR) { np = na + (size_t)z * 2 * plane; nlo = na + (size_t)z * 2 * plane + plane; nld = d.rp; }
+    else { np = (const char*)d.x + z * d.x_stride * esz; nld = d.cols; }
+    az_f4 hh[WT][WT], cross[WT][WT];
+    #pragma unroll
+    for (int i = 0; i < WT; ++i)
+        for (int j = 0; j < WT; ++j) { hh[i][j] = az_f4{0.f, 0.f, 0.f, 0.f}; cross[i][j] = az_f4{0.f, 0.f, 0.f, 0.f}; }
+    OM om;
+    ON on;
+    om.load(mp, mlo, mld, m0, k_lo, d.rows, d.cols, up, tid);
+    on.load(np, nlo, nld, n0, k_lo, d.rows, d.cols, up, tid);
+    int buf = 0;
+    const int mw = (wave & 1) * TILE / 2, nw = (wave >> 1) * TILE / 2;
+    for (int k = k_lo; k < k_hi; k += KSTEP, buf ^= 1) {
+        short* sm = lds + buf * STAGE;
+        short* sn = sm + OM::PARTS * OM::HALVES;
+        om.store(sm, tid);
+        on.store(sn, tid);
+        __syncthreads();                                             // (the other stage was last read before this barrier)
+        if (k + KSTEP < k_hi) {
+            om.load(mp, mlo, mld, m0, k + KSTEP, d.rows, d.cols, up, tid);
+            on.load(np, nlo, nld, n0, k + KSTEP, d.rows, d.cols, up, tid);
+        }
+        az_i4 mf[WT][OM::PARTS];
+        #pragma unroll
+        for (int i = 0; i < WT; ++i)
+            for (int p = 0; p < OM::PARTS; ++p) mf[i][p] = OM::frag(sm, p, mw + i * 16, lane);
+        #pragma unroll
+        for (int j = 0; j < WT; ++j) {
+            az_i4 nf[ON::PARTS];
+            #pragma unroll
+            for (int p = 0; p < ON::PARTS; ++p) nf[p] = ON::frag(sn, p, nw + j * 16, lane);
+            #pragma unroll
+            for (int i = 0; i < WT; ++i) {
+                hh[i][j] = az_mma<1>(mf[i][0], nf[0], hh[i][j]);
+                if constexpr (ON::PARTS == 2) cross[i][j] = az_mma<1>(mf[i][0], nf[1], cross[i][j]);
+                if constexpr (OM::PARTS == 2) cross[i][j] = az_mma<1>(mf[i][1], nf[0], cross[i][j]);
+            }
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < WT; ++i)
+        #pragma unroll
+        for (int j = 0; j < WT; ++j) {
+            az_f4 v = hh[i][j] + cross[i][j] * (1.f / LO);
+            const int m = m0 + mw + i * 16 + q * 4, nn = n0 + nw + j * 16 + (lane & 15);
+            if constexpr (MODE == SYM || GRAM) {
+                if constexpr (GRAM) v *= back * back;
+                if (GRAM && epi == EPI_PARTIAL) { *(az_f4*)(d.partial + ((size_t)z * d.split + sp) * plane + (size_t)nn * d.rp + m) = v; continue; }
+                short* hi = res + (size_t)z * 2 * plane;
+                short* lo = hi + plane;
+                if (MODE == SYM && epi == EPI_POLY) {                 // P = a I + b A + c A A
+                    const az_s4 ah = *(const az_s4*)(ma + (size_t)z * 2 * plane + (size_t)nn * d.rp + m);
+                    const az_s4 al = *(const az_s4*)(ma + (size_t)z * 2 * plane + plane + (size_t)nn * d.rp + m);
+                    #pragma unroll
+                    for (int t = 0; t < 4; ++t) v[t] = (m + t == nn ? d.a : 0.f) + d.b * (az_from16<1>(ah[t]) + az_from16<1>(al[t]) * (1.f / LO)) + d.c * v[t];
+                }
+                az_s4 h, l;
+                #pragma unroll
+                for (int t = 0; t < 4; ++t) { h[t] = az_to16<1>(v[t]); l[t] = az_to16<1>((v[t] - az_from16<1>(h[t])) * LO); }
+                *(az_s4*)(hi + (size_t)nn * d.rp + m) = h;
+                *(az_s4*)(lo + (size_t)nn * d.rp + m) = l;
+                if (m0 != n0)
+                    for (int t = 0; t < 4; ++t) { hi[(size_t)(m + t) * d.rp + nn] = h[t]; lo[(size_t)(m + t) * d.rp + nn] = l[t]; }
+            } else {
+                // the result's line and position in memory: the positions m .. m + 3 of line nn
+                const int nl = d.rows, np_ = d.cols;
+                if (nn >= nl || m >= np_) continue;
+                const float f = back * d.scale;
+                const size_t at = (size_t)nn * d.cols + m;
+                if (d.w) {
+                    const float* w = d.w + z * d.w_stride + at;
+                    float* o = (float*)d.out + z * d.out_stride + at;
+                    if (m + 4 <= np_) { const az_f4 x = *(const az_f4_u*)w; *(az_f4_u*)o = x * d.keep + v * f; }
+                    else for (int t = 0; t < 4; ++t) if (m + t < np_) o[t] = w[t] * d.keep + v[t] * f;
+                } else if (d.out_dtype == AZ_F32) {
+                    float* o = (float*)d.out + z * d.out_stride + at;
+                    if (m + 4 <= np_) *(az_f4_u*)o = v * f;
+                    else for (int t = 0; t < 4; ++t) if (m + t < np_) o[t] = v[t] * f;
+                } else {
+                    short* o = (short*)d.out + z * d.out_stride + at;
+                    const bool h16 = d.out_dtype == AZ_F16;
+                    az_s4 s;
+                    for (int t = 0; t < 4; ++t) s[t] = h16 ? az_to16<1>(v[t] * f) : az_to16<2>(v[t] * f);
+                    if (m + 4 <= np_) *(az_s4_u*)o = s;
+                    else for (int t = 0; t < 4; ++t) if (m + t < np_) o[t] = s[t];
+                }
+            }
+        }
+}
+
+// The slices of a contraction that was split, added in their order: A as pairs, both triangles.
+__global__ void __launch_bounds__(256) az_ortho_join_kernel(OrthoDev d, int tile) {
+    int ti, tj;
+    lower_tile(blockIdx.x, ti, tj);
+    const int z = blockIdx.z;
+    const size_t plane = (size_t)d.rp * d.rp;
+    short* hi = d.A + (size_t)z * 2 * plane;
+    short* lo = hi + plane;
+    for (int i = threadIdx.x + blockIdx.y * 256; i < tile * tile; i += 256 * gridDim.y) {
+        const int nn = ti * tile + i / tile, m = tj * tile + i % tile;
+        float v = 0.f;
+        for (int s = 0; s < d.split; ++s) v += d.partial[((size_t)z * d.split + s) * plane + (size_t)nn * d.rp + m];
+        const short h = az_to16<1>(v), l = az_to16<1>((v - az_from16<1>(h)) * LO);
+        hi[(size_t)nn * d.rp + m] = h; lo[(size_t)nn * d.rp + m] = l;
+        if (ti != tj) { hi[(size_t)m * d.rp + nn] = h; lo[(size_t)m * d.rp + nn] = l; }
+    }
+}
+
+// no step at all: Q = I
+__global__ void __launch_bounds__(256) az_ortho_identity_kernel(short* Q, int rp) {
+    const size_t plane = (size_t)rp * rp;
+    short* q = Q + (size_t)blockIdx.y * 2 * plane;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < 2 * plane; i += (size_t)gridDim.x * 256)
+        q[i] = i < plane && i / rp == i % rp ? az_to16<1>(1.f) : (short)0;
+}
+
+struct Plan {
+    int n, rows, cols, r, k, rp, tile, tiles, low, slices, split, stage;
+    bool muon, restart;
+    size_t off_sq, off_u, off_x1, off_mat, off_partial, bytes;
+    size_t pair_bytes;
+};
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+Plan make_plan(int n, int rows, int cols, int dtype, int steps, bool muon) {
+    Plan p = {};
+    p.n = n; p.rows = rows; p.cols = cols; p.muon = muon;
+    p.r = rows < cols ? rows : cols;
+    p.k = rows < cols ? cols : rows;
+    p.tile = p.r <= 64 ? 64 : 128;
+    p.tiles = (p.r + p.tile - 1) / p.tile;
+    p.rp = p.tiles * p.tile;
+    p.low = p.tiles * (p.tiles + 1) / 2;
+    const long long count = (long long)rows * cols;
+    p.slices = (int)(count / 4096 < 1 ? 1 : count / 4096 > MAX_SLICES ? MAX_SLICES : count / 4096);
+    const int ksteps = (p.k + KSTEP - 1) / KSTEP;
+    p.split = 1;
+    while (p.split < 16 && (long long)p.low * n * p.split < 256 && ksteps / (p.split * 2) >= 4) p.split *= 2;
+    p.stage = dtype == AZ_F32 || muon ? 3 : 5;
+    p.restart = steps > p.stage;
+    p.pair_bytes = up256((size_t)n * 2 * p.rp * p.rp * 2);
+    size_t o = 0;
+    p.off_sq = o; o += up256((size_t)n * p.slices * 8);
+    p.off_u = o; if (muon) o += up256((size_t)n * count * 4);
+    p.off_x1 = o; if (p.restart) o += 2 * up256((size_t)n * count * 4);   // iterates: read one, write the other
+    p.off_mat = o; o += 5 * p.pair_bytes;
+    p.off_partial = o; if (p.split > 1) o += up256((size_t)n * p.split * p.rp * p.rp * 4);
+    p.bytes = o;
+    return p;
+}
+
+template <int TILE, int DT, int MODE> hipError_t product(const OrthoDev& d, dim3 grid, const short* ma, const short* na, short* res, const short* ma2, const short* na2, short* res2,
+                                                         int epi, int n, hipStream_t st) {
+    constexpr int MS = MODE == SYM || MODE == APPLY_TALL ? SRC_PAIR : DT, NS = MODE == SYM || MODE == APPLY_WIDE ? SRC_PAIR : DT;
+    typedef Operand<TILE, MS, !(MODE == GRAM_TALL || MODE == APPLY_WIDE)> OM;
+    typedef Operand<TILE, NS, MODE != GRAM_TALL> ON;
+    const size_t lds = 2 * 2 * ((size_t)OM::PARTS * OM::HALVES + (size_t)ON::PARTS * ON::HALVES);
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void*)az_ortho_product_kernel<TILE, DT, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    az_ortho_product_kernel<TILE, DT, MODE><<<grid, 256, lds, st>>>(d, ma, na, res, ma2, na2, res2, epi, n);
+    return hipGetLastError();
+}
+
+template <int TILE, int DT> hipError_t gram(const Plan& p, const OrthoDev& d, hipStream_t st) {
+    const dim3 grid(p.low, p.split, p.n);
+    const int epi = p.split > 1 ? EPI_PARTIAL : EPI_PAIR;
+    hipError_t e = p.rows <= p.cols ? product<TILE, DT, GRAM_WIDE>(d, grid, nullptr, nullptr, d.A, nullptr, nullptr, nullptr, epi, p.n, st)
+                                    : product<TILE, DT, GRAM_TALL>(d, grid, nullptr, nullptr, d.A, nullptr, nullptr, nullptr, epi, p.n, st);
+    if (e == hipSuccess && p.split > 1) {
+        az_ortho_join_kernel<<<dim3(p.low, TILE * TILE / 1024, p.n), 256, 0, st>>>(d, TILE);
+        e = hipGetLastError();
+    }
+    return e;
+}
+template <int TILE, int DT> hipError_t apply(const Plan& p, const OrthoDev& d, hipStream_t st) {
+    const dim3 grid((p.k + TILE - 1) / TILE, p.tiles, p.n);
+    return p.rows <= p.cols ? product<TILE, DT, APPLY_WIDE>(d, grid, nullptr, d.Q, nullptr, nullptr, nullptr, nullptr, 0, p.n, st)
+                            : product<TILE, DT, APPLY_TALL>(d, grid, d.Q, nullptr, nullptr, nullptr, nullptr, nullptr, 0, p.n, st);
+}
+template <int TILE> hipError_t gram_dt(int dt, const Plan& p, const OrthoDev& d, hipStream_t st) {
+    return dt == AZ_F32 ? gram<TILE, 0>(p, d, st) : dt == AZ_F16 ? gram<TILE, 1>(p, d, st) : gram<TILE, 2>(p, d, st);
+}
+template <int TILE> hipError_t apply_dt(int dt, const Plan& p, const OrthoDev& d, hipStream_t st) {
+    return dt == AZ_F32 ? apply<TILE, 0>(p, d, st) : dt == AZ_F16 ? apply<TILE, 1>(p, d, st) : apply<TILE, 2>(p, d, st);
+}
+
+// `m` steps on A: leaves Q
+template <int TILE> hipError_t iterate(const Plan& p, OrthoDev& d, int m, hipStream_t st) {
+    const dim3 one(p.low, 1, p.n), two(p.low, 2, p.n);
+    hipError_t e = hipSuccess;
+#define RUN(call) do { if (e == hipSuccess) e = (call); } while (0)
+    if (m == 0) { az_ortho_identity_kernel<<<dim3(64, p.n), 256, 0, st>>>(d.Q, p.rp); return hipGetLastError(); }
+    for (int i = 0; i < m; ++i) {
+        const bool first = i == 0, last = i + 1 == m;
+        RUN((product<TILE, 0, SYM>(d, one, d.A, d.A, first ? d.Q : d.P, nullptr, nullptr, nullptr, EPI_POLY, p.n, st)));
+        short* P = first ? d.Q : d.P;                                // the first step's Q is its P
+        if (!last) {
+            if (first) RUN((product<TILE, 0, SYM>(d, one, d.A, P, d.T, nullptr, nullptr, nullptr, EPI_PAIR, p.n, st)));
+            else RUN((product<TILE, 0, SYM>(d, two, d.A, P, d.T, d.Q, P, d.Q2, EPI_PAIR, p.n, st)));
+            RUN((product<TILE, 0, SYM>(d, one, d.T, P, d.A, nullptr, nullptr, nullptr, EPI_PAIR, p.n, st)));
+        } else if (!first) RUN((product<TILE, 0, SYM>(d, one, d.Q, P, d.Q2, nullptr, nullptr, nullptr, EPI_PAIR, p.n, st)));
+        if (!first) { short* t = d.Q; d.Q = d.Q2; d.Q2 = t; }
+    }
+#undef RUN
+    return e;
+}
+
+template <int TILE> hipError_t run_plan(const Plan& p, OrthoDev d, int dtype, int steps, unsigned char* ws, hipStream_t st) {
+    const OrthoDev fin = d;                                          // result pointers of the last application
+    const size_t count = (size_t)p.rows * p.cols;
+    float* x1[2] = {(float*)(ws + p.off_x1), (float*)(ws + p.off_x1 + up256((size_t)p.n * count * 4))};
+    hipError_t e = hipSuccess;
+    int done = 0, which = 0;
+    do {
+        // stages of p.stage steps, the shorter one last: A's error is relative to its largest eigenvalue, which the first
+        // stage starts far below 1 (|X0|_F = 1 spread over the singular values) and the later ones near 1
+        const int left = steps - done, m = left < p.stage ? left : p.stage;
+        done += m;
+        if (m > 0) e = gram_dt<TILE>(dtype, p, d, st);
+        if (e == hipSuccess) e = iterate<TILE>(p, d, m, st);
+        if (done < steps) { d.out = x1[which]; d.out_stride = count; d.out_dtype = AZ_F32; d.scale = 1.f; d.w = nullptr; }
+        else { d.out = fin.out; d.out_stride = fin.out_stride; d.out_dtype = fin.out_dtype; d.scale = fin.scale; d.w = fin.w; }
+        if (e == hipSuccess) e = apply_dt<TILE>(dtype, p, d, st);
+        d.x = x1[which]; d.x_stride = count; dtype = AZ_F32; d.sq = nullptr;
+        d.scale_exp = ilogb(std::sqrt((double)p.k));                 // an iterate's elements: about 1 / sqrt(k)
+        which ^= 1;
+    } while (e == hipSuccess && done < steps);
+    return e;
+}
+
+int check_common(int n, int rows, int cols, int steps, float a, float b, float c, float eps) {
+    if (n < 0) return ofail(AZ_E_ARG, "%d matrices", n);
+    if (n > 65535) return ofail(AZ_E_ARG, "%d matrices are too many for one call (65535)", n);
+    if (rows < 1 || cols < 1) return ofail(AZ_E_ARG, "matrix %d x %d", rows, cols);
+    if ((long long)rows * cols > 0x7fffffffll) return ofail(AZ_E_ARG, "matrix %d x %d has too many elements", rows, cols);
+    if ((rows < cols ? rows : cols) > 8192) return ofail(AZ_E_ARG, "the shorter side of %d x %d is beyond 8192", rows, cols);
+    if (steps < 0 || steps > 100) return ofail(AZ_E_ARG, "%d steps (0..100)", steps);
+    if (!(std::fabs(a) + std::fabs(b) + std::fabs(c) <= 32.f)) return ofail(AZ_E_ARG, "coefficients %g, %g, %g: their magnitudes sum beyond 32", a, b, c);
+    if (!(eps >= 0.f) || std::isinf(eps)) return ofail(AZ_E_ARG, "eps %g", eps);
+    return AZ_OK;
+}
+int check_ortho(const az_orthogonalize_args* p) {
+    if (!p) return ofail(AZ_E_ARG, "null argument: args");
+    const int rc = check_common(p->n, p->rows, p->cols, p->steps, p->a, p->b, p->c, p->eps);
+    if (rc != AZ_OK) return rc;
+    if (p->dtype != AZ_F32 && p->dtype != AZ_F16 && p->dtype != AZ_BF16) return ofail(AZ_E_ARG, "element type %d unknown (AZ_F32, AZ_F16, AZ_BF16)", p->dtype);
+    return AZ_OK;
+}
+int check_muon(const az_muon_step_args* p) {
+    if (!p) return ofail(AZ_E_ARG, "null argument: args");
+    const int rc = check_common(p->n, p->rows, p->cols, p->steps, p->a, p->b, p->c, p->eps);
+    if (rc != AZ_OK) return rc;
+    if (p->grad_dtype != AZ_F32 && p->grad_dtype != AZ_F16 && p->grad_dtype != AZ_BF16) return ofail(AZ_E_ARG, "element type %d unknown (AZ_F32, AZ_F16, AZ_BF16)", p->grad_dtype);
+    return AZ_OK;
+}
+// matrices that are written may not overlap each other: strides of at least a matrix
+int check_stride(const char* name, int64_t stride, int n, int rows, int cols) {
+    if (n > 1 && stride < (int64_t)rows * cols) return ofail(AZ_E_ARG, "%s: stride %lld is shorter than a %d x %d matrix", name, (long long)stride, rows, cols);
+    return AZ_OK;
+}
+// the bytes a batch of matrices spans
+struct Span { const char *lo, *hi; int64_t stride; };
+Span span_of(const void* p, int64_t stride, int n, int rows, int cols, int esz) {
+    const char* c = (const char*)p;
+    return {c, c + ((int64_t)(n - 1) * stride + (int64_t)rows * cols) * esz, stride};
+}
+bool meet(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
+bool same(const Span& a, const Span& b) { return a.lo == b.lo && a.stride == b.stride; }
+int check_ws(const void* ws, size_t have, size_t need) {
+    if (!ws) return ofail(AZ_E_ARG, "null argument: workspace");
+    if ((size_t)ws % 256) return ofail(AZ_E_ARG, "workspace needs 256-byte alignment");
+    if (have < need) return ofail(AZ_E_CAPACITY, "workspace has %zu bytes, the call needs %zu", have, need);
+    return AZ_OK;
+}
+
+int run(const Plan& p, OrthoDev d, int dtype, int steps, unsigned char* ws, hipStream_t st, const char* who) {
+    d.rows = p.rows; d.cols = p.cols; d.r = p.r; d.k = p.k; d.rp = p.rp; d.slices = p.slices; d.split = p.split;
+    d.sq = (const double*)(ws + p.off_sq);
+    short** m[5] = {&d.A, &d.P, &d.T, &d.Q, &d.Q2};
+    for (int i = 0; i < 5; ++i) *m[i] = (short*)(ws + p.off_mat + i * p.pair_bytes);
+    d.partial = (float*)(ws + p.off_partial);
+    const hipError_t e = p.tile == 64 ? run_plan<64>(p, d, dtype, steps, ws, st) : run_plan<128>(p, d, dtype, steps, ws, st);
+    if (e != hipSuccess) return ofail(AZ_E_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
+    return AZ_OK;
+}
+
+}  // namespace
+
+extern "C" size_t az_orthogonalize_workspace(const az_orthogonalize_args* p) {
+    if (check_ortho(p) != AZ_OK) return 0;
+    return make_plan(p->n, p->rows, p->cols, p->dtype, p->steps, false).bytes + 256;
+}
+extern "C" size_t az_muon_step_workspace(const az_muon_step_args* p) {
+    if (check_muon(p) != AZ_OK) return 0;
+    return make_plan(p->n, p->rows, p->cols, AZ_F32, p->steps, true).bytes + 256;
+}
+
+extern "C" int az_orthogonalize_dev(const az_orthogonalize_args* p, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_ortho(p);
+    if (rc != AZ_OK) return rc;
+    if (p->n == 0) return AZ_OK;
+    if (!p->update) return ofail(AZ_E_ARG, "null argument: update");
+    if (!p->out) return ofail(AZ_E_ARG, "null argument: out");
+    if (((size_t)p->update | (size_t)p->out) % (p->dtype == AZ_F32 ? 4 : 2)) return ofail(AZ_E_ARG, "a tensor is not aligned to its element type");
+    if ((rc = check_stride("update", p->update_stride, p->n, p->rows, p->cols)) != AZ_OK || (rc = check_stride("out", p->out_stride, p->n, p->rows, p->cols)) != AZ_OK) return rc;
+    const int esz = p->dtype == AZ_F32 ? 4 : 2;
+    // (a tile of the result is written while other workgroups still read the update)
+    if (meet(span_of(p->update, p->update_stride, p->n, p->rows, p->cols, esz), span_of(p->out, p->out_stride, p->n, p->rows, p->cols, esz)))
+        return ofail(AZ_E_ARG, "out overlaps update");
+    const Plan plan = make_plan(p->n, p->rows, p->cols, p->dtype, p->steps, false);
+    if ((rc = check_ws(workspace, workspace_bytes, plan.bytes + 256)) != AZ_OK) return rc;
+    AzDeviceGuard dev(p->device);
+    if (!dev.ok) return ofail(AZ_E_HIP, "device %d cannot be used (no HIP device: libazhip has no CPU fallback)", p->device);
+    unsigned char* ws = (unsigned char*)workspace;
+    hipStream_t st = (hipStream_t)stream;
+    double* sq = (double*)(ws + plan.off_sq);
+    const dim3 grid(plan.slices, p->n);
+    const int count = p->rows * p->cols;
+    if (p->dtype == AZ_F32) az_ortho_norm_kernel<0><<<grid, 256, 0, st>>>(p->update, p->update_stride, count, plan.slices, sq, nullptr, 0, nullptr, 0, nullptr, 0.f, 0);
+    else if (p->dtype == AZ_F16) az_ortho_norm_kernel<1><<<grid, 256, 0, st>>>(p->update, p->update_stride, count, plan.slices, sq, nullptr, 0, nullptr, 0, nullptr, 0.f, 0);
+    else az_ortho_norm_kernel<2><<<grid, 256, 0, st>>>(p->update, p->update_stride, count, plan.slices, sq, nullptr, 0, nullptr, 0, nullptr, 0.f, 0);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return ofail(AZ_E_HIP, "az_orthogonalize_dev: launch failed: %s", hipGetErrorString(e));
+    OrthoDev d = {};
+    d.x = p->update; d.x_stride = p->update_stride;
+    d.eps = p->eps; d.a = p->a; d.b = p->b; d.c = p->c;
+    d.out = p->out; d.out_stride = p->out_stride; d.out_dtype = p->dtype; d.scale = p->scale;
+    return run(plan, d, p->dtype, p->steps, ws, st, "az_orthogonalize_dev");
+}
+
+extern "C" int az_muon_step_dev(const az_muon_step_args* p, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_muon(p);
+    if (rc != AZ_OK) return rc;
+    if (p->n == 0) return AZ_OK;
+    if (!p->grad) return ofail(AZ_E_ARG, "null argument: grad");
+    if (!p->weight) return ofail(AZ_E_ARG, "null argument: weight");
+    if (!p->momentum) return ofail(AZ_E_ARG, "null argument: momentum");
+    if (!p->weight_out) return ofail(AZ_E_ARG, "null argument: weight_out");
+    if (!p->momentum_out) return ofail(AZ_E_ARG, "null argument: momentum_out");
+    if ((size_t)p->grad % (p->grad_dtype == AZ_F32 ? 4 : 2) || ((size_t)p->weight | (size_t)p->momentum | (size_t)p->weight_out | (size_t)p->momentum_out) % 4)
+        return ofail(AZ_E_ARG, "a tensor is not aligned to its element type");
+    const struct { const char* name; int64_t s; } strides[5] = {{"grad", p->grad_stride}, {"weight", p->weight_stride}, {"momentum", p->momentum_stride},
+                                                                 {"weight_out", p->weight_out_stride}, {"momentum_out", p->momentum_out_stride}};
+    for (const auto& s : strides) if ((rc = check_stride(s.name, s.s, p->n, p->rows, p->cols)) != AZ_OK) return rc;
+    const Span g = span_of(p->grad, p->grad_stride, p->n, p->rows, p->cols, p->grad_dtype == AZ_F32 ? 4 : 2);
+    const Span w = span_of(p->weight, p->weight_stride, p->n, p->rows, p->cols, 4), m = span_of(p->momentum, p->momentum_stride, p->n, p->rows, p->cols, 4);
+    const Span wo = span_of(p->weight_out, p->weight_out_stride, p->n, p->rows, p->cols, 4), mo = span_of(p->momentum_out, p->momentum_out_stride, p->n, p->rows, p->cols, 4);
+    if ((meet(w, wo) && !same(w, wo)) || (meet(m, mo) && !same(m, mo)) || meet(wo, mo) || meet(wo, m) || meet(mo, w) || meet(g, wo) || meet(g, mo))
+        return ofail(AZ_E_ARG, "an output overlaps another tensor (in place means the same address and stride)");
+    const Plan plan = make_plan(p->n, p->rows, p->cols, AZ_F32, p->steps, true);
+    if ((rc = check_ws(workspace, workspace_bytes, plan.bytes + 256)) != AZ_OK) return rc;
+    AzDeviceGuard dev(p->device);
+    if (!dev.ok) return ofail(AZ_E_HIP, "device %d cannot be used (no HIP device: libazhip has no CPU fallback)", p->device);
+    unsigned char* ws = (unsigned char*)workspace;
+    hipStream_t st = (hipStream_t)stream;
+    double* sq = (double*)(ws + plan.off_sq);
+    float* u = (float*)(ws + plan.off_u);
+    const dim3 grid(plan.slices, p->n);
+    const int count = p->rows * p->cols;
+#define NORM(DT) az_ortho_norm_kernel<DT><<<grid, 256, 0, st>>>(p->grad, p->grad_stride, count, plan.slices, sq, p->momentum, p->momentum_stride, \
+                                                                p->momentum_out, p->momentum_out_stride, u, p->beta, p->nesterov)
+    if (p->grad_dtype == AZ_F32) NORM(0);
+    else if (p->grad_dtype == AZ_F16) NORM(1);
+    else NORM(2);
+#undef NORM
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return ofail(AZ_E_HIP, "az_muon_step_dev: launch failed: %s", hipGetErrorString(e));
+    OrthoDev d = {};
+    d.x = u; d.x_stride = count;
+    d.eps = p->eps; d.a = p->a; d.b = p->b; d.c = p->c;
+    d.out = p->weight_out; d.out_stride = p->weight_out_stride; d.out_dtype = AZ_F32; d.scale = -p->lr * p->scale;
+    d.w = p->weight; d.w_stride = p->weight_stride; d.keep = 1.f - p->lr * p->weight_decay;
+    return run(plan, d, AZ_F32, p->steps, ws, st, "az_muon_step_dev");
+}

@@ -406,6 +406,103 @@ int az_blokus_host_info(const void* state, uint8_t* cells /* [400] */, int* to_m
  * rules as the device kernels): returns 1 done, 0 running, AZ_E_ARG illegal. */
 int az_host_env_step(int N, int K, uint8_t* cells, int* to_move, int action, float* reward);
 
+/* ---- The learner's operators: what stands between the rows a drain hands out and the blob az_load_weights_dev takes.
+ * The reference's trainer does this in libtorch (train.cpp:79-128); the loss is its policy term (train.cpp:90-112)
+ * behind PolicyHead's 1x1 convolution (network.hpp:46-65), the optimiser is not the reference's Adam.
+ * These calls belong to no context.  Every pointer is a device pointer, `stream` is the caller's hipStream_t on `device`
+ * (NULL: that device's null stream), everything is queued on it and nothing is allocated, copied or waited for, so a
+ * call can be captured into a HIP graph.  The workspace is the caller's too: 256-byte aligned, at least as large as the
+ * _workspace call says for the same arguments (0 = the arguments are refused, az_last_error says why), in use until the
+ * call's work is done.  Calls that may run at the same time -- two streams, two captured graphs -- need a workspace
+ * each; the calls keep no state of their own and may be made from any thread. */
+#define AZ_F32  0
+#define AZ_F16  1
+#define AZ_BF16 2
+#define AZ_CHANNELS_FIRST 0   /* [B, C, N, N] */
+#define AZ_CHANNELS_LAST  1   /* [B, N, N, C] */
+
+/* Cross entropy of the policy head over all c_out * N * N actions of a board, with its gradients; the logits are never
+ * written.  z = weight . features + bias, loss[b] = sum t (lse_b - z) over the entries with a target, lse_b over the
+ * allowed actions.  Targets need not sum to 1 (a search policy sums to (n - 1) / n, mcts.hpp:136-146).
+ * Gradients are those of sum_b r_b loss_b, r_b = scale * row_scale[b]: d_features in the features' type and layout,
+ * d_weight and d_bias in fp32, written, not added to.
+ * A board without a target has loss 0 and no gradient; so has one without an allowed action and without a target.  A
+ * target on an action that is not allowed makes its board's loss +inf (and that entry's gradient 0). */
+typedef struct az_policy_loss_args {
+    int   device;
+    int   B, N, C, c_out;          /* boards, 1 <= N <= 32, 1 <= C <= 256, 1 <= c_out <= 128; B may be 0 */
+    int   dtype, layout;           /* AZ_F32 / AZ_F16 / AZ_BF16 of features, weight, bias and d_features; AZ_CHANNELS_* */
+    const void* features;          /* contiguous in `layout`: what the last ResBlock leaves (network.hpp:32-38) */
+    const void* weight;            /* [c_out, C] */
+    const void* bias;              /* [c_out] */
+    /* targets: dense, f32 [B, c_out * N * N] as az_replay_drain's policy, or sparse as az_blokus_replay_drain's rows:
+     * the first counts[b] (at most cap) of actions i32 / probs f32 [B, cap]; an action named more than once counts with
+     * the sum, one outside 0 .. c_out * N * N - 1 is left out */
+    const float* target;
+    const int32_t* counts;
+    const int32_t* actions;
+    const float* probs;
+    int   cap;
+    const uint32_t* legal;         /* NULL = all actions; else u32 [B, c_out * N], bit x of word co * N + y: (co, y, x) is
+                                      allowed (the layout of az_tower_forward_masked_dev's `wanted`) */
+    float scale;
+    const float* row_scale;        /* f32 [B] or NULL = 1 */
+    float* loss;                   /* out f32 [B] or NULL */
+    float* stats;                  /* f32 [B, 4] or NULL, 16-byte aligned: {lse, sum of targets, internal, loss}.  Out, unless
+                                      stats_given: then in, as an earlier call without it left them for the same inputs, and
+                                      only the gradients are computed */
+    int   stats_given;
+    void*  d_features;             /* out, all three or none */
+    float* d_weight;               /* [c_out, C] */
+    float* d_bias;                 /* [c_out] */
+} az_policy_loss_args;
+size_t az_policy_loss_workspace(const az_policy_loss_args*);
+int az_policy_loss_dev(const az_policy_loss_args*, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out_i = scale * (update_i with its singular values x taken to what `steps` times x -> a x + b x^3 + c x^5 makes of
+ * x / (|update_i|_F + eps)), for n matrices of rows x cols, row-major and contiguous, `stride` elements apart: the
+ * orthogonalised update of a convolution's weight [C_out, C_in * 9] (a = 3.4445, b = -4.775, c = 2.0315, 5 steps take
+ * singular values between 1/100 and 1 of the norm to about 0.7 .. 1.2).  A strided batch takes the convolutions of all
+ * ResBlocks straight out of the weight blob (az_load_weights).  out may not overlap update. */
+typedef struct az_orthogonalize_args {
+    int   device;
+    int   n, rows, cols;           /* n may be 0; the shorter side at most 8192 */
+    int   dtype;                   /* of update and out */
+    int   steps;                   /* 0..100 */
+    float a, b, c, eps, scale;     /* |a| + |b| + |c| <= 32 */
+    const void* update;
+    int64_t update_stride;
+    void* out;
+    int64_t out_stride;
+} az_orthogonalize_args;
+size_t az_orthogonalize_workspace(const az_orthogonalize_args*);
+int az_orthogonalize_dev(const az_orthogonalize_args*, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One optimiser step of n weight matrices: momentum_out = beta momentum + grad; u = nesterov ? grad + beta momentum_out :
+ * momentum_out; weight_out = (1 - lr weight_decay) weight - lr * az_orthogonalize(u, scale).  Weights and momenta are fp32;
+ * either output may be its input (same address and stride: in place), no other tensors may overlap an output. */
+typedef struct az_muon_step_args {
+    int   device;
+    int   n, rows, cols;
+    int   grad_dtype;
+    int   steps;
+    float a, b, c, eps, scale;
+    float lr, beta, weight_decay;
+    int   nesterov;
+    const void* grad;
+    int64_t grad_stride;
+    const float* weight;
+    int64_t weight_stride;
+    const float* momentum;
+    int64_t momentum_stride;
+    float* weight_out;
+    int64_t weight_out_stride;
+    float* momentum_out;
+    int64_t momentum_out_stride;
+} az_muon_step_args;
+size_t az_muon_step_workspace(const az_muon_step_args*);
+int az_muon_step_dev(const az_muon_step_args*, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Measurement hook (no counterpart in the reference, whose only timers are the
  * verbosity-3 chrono buckets of mcts.hpp:187-201): HIP events on the context's
  * stream around every 3x3-convolution launch and every tree-round launch of
