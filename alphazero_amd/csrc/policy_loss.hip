@@ -7,8 +7,8 @@
 //   dz[b,o,s] = r_b (T_b exp(z - lse_b) - t) on allowed entries, 0 elsewhere;  T_b = sum t
 //   dh = w^T dz      dw = sum dz h^T      dbias = sum dz
 //
-// Rows of the work are cells: row r = b * S + s of the flattened batch, 64 rows a step, whatever the board size (a step
-// may hold parts of several boards).  az_policy_rows_kernel forms the logits of a step in registers and leaves a row's
+// Rows of the work are cells: row r = b * S + s of the flattened batch.  A step is up to 64 rows: a block of one board, or
+// several whole boards where they are small (32 cells or fewer).  az_policy_rows_kernel forms the logits of a step in registers and leaves a row's
 // {max, sum of exp, sum t z, sum t}; az_policy_boards_kernel joins a board's rows; az_policy_grad_kernel forms the same
 // logits again -- 2 C flop an entry against 8 bytes of a kept fp32 logit written and read -- turns them into dz in LDS
 // and multiplies it both ways; az_policy_reduce_kernel adds the workgroups' dw and dbias in a fixed order.
@@ -28,6 +28,8 @@ int lfail(int code, const char* fmt, ...) {
 
 constexpr int ROWS = 64;                     // rows of a step
 constexpr int MAX_GROUPS = 512;              // workgroups of the gradient kernel: two a CU
+constexpr int ENTRIES = 1024;                // sparse targets of a step's boards kept in LDS; longer lists are read from memory
+constexpr int MAX_BOARDS = 16;               // boards of a step
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct PolicyDev {
@@ -41,9 +43,11 @@ struct PolicyDev {
     az_f4* rowstat;                          // [B * S] {max, sum, sum t z, sum t}
     az_f4* stats;                            // [B] {lse, T, 1 where a masked action has a target, loss}
     float *loss, *partial;
+    const float *wpad, *wpadt;               // fp32 weights that do not fit LDS: padded copies
     void* dh;
     int B, N, S, C, O, cap, nchw;
-    int rows, steps;
+    int rows, steps;                         // steps = work items of up to 64 rows
+    int nb, blocks;                          // boards a step holds (blocks = 1), or blocks a board is cut into (nb = 1)
 };
 
 // dynamic LDS of the two product kernels
@@ -51,9 +55,9 @@ template <int DT, int OT> struct Lay {
     static constexpr int EP = AzElem<DT>::EP, KS = AzElem<DT>::KS, SZ = 16 / EP;
     static constexpr int OP = (OT * 16 + KS - 1) / KS * KS;          // planes, padded to a step of the contraction over them
     static constexpr int LDT = OT * 16 + 4, LDO = OP + EP;
-    static int ldc(int Cp) { return Cp + EP; }                       // 16 bytes of padding: rows start in different banks
-    static size_t w_bytes(int Cp) { return (size_t)OP * ldc(Cp) * SZ; }
-    static size_t h_bytes(int Cp) { return (size_t)ROWS * ldc(Cp) * SZ; }
+    __host__ __device__ static int ldc(int Cp) { return Cp + EP; }                       // 16 bytes of padding: rows start in different banks
+    __host__ __device__ static size_t w_bytes(int Cp) { return (size_t)OP * ldc(Cp) * SZ; }
+    __host__ __device__ static size_t h_bytes(int Cp) { return (size_t)ROWS * ldc(Cp) * SZ; }
     static constexpr size_t z_bytes = (size_t)ROWS * (LDO > LDT ? LDO : LDT) * 4;
 };
 
@@ -77,12 +81,26 @@ template <int DT, int OT> __device__ void stage_w(const PolicyDev& a, void* wl, 
     }
 }
 
+// A step: rows rbase .. rbase + n - 1 of the flattened batch, cells cell0 .. of board b0 (or whole boards b0 ..).
+struct Step { int b0, cell0, rbase, n; };
+__device__ __forceinline__ Step step_at(const PolicyDev& a, int it) {
+    Step s;
+    if (a.nb > 1) {
+        s.b0 = it * a.nb; s.cell0 = 0; s.rbase = s.b0 * a.S;
+        s.n = min(a.nb, a.B - s.b0) * a.S;
+    } else {
+        s.b0 = it / a.blocks; s.cell0 = (it - s.b0 * a.blocks) * ROWS; s.rbase = s.b0 * a.S + s.cell0;
+        s.n = min(ROWS, a.S - s.cell0);
+    }
+    return s;
+}
+
 // The 16-byte pieces of a step's features a thread carries from memory to LDS: rows r0 .., piece p of row r holds
 // channels EP * p .. + EP - 1 (zero beyond C and beyond the last row).  Channels last: one load where the piece is whole.
 // Channels first: consecutive threads take consecutive cells, EP loads of one element each.
 template <int DT, int NP> struct Feat {
     az_i4 v[NP];
-    template <int NT> __device__ __forceinline__ void load(const PolicyDev& a, int r0, int pieces, int tid) {
+    template <int NT> __device__ __forceinline__ void load(const PolicyDev& a, const Step& st, int pieces, int tid) {
         constexpr int EP = AzElem<DT>::EP;
         typedef typename AzElem<DT>::T T;
         #pragma unroll
@@ -90,11 +108,11 @@ template <int DT, int NP> struct Feat {
             const int k = tid + i * NT;
             int row, p;
             if (a.nchw) { row = k % ROWS; p = k / ROWS; } else { row = k / pieces; p = k % pieces; }
-            const int r = r0 + row, c0 = p * EP;
+            const int r = st.rbase + row, c0 = p * EP;
             T e[EP];
             #pragma unroll
             for (int j = 0; j < EP; ++j) e[j] = (T)0.f;
-            if (row < ROWS && p < pieces && r < a.rows) {
+            if (row < st.n && p < pieces) {
                 if (!a.nchw) {
                     const T* src = (const T*)a.h + (size_t)r * a.C + c0;
                     if (c0 + EP <= a.C) {
@@ -126,106 +144,162 @@ template <int DT, int NP> struct Feat {
     }
 };
 
-// The sparse targets of a step into t [ROWS][LDT] (zeroed before).  One wave takes a board's entries in their order and
-// an LDS add of one wave takes its lanes in theirs, so an action that is named more than once is summed in one order.
-// Entries outside 0 .. O * S - 1 are left out.
-template <int LDT> __device__ __forceinline__ void scatter_targets(const PolicyDev& a, float* t, int r0, int wave, int waves, int lane) {
-    const int last = min(r0 + ROWS, a.rows) - 1;
-    const int b0 = r0 / a.S, b1 = last / a.S;
-    for (int b = b0 + wave; b <= b1; b += waves) {
-        const int n = min(a.counts[b], a.cap);
-        const int base = b * a.S - r0;
-        for (int e = lane; e < n; e += 64) {
-            const int act = a.actions[(size_t)b * a.cap + e];
-            if ((unsigned)act >= (unsigned)(a.O * a.S)) continue;
-            const int o = act / a.S, idx = base + (act - o * a.S);
-            if ((unsigned)idx < (unsigned)ROWS) __hip_atomic_fetch_add(t + idx * LDT + o, a.probs[(size_t)b * a.cap + e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+// What a step's boards need beside the features, brought to LDS when the board changes: the legal-move words, and the
+// sparse targets as {row of the step's boards * 256 + plane, value} (entries that are left out: -1).
+struct BoardLds {
+    unsigned* words;
+    int* key;
+    float* val;
+    bool listed;                                                     // the entries fit
+};
+__host__ __device__ inline int entry_room(int nb, int cap) { return (long long)nb * cap <= ENTRIES ? nb * cap : 0; }
+__device__ __forceinline__ int entry_key(const PolicyDev& a, int act, int bb) {
+    if ((unsigned)act >= (unsigned)(a.O * a.S)) return -1;
+    const int o = act / a.S;
+    return (bb * a.S + act - o * a.S) * 256 + o;
+}
+__device__ __forceinline__ void stage_boards(const PolicyDev& a, const BoardLds& l, int b0, int tid, int nt) {
+    const int boards = min(a.nb, a.B - b0);
+    if (a.legal) for (int i = tid; i < boards * a.O * a.N; i += nt) l.words[i] = a.legal[(size_t)b0 * a.O * a.N + i];
+    if (a.counts && l.listed)
+        for (int e = tid; e < boards * a.cap; e += nt) {
+            const int bb = a.nb > 1 ? e / a.cap : 0, k = e - bb * a.cap;
+            const size_t at = (size_t)(b0 + bb) * a.cap + k;
+            const bool live = k < a.counts[b0 + bb];
+            l.key[e] = live ? entry_key(a, a.actions[at], bb) : -1;
+            l.val[e] = live ? a.probs[at] : 0.f;
         }
+}
+// The sparse targets of a step into t [ROWS][LDT] (zeroed before).  A wave adds the entries of its own planes in their
+// order (an LDS add takes a wave's lanes in theirs), so an action that is named more than once is summed in one order.
+template <int LDT, int WAVES> __device__ __forceinline__ void scatter_targets(const PolicyDev& a, const BoardLds& l, float* t, const Step& st, int wave, int lane) {
+    const int boards = min(a.nb, a.B - st.b0), n = boards * a.cap;
+    for (int e = lane; e < n; e += 64) {
+        int key;
+        float v;
+        if (l.listed) { key = l.key[e]; v = l.val[e]; }
+        else {
+            const int bb = a.nb > 1 ? e / a.cap : 0, k = e - bb * a.cap;
+            const size_t at = (size_t)(st.b0 + bb) * a.cap + k;
+            key = k < a.counts[st.b0 + bb] ? entry_key(a, a.actions[at], bb) : -1;
+            v = a.probs[at];
+        }
+        const int o = key & 255, row = (key >> 8) - st.cell0;
+        if (key >= 0 && o % WAVES == wave && (unsigned)row < (unsigned)ROWS)
+            __hip_atomic_fetch_add(t + row * LDT + o, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
 }
 
-__device__ __forceinline__ bool allowed(const PolicyDev& a, size_t word0, int o, int x) {
-    return (a.legal[word0 + (size_t)o * a.N] >> x) & 1u;
+// fp32 weights of more than 32 planes and 128 channels do not fit LDS beside a step: a zero-padded copy [OP][Cp] and one
+// transposed [Cp][OP] lie in the workspace, and fragments come from the caches (the fp32 matrix instructions take 32
+// cycles for the 512 bytes of operands that a wave loads).
+__global__ void __launch_bounds__(256) az_policy_pad_weight_kernel(const float* w, float* pad, float* padt, int O, int C, int OP, int Cp) {
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < OP * Cp; i += gridDim.x * 256) {
+        const int o = i / Cp, c = i % Cp;
+        const float v = o < O && c < C ? w[(size_t)o * C + c] : 0.f;
+        pad[i] = v;
+        padt[c * OP + o] = v;
+    }
 }
+template <int DT, int OT, int CB> __host__ __device__ constexpr bool w_in_lds() { return !(DT == 0 && CB == 2 && OT >= 4); }
+
+// LDS of both product kernels, in this order
+template <int DT, int OT, int CB> struct Smem {
+    typedef Lay<DT, OT> L;
+    unsigned char *w, *h;
+    float *t, *bias;
+    BoardLds b;
+    __device__ __forceinline__ Smem(unsigned char* p, const PolicyDev& a, int Cp) {
+        w = p; p += w_in_lds<DT, OT, CB>() ? L::w_bytes(Cp) : 0;
+        h = p; p += L::h_bytes(Cp);
+        t = (float*)p; p += L::z_bytes;
+        bias = (float*)p; p += OT * 16 * 4;
+        const int room = a.counts ? entry_room(a.nb, a.cap) : 0;
+        b.listed = room > 0;
+        b.key = (int*)p; p += (size_t)room * 4;
+        b.val = (float*)p; p += (size_t)room * 4;
+        b.words = (unsigned*)p;
+    }
+    static size_t bytes(const PolicyDev& a, int Cp) {
+        return (w_in_lds<DT, OT, CB>() ? L::w_bytes(Cp) : 0) + L::h_bytes(Cp) + L::z_bytes + OT * 16 * 4 + (a.counts ? (size_t)entry_room(a.nb, a.cap) * 8 : 0) +
+               (a.legal ? (size_t)a.nb * a.O * a.N * 4 : 0);
+    }
+};
 
 // Row statistics.  Four waves, 16 rows each, all planes.
 template <int DT, int OT, int CB> __global__ void __launch_bounds__(256) az_policy_rows_kernel(PolicyDev a) {
     typedef Lay<DT, OT> L;
     constexpr int NT = 256, NP = CB * 128 / L::EP * ROWS / NT;
-    constexpr bool WLDS = !(DT == 0 && CB == 2 && OT >= 6);
+    constexpr bool WLDS = w_in_lds<DT, OT, CB>();
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int Cp = (a.C + 31) / 32 * 32, ldc = Cp + L::EP, pieces = Cp / L::EP;
-    unsigned char* wl = smem;
-    unsigned char* hl = wl + (WLDS ? (size_t)L::OP * ldc * L::SZ : 0);
-    float* t = (float*)(hl + (size_t)ROWS * ldc * L::SZ);
+    const Smem<DT, OT, CB> m(smem, a, Cp);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
-    if (WLDS) stage_w<DT, OT>(a, wl, Cp, tid, NT);
+    if (WLDS) stage_w<DT, OT>(a, m.w, Cp, tid, NT);
+    for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
     const int s_lo = (int)((long long)blockIdx.x * a.steps / gridDim.x), s_hi = (int)((long long)(blockIdx.x + 1) * a.steps / gridDim.x);
     Feat<DT, NP> f;
-    if (s_lo < s_hi) f.template load<NT>(a, s_lo * ROWS, pieces, tid);
-    for (int st = s_lo; st < s_hi; ++st) {
-        const int r0 = st * ROWS;
-        __syncthreads();                                             // the step before has read hl and t
-        f.template store<NT>(a, hl, Cp, pieces, tid);
-        if (a.counts) for (int i = tid; i < ROWS * L::LDT; i += NT) t[i] = 0.f;
+    if (s_lo < s_hi) f.template load<NT>(a, step_at(a, s_lo), pieces, tid);
+    int board = -1;
+    for (int it = s_lo; it < s_hi; ++it) {
+        const Step st = step_at(a, it);
+        __syncthreads();                                             // the step before has read its LDS
+        f.template store<NT>(a, m.h, Cp, pieces, tid);
+        if (a.counts) for (int i = tid; i < ROWS * L::LDT / 4; i += NT) ((az_f4*)m.t)[i] = az_f4{0.f, 0.f, 0.f, 0.f};
+        if (st.b0 != board) { stage_boards(a, m.b, st.b0, tid, NT); board = st.b0; }
         __syncthreads();
-        if (st + 1 < s_hi) f.template load<NT>(a, r0 + ROWS, pieces, tid);
-        if (a.counts) { scatter_targets<L::LDT>(a, t, r0, wave, 4, lane); __syncthreads(); }
+        if (it + 1 < s_hi) f.template load<NT>(a, step_at(a, it + 1), pieces, tid);
+        if (a.counts) { scatter_targets<L::LDT, 4>(a, m.b, m.t, st, wave, lane); __syncthreads(); }
+        if (wave * 16 >= st.n) continue;
         az_f4 acc[OT];
         #pragma unroll
-        for (int ot = 0; ot < OT; ++ot)
-            for (int i = 0; i < 4; ++i) { const int o = ot * 16 + q * 4 + i; acc[ot][i] = o < a.O ? az_load<DT>(a.bias, o) : 0.f; }
+        for (int ot = 0; ot < OT; ++ot) acc[ot] = *(const az_f4*)(m.bias + ot * 16 + q * 4);
         for (int k = 0; k < Cp; k += L::KS) {
-            const az_i4 hb = az_row_frag<DT>(hl, ldc, wave * 16, k, lane);
+            const az_i4 hb = az_row_frag<DT>(m.h, ldc, wave * 16, k, lane);
             #pragma unroll
-            for (int ot = 0; ot < OT; ++ot) {
-                az_i4 wa;
-                if constexpr (WLDS) wa = az_row_frag<DT>(wl, ldc, ot * 16, k, lane);
-                else {
-                    const int o = ot * 16 + (lane & 15), c = k + L::EP * q;
-                    az_f4 x = {0.f, 0.f, 0.f, 0.f};
-                    for (int j = 0; j < 4; ++j) if (o < a.O && c + j < a.C) x[j] = ((const float*)a.w)[(size_t)o * a.C + c + j];
-                    wa = __builtin_bit_cast(az_i4, x);
-                }
-                acc[ot] = az_mma<DT>(wa, hb, acc[ot]);
-            }
+            for (int ot = 0; ot < OT; ++ot)
+                acc[ot] = az_mma<DT>(WLDS ? az_row_frag<DT>(m.w, ldc, ot * 16, k, lane) : az_row_frag<DT>(a.wpad, Cp, ot * 16, k, lane), hb, acc[ot]);
         }
-        const int rl = wave * 16 + (lane & 15), r = r0 + rl;
-        if (r < a.rows) {
-            const int b = r / a.S, s = r - b * a.S, y = s / a.N, x = s - y * a.N;
-            const size_t word0 = (size_t)b * a.O * a.N + y;
-            float m = -INFINITY, tz = 0.f, tm = 0.f;
+        const int rl = wave * 16 + (lane & 15);
+        if (rl < st.n) {
+            const int bb = a.nb > 1 ? rl / a.S : 0, s = st.cell0 + rl - bb * a.S, y = s / a.N, x = s - y * a.N;
+            const unsigned* words = m.b.words + (bb * a.O + q * 4) * a.N + y;
+            const float* dense = a.counts ? nullptr : a.dense + ((size_t)(st.b0 + bb) * a.O + q * 4) * a.S + s;
+            float mx = -INFINITY, tz = 0.f, tm = 0.f;
             #pragma unroll
             for (int ot = 0; ot < OT; ++ot) {
+                az_f4 tv = {0.f, 0.f, 0.f, 0.f};
+                if (a.counts) tv = *(const az_f4*)(m.t + rl * L::LDT + ot * 16 + q * 4);
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int o = ot * 16 + q * 4 + i;
                     if (o < a.O) {
-                        const float tv = a.counts ? t[rl * L::LDT + o] : a.dense[((size_t)b * a.O + o) * a.S + s];
-                        if (a.legal && !allowed(a, word0, o, x)) acc[ot][i] = -INFINITY;
+                        if (!a.counts) tv[i] = dense[(size_t)(ot * 16 + i) * a.S];
+                        if (a.legal && !((words[(ot * 16 + i) * a.N] >> x) & 1u)) acc[ot][i] = -INFINITY;
                         const float z = acc[ot][i];
-                        if (tv != 0.f) { tz += tv * z; tm += tv; }
-                        if (!(z <= m)) m = z;                        // (a NaN logit stays in sight: it compares false)
+                        if (tv[i] != 0.f) { tz += tv[i] * z; tm += tv[i]; }
+                        if (!(z <= mx)) mx = z;                      // (a NaN logit is not lost: its exponential joins the sum)
                     } else acc[ot][i] = -INFINITY;
                 }
             }
             // four groups of lanes hold a row's planes
             for (int d = 16; d <= 32; d <<= 1) {
-                const float om = __shfl_xor(m, d, 64);
-                if (!(om <= m)) m = om;
+                const float om = __shfl_xor(mx, d, 64);
+                if (!(om <= mx)) mx = om;
                 tz += __shfl_xor(tz, d, 64);
                 tm += __shfl_xor(tm, d, 64);
             }
             float l = 0.f;
-            if (m != -INFINITY) {
+            if (mx != -INFINITY) {
+                const float ml = mx * LOG2E;
                 #pragma unroll
                 for (int ot = 0; ot < OT; ++ot)
                     #pragma unroll
-                    for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f((acc[ot][i] - m) * LOG2E);
+                    for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[ot][i], LOG2E, -ml));
             }
             for (int d = 16; d <= 32; d <<= 1) l += __shfl_xor(l, d, 64);
             if (q == 0) {
-                a.rowstat[r] = az_f4{m, l, tz, tm};
+                a.rowstat[st.rbase + rl] = az_f4{mx, l, tz, tm};
                 asm volatile("s_nop 1");                             // (a wide store reads its registers after it has issued)
             }
         }
@@ -261,43 +335,47 @@ __global__ void __launch_bounds__(256) az_policy_boards_kernel(PolicyDev a) {
     }
 }
 
-// Gradients.  Eight waves.  A step: dz of 64 rows (16 rows and half of the planes a wave), then its product with w (16
-// rows and half of the channels a wave) and its product with the features (every eighth 16 channels a wave, all planes,
-// kept in registers over all of a workgroup's steps).  16-bit features: dz goes to LDS as hi + lo of the type, hi alone
-// feeds dh (whose result is rounded to that type anyway), both feed dw (an fp32 sum over all rows: one rounding to 16
-// bits of each term would stay in it).
+// Gradients.  Eight waves.  A step: dz of 64 rows (16 rows and half of the planes a wave), then its product with w (32
+// rows and a quarter of the channels a wave) and its product with the features (half of the planes and a quarter of the
+// channels a wave, kept in registers over all of a workgroup's steps).  16-bit features: dz goes to LDS as hi + lo of the
+// type, hi alone feeds dh (whose result is rounded to that type anyway), both feed dw (an fp32 sum over all rows: one
+// rounding to 16 bits of each term would stay in it).
 template <int DT, int OT, int CB> __global__ void __launch_bounds__(512) az_policy_grad_kernel(PolicyDev a) {
     typedef Lay<DT, OT> L;
     typedef typename AzElem<DT>::T T;
-    constexpr int NT = 512, NP = CB * 128 / L::EP * ROWS / NT, OTH = (OT + 1) / 2;
-    constexpr bool WLDS = !(DT == 0 && CB == 2 && OT >= 6);
+    constexpr int NT = 512, NP = CB * 128 / L::EP * ROWS / NT, OTH = (OT + 1) / 2, KO = L::OP / L::KS;
+    constexpr int OG = OT > 1 ? 2 : 1, CG = 8 / OG, OTN = OT / OG, CTN = CB * 8 / CG;   // dw: groups of planes and channels, tiles of a wave
+    constexpr bool WLDS = w_in_lds<DT, OT, CB>();
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int Cp = (a.C + 31) / 32 * 32, ldc = Cp + L::EP, pieces = Cp / L::EP;
-    unsigned char* wl = smem;
-    unsigned char* hl = wl + (WLDS ? (size_t)L::OP * ldc * L::SZ : 0);
-    float* t = (float*)(hl + (size_t)ROWS * ldc * L::SZ);            // the step's targets, then its dz in the same place
+    const Smem<DT, OT, CB> m(smem, a, Cp);
+    float* t = m.t;                                                  // the step's targets, then its dz in the same place
     T* zhi = (T*)t;
     T* zlo = zhi + ROWS * L::LDO;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, rt = wave & 3, half = wave >> 2;
-    if (WLDS) stage_w<DT, OT>(a, wl, Cp, tid, NT);
+    if (WLDS) stage_w<DT, OT>(a, m.w, Cp, tid, NT);
+    for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
     const int s_lo = (int)((long long)blockIdx.x * a.steps / gridDim.x), s_hi = (int)((long long)(blockIdx.x + 1) * a.steps / gridDim.x);
-    az_f4 dw[CB][OT];
+    const int og = OG == 2 ? wave & 1 : 0, cg = OG == 2 ? wave >> 1 : wave;
+    az_f4 dw[CTN][OTN];
     #pragma unroll
-    for (int i = 0; i < CB; ++i)
-        for (int j = 0; j < OT; ++j) dw[i][j] = az_f4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < CTN; ++i)
+        #pragma unroll
+        for (int j = 0; j < OTN; ++j) dw[i][j] = az_f4{0.f, 0.f, 0.f, 0.f};
     az_f4 db[OTH];
     #pragma unroll
     for (int j = 0; j < OTH; ++j) db[j] = az_f4{0.f, 0.f, 0.f, 0.f};
     Feat<DT, NP> f;
-    if (s_lo < s_hi) f.template load<NT>(a, s_lo * ROWS, pieces, tid);
+    if (s_lo < s_hi) f.template load<NT>(a, step_at(a, s_lo), pieces, tid);
     // fp16: dz is r_b (a mean over the batch: 1 / B) times probabilities that may be 1e-5, below what fp16 resolves.  The
     // workgroup's dz carry a power of two that puts the largest r_b T_b of its boards at 2^9 .. 2^10; it comes off the
     // fp32 sums again.
     float up = 1.f, down = 1.f;
     if constexpr (DT == 1) {
-        const int b0 = s_lo * ROWS / a.S, b1 = (min(s_hi * ROWS, a.rows) - 1) / a.S;
+        const Step first = step_at(a, s_lo), last = step_at(a, s_hi - 1);
+        const int b1 = min(last.b0 + a.nb, a.B);
         float mx = 0.f;
-        for (int b = b0 + tid; b <= b1; b += NT) mx = fmaxf(mx, fabsf(a.scale * (a.row_scale ? a.row_scale[b] : 1.f) * a.stats[b][1]));
+        for (int b = first.b0 + tid; b < b1; b += NT) mx = fmaxf(mx, fabsf(a.scale * (a.row_scale ? a.row_scale[b] : 1.f) * a.stats[b][1]));
         mx = wave_max(mx);
         if (lane == 0) t[wave] = mx;
         __syncthreads();
@@ -308,19 +386,21 @@ template <int DT, int OT, int CB> __global__ void __launch_bounds__(512) az_poli
             down = ldexpf(1.f, -e);
         }
     }
-    for (int st = s_lo; st < s_hi; ++st) {
-        const int r0 = st * ROWS;
-        __syncthreads();                                             // the step before has read hl and dz
-        f.template store<NT>(a, hl, Cp, pieces, tid);
-        if (a.counts) for (int i = tid; i < ROWS * L::LDT; i += NT) t[i] = 0.f;
+    int board = -1;
+    for (int it = s_lo; it < s_hi; ++it) {
+        const Step st = step_at(a, it);
+        __syncthreads();                                             // the step before has read its LDS
+        f.template store<NT>(a, m.h, Cp, pieces, tid);
+        if (a.counts) for (int i = tid; i < ROWS * L::LDT / 4; i += NT) ((az_f4*)t)[i] = az_f4{0.f, 0.f, 0.f, 0.f};
+        if (st.b0 != board) { stage_boards(a, m.b, st.b0, tid, NT); board = st.b0; }
         __syncthreads();
-        if (st + 1 < s_hi) f.template load<NT>(a, r0 + ROWS, pieces, tid);
-        const int rl = rt * 16 + (lane & 15), r = r0 + rl;
-        const bool live = r < a.rows;
-        const int b = live ? r / a.S : 0, s = live ? r - b * a.S : 0, y = s / a.N, x = s - y * a.N;
+        if (it + 1 < s_hi) f.template load<NT>(a, step_at(a, it + 1), pieces, tid);
+        const int rl = rt * 16 + (lane & 15);
+        const bool live = rl < st.n;
+        const int bb = live && a.nb > 1 ? rl / a.S : 0, b = st.b0 + bb, s = live ? st.cell0 + rl - bb * a.S : 0, y = s / a.N, x = s - y * a.N;
         az_f4 tv[OTH];
         if (a.counts) {
-            scatter_targets<L::LDT>(a, t, r0, wave, 8, lane);
+            scatter_targets<L::LDT, 8>(a, m.b, t, st, wave, lane);
             __syncthreads();
             #pragma unroll
             for (int j = 0; j < OTH; ++j) {
@@ -329,38 +409,27 @@ template <int DT, int OT, int CB> __global__ void __launch_bounds__(512) az_poli
             }
             __syncthreads();                                         // dz takes the targets' place
         } else {
+            const float* dense = a.dense + ((size_t)b * a.O + half * OTH * 16 + q * 4) * a.S + s;
             #pragma unroll
             for (int j = 0; j < OTH; ++j)
-                for (int i = 0; i < 4; ++i) {
-                    const int o = (half * OTH + j) * 16 + q * 4 + i;
-                    tv[j][i] = live && o < a.O ? a.dense[((size_t)b * a.O + o) * a.S + s] : 0.f;
-                }
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) tv[j][i] = live && (half * OTH + j) * 16 + q * 4 + i < a.O ? dense[(size_t)(j * 16 + i) * a.S] : 0.f;
         }
         az_f4 acc[OTH];
         #pragma unroll
-        for (int j = 0; j < OTH; ++j)
-            for (int i = 0; i < 4; ++i) { const int o = (half * OTH + j) * 16 + q * 4 + i; acc[j][i] = o < a.O ? az_load<DT>(a.bias, o) : 0.f; }
+        for (int j = 0; j < OTH; ++j) acc[j] = half * OTH + j < OT ? *(const az_f4*)(m.bias + (half * OTH + j) * 16 + q * 4) : az_f4{0.f, 0.f, 0.f, 0.f};
         for (int k = 0; k < Cp; k += L::KS) {
-            const az_i4 hb = az_row_frag<DT>(hl, ldc, rt * 16, k, lane);
+            const az_i4 hb = az_row_frag<DT>(m.h, ldc, rt * 16, k, lane);
             #pragma unroll
             for (int j = 0; j < OTH; ++j) {
                 const int ot = half * OTH + j;
-                if (ot >= OT) continue;
-                az_i4 wa;
-                if constexpr (WLDS) wa = az_row_frag<DT>(wl, ldc, ot * 16, k, lane);
-                else {
-                    const int o = ot * 16 + (lane & 15), c = k + L::EP * q;
-                    az_f4 v = {0.f, 0.f, 0.f, 0.f};
-                    for (int e = 0; e < 4; ++e) if (o < a.O && c + e < a.C) v[e] = ((const float*)a.w)[(size_t)o * a.C + c + e];
-                    wa = __builtin_bit_cast(az_i4, v);
-                }
-                acc[j] = az_mma<DT>(wa, hb, acc[j]);
+                if (ot < OT) acc[j] = az_mma<DT>(WLDS ? az_row_frag<DT>(m.w, ldc, ot * 16, k, lane) : az_row_frag<DT>(a.wpad, Cp, ot * 16, k, lane), hb, acc[j]);
             }
         }
         const az_f4 bst = live ? a.stats[b] : az_f4{0.f, 0.f, 0.f, 0.f};
         const float rs = live ? up * (a.scale * (a.row_scale ? a.row_scale[b] : 1.f)) : 0.f;
-        const float rT = rs * bst[1];
-        const size_t word0 = (size_t)b * a.O * a.N + y;
+        const float rT = rs * bst[1], lse2 = bst[0] * LOG2E;
+        const unsigned* words = m.b.words + (bb * a.O + half * OTH * 16 + q * 4) * a.N + y;
         // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
         const bool bias_counts = a.O > 1 || bst[2] != 0.f;
         #pragma unroll
@@ -370,9 +439,9 @@ template <int DT, int OT, int CB> __global__ void __launch_bounds__(512) az_poli
             az_f4 dz;
             #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int o = ot * 16 + q * 4 + i;
-                const bool on = live && o < a.O && !(a.legal && !allowed(a, word0, o, x));
-                dz[i] = on ? rT * __builtin_amdgcn_exp2f((acc[j][i] - bst[0]) * LOG2E) - rs * tv[j][i] : 0.f;
+                bool on = live && ot * 16 + q * 4 + i < a.O;
+                if (a.legal && on) on = (words[(j * 16 + i) * a.N] >> x) & 1u;
+                dz[i] = on ? rT * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -lse2)) - rs * tv[j][i] : 0.f;
                 if (bias_counts) db[j][i] += dz[i];
             }
             if constexpr (DT == 0) *(az_f4*)((float*)zhi + rl * L::LDO + ot * 16 + q * 4) = dz;
@@ -385,58 +454,81 @@ template <int DT, int OT, int CB> __global__ void __launch_bounds__(512) az_poli
             }
         }
         __syncthreads();
-        // dh: rows of the tile are channels, columns are cells
-        for (int ct = half; ct * 16 < Cp; ct += 2) {
-            az_f4 d = {0.f, 0.f, 0.f, 0.f};
+        // dh: rows of a tile are channels, columns are cells
+        {
+            const int pair = wave & 1, cq = wave >> 1;
+            az_i4 zf[2][KO];
             #pragma unroll
-            for (int k = 0; k < L::OP; k += L::KS) {
-                az_i4 wa;
-                if constexpr (WLDS) wa = az_col_frag<DT>(wl, ldc, k, ct * 16, lane);
-                else {
-                    const int c = ct * 16 + (lane & 15);
-                    az_f4 v = {0.f, 0.f, 0.f, 0.f};
-                    for (int e = 0; e < 4; ++e) { const int o = k + 4 * q + e; if (o < a.O && c < a.C) v[e] = ((const float*)a.w)[(size_t)o * a.C + c]; }
-                    wa = __builtin_bit_cast(az_i4, v);
+            for (int k = 0; k < KO; ++k)
+                #pragma unroll
+                for (int e = 0; e < 2; ++e) zf[e][k] = az_row_frag<DT>(zhi, L::LDO, (pair * 2 + e) * 16, k * L::KS, lane);
+            #pragma unroll
+            for (int j = 0; j < CB * 2; ++j) {
+                const int ct = cq + 4 * j;
+                if (ct * 16 >= Cp) continue;
+                az_f4 d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                #pragma unroll
+                for (int k = 0; k < KO; ++k) {
+                    az_i4 wa;
+                    if constexpr (WLDS) wa = az_col_frag<DT>(m.w, ldc, k * L::KS, ct * 16, lane);
+                    else wa = az_row_frag<DT>(a.wpadt, L::OP, ct * 16, k * L::KS, lane);
+                    d[0] = az_mma<DT>(wa, zf[0][k], d[0]);
+                    d[1] = az_mma<DT>(wa, zf[1][k], d[1]);
                 }
-                d = az_mma<DT>(wa, az_row_frag<DT>(zhi, L::LDO, rt * 16, k, lane), d);
-            }
-            if constexpr (DT == 1) d *= down;
-            const int c = ct * 16 + q * 4;
-            if (live && c < a.C) {
-                if (!a.nchw) {
-                    const size_t at = (size_t)r * a.C + c;
-                    if (c + 4 <= a.C) {
-                        if constexpr (DT == 0) *(az_f4_u*)((float*)a.dh + at) = d;
-                        else *(az_s4_u*)((short*)a.dh + at) = az_s4{az_to16<DT>(d[0]), az_to16<DT>(d[1]), az_to16<DT>(d[2]), az_to16<DT>(d[3])};
-                    } else for (int i = 0; i < 4; ++i) if (c + i < a.C) az_store<DT>(a.dh, at + i, d[i]);
-                } else for (int i = 0; i < 4; ++i) if (c + i < a.C) az_store<DT>(a.dh, ((size_t)b * a.C + c + i) * a.S + s, d[i]);
+                const int c = ct * 16 + q * 4;
+                #pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = (pair * 2 + e) * 16 + (lane & 15);
+                    if (row >= st.n || c >= a.C) continue;
+                    if constexpr (DT == 1) d[e] *= down;
+                    if (!a.nchw) {
+                        const size_t at = (size_t)(st.rbase + row) * a.C + c;
+                        if (c + 4 <= a.C) {
+                            if constexpr (DT == 0) *(az_f4_u*)((float*)a.dh + at) = d[e];
+                            else *(az_s4_u*)((short*)a.dh + at) = az_s4{az_to16<DT>(d[e][0]), az_to16<DT>(d[e][1]), az_to16<DT>(d[e][2]), az_to16<DT>(d[e][3])};
+                        } else for (int i = 0; i < 4; ++i) if (c + i < a.C) az_store<DT>(a.dh, at + i, d[e][i]);
+                    } else {
+                        const int b2 = a.nb > 1 ? row / a.S : 0, s2 = st.cell0 + row - b2 * a.S;
+                        const size_t at = ((size_t)(st.b0 + b2) * a.C + c) * a.S + s2;
+                        for (int i = 0; i < 4; ++i) if (c + i < a.C) az_store<DT>(a.dh, at + (size_t)i * a.S, d[e][i]);
+                    }
+                }
             }
         }
-        // dw: rows of the tile are planes, columns are channels, the contraction runs over the step's rows
+        // dw: rows of a tile are planes, columns are channels, the contraction runs over the step's rows (rows beyond the
+        // step have dz = 0 and features of 0)
         #pragma unroll
-        for (int ci = 0; ci < CB; ++ci) {
-            const int ct = wave + 8 * ci;
-            if (ct * 16 >= Cp) continue;
+        for (int k = 0; k < ROWS; k += L::KS) {
+            if (k >= st.n) break;
+            az_i4 zf[OTN][DT == 0 ? 1 : 2];
             #pragma unroll
-            for (int k = 0; k < ROWS; k += L::KS) {
-                const az_i4 hb = az_col_frag<DT>(hl, ldc, k, ct * 16, lane);
+            for (int j = 0; j < OTN; ++j) {
+                zf[j][0] = az_col_frag<DT>(zhi, L::LDO, k, (og * OTN + j) * 16, lane);
+                if constexpr (DT != 0) zf[j][1] = az_col_frag<DT>(zlo, L::LDO, k, (og * OTN + j) * 16, lane);
+            }
+            #pragma unroll
+            for (int i = 0; i < CTN; ++i) {
+                const int ct = cg + CG * i;
+                if (ct * 16 >= Cp) continue;
+                const az_i4 hb = az_col_frag<DT>(m.h, ldc, k, ct * 16, lane);
                 #pragma unroll
-                for (int ot = 0; ot < OT; ++ot) {
-                    dw[ci][ot] = az_mma<DT>(az_col_frag<DT>(zhi, L::LDO, k, ot * 16, lane), hb, dw[ci][ot]);
-                    if constexpr (DT != 0) dw[ci][ot] = az_mma<DT>(az_col_frag<DT>(zlo, L::LDO, k, ot * 16, lane), hb, dw[ci][ot]);
+                for (int j = 0; j < OTN; ++j) {
+                    dw[i][j] = az_mma<DT>(zf[j][0], hb, dw[i][j]);
+                    if constexpr (DT != 0) dw[i][j] = az_mma<DT>(zf[j][1], hb, dw[i][j]);
                 }
             }
         }
     }
     float* out = a.partial + (size_t)blockIdx.x * ((size_t)a.O * a.C + a.O);
     #pragma unroll
-    for (int ci = 0; ci < CB; ++ci) {
-        const int c = (wave + 8 * ci) * 16 + (lane & 15);
+    for (int i = 0; i < CTN; ++i) {
+        const int c = (cg + CG * i) * 16 + (lane & 15);
         #pragma unroll
-        for (int ot = 0; ot < OT; ++ot)
-            for (int i = 0; i < 4; ++i) {
-                const int o = ot * 16 + q * 4 + i;
-                if (o < a.O && c < a.C) out[(size_t)o * a.C + c] = dw[ci][ot][i] * down;
+        for (int j = 0; j < OTN; ++j)
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int o = (og * OTN + j) * 16 + q * 4 + e;
+                if (o < a.O && c < a.C) out[(size_t)o * a.C + c] = dw[i][j][e] * down;
             }
     }
     __syncthreads();
@@ -474,10 +566,8 @@ __global__ void __launch_bounds__(512) az_policy_reduce_kernel(const float* part
 }
 
 template <int DT, int OT, int CB> hipError_t launch_products(const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
-    typedef Lay<DT, OT> L;
     const int Cp = (a.C + 31) / 32 * 32;
-    const bool wlds = !(DT == 0 && CB == 2 && OT >= 6);
-    const size_t lds = (wlds ? L::w_bytes(Cp) : 0) + L::h_bytes(Cp) + L::z_bytes;
+    const size_t lds = Smem<DT, OT, CB>::bytes(a, Cp);
     const void* fn = grad ? (const void*)az_policy_grad_kernel<DT, OT, CB> : (const void*)az_policy_rows_kernel<DT, OT, CB>;
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -507,6 +597,17 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 int groups_of(long long steps) { return (int)(steps < MAX_GROUPS ? steps : MAX_GROUPS); }
 
+// how boards map to steps
+void geometry(int B, int N, int& nb, int& blocks, long long& steps) {
+    const int S = N * N;
+    nb = S <= 32 ? (ROWS / S < MAX_BOARDS ? ROWS / S : MAX_BOARDS) : 1;
+    blocks = nb > 1 ? 1 : (S + ROWS - 1) / ROWS;
+    steps = nb > 1 ? ((long long)B + nb - 1) / nb : (long long)B * blocks;
+}
+// fp32 weights beyond LDS (w_in_lds): padded copies of at most 128 x 256
+bool pads_weight(const az_policy_loss_args* p) { return p->dtype == AZ_F32 && p->C > 128 && p->c_out > 32; }
+constexpr size_t PAD_BYTES = (size_t)128 * 256 * 4;
+
 // shape and range checks that need no pointer; 0 or the recorded error
 int check_shape(const az_policy_loss_args* p) {
     if (!p) return lfail(AZ_E_ARG, "null argument: args");
@@ -526,7 +627,11 @@ extern "C" size_t az_policy_loss_workspace(const az_policy_loss_args* p) {
     if (check_shape(p) != AZ_OK) return 0;
     const size_t rows = (size_t)p->B * p->N * p->N;
     size_t n = up256(rows * sizeof(az_f4)) + up256((size_t)p->B * sizeof(az_f4));
-    if (p->d_weight) n += up256((size_t)groups_of((long long)(rows + ROWS - 1) / ROWS) * ((size_t)p->c_out * p->C + p->c_out) * 4);
+    int nb, blocks;
+    long long steps;
+    geometry(p->B, p->N, nb, blocks, steps);
+    if (pads_weight(p)) n += 2 * PAD_BYTES;
+    if (p->d_weight) n += up256((size_t)groups_of(steps) * ((size_t)p->c_out * p->C + p->c_out) * 4);
     return n ? n : 256;
 }
 
@@ -561,14 +666,23 @@ extern "C" int az_policy_loss_dev(const az_policy_loss_args* p, void* workspace,
     a.h = p->features; a.w = p->weight; a.bias = p->bias; a.dense = p->target; a.counts = p->counts; a.actions = p->actions; a.probs = p->probs;
     a.legal = p->legal; a.row_scale = p->row_scale; a.scale = p->scale; a.loss = p->loss; a.dh = p->d_features;
     a.B = p->B; a.N = p->N; a.S = p->N * p->N; a.C = p->C; a.O = p->c_out; a.cap = p->cap; a.nchw = p->layout == AZ_CHANNELS_FIRST;
-    a.rows = a.B * a.S; a.steps = (a.rows + ROWS - 1) / ROWS;
+    long long steps;
+    geometry(p->B, p->N, a.nb, a.blocks, steps);
+    a.rows = a.B * a.S; a.steps = (int)steps;
     unsigned char* ws = (unsigned char*)workspace;
     a.rowstat = (az_f4*)ws; ws += up256((size_t)a.rows * sizeof(az_f4));
     a.stats = p->stats ? (az_f4*)p->stats : (az_f4*)ws; ws += up256((size_t)a.B * sizeof(az_f4));
+    const bool pads = pads_weight(p);
+    float* pad = (float*)ws;
+    if (pads) { a.wpad = pad; a.wpadt = pad + PAD_BYTES / 4; ws += 2 * PAD_BYTES; }
     a.partial = (float*)ws;
     const int groups = groups_of(a.steps);
     hipError_t e = hipSuccess;
-    if (a.B > 0 && !p->stats_given) {
+    if (a.B > 0 && pads) {
+        az_policy_pad_weight_kernel<<<64, 256, 0, st>>>((const float*)p->weight, pad, pad + PAD_BYTES / 4, a.O, a.C, a.O <= 64 ? 64 : a.O <= 96 ? 96 : 128, (a.C + 31) / 32 * 32);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess && a.B > 0 && !p->stats_given) {
         e = launch_dt(p->dtype, a, false, groups, st);
         if (e == hipSuccess) { az_policy_boards_kernel<<<(a.B + 3) / 4, 256, 0, st>>>(a); e = hipGetLastError(); }
     }
