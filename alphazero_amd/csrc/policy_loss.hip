@@ -27,6 +27,7 @@ int lfail(int code, const char* fmt, ...) {
 }
 
 constexpr int ROWS = 64;                     // rows of a step
+constexpr size_t LDS_BYTES = 160 * 1024;
 constexpr int MAX_GROUPS = 512;              // workgroups of the gradient kernel: two a CU
 constexpr int ENTRIES = 1024;                // sparse targets of a step's boards kept in LDS; longer lists are read from memory
 constexpr int MAX_BOARDS = 16;               // boards of a step
@@ -148,6 +149,7 @@ template <int DT, int NP> struct Feat {
 // sparse targets as {row of the step's boards * 256 + plane, value} (entries that are left out: -1).
 struct BoardLds {
     unsigned* words;
+    int planes;                                                      // words of a line: the planes, padded to 16
     int* key;
     float* val;
     bool listed;                                                     // the entries fit
@@ -158,9 +160,20 @@ __device__ __forceinline__ int entry_key(const PolicyDev& a, int act, int bb) {
     const int o = act / a.S;
     return (bb * a.S + act - o * a.S) * 256 + o;
 }
+__device__ __forceinline__ int entry_at(const PolicyDev& a, const Step& st, int e, float& v) {
+    const int bb = a.nb > 1 ? e / a.cap : 0, k = e - bb * a.cap;
+    const size_t at = (size_t)(st.b0 + bb) * a.cap + k;
+    if (k >= a.counts[st.b0 + bb]) return -1;
+    v = a.probs[at];
+    return entry_key(a, a.actions[at], bb);
+}
 __device__ __forceinline__ void stage_boards(const PolicyDev& a, const BoardLds& l, int b0, int tid, int nt) {
     const int boards = min(a.nb, a.B - b0);
-    if (a.legal) for (int i = tid; i < boards * a.O * a.N; i += nt) l.words[i] = a.legal[(size_t)b0 * a.O * a.N + i];
+    if (a.legal)                                                     // [board, plane, row] -> [board, row][plane]: a lane reads its row's words four at a time
+        for (int i = tid; i < boards * a.O * a.N; i += nt) {
+            const int bo = i / a.N, y = i - bo * a.N, bb = a.nb > 1 ? bo / a.O : 0;
+            l.words[(bb * a.N + y) * l.planes + bo - bb * a.O] = a.legal[(size_t)b0 * a.O * a.N + i];
+        }
     if (a.counts && l.listed)
         for (int e = tid; e < boards * a.cap; e += nt) {
             const int bb = a.nb > 1 ? e / a.cap : 0, k = e - bb * a.cap;
@@ -176,14 +189,9 @@ template <int LDT, int WAVES> __device__ __forceinline__ void scatter_targets(co
     const int boards = min(a.nb, a.B - st.b0), n = boards * a.cap;
     for (int e = lane; e < n; e += 64) {
         int key;
-        float v;
+        float v = 0.f;
         if (l.listed) { key = l.key[e]; v = l.val[e]; }
-        else {
-            const int bb = a.nb > 1 ? e / a.cap : 0, k = e - bb * a.cap;
-            const size_t at = (size_t)(st.b0 + bb) * a.cap + k;
-            key = k < a.counts[st.b0 + bb] ? entry_key(a, a.actions[at], bb) : -1;
-            v = a.probs[at];
-        }
+        else key = entry_at(a, st, e, v);
         const int o = key & 255, row = (key >> 8) - st.cell0;
         if (key >= 0 && o % WAVES == wave && (unsigned)row < (unsigned)ROWS)
             __hip_atomic_fetch_add(t + row * LDT + o, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
@@ -203,105 +211,190 @@ __global__ void __launch_bounds__(256) az_policy_pad_weight_kernel(const float* 
 }
 template <int DT, int OT, int CB> __host__ __device__ constexpr bool w_in_lds() { return !(DT == 0 && CB == 2 && OT >= 4); }
 
-// LDS of both product kernels, in this order
-template <int DT, int OT, int CB> struct Smem {
+// LDS of the product kernels, in this order; zb: bytes of the kernel's own tile (logits or dz)
+template <int DT, int OT, int CB, bool HBUF> struct Smem {
     typedef Lay<DT, OT> L;
     unsigned char *w, *h;
     float *t, *bias;
     BoardLds b;
-    __device__ __forceinline__ Smem(unsigned char* p, const PolicyDev& a, int Cp) {
+    __device__ __forceinline__ Smem(unsigned char* p, const PolicyDev& a, int Cp, size_t zb) {
         w = p; p += w_in_lds<DT, OT, CB>() ? L::w_bytes(Cp) : 0;
-        h = p; p += L::h_bytes(Cp);
-        t = (float*)p; p += L::z_bytes;
+        h = p; p += HBUF ? L::h_bytes(Cp) : 0;
+        t = (float*)p; p += zb;
         bias = (float*)p; p += OT * 16 * 4;
+        b.words = (unsigned*)p; p += a.legal ? (size_t)a.nb * a.N * OT * 16 * 4 : 0;
+        b.planes = OT * 16;
         const int room = a.counts ? entry_room(a.nb, a.cap) : 0;
         b.listed = room > 0;
         b.key = (int*)p; p += (size_t)room * 4;
-        b.val = (float*)p; p += (size_t)room * 4;
-        b.words = (unsigned*)p;
+        b.val = (float*)p;
     }
-    static size_t bytes(const PolicyDev& a, int Cp) {
-        return (w_in_lds<DT, OT, CB>() ? L::w_bytes(Cp) : 0) + L::h_bytes(Cp) + L::z_bytes + OT * 16 * 4 + (a.counts ? (size_t)entry_room(a.nb, a.cap) * 8 : 0) +
-               (a.legal ? (size_t)a.nb * a.O * a.N * 4 : 0);
+    static size_t bytes(const PolicyDev& a, int Cp, size_t zb) {
+        return (w_in_lds<DT, OT, CB>() ? L::w_bytes(Cp) : 0) + (HBUF ? L::h_bytes(Cp) : 0) + zb + OT * 16 * 4 + (a.counts ? (size_t)entry_room(a.nb, a.cap) * 8 : 0) +
+               (a.legal ? (size_t)a.nb * a.N * OT * 16 * 4 : 0);
     }
 };
 
-// Row statistics.  Four waves, 16 rows each, all planes.
-template <int DT, int OT, int CB> __global__ void __launch_bounds__(256) az_policy_rows_kernel(PolicyDev a) {
+// Fragments of 16 rows of the features straight from memory: row r of the batch (this lane's, live or not), all channels.
+template <int DT, int KT> struct RowFrags {
+    az_i4 v[KT];
+    __device__ __forceinline__ void load(const PolicyDev& a, const Step& st, int rl, int q) {
+        constexpr int EP = AzElem<DT>::EP, KS = AzElem<DT>::KS;
+        typedef typename AzElem<DT>::T T;
+        #pragma unroll
+        for (int k = 0; k < KT; ++k) v[k] = az_i4{0, 0, 0, 0};
+        if (rl >= st.n) return;
+        const int bb = a.nb > 1 ? rl / a.S : 0, s = st.cell0 + rl - bb * a.S;
+        const T* src = a.nchw ? (const T*)a.h + (size_t)(st.b0 + bb) * a.C * a.S + s : (const T*)a.h + (size_t)(st.rbase + rl) * a.C;
+        const size_t cs = a.nchw ? a.S : 1;
+        #pragma unroll
+        for (int k = 0; k < KT; ++k) {
+            const int c0 = k * KS + q * EP;
+            if (k * KS >= a.C) break;
+            T e[EP];
+            if (c0 + EP <= a.C) {
+                if (!a.nchw) {
+                    if constexpr (DT == 0) *(az_f4*)e = *(const az_f4_u*)(src + c0);
+                    else *(az_s8*)e = *(const az_s8_u*)(src + c0);
+                } else {
+                    #pragma unroll
+                    for (int j = 0; j < EP; ++j) e[j] = src[(size_t)(c0 + j) * cs];
+                }
+            } else {
+                #pragma unroll
+                for (int j = 0; j < EP; ++j) e[j] = c0 + j < a.C ? src[(size_t)(c0 + j) * cs] : (T)0.f;
+            }
+            v[k] = *(az_i4*)e;
+        }
+    }
+};
+
+// Row statistics.  Four waves; a wave takes 16 rows of a step, all planes, and meets the others only where the board
+// changes.  The features go from memory to fragments (no other wave wants these rows), the next tile's while this one is
+// worked on.  Sparse targets: the tile's logits pass through LDS, half of the planes at a time where there are many, and
+// the lanes pick out those that the entries name.
+template <int DT, int OT, int CB> struct RowsCfg {
+    static constexpr int PASSES = OT >= 6 ? 2 : 1, OTP = OT / PASSES, LDZ = OTP * 16 + 4;
+    static constexpr size_t tile = (size_t)16 * LDZ * 4;             // of one wave
+};
+template <int DT, int OT, int CB> __global__ void __launch_bounds__(256, DT != 0 && CB == 1 ? 3 : DT == 0 && CB == 2 && OT >= 4 ? 1 : 2) az_policy_rows_kernel(PolicyDev a) {
     typedef Lay<DT, OT> L;
-    constexpr int NT = 256, NP = CB * 128 / L::EP * ROWS / NT;
+    typedef RowsCfg<DT, OT, CB> R;
+    constexpr int NT = 256, KT = CB * 128 / L::KS;
     constexpr bool WLDS = w_in_lds<DT, OT, CB>();
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int Cp = (a.C + 31) / 32 * 32, ldc = Cp + L::EP, pieces = Cp / L::EP;
-    const Smem<DT, OT, CB> m(smem, a, Cp);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
+    const int Cp = (a.C + 31) / 32 * 32, ldc = Cp + L::EP;
+    const Smem<DT, OT, CB, false> m(smem, a, Cp, a.counts ? 4 * R::tile : 0);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, rl = wave * 16 + (lane & 15);
+    float* zt = m.t + wave * (R::tile / 4);
     if (WLDS) stage_w<DT, OT>(a, m.w, Cp, tid, NT);
     for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
     const int s_lo = (int)((long long)blockIdx.x * a.steps / gridDim.x), s_hi = (int)((long long)(blockIdx.x + 1) * a.steps / gridDim.x);
-    Feat<DT, NP> f;
-    if (s_lo < s_hi) f.template load<NT>(a, step_at(a, s_lo), pieces, tid);
+    RowFrags<DT, KT> f;
+    f.load(a, step_at(a, s_lo), rl, q);
     int board = -1;
     for (int it = s_lo; it < s_hi; ++it) {
         const Step st = step_at(a, it);
-        __syncthreads();                                             // the step before has read its LDS
-        f.template store<NT>(a, m.h, Cp, pieces, tid);
-        if (a.counts) for (int i = tid; i < ROWS * L::LDT / 4; i += NT) ((az_f4*)m.t)[i] = az_f4{0.f, 0.f, 0.f, 0.f};
-        if (st.b0 != board) { stage_boards(a, m.b, st.b0, tid, NT); board = st.b0; }
-        __syncthreads();
-        if (it + 1 < s_hi) f.template load<NT>(a, step_at(a, it + 1), pieces, tid);
-        if (a.counts) { scatter_targets<L::LDT, 4>(a, m.b, m.t, st, wave, lane); __syncthreads(); }
-        if (wave * 16 >= st.n) continue;
-        az_f4 acc[OT];
-        #pragma unroll
-        for (int ot = 0; ot < OT; ++ot) acc[ot] = *(const az_f4*)(m.bias + ot * 16 + q * 4);
-        for (int k = 0; k < Cp; k += L::KS) {
-            const az_i4 hb = az_row_frag<DT>(m.h, ldc, wave * 16, k, lane);
-            #pragma unroll
-            for (int ot = 0; ot < OT; ++ot)
-                acc[ot] = az_mma<DT>(WLDS ? az_row_frag<DT>(m.w, ldc, ot * 16, k, lane) : az_row_frag<DT>(a.wpad, Cp, ot * 16, k, lane), hb, acc[ot]);
+        if (st.b0 != board) {
+            if (a.legal || a.counts || board < 0) {
+                __syncthreads();
+                stage_boards(a, m.b, st.b0, tid, NT);
+                __syncthreads();
+            }
+            board = st.b0;
         }
-        const int rl = wave * 16 + (lane & 15);
-        if (rl < st.n) {
-            const int bb = a.nb > 1 ? rl / a.S : 0, s = st.cell0 + rl - bb * a.S, y = s / a.N, x = s - y * a.N;
-            const unsigned* words = m.b.words + (bb * a.O + q * 4) * a.N + y;
-            const float* dense = a.counts ? nullptr : a.dense + ((size_t)(st.b0 + bb) * a.O + q * 4) * a.S + s;
-            float mx = -INFINITY, tz = 0.f, tm = 0.f;
+        az_f4 acc[OT];
+        if (wave * 16 < st.n) {
+            #pragma unroll
+            for (int ot = 0; ot < OT; ++ot) acc[ot] = *(const az_f4*)(m.bias + ot * 16 + q * 4);
+            #pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                if (k * L::KS >= Cp) break;
+                #pragma unroll
+                for (int ot = 0; ot < OT; ++ot)
+                    acc[ot] = az_mma<DT>(WLDS ? az_row_frag<DT>(m.w, ldc, ot * 16, k * L::KS, lane) : az_row_frag<DT>(a.wpad, Cp, ot * 16, k * L::KS, lane), f.v[k], acc[ot]);
+            }
+        }
+        if (it + 1 < s_hi) f.load(a, step_at(a, it + 1), rl, q);
+        if (wave * 16 >= st.n) continue;
+        const int bb = a.nb > 1 ? rl / a.S : 0, s = st.cell0 + rl - bb * a.S, y = s / a.N;
+        // entries that no action stands for: planes beyond the last, actions that are not allowed
+        if (a.legal) {
+            const unsigned bit = 1u << (s - y * a.N);
+            const unsigned* words = m.b.words + (bb * a.N + (rl < st.n ? y : 0)) * (OT * 16) + q * 4;
             #pragma unroll
             for (int ot = 0; ot < OT; ++ot) {
-                az_f4 tv = {0.f, 0.f, 0.f, 0.f};
-                if (a.counts) tv = *(const az_f4*)(m.t + rl * L::LDT + ot * 16 + q * 4);
+                const az_i4 w = *(const az_i4*)(words + ot * 16);
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int o = ot * 16 + q * 4 + i;
-                    if (o < a.O) {
-                        if (!a.counts) tv[i] = dense[(size_t)(ot * 16 + i) * a.S];
-                        if (a.legal && !((words[(ot * 16 + i) * a.N] >> x) & 1u)) acc[ot][i] = -INFINITY;
-                        const float z = acc[ot][i];
-                        if (tv[i] != 0.f) { tz += tv[i] * z; tm += tv[i]; }
-                        if (!(z <= mx)) mx = z;                      // (a NaN logit is not lost: its exponential joins the sum)
-                    } else acc[ot][i] = -INFINITY;
-                }
+                for (int i = 0; i < 4; ++i) acc[ot][i] = (unsigned)w[i] & bit ? acc[ot][i] : -INFINITY;
             }
-            // four groups of lanes hold a row's planes
-            for (int d = 16; d <= 32; d <<= 1) {
-                const float om = __shfl_xor(mx, d, 64);
-                if (!(om <= mx)) mx = om;
-                tz += __shfl_xor(tz, d, 64);
-                tm += __shfl_xor(tm, d, 64);
+        }
+        #pragma unroll
+        for (int ot = 0; ot < OT; ++ot)
+            if (ot * 16 + 16 > a.O) {
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) if (ot * 16 + q * 4 + i >= a.O) acc[ot][i] = -INFINITY;
             }
-            float l = 0.f;
-            if (mx != -INFINITY) {
-                const float ml = mx * LOG2E;
+        float tz = 0.f, tm = 0.f;
+        // (an entry without a target does not count, whatever its logit; one with a target whose action is not allowed
+        // gives -inf)
+        if (!a.counts) {
+            if (rl < st.n) {
+                const float* dense = a.dense + ((size_t)(st.b0 + bb) * a.O + q * 4) * a.S + s;
                 #pragma unroll
                 for (int ot = 0; ot < OT; ++ot)
                     #pragma unroll
-                    for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[ot][i], LOG2E, -ml));
+                    for (int i = 0; i < 4; ++i)
+                        if (ot * 16 + q * 4 + i < a.O) {
+                            const float tv = dense[(size_t)(ot * 16 + i) * a.S];
+                            tz += tv != 0.f ? tv * acc[ot][i] : 0.f;
+                            tm += tv;
+                        }
             }
-            for (int d = 16; d <= 32; d <<= 1) l += __shfl_xor(l, d, 64);
-            if (q == 0) {
-                a.rowstat[st.rbase + rl] = az_f4{mx, l, tz, tm};
-                asm volatile("s_nop 1");                             // (a wide store reads its registers after it has issued)
+        } else {
+            const int n = min(a.nb, a.B - st.b0) * a.cap, lo = st.cell0 + wave * 16, hi = min(lo + 16, st.cell0 + st.n);
+            #pragma unroll
+            for (int p = 0; p < R::PASSES; ++p) {
+                #pragma unroll
+                for (int j = 0; j < R::OTP; ++j) *(az_f4*)(zt + (lane & 15) * R::LDZ + j * 16 + q * 4) = acc[p * R::OTP + j];
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                // one board: every lane takes an entry, whichever row it names; several: a lane takes its own row's
+                for (int e = a.nb > 1 ? q : lane; e < n; e += a.nb > 1 ? 4 : 64) {
+                    int key;
+                    float v = 0.f;
+                    if (m.b.listed) key = m.b.key[e];
+                    else key = entry_at(a, st, e, v);
+                    const int row = key >> 8, o = (key & 255) - p * R::OTP * 16;
+                    if (row >= lo && row < hi && (unsigned)o < (unsigned)(R::OTP * 16) && (a.nb == 1 || row == rl)) {
+                        if (m.b.listed) v = m.b.val[e];
+                        tz += v != 0.f ? v * zt[(row - lo) * R::LDZ + o] : 0.f;
+                        tm += v;
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
             }
+        }
+        float mx = -INFINITY;
+        #pragma unroll
+        for (int ot = 0; ot < OT; ++ot) mx = fmaxf(mx, fmaxf(fmaxf(acc[ot][0], acc[ot][1]), fmaxf(acc[ot][2], acc[ot][3])));
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));                      // four groups of lanes hold a row's planes
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float ml = mx == -INFINITY ? 0.f : mx * LOG2E;         // (a NaN logit is not the maximum, but its exponential joins the sum)
+        float l = 0.f;
+        #pragma unroll
+        for (int ot = 0; ot < OT; ++ot)
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[ot][i], LOG2E, -ml));
+        for (int d = 16; d <= 32; d <<= 1) {
+            l += __shfl_xor(l, d, 64);
+            tz += __shfl_xor(tz, d, 64);
+            tm += __shfl_xor(tm, d, 64);
+        }
+        if (q == 0 && rl < st.n) {                                   // (sparse, one board: tz and tm are the tile's entries' sums, spread over its rows)
+            a.rowstat[st.rbase + rl] = az_f4{mx, l, tz, tm};
+            asm volatile("s_nop 1");                                 // (a wide store reads its registers after it has issued)
         }
     }
 }
@@ -316,18 +409,18 @@ __global__ void __launch_bounds__(256) az_policy_boards_kernel(PolicyDev a) {
         const az_f4 v = rs[s];
         tz += v[2];
         tm += v[3];
-        if (v[0] == -INFINITY) continue;
+        if (v[0] == -INFINITY) { l += v[1]; continue; }              // nothing allowed in the row: 0, or a NaN that stays
         if (v[0] <= m) l += v[1] * __builtin_amdgcn_exp2f((v[0] - m) * LOG2E);
-        else { l = (m == -INFINITY ? 0.f : l * __builtin_amdgcn_exp2f((m - v[0]) * LOG2E)) + v[1]; m = v[0]; }
+        else { l = (m == -INFINITY ? l : l * __builtin_amdgcn_exp2f((m - v[0]) * LOG2E)) + v[1]; m = v[0]; }
     }
     float M = m;
     for (int d = 32; d > 0; d >>= 1) { const float om = __shfl_xor(M, d, 64); if (!(om <= M)) M = om; }
-    l = m == -INFINITY ? 0.f : l * __builtin_amdgcn_exp2f((m - M) * LOG2E);
+    l = m == -INFINITY ? l : l * __builtin_amdgcn_exp2f((m - M) * LOG2E);
     l = wave_sum(l);
     tz = wave_sum(tz);
     tm = wave_sum(tm);
     if (lane == 0) {
-        const float lse = M == -INFINITY ? -INFINITY : M + logf(l);
+        const float lse = M == -INFINITY ? (l == l ? -INFINITY : l) : M + logf(l);
         const bool masked = tz == -INFINITY;                         // a target on an action that is not allowed
         const float loss = masked ? INFINITY : (tm != 0.f ? tm * lse : 0.f) - tz;
         a.stats[b] = az_f4{lse, tm, masked ? 1.f : 0.f, loss};
@@ -348,7 +441,7 @@ template <int DT, int OT, int CB> __global__ void __launch_bounds__(512) az_poli
     constexpr bool WLDS = w_in_lds<DT, OT, CB>();
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int Cp = (a.C + 31) / 32 * 32, ldc = Cp + L::EP, pieces = Cp / L::EP;
-    const Smem<DT, OT, CB> m(smem, a, Cp);
+    const Smem<DT, OT, CB, true> m(smem, a, Cp, L::z_bytes);
     float* t = m.t;                                                  // the step's targets, then its dz in the same place
     T* zhi = (T*)t;
     T* zlo = zhi + ROWS * L::LDO;
@@ -397,7 +490,8 @@ template <int DT, int OT, int CB> __global__ void __launch_bounds__(512) az_poli
         if (it + 1 < s_hi) f.template load<NT>(a, step_at(a, it + 1), pieces, tid);
         const int rl = rt * 16 + (lane & 15);
         const bool live = rl < st.n;
-        const int bb = live && a.nb > 1 ? rl / a.S : 0, b = st.b0 + bb, s = live ? st.cell0 + rl - bb * a.S : 0, y = s / a.N, x = s - y * a.N;
+        const int bb = live && a.nb > 1 ? rl / a.S : 0, b = st.b0 + bb, s = live ? st.cell0 + rl - bb * a.S : 0, y = s / a.N;
+        const unsigned bit = 1u << (s - y * a.N);
         az_f4 tv[OTH];
         if (a.counts) {
             scatter_targets<L::LDT, 8>(a, m.b, t, st, wave, lane);
@@ -429,7 +523,7 @@ template <int DT, int OT, int CB> __global__ void __launch_bounds__(512) az_poli
         const az_f4 bst = live ? a.stats[b] : az_f4{0.f, 0.f, 0.f, 0.f};
         const float rs = live ? up * (a.scale * (a.row_scale ? a.row_scale[b] : 1.f)) : 0.f;
         const float rT = rs * bst[1], lse2 = bst[0] * LOG2E;
-        const unsigned* words = m.b.words + (bb * a.O + half * OTH * 16 + q * 4) * a.N + y;
+        const unsigned* words = m.b.words + (bb * a.N + y) * (OT * 16) + half * OTH * 16 + q * 4;
         // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
         const bool bias_counts = a.O > 1 || bst[2] != 0.f;
         #pragma unroll
@@ -438,12 +532,18 @@ template <int DT, int OT, int CB> __global__ void __launch_bounds__(512) az_poli
             if (ot * 16 >= L::OP) continue;
             az_f4 dz;
             #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                bool on = live && ot * 16 + q * 4 + i < a.O;
-                if (a.legal && on) on = (words[(j * 16 + i) * a.N] >> x) & 1u;
-                dz[i] = on ? rT * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -lse2)) - rs * tv[j][i] : 0.f;
-                if (bias_counts) db[j][i] += dz[i];
+            for (int i = 0; i < 4; ++i) dz[i] = rT * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -lse2)) - rs * tv[j][i];
+            if (a.legal && ot < OT) {
+                const az_i4 w = *(const az_i4*)(words + j * 16);
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) dz[i] = (unsigned)w[i] & bit ? dz[i] : 0.f;
             }
+            if (ot * 16 + 16 > a.O) {
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) if (ot * 16 + q * 4 + i >= a.O) dz[i] = 0.f;
+            }
+            if (!live) dz = az_f4{0.f, 0.f, 0.f, 0.f};
+            if (bias_counts) db[j] += dz;
             if constexpr (DT == 0) *(az_f4*)((float*)zhi + rl * L::LDO + ot * 16 + q * 4) = dz;
             else {
                 az_s4 hi, lo;
@@ -567,14 +667,18 @@ __global__ void __launch_bounds__(512) az_policy_reduce_kernel(const float* part
 
 template <int DT, int OT, int CB> hipError_t launch_products(const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
     const int Cp = (a.C + 31) / 32 * 32;
-    const size_t lds = Smem<DT, OT, CB>::bytes(a, Cp);
+    const size_t lds = grad ? Smem<DT, OT, CB, true>::bytes(a, Cp, Lay<DT, OT>::z_bytes) : Smem<DT, OT, CB, false>::bytes(a, Cp, a.counts ? 4 * RowsCfg<DT, OT, CB>::tile : 0);
     const void* fn = grad ? (const void*)az_policy_grad_kernel<DT, OT, CB> : (const void*)az_policy_rows_kernel<DT, OT, CB>;
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
     if (grad) az_policy_grad_kernel<DT, OT, CB><<<groups, 512, lds, stream>>>(a);
-    else az_policy_rows_kernel<DT, OT, CB><<<groups, 256, lds, stream>>>(a);
+    else {
+        // as many workgroups as the chip holds: 160 KB of LDS a CU, at most four of four waves
+        const int per_cu = lds * 4 <= LDS_BYTES ? 4 : (int)(LDS_BYTES / lds), room = 256 * per_cu;
+        az_policy_rows_kernel<DT, OT, CB><<<a.steps < room ? a.steps : room, 256, lds, stream>>>(a);
+    }
     return hipGetLastError();
 }
 template <int DT, int OT> hipError_t launch_c(const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
