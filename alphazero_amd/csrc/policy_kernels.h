@@ -1,0 +1,883 @@
+// policy_kernels.h -- the kernels of policy_loss.h, templates over the element type DT, planes OT (in 16s), channels CB (in
+// 128s) and the way the features are read.
+#pragma once
+#include "policy_loss.h"
+
+namespace {
+
+// dynamic LDS of the two product kernels
+template <int DT, int OT> struct Lay {
+    static constexpr int EP = AzElem<DT>::EP, KS = AzElem<DT>::KS, SZ = 16 / EP;
+    static constexpr int OP = (OT * 16 + KS - 1) / KS * KS;          // planes, padded to a step of the contraction over them
+    static constexpr int LDT = OT * 16 + 4, LDO = OP + EP;
+    // rows are padded by 16 bytes, so that they start in different banks
+    __host__ __device__ static size_t w_bytes(int Cp) { return (size_t)OP * (Cp + EP) * SZ; }
+    __host__ __device__ static size_t h_bytes(int Cp) { return (size_t)ROWS * (Cp + EP) * SZ; }
+    static constexpr size_t z_bytes = (size_t)ROWS * (LDO > LDT ? LDO : LDT) * 4;
+};
+
+__device__ __forceinline__ float wave_max(float x) {
+    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+    return x;
+}
+
+// How the features are read.  A load that is to stay in flight is unconditional, its address clamped into the tensor, and
+// what it should not have brought is dropped where it is used.
+//   WHOLE_LAST   channels last, C a multiple of a product step (32; fp32: 16): 16-byte loads
+//   WHOLE_FIRST  channels first, C such a multiple: one element a load, neighbouring lanes neighbouring cells
+//   ANY          anything else: one element a load, every index clamped
+enum { WHOLE_LAST, WHOLE_FIRST, ANY };
+
+// A value the compiler may not carry over from an earlier iteration: index arithmetic of the one-element loads is done
+// anew for each tile instead of filling the registers.
+__device__ __forceinline__ int anew(int x) { asm volatile("" : "+v"(x)); return x; }
+__device__ __forceinline__ int anew_s(int x) { asm volatile("" : "+s"(x)); return x; }      // (of a wave-uniform value)
+
+// (policy_loss.hip: az_policy_pad_weight_kernel)
+template <int DT, int OT, int CB> __host__ __device__ constexpr bool w_in_lds() { return !(DT == 0 && CB == 2 && OT >= 4); }
+
+// w [O][C] -> LDS [OP][Cp + EP], zero beyond O and C, in pieces of 16 bytes; eight loads of a thread in flight
+template <int DT, int OT> __device__ __forceinline__ void stage_w(const PolicyDev& a, void* wl, int Cp, int tid) {
+    typedef Lay<DT, OT> L;
+    typedef typename AzElem<DT>::T T;
+    constexpr int EP = L::EP, U = 8;
+    const int per = Cp / EP, total = L::OP * per;
+    for (int base = tid; base < total; base += NT * U) {
+        az_i4 v[U];
+        if (a.C % EP == 0) {
+            #pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = min(base + u * NT, total - 1), o = i / per, c = (i - o * per) * EP;
+                const T* src = (const T*)a.w + (size_t)min(o, a.O - 1) * a.C + min(c, a.C - EP);
+                if constexpr (DT == 0) v[u] = __builtin_bit_cast(az_i4, *(const az_f4_u*)src);
+                else v[u] = __builtin_bit_cast(az_i4, *(const az_s8_u*)src);
+            }
+        } else {
+            #pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = min(base + u * NT, total - 1), o = i / per, c = (i - o * per) * EP;
+                const T* src = (const T*)a.w + (size_t)min(o, a.O - 1) * a.C;
+                T e[EP];
+                #pragma unroll
+                for (int k = 0; k < EP; ++k) { const T x = src[min(c + k, a.C - 1)]; e[k] = c + k < a.C ? x : (T)0.f; }
+                v[u] = *(az_i4*)e;
+            }
+        }
+        #pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = base + u * NT, o = i / per, c = (i - o * per) * EP;
+            if (i < total) *(az_i4*)((char*)wl + ((size_t)o * (Cp + EP) + c) * L::SZ) = o < a.O && c < a.C ? v[u] : az_i4{0, 0, 0, 0};
+        }
+    }
+}
+
+// What a workgroup's boards need beside the features, brought to LDS when the board changes: the legal-move words as
+// [board, row][plane], and the sparse targets sorted by tile as {row of the boards * 256 + plane, value}.
+struct BoardLds {
+    unsigned* words;                                                 // bit 0 = no action stands for the entry: a plane beyond the last, or not allowed
+    int planes;                                                      // words of a line: the planes, padded to 16
+    int* key;
+    float* val;
+    int* cnt;                                                        // [64-entry chunk][64 tiles]
+    int* start;                                                      // [65]: a tile's first entry
+    bool listed;                                                     // the entries fit
+};
+__host__ __device__ inline int entry_room(int nb, int cap) { return (long long)nb * cap <= ENTRIES ? nb * cap : 0; }
+// entries outside the board's actions: -1
+__device__ __forceinline__ int entry_key(const PolicyDev& a, int act, int bb) {
+    if ((unsigned)act >= (unsigned)(a.O * a.S)) return -1;
+    const int o = act / a.S;
+    return (bb * a.S + act - o * a.S) * 256 + o;
+}
+__device__ __forceinline__ int entry_at(const PolicyDev& a, int b0, int e, float& v) {
+    const int bb = a.nb > 1 ? e / a.cap : 0, k = e - bb * a.cap;
+    const size_t at = (size_t)(b0 + bb) * a.cap + k;
+    if (k >= a.counts[b0 + bb]) return -1;
+    v = a.probs[at];
+    return entry_key(a, a.actions[at], bb);
+}
+
+// The words before any board's are there: without legal-move words every action of the planes there are is allowed.
+__device__ __forceinline__ void init_words(const PolicyDev& a, const BoardLds& l, int tid) {
+    for (int i = tid; i < a.nb * a.N * l.planes; i += NT) l.words[i] = !a.legal && i % l.planes < a.O ? ~0u : 0u;
+}
+
+// One group's words and entries on their way: the first loads of a thread wait in registers while the group before is
+// worked on.
+struct BoardLoads {
+    static constexpr int W = 4, E = ENTRIES / NT;
+    unsigned w[W];
+    int act[E], cnt[E];
+    float val[E];
+    __device__ __forceinline__ void load(const PolicyDev& a, const BoardLds& l, int b0, int tid) {
+        const int boards = min(a.nb, a.B - b0);
+        if (a.legal) {
+            const int n = boards * a.O * a.N;
+            const unsigned* src = a.legal + (size_t)b0 * a.O * a.N;
+            #pragma unroll
+            for (int u = 0; u < W; ++u) w[u] = src[min(tid + u * NT, n - 1)];
+        }
+        if (l.listed) {
+            const int n = boards * a.cap;
+            #pragma unroll
+            for (int u = 0; u < E; ++u) {
+                const int e = min(tid + u * NT, n - 1);
+                cnt[u] = a.counts[b0 + (a.nb > 1 ? e / a.cap : 0)];
+                act[u] = a.actions[(size_t)b0 * a.cap + e];
+                val[u] = a.probs[(size_t)b0 * a.cap + e];
+            }
+        }
+    }
+    __device__ __forceinline__ void put_word(const PolicyDev& a, const BoardLds& l, int i, unsigned v) const {
+        const int bo = (int)((unsigned)i * a.mag_w >> 20), y = i - bo * a.N, bb = a.nb > 1 ? bo / a.O : 0;
+        l.words[(bb * a.N + y) * l.planes + bo - bb * a.O] = v;
+    }
+    // every thread; ends in a barrier
+    __device__ __forceinline__ void store(const PolicyDev& a, const BoardLds& l, int b0, int tid) const {
+        const int boards = min(a.nb, a.B - b0), lane = tid & 63, wave = tid >> 6;
+        if (a.legal) {
+            const int n = boards * a.O * a.N;
+            #pragma unroll
+            for (int u = 0; u < W; ++u) if (tid + u * NT < n) put_word(a, l, tid + u * NT, w[u]);
+            const unsigned* src = a.legal + (size_t)b0 * a.O * a.N;
+            for (int i = tid + W * NT; i < n; i += NT) put_word(a, l, i, src[i]);
+        }
+        if (l.listed) {
+            // a stable counting sort by tile: the entries of a tile keep their order, whatever the waves' timing
+            const int n = boards * a.cap, chunks = (n + 63) / 64, tiles = (boards * a.S + 15) / 16;
+            int key[E], rank[E];
+            #pragma unroll
+            for (int u = 0; u < E; ++u) {
+                const int e = tid + u * NT, chunk = wave + u * WAVES;
+                const int bb = a.nb > 1 ? min(e, n - 1) / a.cap : 0;
+                key[u] = e < n && e - bb * a.cap < cnt[u] ? entry_key(a, act[u], bb) : -1;
+                if (chunk >= chunks) continue;
+                const int tile = key[u] < 0 ? -1 : key[u] >> 12;
+                int mine = 0;
+                for (int t = 0; t < tiles; ++t) {
+                    const unsigned long long m = __ballot(tile == t);
+                    if (tile == t) rank[u] = __popcll(m & ((1ull << lane) - 1));
+                    if (lane == t) mine = __popcll(m);
+                }
+                l.cnt[chunk * 64 + lane] = mine;
+            }
+            __syncthreads();
+            if (wave == 0) {
+                int sum = 0;
+                for (int c = 0; c < chunks; ++c) sum += l.cnt[c * 64 + lane];
+                int incl = sum;
+                for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
+                int at = incl - sum;
+                l.start[lane] = at;
+                if (lane == 63) l.start[64] = incl;
+                for (int c = 0; c < chunks; ++c) { const int k = l.cnt[c * 64 + lane]; l.cnt[c * 64 + lane] = at; at += k; }
+            }
+            __syncthreads();
+            #pragma unroll
+            for (int u = 0; u < E; ++u)
+                if (key[u] >= 0) {
+                    const int at = l.cnt[(wave + u * WAVES) * 64 + (key[u] >> 12)] + rank[u];
+                    l.key[at] = key[u];
+                    l.val[at] = val[u];
+                }
+        }
+        __syncthreads();
+    }
+};
+
+// LDS of the product kernels, in this order; zb: bytes of the kernel's own tile (logits or dz)
+template <int DT, int OT, int CB, int HBUF, bool WBUF> struct Smem {
+    typedef Lay<DT, OT> L;
+    unsigned char *w, *h;
+    float *t, *bias;
+    BoardLds b;
+    __device__ __forceinline__ Smem(unsigned char* p, const PolicyDev& a, int Cp, size_t zb) {
+        w = p; p += WBUF ? L::w_bytes(Cp) : 0;
+        h = p; p += HBUF * L::h_bytes(Cp);
+        t = (float*)p; p += zb;
+        bias = (float*)p; p += OT * 16 * 4;
+        b.words = (unsigned*)p; p += (size_t)a.nb * a.N * OT * 16 * 4;
+        b.planes = OT * 16;
+        const int room = a.counts ? entry_room(a.nb, a.cap) : 0;
+        b.listed = room > 0;
+        b.key = (int*)p; p += (size_t)room * 4;
+        b.val = (float*)p; p += (size_t)room * 4;
+        b.start = (int*)p; p += 65 * 4;
+        b.cnt = (int*)p;
+    }
+    static size_t bytes(const PolicyDev& a, int Cp, size_t zb) {
+        const size_t room = a.counts ? (size_t)entry_room(a.nb, a.cap) : 0;
+        return (WBUF ? L::w_bytes(Cp) : 0) + HBUF * L::h_bytes(Cp) + zb + OT * 16 * 4 + (size_t)a.nb * a.N * OT * 16 * 4 +
+               (room ? room * 8 + 65 * 4 + (room + 63) / 64 * 256 : 0);
+    }
+};
+
+// Running {max, sum of exp} of a set of logits, joined.  Nothing in it yet: {-inf, 0}; a NaN logit is not the maximum, but
+// its exponential joins the sum.
+__device__ __forceinline__ float rescale(float m, float to) { return m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - to) * LOG2E); }
+__device__ __forceinline__ void join(float& m, float& l, float om, float ol) {
+    const float to = fmaxf(m, om);
+    l = l * rescale(m, to) + ol * rescale(om, to);
+    m = to;
+}
+__device__ __forceinline__ void finish_board(const PolicyDev& a, int b, float m, float l, float tz, float tm) {
+    const float lse = m == -INFINITY ? (l == l ? -INFINITY : l) : m + logf(l);
+    const bool masked = tz == -INFINITY;                             // a target on an action that is not allowed
+    const float loss = masked ? INFINITY : (tm != 0.f ? tm * lse : 0.f) - tz;
+    a.stats[b] = az_f4{lse, tm, masked ? 1.f : 0.f, loss};
+    if (a.loss) a.loss[b] = loss;
+}
+
+// Fragments of 16 rows of the features straight from memory, all channels.  Rows beyond the last are the last one again
+// (nobody reads their columns of the product).
+template <int DT, int KT, int MODE> struct RowFrags {
+    az_i4 v[KT];
+    __device__ __forceinline__ void load(const PolicyDev& a, int b0, int row, int rows, int q) {
+        constexpr int EP = AzElem<DT>::EP, KS = AzElem<DT>::KS;
+        typedef typename AzElem<DT>::T T;
+        row = min(row, rows - 1);
+        const T* group = (const T*)a.h + (size_t)b0 * a.S * a.C;
+        const int bb = MODE != WHOLE_LAST && a.nb > 1 ? (int)((unsigned)row * a.mag_s >> 16) : 0;
+        if constexpr (MODE == WHOLE_LAST) {
+            const int at = row * a.C + q * EP;
+            #pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                const T* p = group + min(k * KS, a.C - KS) + at;
+                if constexpr (DT == 0) v[k] = __builtin_bit_cast(az_i4, *(const az_f4_u*)p);
+                else v[k] = __builtin_bit_cast(az_i4, *(const az_s8_u*)p);
+            }
+        } else if constexpr (MODE == WHOLE_FIRST) {
+            const int at = anew(bb * (a.C - 1) * a.S + row + q * EP * a.S), S = anew_s(a.S);
+            #pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                T e[EP];
+                #pragma unroll
+                for (int j = 0; j < EP; ++j) e[j] = (group + (min(k * KS, a.C - KS) + j) * S)[at];
+                v[k] = *(az_i4*)e;
+            }
+        } else {
+            const int cs = anew_s(a.nchw ? a.S : 1), at = a.nchw ? bb * (a.C - 1) * a.S + row : row * a.C, c0 = anew(q * EP);
+            #pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                T e[EP];
+                #pragma unroll
+                for (int j = 0; j < EP; ++j) e[j] = group[at + min(c0 + k * KS + j, a.C - 1) * cs];
+                v[k] = *(az_i4*)e;
+            }
+        }
+    }
+    // channels beyond the last are zero
+    __device__ __forceinline__ az_i4 frag(const PolicyDev& a, int k, int q) const {
+        constexpr int EP = AzElem<DT>::EP, KS = AzElem<DT>::KS;
+        typedef typename AzElem<DT>::T T;
+        if (MODE != ANY) return v[k];
+        T e[EP];
+        *(az_i4*)e = v[k];
+        const int c0 = k * KS + q * EP;
+        #pragma unroll
+        for (int j = 0; j < EP; ++j) e[j] = c0 + j < a.C ? e[j] : (T)0.f;
+        return *(az_i4*)e;
+    }
+};
+
+// acc += w h over the channels: step(k, w) multiplies the fragments that fetch(k, w) brings.  All KT steps of the width
+// the kernel is built for as straight code (the LDS reads run ahead of the products by themselves); fewer under checks.
+// AHEAD: the fragments come from memory, so they are asked for one step early, and no earlier (all at once they would
+// take more registers than there are).
+template <int KT, int KS, int W, bool AHEAD, class F, class S> __device__ __forceinline__ void product(int C, const F& fetch, const S& step) {
+    if constexpr (AHEAD) {
+        az_i4 w[2][W];
+        fetch(0, w[0]);
+        #pragma unroll
+        for (int k = 0; k < KT; ++k) {
+            if (k * KS >= C) break;
+            if (k + 1 < KT) fetch(k + 1, w[(k + 1) & 1]);            // (the padded copy is as wide as the kernel)
+            step(k, w[k & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    } else if (C > (KT - 1) * KS) {
+        #pragma unroll
+        for (int k = 0; k < KT; ++k) { az_i4 w[W]; fetch(k, w); step(k, w); }
+    } else {
+        #pragma unroll
+        for (int k = 0; k < KT - 1; ++k)
+            if (k * KS < C) { az_i4 w[W]; fetch(k, w); step(k, w); }
+    }
+}
+
+// Losses.  A workgroup takes a board (or nb small ones) at a time, its waves the tiles of 16 rows in turn, all planes.  The
+// features go from memory to fragments (no other wave wants these rows), the next tile's while this one is worked on; the
+// waves meet only where the board changes.  Planes are taken half at a time where there are many (all at
+// once leaves a wave too few registers for four waves a SIMD).  Sparse targets: the logits pass through LDS, and lanes
+// pick out those that the tile's entries name.
+template <int OT> struct LossTile {
+    static constexpr int PASSES = OT >= 4 ? 2 : 1, OTP = OT / PASSES, LDZ = OTP * 16 + 4;
+    static constexpr size_t bytes = (size_t)16 * LDZ * 4;            // of one wave
+};
+template <int DT, int OT, int CB> __host__ __device__ constexpr int loss_waves() { return DT != 0 && CB == 1 ? 4 : 2; }   // a SIMD
+template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT, (loss_waves<DT, OT, CB>())) az_policy_loss_kernel(PolicyDev a, int groups) {
+    typedef Lay<DT, OT> L;
+    typedef LossTile<OT> R;
+    constexpr int KT = CB * 128 / L::KS;
+    constexpr bool WLDS = w_in_lds<DT, OT, CB>();
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    __shared__ az_f4 red[4 * ROWS];
+    const int Cp = (a.C + 31) / 32 * 32, ldc = Cp + L::EP;
+    const Smem<DT, OT, CB, 0, WLDS> m(smem, a, Cp, a.counts ? WAVES * R::bytes : 0);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
+    float* zt = m.t + wave * (R::bytes / 4);
+    const int g_lo = (int)((long long)blockIdx.x * groups / gridDim.x), g_hi = (int)((long long)(blockIdx.x + 1) * groups / gridDim.x);
+    RowFrags<DT, KT, MODE> f;
+    f.load(a, g_lo * a.nb, wave * 16 + (lane & 15), min(a.nb, a.B - g_lo * a.nb) * a.S, q);
+    BoardLoads next;
+    next.load(a, m.b, g_lo * a.nb, tid);
+    if (WLDS) stage_w<DT, OT>(a, m.w, Cp, tid);
+    for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
+    init_words(a, m.b, tid);
+    __syncthreads();
+    for (int g = g_lo; g < g_hi; ++g) {
+        const int b0 = g * a.nb, rows = min(a.nb, a.B - b0) * a.S;
+        next.store(a, m.b, b0, tid);
+        if (g + 1 < g_hi) next.load(a, m.b, b0 + a.nb, tid);
+        float mx = -INFINITY, l = 0.f, tz = 0.f, tm = 0.f;
+        for (int r0 = wave * 16; r0 < rows; r0 += WAVES * 16) {
+            const int rl = r0 + (lane & 15);
+            const bool live = rl < rows;
+            const int bb = a.nb > 1 ? (int)((unsigned)min(rl, ROWS - 1) * a.mag_s >> 16) : 0, s = live ? rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
+            const unsigned bit = live ? 1u << (s - y * a.N) : 0u;
+            const unsigned* words = m.b.words + ((live ? bb : 0) * a.N + y) * (OT * 16) + q * 4;
+            const float* dense = a.dense + (size_t)b0 * a.O * a.S;
+            const int hi = min(r0 + 16, rows), e0 = m.b.listed ? m.b.start[r0 >> 4] : 0, e1 = m.b.listed ? m.b.start[(r0 >> 4) + 1] : min(a.nb, a.B - b0) * a.cap;
+            int key0 = -1;
+            float val0 = 0.f;
+            if (m.b.listed && e0 + lane < e1) { key0 = m.b.key[e0 + lane]; val0 = m.b.val[e0 + lane]; }
+            #pragma unroll 1
+            for (int o0 = 0; o0 < OT * 16; o0 += R::OTP * 16) {      // planes o0 .. o0 + 16 OTP - 1
+                az_f4 acc[R::OTP];
+                #pragma unroll
+                for (int j = 0; j < R::OTP; ++j) acc[j] = *(const az_f4*)(m.bias + o0 + j * 16 + q * 4);
+                const auto step = [&](int k, const az_i4* w) __attribute__((always_inline)) {
+                    const az_i4 hb = f.frag(a, k, q);
+                    #pragma unroll
+                    for (int j = 0; j < R::OTP; ++j) acc[j] = az_mma<DT>(w[j], hb, acc[j]);
+                };
+                const auto fetch = [&](int k, az_i4* w) __attribute__((always_inline)) {
+                    #pragma unroll
+                    for (int j = 0; j < R::OTP; ++j) w[j] = WLDS ? az_row_frag<DT>(m.w, ldc, o0 + j * 16, k * L::KS, lane) : az_row_frag<DT>(a.wpad, Cp, o0 + j * 16, k * L::KS, lane);
+                };
+                product<KT, L::KS, R::OTP, !WLDS>(a.C, fetch, step);
+                // the wave's next tile: of this group, or the first of the next one (which the barriers between do not touch)
+                if (o0 + R::OTP * 16 >= OT * 16) {
+                    if (r0 + WAVES * 16 < rows) f.load(a, b0, rl + WAVES * 16, rows, q);
+                    else if (g + 1 < g_hi) f.load(a, b0 + a.nb, wave * 16 + (lane & 15), min(a.nb, a.B - b0 - a.nb) * a.S, q);
+                }
+                #pragma unroll
+                for (int j = 0; j < R::OTP; ++j) {
+                    const az_i4 w = *(const az_i4*)(words + o0 + j * 16);
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[j][i] = (unsigned)w[i] & bit ? acc[j][i] : -INFINITY;
+                }
+                // (an entry without a target does not count, whatever its logit; one with a target whose action is not
+                // allowed gives -inf)
+                if (!a.counts) {
+                    const int at = (bb * a.O + o0 + q * 4) * a.S + s, last = ((bb + 1) * a.O - 1) * a.S + s;
+                    float tv[R::OTP][4];
+                    #pragma unroll
+                    for (int j = 0; j < R::OTP; ++j)
+                        #pragma unroll
+                        for (int i = 0; i < 4; ++i) tv[j][i] = dense[min(at + (j * 16 + i) * a.S, last)];
+                    #pragma unroll
+                    for (int j = 0; j < R::OTP; ++j)
+                        #pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float v = live && o0 + j * 16 + q * 4 + i < a.O ? tv[j][i] : 0.f;
+                            tz += v != 0.f ? v * acc[j][i] : 0.f;
+                            tm += v;
+                        }
+                } else {
+                    #pragma unroll
+                    for (int j = 0; j < R::OTP; ++j) *(az_f4*)(zt + (lane & 15) * R::LDZ + j * 16 + q * 4) = acc[j];
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                    const auto take = [&](int k, float v) __attribute__((always_inline)) {
+                        const int row = (k >> 8) - r0, o = (k & 255) - o0;
+                        if ((unsigned)row < (unsigned)(hi - r0) && (unsigned)o < (unsigned)(R::OTP * 16)) {
+                            tz += v != 0.f ? v * zt[row * R::LDZ + o] : 0.f;
+                            tm += v;
+                        }
+                    };
+                    if (m.b.listed && a.nb == 1) {                   // every lane takes an entry, whichever row it names
+                        take(key0, val0);
+                        for (int e = e0 + 64 + lane; e < e1; e += 64) take(m.b.key[e], m.b.val[e]);
+                    } else                                           // several boards: a lane takes its own row's
+                        for (int e = e0 + (a.nb > 1 ? q : lane); e < e1; e += a.nb > 1 ? 4 : 64) {
+                            float v = 0.f;
+                            int k;
+                            if (m.b.listed) { k = m.b.key[e]; v = m.b.val[e]; } else k = entry_at(a, b0, e, v);
+                            if (k >= 0 && (a.nb == 1 || k >> 8 == rl)) take(k, v);
+                        }
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                }
+                float to = mx;
+                #pragma unroll
+                for (int j = 0; j < R::OTP; ++j) to = fmaxf(to, fmaxf(fmaxf(acc[j][0], acc[j][1]), fmaxf(acc[j][2], acc[j][3])));
+                const float ml = to == -INFINITY ? 0.f : to * LOG2E;
+                l *= rescale(mx, to);
+                #pragma unroll
+                for (int j = 0; j < R::OTP; ++j)
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -ml));
+                mx = to;
+            }
+        }
+        if (a.nb == 1) {
+            for (int d = 32; d > 0; d >>= 1) {
+                join(mx, l, __shfl_xor(mx, d, 64), __shfl_xor(l, d, 64));
+                tz += __shfl_xor(tz, d, 64);
+                tm += __shfl_xor(tm, d, 64);
+            }
+            if (lane == 0) red[wave] = az_f4{mx, l, tz, tm};
+        } else if (wave < 4) red[wave * 64 + (lane & 15) * 4 + q] = az_f4{mx, l, tz, tm};
+        __syncthreads();
+        if (a.nb == 1) {
+            if (tid == 0) {
+                az_f4 r = red[0];
+                float fm = r[0], fl = r[1], fz = r[2], ft = r[3];
+                for (int w = 1; w < WAVES; ++w) { r = red[w]; join(fm, fl, r[0], r[1]); fz += r[2]; ft += r[3]; }
+                finish_board(a, b0, fm, fl, fz, ft);
+            }
+        } else
+            for (int bb = wave; bb * a.S < rows; bb += WAVES) {
+                float fm = -INFINITY, fl = 0.f, fz = 0.f, ft = 0.f;
+                for (int i = lane; i < a.S * 4; i += 64) { const az_f4 r = red[bb * a.S * 4 + i]; join(fm, fl, r[0], r[1]); fz += r[2]; ft += r[3]; }
+                for (int d = 32; d > 0; d >>= 1) {
+                    join(fm, fl, __shfl_xor(fm, d, 64), __shfl_xor(fl, d, 64));
+                    fz += __shfl_xor(fz, d, 64);
+                    ft += __shfl_xor(ft, d, 64);
+                }
+                if (lane == 0) finish_board(a, b0 + bb, fm, fl, fz, ft);
+            }
+    }
+}
+
+// A step of the gradients: up to 64 rows, a block of a board or whole boards; cells cell0 .. of board b0.
+struct Step {
+    int b0, blk, cell0, rows;
+    __device__ __forceinline__ void set(const PolicyDev& a) {
+        cell0 = blk * ROWS;
+        rows = a.nb > 1 ? min(a.nb, a.B - b0) * a.S : min(ROWS, a.S - cell0);
+    }
+    __device__ __forceinline__ Step(const PolicyDev& a, int it) {
+        const int g = it / a.blocks;
+        b0 = g * a.nb; blk = it - g * a.blocks;
+        set(a);
+    }
+    __device__ __forceinline__ void next(const PolicyDev& a) {
+        if (++blk == a.blocks) { blk = 0; b0 += a.nb; }
+        set(a);
+    }
+};
+
+// The 16-byte pieces of a step's features that a thread carries from memory to LDS.  WHOLE_LAST: consecutive threads take
+// consecutive pieces of a row; otherwise a wave takes one piece of all 64 rows.
+template <int DT, int NP, int MODE> struct Feat {
+    az_i4 v[NP];
+    __device__ __forceinline__ void place(int i, int pieces, int tid, int& row, int& p) const {
+        const int k = tid + i * NT;
+        if constexpr (MODE == WHOLE_LAST) { row = k / pieces; p = k - row * pieces; }
+        else { row = tid & (ROWS - 1); p = __builtin_amdgcn_readfirstlane(tid / ROWS) + i * WAVES; }
+    }
+    __device__ __forceinline__ void load(const PolicyDev& a, const Step& st, int pieces, int tid) {
+        constexpr int EP = AzElem<DT>::EP;
+        typedef typename AzElem<DT>::T T;
+        const bool first = MODE == WHOLE_FIRST || (MODE == ANY && a.nchw);
+        const T* group = (const T*)a.h + (size_t)st.b0 * a.S * a.C + (first ? st.cell0 : st.cell0 * a.C);
+        #pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            int row, p;
+            place(i, pieces, tid, row, p);
+            row = min(row, st.rows - 1);
+            const int bb = first && a.nb > 1 ? (int)((unsigned)row * a.mag_s >> 16) : 0;
+            if constexpr (MODE == WHOLE_LAST) {
+                const T* src = group + row * a.C + min(p * EP, a.C - EP);
+                if constexpr (DT == 0) v[i] = __builtin_bit_cast(az_i4, *(const az_f4_u*)src);
+                else v[i] = __builtin_bit_cast(az_i4, *(const az_s8_u*)src);
+            } else {
+                const int at = first ? bb * (a.C - 1) * a.S + row : row * a.C, cs = anew_s(first ? a.S : 1);
+                T e[EP];
+                #pragma unroll
+                for (int j = 0; j < EP; ++j) e[j] = (group + min(p * EP + j, a.C - 1) * cs)[at];
+                v[i] = *(az_i4*)e;
+            }
+        }
+    }
+    // Rows beyond the step are zero; channels beyond C were zeroed when the kernel began and stay so.
+    __device__ __forceinline__ void store(const PolicyDev& a, const Step& st, void* hl, int Cp, int pieces, int tid) const {
+        constexpr int EP = AzElem<DT>::EP;
+        typedef typename AzElem<DT>::T T;
+        #pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            int row, p;
+            place(i, pieces, tid, row, p);
+            const az_i4 x = row < st.rows ? v[i] : az_i4{0, 0, 0, 0};
+            if (row >= ROWS || p >= pieces) continue;
+            T* dst = (T*)hl + row * (Cp + EP) + p * EP;
+            if (p * EP + EP <= a.C) *(az_i4*)dst = x;
+            else if (MODE == ANY) {
+                T e[EP];
+                *(az_i4*)e = x;
+                #pragma unroll
+                for (int j = 0; j < EP; ++j) if (p * EP + j < a.C) dst[j] = e[j];
+            }
+        }
+    }
+};
+
+// The sparse targets of 16 rows (tile rt of the step) and planes o0 .. o0 + n - 1 into t [16][LD], cleared before: one
+// wave, the entries in their order (an LDS add takes a wave's lanes in theirs), so an action that is named more than once
+// is summed in one order.
+template <int LD> __device__ __forceinline__ void scatter_targets(const PolicyDev& a, const BoardLds& l, float* t, const Step& st, int rt, int o0, int n, int lane) {
+    const int row0 = st.cell0 + rt * 16, tile = min(row0 >> 4, 63);
+    const int e0 = l.listed ? l.start[tile] : 0, e1 = l.listed ? l.start[tile + 1] : min(a.nb, a.B - st.b0) * a.cap;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    for (int e = e0 + lane; e < e1; e += 64) {
+        int key;
+        float v = 0.f;
+        if (l.listed) { key = l.key[e]; v = l.val[e]; }
+        else key = entry_at(a, st.b0, e, v);
+        const int o = (key & 255) - o0, row = (key >> 8) - row0;
+        if (key >= 0 && (unsigned)o < (unsigned)n && (unsigned)row < 16u)
+            __hip_atomic_fetch_add(t + row * LD + o, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Gradients.  Eight waves.  A step: dz of 64 rows (16 rows and half of the planes a wave), then its product with w (32
+// rows and a quarter of the channels a wave) and its product with the features (half of the planes and a quarter of the
+// channels a wave, kept in registers over all of a workgroup's steps).  16-bit features: dz goes to LDS as hi + lo of the
+// type, hi alone feeds dh (whose result is rounded to that type anyway), both feed dw (an fp32 sum over all rows: one
+// rounding to 16 bits of each term would stay in it).
+//
+// The LDS port bounds the step (128 bytes a cycle for operands that the matrix units eat at 1 KB per 16 cycles and SIMD),
+// so 16-bit kernels of up to 128 channels (LEAN) hold their shares of w in registers in both roles, 72 of a wave's 256
+// for 96 planes; the room that leaves in LDS takes a second buffer of features and each wave's own targets, and a step
+// has two barriers instead of five.
+template <int DT, int OT, int CB> struct GradCfg {
+    typedef Lay<DT, OT> L;
+    static constexpr bool LEAN = DT != 0 && CB == 1;
+    static constexpr bool WLDS = !LEAN && w_in_lds<DT, OT, CB>();
+    static constexpr int OTH = (OT + 1) / 2, HBUF = LEAN ? 2 : 1, LDP = OTH * 16 + 4;   // LDP: a wave's own targets [16][LDP]
+    static constexpr size_t own = (size_t)16 * LDP * 4;
+    static constexpr int WAVES_EU = LEAN && OT <= 2 ? 4 : 2;
+    static size_t zb(const PolicyDev& a) { return L::z_bytes + (LEAN && a.counts ? WAVES * own : 0); }
+};
+template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT, (GradCfg<DT, OT, CB>::WAVES_EU)) az_policy_grad_kernel(PolicyDev a) {
+    typedef Lay<DT, OT> L;
+    typedef GradCfg<DT, OT, CB> G;
+    typedef typename AzElem<DT>::T T;
+    constexpr int NP = CB * 128 / L::EP * ROWS / NT, OTH = G::OTH, KO = L::OP / L::KS, KT = CB * 128 / L::KS;
+    constexpr int OG = OT > 1 ? 2 : 1, CG = 8 / OG, OTN = OT / OG, CTN = CB * 8 / CG;   // dw: groups of planes and channels, tiles of a wave
+    constexpr bool LEAN = G::LEAN, WLDS = G::WLDS;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int Cp = (a.C + 31) / 32 * 32, ldc = Cp + L::EP, pieces = Cp / L::EP;
+    const Smem<DT, OT, CB, G::HBUF, WLDS> m(smem, a, Cp, L::z_bytes + (LEAN && a.counts ? WAVES * G::own : 0));
+    T* zhi = (T*)m.t;
+    T* zlo = zhi + ROWS * L::LDO;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, rt = wave & 3, half = wave >> 2;
+    float* own = (float*)((unsigned char*)m.t + L::z_bytes + wave * G::own);
+    const int s_lo = (int)((long long)blockIdx.x * a.steps / gridDim.x), s_hi = (int)((long long)(blockIdx.x + 1) * a.steps / gridDim.x);
+    const int og = OG == 2 ? wave & 1 : 0, cg = OG == 2 ? wave >> 1 : wave, pair = wave & 1, cq = wave >> 1;
+    az_f4 dw[CTN][OTN];
+    #pragma unroll
+    for (int i = 0; i < CTN; ++i)
+        #pragma unroll
+        for (int j = 0; j < OTN; ++j) dw[i][j] = az_f4{0.f, 0.f, 0.f, 0.f};
+    az_f4 db[OTH];
+    #pragma unroll
+    for (int j = 0; j < OTH; ++j) db[j] = az_f4{0.f, 0.f, 0.f, 0.f};
+    Step st(a, s_lo);
+    Feat<DT, NP, MODE> f;
+    f.load(a, st, pieces, tid);
+    BoardLoads nextb;
+    nextb.load(a, m.b, st.b0, tid);
+    for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
+    init_words(a, m.b, tid);
+    // this wave's shares of w: rows of its planes for the logits, columns of its channels for dh
+    az_i4 wr[LEAN ? OTH : 1][LEAN ? KT : 1], wc[LEAN ? CB * 2 : 1][LEAN ? KO : 1];
+    if constexpr (WLDS) stage_w<DT, OT>(a, m.w, Cp, tid);
+    if constexpr (LEAN) {
+        // through the features' and dz' room
+        unsigned char* w = m.h;
+        static_assert(L::OP * (128 + L::EP) * L::SZ <= 2 * ROWS * (128 + L::EP) * L::SZ, "w fits where the two feature buffers lie");
+        stage_w<DT, OT>(a, w, Cp, tid);
+        __syncthreads();
+        #pragma unroll
+        for (int j = 0; j < OTH; ++j)
+            #pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                const int ot = min(half * OTH + j, OT - 1);
+                wr[j][k] = k * L::KS < Cp ? az_row_frag<DT>(w, ldc, ot * 16, k * L::KS, lane) : az_i4{0, 0, 0, 0};
+            }
+        #pragma unroll
+        for (int j = 0; j < CB * 2; ++j)
+            #pragma unroll
+            for (int k = 0; k < KO; ++k) wc[j][k] = (cq + 4 * j) * 16 < Cp ? az_col_frag<DT>(w, ldc, k * L::KS, (cq + 4 * j) * 16, lane) : az_i4{0, 0, 0, 0};
+        __syncthreads();
+    }
+    if (a.C < Cp) for (int i = tid; i < G::HBUF * ROWS * ldc; i += NT) ((T*)m.h)[i] = (T)0.f;
+    // fp16: dz is r_b (a mean over the batch: 1 / B) times probabilities that may be 1e-5, below what fp16 resolves.  The
+    // workgroup's dz carry a power of two that puts the largest r_b T_b of its boards at 2^9 .. 2^10; it comes off the
+    // fp32 sums again.
+    float up = 1.f, down = 1.f;
+    if constexpr (DT == 1) {
+        const Step last(a, s_hi - 1);
+        const int b1 = min(last.b0 + a.nb, a.B);
+        float mx = 0.f;
+        for (int b = st.b0 + tid; b < b1; b += NT) mx = fmaxf(mx, fabsf(a.scale * (a.row_scale ? a.row_scale[b] : 1.f) * a.stats[b][1]));
+        mx = wave_max(mx);
+        if (lane == 0) m.t[wave] = mx;
+        __syncthreads();
+        for (int w = 0; w < 8; ++w) mx = fmaxf(mx, m.t[w]);
+        if (mx > 0.f && mx < INFINITY) {
+            const int e = min(max(10 - (ilogbf(mx) + 1), -100), 100);
+            up = ldexpf(1.f, e);
+            down = ldexpf(1.f, -e);
+        }
+    }
+    __syncthreads();
+    T* h = (T*)m.h;
+    f.store(a, st, h, Cp, pieces, tid);
+    nextb.store(a, m.b, st.b0, tid);                                 // (ends in a barrier)
+    Step nx = st;
+    if (s_lo + 1 < s_hi) { nx.next(a); f.load(a, nx, pieces, tid); }
+    for (int it = s_lo; it < s_hi; ++it) {
+        // dz of the step
+        const int rl = rt * 16 + (lane & 15);
+        const bool live = rl < st.rows;
+        const int bb = live && a.nb > 1 ? (int)((unsigned)rl * a.mag_s >> 16) : 0, b = st.b0 + bb, s = live ? st.cell0 + rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
+        const unsigned bit = live ? 1u << (s - y * a.N) : 0u;
+        const unsigned* words = m.b.words + (bb * a.N + y) * (OT * 16) + half * OTH * 16 + q * 4;
+        const az_f4 bst = a.stats[b];
+        const float rs = up * (a.scale * (a.row_scale ? a.row_scale[b] : 1.f));
+        az_f4 tv[OTH];
+        if (a.counts) {
+            if constexpr (LEAN) {                                    // the wave's own rows and planes, by itself
+                #pragma unroll
+                for (int i = 0; i < (int)(G::own / 16 + 63) / 64; ++i)
+                    if (i * 64 + lane < (int)(G::own / 16)) ((az_f4*)own)[i * 64 + lane] = az_f4{0.f, 0.f, 0.f, 0.f};
+                scatter_targets<G::LDP>(a, m.b, own, st, rt, half * OTH * 16, OTH * 16, lane);
+                #pragma unroll
+                for (int j = 0; j < OTH; ++j) tv[j] = *(const az_f4*)(own + (lane & 15) * G::LDP + j * 16 + q * 4);
+            } else {
+                float* t = m.t + rt * 16 * L::LDT;                   // where dz will lie: the waves clear and read it together
+                for (int i = tid; i < ROWS * L::LDT / 4; i += NT) ((az_f4*)m.t)[i] = az_f4{0.f, 0.f, 0.f, 0.f};
+                __syncthreads();
+                scatter_targets<L::LDT>(a, m.b, t + half * OTH * 16, st, rt, half * OTH * 16, OTH * 16, lane);
+                #pragma unroll
+                for (int j = 0; j < OTH; ++j) tv[j] = half * OTH + j < OT ? *(const az_f4*)(t + (lane & 15) * L::LDT + (half * OTH + j) * 16 + q * 4) : az_f4{0.f, 0.f, 0.f, 0.f};
+                __syncthreads();
+            }
+        } else {
+            const float* dense = a.dense + (size_t)st.b0 * a.O * a.S;
+            const int at = (bb * a.O + half * OTH * 16 + q * 4) * a.S + s, last = ((bb + 1) * a.O - 1) * a.S + s;
+            #pragma unroll
+            for (int j = 0; j < OTH; ++j)
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) tv[j][i] = dense[min(at + (j * 16 + i) * a.S, last)];   // (dropped below where no action stands for it)
+        }
+        az_f4 acc[OTH];
+        #pragma unroll
+        for (int j = 0; j < OTH; ++j) acc[j] = *(const az_f4*)(m.bias + min(half * OTH + j, OT - 1) * 16 + q * 4);
+        const auto step = [&](int k, const az_i4* w) __attribute__((always_inline)) {
+            const az_i4 hb = az_row_frag<DT>(h, ldc, rt * 16, k * L::KS, lane);
+            #pragma unroll
+            for (int j = 0; j < OTH; ++j) acc[j] = az_mma<DT>(w[j], hb, acc[j]);
+        };
+        const auto fetch = [&](int k, az_i4* w) __attribute__((always_inline)) {
+            #pragma unroll
+            for (int j = 0; j < OTH; ++j) {
+                const int ot = min(half * OTH + j, OT - 1);
+                if constexpr (LEAN) w[j] = wr[j][k];
+                else if constexpr (WLDS) w[j] = az_row_frag<DT>(m.w, ldc, ot * 16, k * L::KS, lane);
+                else w[j] = az_row_frag<DT>(a.wpad, Cp, ot * 16, k * L::KS, lane);
+            }
+        };
+        product<KT, L::KS, OTH, !LEAN && !WLDS>(a.C, fetch, step);
+        const float rT = rs * bst[1], lse2 = bst[0] * LOG2E;
+        // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
+        const bool bias_counts = a.O > 1 || bst[2] != 0.f;
+        #pragma unroll
+        for (int j = 0; j < OTH; ++j) {
+            const int ot = half * OTH + j;
+            if (ot * 16 >= L::OP) continue;
+            az_f4 dz = {0.f, 0.f, 0.f, 0.f};
+            if (ot < OT) {
+                const az_i4 w = *(const az_i4*)(words + j * 16);
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float v = rT * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -lse2)) - rs * tv[j][i];
+                    dz[i] = (unsigned)w[i] & bit ? v : 0.f;
+                }
+            }
+            if (bias_counts) db[j] += dz;
+            if constexpr (DT == 0) *(az_f4*)((float*)zhi + rl * L::LDO + ot * 16 + q * 4) = dz;
+            else {
+                az_s4 hi, lo;
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) { hi[i] = az_to16<DT>(dz[i]); lo[i] = az_to16<DT>(dz[i] - az_from16<DT>(hi[i])); }
+                *(az_s4*)((short*)zhi + rl * L::LDO + ot * 16 + q * 4) = hi;
+                *(az_s4*)((short*)zlo + rl * L::LDO + ot * 16 + q * 4) = lo;
+            }
+        }
+        __syncthreads();
+        const T* hcur = h;
+        if constexpr (LEAN) {                                        // the next step's features into the other buffer, the one after it on its way
+            h = (T*)m.h + ((it + 1 - s_lo) & 1) * ROWS * ldc;
+            if (it + 1 < s_hi) f.store(a, nx, h, Cp, pieces, tid);
+        }
+        Step after = nx;
+        if (it + 2 < s_hi) after.next(a);
+        if constexpr (LEAN) if (it + 2 < s_hi) f.load(a, after, pieces, tid);
+        // dh: rows of a tile are channels, columns are cells
+        {
+            az_i4 zf[2][KO];
+            #pragma unroll
+            for (int k = 0; k < KO; ++k)
+                #pragma unroll
+                for (int e = 0; e < 2; ++e) zf[e][k] = az_row_frag<DT>(zhi, L::LDO, (pair * 2 + e) * 16, k * L::KS, lane);
+            #pragma unroll
+            for (int j = 0; j < CB * 2; ++j) {
+                const int ct = cq + 4 * j;
+                if (ct * 16 >= Cp) continue;
+                az_f4 d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                #pragma unroll
+                for (int k = 0; k < KO; ++k) {
+                    az_i4 wa;
+                    if constexpr (LEAN) wa = wc[j][k];
+                    else if constexpr (WLDS) wa = az_col_frag<DT>(m.w, ldc, k * L::KS, ct * 16, lane);
+                    else wa = az_row_frag<DT>(a.wpadt, L::OP, ct * 16, k * L::KS, lane);
+                    d[0] = az_mma<DT>(wa, zf[0][k], d[0]);
+                    d[1] = az_mma<DT>(wa, zf[1][k], d[1]);
+                }
+                const int c = ct * 16 + q * 4;
+                #pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = (pair * 2 + e) * 16 + (lane & 15);
+                    if (row >= st.rows || c >= a.C) continue;
+                    if constexpr (DT == 1) d[e] *= down;
+                    if (MODE == WHOLE_LAST || (MODE == ANY && !a.nchw)) {
+                        T* dst = (T*)a.dh + ((size_t)st.b0 * a.S + st.cell0) * a.C + (row * a.C + c);
+                        if (MODE == WHOLE_LAST || c + 4 <= a.C) {
+                            if constexpr (DT == 0) *(az_f4_u*)dst = d[e];
+                            else *(az_s4_u*)dst = az_s4{az_to16<DT>(d[e][0]), az_to16<DT>(d[e][1]), az_to16<DT>(d[e][2]), az_to16<DT>(d[e][3])};
+                        } else for (int i = 0; i < 4; ++i) if (c + i < a.C) az_store<DT>(dst, i, d[e][i]);
+                    } else {
+                        const int b2 = a.nb > 1 ? (int)((unsigned)row * a.mag_s >> 16) : 0, s2 = st.cell0 + row - b2 * a.S;
+                        T* dst = (T*)a.dh + (size_t)st.b0 * a.C * a.S + ((b2 * a.C + c) * a.S + s2);
+                        for (int i = 0; i < 4; ++i) if (MODE == WHOLE_FIRST || c + i < a.C) az_store<DT>(dst, (size_t)i * a.S, d[e][i]);
+                    }
+                }
+            }
+        }
+        // dw: rows of a tile are planes, columns are channels, the contraction runs over the step's rows (rows beyond the
+        // step have dz = 0 and features of 0)
+        #pragma unroll
+        for (int k = 0; k < ROWS; k += L::KS) {
+            if (k >= st.rows) break;
+            az_i4 zf[OTN][DT == 0 ? 1 : 2];
+            #pragma unroll
+            for (int j = 0; j < OTN; ++j) {
+                zf[j][0] = az_col_frag<DT>(zhi, L::LDO, k, (og * OTN + j) * 16, lane);
+                if constexpr (DT != 0) zf[j][1] = az_col_frag<DT>(zlo, L::LDO, k, (og * OTN + j) * 16, lane);
+            }
+            #pragma unroll
+            for (int i = 0; i < CTN; ++i) {
+                const int ct = cg + CG * i;
+                if (ct * 16 >= Cp) continue;
+                const az_i4 hb = az_col_frag<DT>(hcur, ldc, k, ct * 16, lane);
+                #pragma unroll
+                for (int j = 0; j < OTN; ++j) {
+                    dw[i][j] = az_mma<DT>(zf[j][0], hb, dw[i][j]);
+                    if constexpr (DT != 0) dw[i][j] = az_mma<DT>(zf[j][1], hb, dw[i][j]);
+                }
+            }
+        }
+        __syncthreads();                                             // everything of this step has been read
+        if constexpr (!LEAN)
+            if (it + 1 < s_hi) {
+                f.store(a, nx, h, Cp, pieces, tid);
+                if (it + 2 < s_hi) f.load(a, after, pieces, tid);
+                if (nx.b0 == st.b0) __syncthreads();                 // (else the boards' staging ends in one)
+            }
+        if (it + 1 < s_hi && nx.b0 != st.b0) {
+            nextb.load(a, m.b, nx.b0, tid);
+            nextb.store(a, m.b, nx.b0, tid);
+        }
+        st = nx;
+        nx = after;
+    }
+    float* out = a.partial + (size_t)blockIdx.x * ((size_t)a.O * a.C + a.O);
+    #pragma unroll
+    for (int i = 0; i < CTN; ++i) {
+        const int c = (cg + CG * i) * 16 + (lane & 15);
+        #pragma unroll
+        for (int j = 0; j < OTN; ++j)
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int o = (og * OTN + j) * 16 + q * 4 + e;
+                if (o < a.O && c < a.C) out[(size_t)o * a.C + c] = dw[i][j][e] * down;
+            }
+    }
+    float* red = m.t;                                                // [4][OT * 16]
+    #pragma unroll
+    for (int j = 0; j < OTH; ++j) {
+        const int ot = half * OTH + j;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v = db[j][i];
+            for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d, 64);
+            if (ot < OT && (lane & 15) == 0) red[rt * OT * 16 + ot * 16 + q * 4 + i] = v;
+        }
+    }
+    __syncthreads();
+    for (int o = tid; o < a.O; o += NT) out[(size_t)a.O * a.C + o] = ((red[o] + red[OT * 16 + o]) + (red[2 * OT * 16 + o] + red[3 * OT * 16 + o])) * down;
+}
+
+template <int DT, int OT, int CB, int MODE> hipError_t launch_products(const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
+    const int Cp = (a.C + 31) / 32 * 32;
+    typedef GradCfg<DT, OT, CB> G;
+    const size_t lds = grad ? Smem<DT, OT, CB, G::HBUF, G::WLDS>::bytes(a, Cp, G::zb(a))
+                            : Smem<DT, OT, CB, 0, w_in_lds<DT, OT, CB>()>::bytes(a, Cp, a.counts ? WAVES * LossTile<OT>::bytes : 0);
+    const void* fn = grad ? (const void*)az_policy_grad_kernel<DT, OT, CB, MODE> : (const void*)az_policy_loss_kernel<DT, OT, CB, MODE>;
+    if (lds > 32 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    if (grad) az_policy_grad_kernel<DT, OT, CB, MODE><<<groups, NT, lds, stream>>>(a);
+    else {
+        // as many workgroups as the chip holds at once, the boards in even shares
+        const int per_cu = loss_waves<DT, OT, CB>() * 4 / WAVES >= 2 && (lds + 4 * ROWS * 16) * 2 <= LDS_BYTES ? 2 : 1;
+        const int work = (a.B + a.nb - 1) / a.nb, room = CUS * per_cu, rounds = (work + room - 1) / room;
+        az_policy_loss_kernel<DT, OT, CB, MODE><<<(work + rounds - 1) / rounds, NT, lds, stream>>>(a, work);
+    }
+    return hipGetLastError();
+}
+template <int DT, int OT, int CB> hipError_t launch_mode(const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
+    if (a.C % AzElem<DT>::KS) return launch_products<DT, OT, CB, ANY>(a, grad, groups, stream);
+    return a.nchw ? launch_products<DT, OT, CB, WHOLE_FIRST>(a, grad, groups, stream) : launch_products<DT, OT, CB, WHOLE_LAST>(a, grad, groups, stream);
+}
+template <int DT, int OT> hipError_t launch_c(const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
+    return a.C <= 128 ? launch_mode<DT, OT, 1>(a, grad, groups, stream) : launch_mode<DT, OT, 2>(a, grad, groups, stream);
+}
+template <int DT> hipError_t launch_o(const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
+    if (a.O <= 16) return launch_c<DT, 1>(a, grad, groups, stream);
+    if (a.O <= 32) return launch_c<DT, 2>(a, grad, groups, stream);
+    if (a.O <= 64) return launch_c<DT, 4>(a, grad, groups, stream);
+    if (a.O <= 96) return launch_c<DT, 6>(a, grad, groups, stream);
+    return launch_c<DT, 8>(a, grad, groups, stream);
+}
+
+}  // namespace
