@@ -58,20 +58,20 @@ template <int DT> __device__ __forceinline__ void az_store(void* p, size_t i, fl
 // Fragment whose contraction runs along a row of the LDS matrix m [rows][ld]: row r0 + l % 16, elements k0 + EP * (l / 16) ..
 template <int DT> __device__ __forceinline__ az_i4 az_row_frag(const void* m, int ld, int r0, int k0, int lane) {
     constexpr int EP = AzElem<DT>::EP, SZ = 16 / EP;
-    return *(const az_i4*)((const char*)m + ((size_t)(r0 + (lane & 15)) * ld + k0 + EP * (lane >> 4)) * SZ);
+    return *(const az_i4*)((const char*)m + ((r0 + (lane & 15)) * ld + k0 + EP * (lane >> 4)) * SZ);
 }
 // Fragment whose contraction runs down a column: column n0 + l % 16, rows k0 + EP * (l / 16) ..  For 16-bit elements the
 // LDS read transposes: in each group of 16 lanes, lane i's address names 4 elements of row i / 4 and the lane gets
 // column i of the 4 x 16 block.
 template <int DT> __device__ __forceinline__ az_i4 az_col_frag(const void* m, int ld, int k0, int n0, int lane) {
     if constexpr (DT == 0) {
-        const float* p = (const float*)m + (size_t)(k0 + 4 * (lane >> 4)) * ld + n0 + (lane & 15);
+        const float* p = (const float*)m + (k0 + 4 * (lane >> 4)) * ld + n0 + (lane & 15);
         az_f4 v;
-        for (int j = 0; j < 4; ++j) v[j] = p[(size_t)j * ld];
+        for (int j = 0; j < 4; ++j) v[j] = p[j * ld];
         return __builtin_bit_cast(az_i4, v);
     } else {
         typedef __attribute__((address_space(3))) az_s4* lds_s4;
-        const short* p = (const short*)m + (size_t)(k0 + 8 * (lane >> 4) + ((lane & 15) >> 2)) * ld + n0 + (lane & 3) * 4;
+        const short* p = (const short*)m + (k0 + 8 * (lane >> 4) + ((lane & 15) >> 2)) * ld + n0 + (lane & 3) * 4;
         const az_s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p);
         const az_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 4 * ld));
         return __builtin_bit_cast(az_i4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));

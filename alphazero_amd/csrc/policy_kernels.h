@@ -6,13 +6,14 @@
 namespace {
 
 // dynamic LDS of the two product kernels
-template <int DT, int OT> struct Lay {
+template <int DT, int OT, int CB> struct Lay {
     static constexpr int EP = AzElem<DT>::EP, KS = AzElem<DT>::KS, SZ = 16 / EP;
     static constexpr int OP = (OT * 16 + KS - 1) / KS * KS;          // planes, padded to a step of the contraction over them
     static constexpr int LDT = OT * 16 + 4, LDO = OP + EP;
-    // rows are padded by 16 bytes, so that they start in different banks
-    __host__ __device__ static size_t w_bytes(int Cp) { return (size_t)OP * (Cp + EP) * SZ; }
-    __host__ __device__ static size_t h_bytes(int Cp) { return (size_t)ROWS * (Cp + EP) * SZ; }
+    // channels are padded to what the kernel is built for (every LDS address is then a base and a constant), rows by 16
+    // bytes more, so that they start in different banks
+    static constexpr int CP = CB * 128, LDC = CP + EP, PIECES = CP / EP;
+    static constexpr size_t w_bytes = (size_t)OP * LDC * SZ, h_bytes = (size_t)ROWS * LDC * SZ;
     static constexpr size_t z_bytes = (size_t)ROWS * (LDO > LDT ? LDO : LDT) * 4;
 };
 
@@ -28,6 +29,15 @@ __device__ __forceinline__ float wave_max(float x) {
 //   ANY          anything else: one element a load, every index clamped
 enum { WHOLE_LAST, WHOLE_FIRST, ANY };
 
+// The kernel's arguments, read again from the argument segment: called at the top of a loop's body, what is derived from
+// them does not have to live through the whole loop (it would fill the scalar registers, and spill into vector ones).
+__device__ __forceinline__ PolicyDev arguments() {
+    typedef const __attribute__((address_space(4))) PolicyDev* Args;
+    Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const PolicyDev*)p;
+}
+
 // A value the compiler may not carry over from an earlier iteration: index arithmetic of the one-element loads is done
 // anew for each tile instead of filling the registers.
 __device__ __forceinline__ int anew(int x) { asm volatile("" : "+v"(x)); return x; }
@@ -37,11 +47,11 @@ __device__ __forceinline__ int anew_s(int x) { asm volatile("" : "+s"(x)); retur
 template <int DT, int OT, int CB> __host__ __device__ constexpr bool w_in_lds() { return !(DT == 0 && CB == 2 && OT >= 4); }
 
 // w [O][C] -> LDS [OP][Cp + EP], zero beyond O and C, in pieces of 16 bytes; eight loads of a thread in flight
-template <int DT, int OT> __device__ __forceinline__ void stage_w(const PolicyDev& a, void* wl, int Cp, int tid) {
-    typedef Lay<DT, OT> L;
+template <int DT, int OT, int CB> __device__ __forceinline__ void stage_w(const PolicyDev& a, void* wl, int tid) {
+    typedef Lay<DT, OT, CB> L;
     typedef typename AzElem<DT>::T T;
     constexpr int EP = L::EP, U = 8;
-    const int per = Cp / EP, total = L::OP * per;
+    constexpr int per = L::PIECES, total = L::OP * per;
     for (int base = tid; base < total; base += NT * U) {
         az_i4 v[U];
         if (a.C % EP == 0) {
@@ -66,7 +76,7 @@ template <int DT, int OT> __device__ __forceinline__ void stage_w(const PolicyDe
         #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = base + u * NT, o = i / per, c = (i - o * per) * EP;
-            if (i < total) *(az_i4*)((char*)wl + ((size_t)o * (Cp + EP) + c) * L::SZ) = o < a.O && c < a.C ? v[u] : az_i4{0, 0, 0, 0};
+            if (i < total) *(az_i4*)((char*)wl + ((size_t)o * L::LDC + c) * L::SZ) = o < a.O && c < a.C ? v[u] : az_i4{0, 0, 0, 0};
         }
     }
 }
@@ -80,6 +90,7 @@ struct BoardLds {
     float* val;
     int* cnt;                                                        // [64-entry chunk][64 tiles]
     int* start;                                                      // [65]: a tile's first entry
+    az_f4* stat;                                                     // [MAX_BOARDS] of the gradients: {lse, r T, r, is there a target that is not allowed}
     bool listed;                                                     // the entries fit
 };
 __host__ __device__ inline int entry_room(int nb, int cap) { return (long long)nb * cap <= ENTRIES ? nb * cap : 0; }
@@ -102,8 +113,7 @@ __device__ __forceinline__ void init_words(const PolicyDev& a, const BoardLds& l
     for (int i = tid; i < a.nb * a.N * l.planes; i += NT) l.words[i] = !a.legal && i % l.planes < a.O ? ~0u : 0u;
 }
 
-// One group's words and entries on their way: the first loads of a thread wait in registers while the group before is
-// worked on.
+// One group's words and entries: a thread's first loads go out together.
 struct BoardLoads {
     static constexpr int W = 4, E = ENTRIES / NT;
     unsigned w[W];
@@ -133,8 +143,13 @@ struct BoardLoads {
         l.words[(bb * a.N + y) * l.planes + bo - bb * a.O] = v;
     }
     // every thread; ends in a barrier
-    __device__ __forceinline__ void store(const PolicyDev& a, const BoardLds& l, int b0, int tid) const {
+    template <bool GRAD> __device__ __forceinline__ void store(const PolicyDev& a, const BoardLds& l, int b0, int tid) const {
         const int boards = min(a.nb, a.B - b0), lane = tid & 63, wave = tid >> 6;
+        if (GRAD && tid < boards) {
+            const az_f4 st = a.stats[b0 + tid];
+            const float r = a.scale * (a.row_scale ? a.row_scale[b0 + tid] : 1.f);
+            l.stat[tid] = az_f4{st[0], r * st[1], r, st[2]};
+        }
         if (a.legal) {
             const int n = boards * a.O * a.N;
             #pragma unroll
@@ -185,17 +200,24 @@ struct BoardLoads {
     }
 };
 
+template <bool GRAD> __device__ __forceinline__ void stage_boards(const PolicyDev& a, const BoardLds& l, int b0, int tid) {
+    BoardLoads x;
+    x.load(a, l, b0, tid);
+    x.store<GRAD>(a, l, b0, tid);
+}
+
 // LDS of the product kernels, in this order; zb: bytes of the kernel's own tile (logits or dz)
 template <int DT, int OT, int CB, int HBUF, bool WBUF> struct Smem {
-    typedef Lay<DT, OT> L;
+    typedef Lay<DT, OT, CB> L;
     unsigned char *w, *h;
     float *t, *bias;
     BoardLds b;
-    __device__ __forceinline__ Smem(unsigned char* p, const PolicyDev& a, int Cp, size_t zb) {
-        w = p; p += WBUF ? L::w_bytes(Cp) : 0;
-        h = p; p += HBUF * L::h_bytes(Cp);
+    __device__ __forceinline__ Smem(unsigned char* p, const PolicyDev& a, size_t zb) {
+        w = p; p += WBUF ? L::w_bytes : 0;
+        h = p; p += HBUF * L::h_bytes;
         t = (float*)p; p += zb;
         bias = (float*)p; p += OT * 16 * 4;
+        b.stat = (az_f4*)p; p += MAX_BOARDS * 16;
         b.words = (unsigned*)p; p += (size_t)a.nb * a.N * OT * 16 * 4;
         b.planes = OT * 16;
         const int room = a.counts ? entry_room(a.nb, a.cap) : 0;
@@ -205,9 +227,9 @@ template <int DT, int OT, int CB, int HBUF, bool WBUF> struct Smem {
         b.start = (int*)p; p += 65 * 4;
         b.cnt = (int*)p;
     }
-    static size_t bytes(const PolicyDev& a, int Cp, size_t zb) {
+    static size_t bytes(const PolicyDev& a, size_t zb) {
         const size_t room = a.counts ? (size_t)entry_room(a.nb, a.cap) : 0;
-        return (WBUF ? L::w_bytes(Cp) : 0) + HBUF * L::h_bytes(Cp) + zb + OT * 16 * 4 + (size_t)a.nb * a.N * OT * 16 * 4 +
+        return (WBUF ? L::w_bytes : 0) + HBUF * L::h_bytes + zb + OT * 16 * 4 + MAX_BOARDS * 16 + (size_t)a.nb * a.N * OT * 16 * 4 +
                (room ? room * 8 + 65 * 4 + (room + 63) / 64 * 256 : 0);
     }
 };
@@ -316,31 +338,30 @@ template <int OT> struct LossTile {
 };
 template <int DT, int OT, int CB> __host__ __device__ constexpr int loss_waves() { return DT != 0 && CB == 1 ? 4 : 2; }   // a SIMD
 template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT, (loss_waves<DT, OT, CB>())) az_policy_loss_kernel(PolicyDev a, int groups) {
-    typedef Lay<DT, OT> L;
+    typedef Lay<DT, OT, CB> L;
     typedef LossTile<OT> R;
     constexpr int KT = CB * 128 / L::KS;
     constexpr bool WLDS = w_in_lds<DT, OT, CB>();
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ az_f4 red[4 * ROWS];
-    const int Cp = (a.C + 31) / 32 * 32, ldc = Cp + L::EP;
-    const Smem<DT, OT, CB, 0, WLDS> m(smem, a, Cp, a.counts ? WAVES * R::bytes : 0);
+    constexpr int Cp = L::CP, ldc = L::LDC;
+    const Smem<DT, OT, CB, 0, WLDS> m(smem, a, a.counts ? WAVES * R::bytes : 0);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
     float* zt = m.t + wave * (R::bytes / 4);
     const int g_lo = (int)((long long)blockIdx.x * groups / gridDim.x), g_hi = (int)((long long)(blockIdx.x + 1) * groups / gridDim.x);
     RowFrags<DT, KT, MODE> f;
     f.load(a, g_lo * a.nb, wave * 16 + (lane & 15), min(a.nb, a.B - g_lo * a.nb) * a.S, q);
-    BoardLoads next;
-    next.load(a, m.b, g_lo * a.nb, tid);
-    if (WLDS) stage_w<DT, OT>(a, m.w, Cp, tid);
+    if (WLDS) stage_w<DT, OT, CB>(a, m.w, tid);
     for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
     init_words(a, m.b, tid);
     __syncthreads();
     for (int g = g_lo; g < g_hi; ++g) {
         const int b0 = g * a.nb, rows = min(a.nb, a.B - b0) * a.S;
-        next.store(a, m.b, b0, tid);
-        if (g + 1 < g_hi) next.load(a, m.b, b0 + a.nb, tid);
+        stage_boards<false>(a, m.b, b0, tid);
         float mx = -INFINITY, l = 0.f, tz = 0.f, tm = 0.f;
+        #pragma unroll 1
         for (int r0 = wave * 16; r0 < rows; r0 += WAVES * 16) {
+            const PolicyDev a = arguments();
             const int rl = r0 + (lane & 15);
             const bool live = rl < rows;
             const int bb = a.nb > 1 ? (int)((unsigned)min(rl, ROWS - 1) * a.mag_s >> 16) : 0, s = live ? rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
@@ -353,6 +374,15 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             if (m.b.listed && e0 + lane < e1) { key0 = m.b.key[e0 + lane]; val0 = m.b.val[e0 + lane]; }
             #pragma unroll 1
             for (int o0 = 0; o0 < OT * 16; o0 += R::OTP * 16) {      // planes o0 .. o0 + 16 OTP - 1
+                // loads return in order: the targets are asked for ahead of the next tile's features
+                float tv[R::OTP][4];
+                if (!a.counts) {
+                    const int at = (bb * a.O + o0 + q * 4) * a.S + s, last = ((bb + 1) * a.O - 1) * a.S + s;
+                    #pragma unroll
+                    for (int j = 0; j < R::OTP; ++j)
+                        #pragma unroll
+                        for (int i = 0; i < 4; ++i) tv[j][i] = dense[min(at + (j * 16 + i) * a.S, last)];
+                }
                 az_f4 acc[R::OTP];
                 #pragma unroll
                 for (int j = 0; j < R::OTP; ++j) acc[j] = *(const az_f4*)(m.bias + o0 + j * 16 + q * 4);
@@ -380,12 +410,6 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                 // (an entry without a target does not count, whatever its logit; one with a target whose action is not
                 // allowed gives -inf)
                 if (!a.counts) {
-                    const int at = (bb * a.O + o0 + q * 4) * a.S + s, last = ((bb + 1) * a.O - 1) * a.S + s;
-                    float tv[R::OTP][4];
-                    #pragma unroll
-                    for (int j = 0; j < R::OTP; ++j)
-                        #pragma unroll
-                        for (int i = 0; i < 4; ++i) tv[j][i] = dense[min(at + (j * 16 + i) * a.S, last)];
                     #pragma unroll
                     for (int j = 0; j < R::OTP; ++j)
                         #pragma unroll
@@ -482,13 +506,14 @@ struct Step {
 // The 16-byte pieces of a step's features that a thread carries from memory to LDS.  WHOLE_LAST: consecutive threads take
 // consecutive pieces of a row; otherwise a wave takes one piece of all 64 rows.
 template <int DT, int NP, int MODE> struct Feat {
+    static constexpr int pieces = NP * NT / ROWS, LDC = pieces * AzElem<DT>::EP + AzElem<DT>::EP;
     az_i4 v[NP];
-    __device__ __forceinline__ void place(int i, int pieces, int tid, int& row, int& p) const {
+    __device__ __forceinline__ void place(int i, int tid, int& row, int& p) const {
         const int k = tid + i * NT;
         if constexpr (MODE == WHOLE_LAST) { row = k / pieces; p = k - row * pieces; }
         else { row = tid & (ROWS - 1); p = __builtin_amdgcn_readfirstlane(tid / ROWS) + i * WAVES; }
     }
-    __device__ __forceinline__ void load(const PolicyDev& a, const Step& st, int pieces, int tid) {
+    __device__ __forceinline__ void load(const PolicyDev& a, const Step& st, int tid) {
         constexpr int EP = AzElem<DT>::EP;
         typedef typename AzElem<DT>::T T;
         const bool first = MODE == WHOLE_FIRST || (MODE == ANY && a.nchw);
@@ -496,7 +521,7 @@ template <int DT, int NP, int MODE> struct Feat {
         #pragma unroll
         for (int i = 0; i < NP; ++i) {
             int row, p;
-            place(i, pieces, tid, row, p);
+            place(i, tid, row, p);
             row = min(row, st.rows - 1);
             const int bb = first && a.nb > 1 ? (int)((unsigned)row * a.mag_s >> 16) : 0;
             if constexpr (MODE == WHOLE_LAST) {
@@ -513,16 +538,15 @@ template <int DT, int NP, int MODE> struct Feat {
         }
     }
     // Rows beyond the step are zero; channels beyond C were zeroed when the kernel began and stay so.
-    __device__ __forceinline__ void store(const PolicyDev& a, const Step& st, void* hl, int Cp, int pieces, int tid) const {
+    __device__ __forceinline__ void store(const PolicyDev& a, const Step& st, void* hl, int tid) const {
         constexpr int EP = AzElem<DT>::EP;
         typedef typename AzElem<DT>::T T;
         #pragma unroll
         for (int i = 0; i < NP; ++i) {
             int row, p;
-            place(i, pieces, tid, row, p);
+            place(i, tid, row, p);
             const az_i4 x = row < st.rows ? v[i] : az_i4{0, 0, 0, 0};
-            if (row >= ROWS || p >= pieces) continue;
-            T* dst = (T*)hl + row * (Cp + EP) + p * EP;
+            T* dst = (T*)hl + row * LDC + p * EP;
             if (p * EP + EP <= a.C) *(az_i4*)dst = x;
             else if (MODE == ANY) {
                 T e[EP];
@@ -566,7 +590,7 @@ template <int LD> __device__ __forceinline__ void scatter_targets(const PolicyDe
 // for 96 planes; the room that leaves in LDS takes a second buffer of features and each wave's own targets, and a step
 // has two barriers instead of five.
 template <int DT, int OT, int CB> struct GradCfg {
-    typedef Lay<DT, OT> L;
+    typedef Lay<DT, OT, CB> L;
     static constexpr bool LEAN = DT != 0 && CB == 1;
     static constexpr bool WLDS = !LEAN && w_in_lds<DT, OT, CB>();
     static constexpr int OTH = (OT + 1) / 2, HBUF = LEAN ? 2 : 1, LDP = OTH * 16 + 4;   // LDP: a wave's own targets [16][LDP]
@@ -575,15 +599,15 @@ template <int DT, int OT, int CB> struct GradCfg {
     static size_t zb(const PolicyDev& a) { return L::z_bytes + (LEAN && a.counts ? WAVES * own : 0); }
 };
 template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT, (GradCfg<DT, OT, CB>::WAVES_EU)) az_policy_grad_kernel(PolicyDev a) {
-    typedef Lay<DT, OT> L;
+    typedef Lay<DT, OT, CB> L;
     typedef GradCfg<DT, OT, CB> G;
     typedef typename AzElem<DT>::T T;
     constexpr int NP = CB * 128 / L::EP * ROWS / NT, OTH = G::OTH, KO = L::OP / L::KS, KT = CB * 128 / L::KS;
     constexpr int OG = OT > 1 ? 2 : 1, CG = 8 / OG, OTN = OT / OG, CTN = CB * 8 / CG;   // dw: groups of planes and channels, tiles of a wave
     constexpr bool LEAN = G::LEAN, WLDS = G::WLDS;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int Cp = (a.C + 31) / 32 * 32, ldc = Cp + L::EP, pieces = Cp / L::EP;
-    const Smem<DT, OT, CB, G::HBUF, WLDS> m(smem, a, Cp, L::z_bytes + (LEAN && a.counts ? WAVES * G::own : 0));
+    constexpr int Cp = L::CP, ldc = L::LDC;
+    const Smem<DT, OT, CB, G::HBUF, WLDS> m(smem, a, L::z_bytes + (LEAN && a.counts ? WAVES * G::own : 0));
     T* zhi = (T*)m.t;
     T* zlo = zhi + ROWS * L::LDO;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, rt = wave & 3, half = wave >> 2;
@@ -600,31 +624,29 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
     for (int j = 0; j < OTH; ++j) db[j] = az_f4{0.f, 0.f, 0.f, 0.f};
     Step st(a, s_lo);
     Feat<DT, NP, MODE> f;
-    f.load(a, st, pieces, tid);
-    BoardLoads nextb;
-    nextb.load(a, m.b, st.b0, tid);
+    f.load(a, st, tid);
     for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
     init_words(a, m.b, tid);
     // this wave's shares of w: rows of its planes for the logits, columns of its channels for dh
     az_i4 wr[LEAN ? OTH : 1][LEAN ? KT : 1], wc[LEAN ? CB * 2 : 1][LEAN ? KO : 1];
-    if constexpr (WLDS) stage_w<DT, OT>(a, m.w, Cp, tid);
+    if constexpr (WLDS) stage_w<DT, OT, CB>(a, m.w, tid);
     if constexpr (LEAN) {
         // through the features' and dz' room
         unsigned char* w = m.h;
-        static_assert(L::OP * (128 + L::EP) * L::SZ <= 2 * ROWS * (128 + L::EP) * L::SZ, "w fits where the two feature buffers lie");
-        stage_w<DT, OT>(a, w, Cp, tid);
+        static_assert(L::w_bytes <= 2 * L::h_bytes, "w fits where the two feature buffers lie");
+        stage_w<DT, OT, CB>(a, w, tid);
         __syncthreads();
         #pragma unroll
         for (int j = 0; j < OTH; ++j)
             #pragma unroll
             for (int k = 0; k < KT; ++k) {
                 const int ot = min(half * OTH + j, OT - 1);
-                wr[j][k] = k * L::KS < Cp ? az_row_frag<DT>(w, ldc, ot * 16, k * L::KS, lane) : az_i4{0, 0, 0, 0};
+                wr[j][k] = az_row_frag<DT>(w, ldc, ot * 16, k * L::KS, lane);
             }
         #pragma unroll
         for (int j = 0; j < CB * 2; ++j)
             #pragma unroll
-            for (int k = 0; k < KO; ++k) wc[j][k] = (cq + 4 * j) * 16 < Cp ? az_col_frag<DT>(w, ldc, k * L::KS, (cq + 4 * j) * 16, lane) : az_i4{0, 0, 0, 0};
+            for (int k = 0; k < KO; ++k) wc[j][k] = az_col_frag<DT>(w, ldc, k * L::KS, (cq + 4 * j) * 16, lane);
         __syncthreads();
     }
     if (a.C < Cp) for (int i = tid; i < G::HBUF * ROWS * ldc; i += NT) ((T*)m.h)[i] = (T)0.f;
@@ -649,20 +671,33 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
     }
     __syncthreads();
     T* h = (T*)m.h;
-    f.store(a, st, h, Cp, pieces, tid);
-    nextb.store(a, m.b, st.b0, tid);                                 // (ends in a barrier)
+    f.store(a, st, h, tid);
+    stage_boards<true>(a, m.b, st.b0, tid);                          // (ends in a barrier)
+    // dense targets of a step, on their way during the step before, ahead of the features (loads return in order)
+    az_f4 tv[OTH];
+    const auto targets = [&](const PolicyDev& a, const Step& st) __attribute__((always_inline)) {
+        const int row = min(rt * 16 + (lane & 15), st.rows - 1), bb = a.nb > 1 ? (int)((unsigned)row * a.mag_s >> 16) : 0, s = st.cell0 + row - bb * a.S;
+        const float* dense = a.dense + (size_t)st.b0 * a.O * a.S;
+        const int at = (bb * a.O + half * OTH * 16 + q * 4) * a.S + s, last = ((bb + 1) * a.O - 1) * a.S + s;
+        #pragma unroll
+        for (int j = 0; j < OTH; ++j)
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) tv[j][i] = dense[min(at + (j * 16 + i) * a.S, last)];   // (dropped where no action stands for it)
+    };
+    if (!a.counts) targets(a, st);
     Step nx = st;
-    if (s_lo + 1 < s_hi) { nx.next(a); f.load(a, nx, pieces, tid); }
+    if (s_lo + 1 < s_hi) { nx.next(a); f.load(a, nx, tid); }
+    #pragma unroll 1
     for (int it = s_lo; it < s_hi; ++it) {
+        const PolicyDev a = arguments();
         // dz of the step
         const int rl = rt * 16 + (lane & 15);
         const bool live = rl < st.rows;
         const int bb = live && a.nb > 1 ? (int)((unsigned)rl * a.mag_s >> 16) : 0, b = st.b0 + bb, s = live ? st.cell0 + rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
         const unsigned bit = live ? 1u << (s - y * a.N) : 0u;
         const unsigned* words = m.b.words + (bb * a.N + y) * (OT * 16) + half * OTH * 16 + q * 4;
-        const az_f4 bst = a.stats[b];
-        const float rs = up * (a.scale * (a.row_scale ? a.row_scale[b] : 1.f));
-        az_f4 tv[OTH];
+        const az_f4 bst = m.b.stat[bb];                              // {lse, r T, r, is there a target that is not allowed}
+        const float rs = up * bst[2];
         if (a.counts) {
             if constexpr (LEAN) {                                    // the wave's own rows and planes, by itself
                 #pragma unroll
@@ -680,13 +715,6 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                 for (int j = 0; j < OTH; ++j) tv[j] = half * OTH + j < OT ? *(const az_f4*)(t + (lane & 15) * L::LDT + (half * OTH + j) * 16 + q * 4) : az_f4{0.f, 0.f, 0.f, 0.f};
                 __syncthreads();
             }
-        } else {
-            const float* dense = a.dense + (size_t)st.b0 * a.O * a.S;
-            const int at = (bb * a.O + half * OTH * 16 + q * 4) * a.S + s, last = ((bb + 1) * a.O - 1) * a.S + s;
-            #pragma unroll
-            for (int j = 0; j < OTH; ++j)
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) tv[j][i] = dense[min(at + (j * 16 + i) * a.S, last)];   // (dropped below where no action stands for it)
         }
         az_f4 acc[OTH];
         #pragma unroll
@@ -706,9 +734,9 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             }
         };
         product<KT, L::KS, OTH, !LEAN && !WLDS>(a.C, fetch, step);
-        const float rT = rs * bst[1], lse2 = bst[0] * LOG2E;
+        const float rT = up * bst[1], lse2 = bst[0] * LOG2E;
         // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
-        const bool bias_counts = a.O > 1 || bst[2] != 0.f;
+        const bool bias_counts = a.O > 1 || bst[3] != 0.f;
         #pragma unroll
         for (int j = 0; j < OTH; ++j) {
             const int ot = half * OTH + j;
@@ -736,11 +764,12 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         const T* hcur = h;
         if constexpr (LEAN) {                                        // the next step's features into the other buffer, the one after it on its way
             h = (T*)m.h + ((it + 1 - s_lo) & 1) * ROWS * ldc;
-            if (it + 1 < s_hi) f.store(a, nx, h, Cp, pieces, tid);
+            if (it + 1 < s_hi) f.store(a, nx, h, tid);
         }
         Step after = nx;
         if (it + 2 < s_hi) after.next(a);
-        if constexpr (LEAN) if (it + 2 < s_hi) f.load(a, after, pieces, tid);
+        if (!a.counts && it + 1 < s_hi) targets(a, nx);
+        if constexpr (LEAN) if (it + 2 < s_hi) f.load(a, after, tid);
         // dh: rows of a tile are channels, columns are cells
         {
             az_i4 zf[2][KO];
@@ -751,7 +780,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             #pragma unroll
             for (int j = 0; j < CB * 2; ++j) {
                 const int ct = cq + 4 * j;
-                if (ct * 16 >= Cp) continue;
+                if (ct * 16 >= a.C) continue;
                 az_f4 d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
                 #pragma unroll
                 for (int k = 0; k < KO; ++k) {
@@ -796,7 +825,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             #pragma unroll
             for (int i = 0; i < CTN; ++i) {
                 const int ct = cg + CG * i;
-                if (ct * 16 >= Cp) continue;
+                if (ct * 16 >= a.C) continue;
                 const az_i4 hb = az_col_frag<DT>(hcur, ldc, k, ct * 16, lane);
                 #pragma unroll
                 for (int j = 0; j < OTN; ++j) {
@@ -808,14 +837,11 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         __syncthreads();                                             // everything of this step has been read
         if constexpr (!LEAN)
             if (it + 1 < s_hi) {
-                f.store(a, nx, h, Cp, pieces, tid);
-                if (it + 2 < s_hi) f.load(a, after, pieces, tid);
+                f.store(a, nx, h, tid);
+                if (it + 2 < s_hi) f.load(a, after, tid);
                 if (nx.b0 == st.b0) __syncthreads();                 // (else the boards' staging ends in one)
             }
-        if (it + 1 < s_hi && nx.b0 != st.b0) {
-            nextb.load(a, m.b, nx.b0, tid);
-            nextb.store(a, m.b, nx.b0, tid);
-        }
+        if (it + 1 < s_hi && nx.b0 != st.b0) stage_boards<true>(a, m.b, nx.b0, tid);
         st = nx;
         nx = after;
     }
@@ -847,10 +873,9 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
 }
 
 template <int DT, int OT, int CB, int MODE> hipError_t launch_products(const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
-    const int Cp = (a.C + 31) / 32 * 32;
     typedef GradCfg<DT, OT, CB> G;
-    const size_t lds = grad ? Smem<DT, OT, CB, G::HBUF, G::WLDS>::bytes(a, Cp, G::zb(a))
-                            : Smem<DT, OT, CB, 0, w_in_lds<DT, OT, CB>()>::bytes(a, Cp, a.counts ? WAVES * LossTile<OT>::bytes : 0);
+    const size_t lds = grad ? Smem<DT, OT, CB, G::HBUF, G::WLDS>::bytes(a, G::zb(a))
+                            : Smem<DT, OT, CB, 0, w_in_lds<DT, OT, CB>()>::bytes(a, a.counts ? WAVES * LossTile<OT>::bytes : 0);
     const void* fn = grad ? (const void*)az_policy_grad_kernel<DT, OT, CB, MODE> : (const void*)az_policy_loss_kernel<DT, OT, CB, MODE>;
     if (lds > 32 * 1024) {
         const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

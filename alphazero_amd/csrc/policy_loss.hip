@@ -131,7 +131,7 @@ extern "C" int az_policy_loss_dev(const az_policy_loss_args* p, void* workspace,
     const int groups = groups_of(a.steps);
     hipError_t e = hipSuccess;
     if (a.B > 0 && pads) {
-        az_policy_pad_weight_kernel<<<64, 256, 0, st>>>((const float*)p->weight, pad, pad + PAD_BYTES / 4, a.O, a.C, a.O <= 64 ? 64 : a.O <= 96 ? 96 : 128, (a.C + 31) / 32 * 32);
+        az_policy_pad_weight_kernel<<<64, 256, 0, st>>>((const float*)p->weight, pad, pad + PAD_BYTES / 4, a.O, a.C, a.O <= 64 ? 64 : a.O <= 96 ? 96 : 128, 256);
         e = hipGetLastError();
     }
     if (e == hipSuccess && a.B > 0 && !p->stats_given) {
