@@ -1,4 +1,4 @@
 // policy_f32.hip -- policy_kernels.h for one element type
 #include "policy_kernels.h"
 
-hipError_t az_policy_launch_f32(const PolicyDev& a, bool grad, int groups, hipStream_t stream) { return launch_o<0>(a, grad, groups, stream); }
+hipError_t az_policy_launch_f32(const PolicyDev& a, bool grad, int& groups, hipStream_t stream) { return launch_o<0>(a, grad, groups, stream); }

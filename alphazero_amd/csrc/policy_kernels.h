@@ -312,10 +312,11 @@ template <int KT, int KS, int W, bool AHEAD, class F, class S> __device__ __forc
         fetch(0, w[0]);
         #pragma unroll
         for (int k = 0; k < KT; ++k) {
-            if (k * KS >= C) break;
-            if (k + 1 < KT) fetch(k + 1, w[(k + 1) & 1]);            // (the padded copy is as wide as the kernel)
-            step(k, w[k & 1]);
-            __builtin_amdgcn_sched_barrier(0);
+            if (k * KS < C) {
+                if (k + 1 < KT) fetch(k + 1, w[(k + 1) & 1]);        // (the padded copy is as wide as the kernel)
+                step(k, w[k & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     } else if (C > (KT - 1) * KS) {
         #pragma unroll
@@ -505,13 +506,13 @@ struct Step {
 
 // The 16-byte pieces of a step's features that a thread carries from memory to LDS.  WHOLE_LAST: consecutive threads take
 // consecutive pieces of a row; otherwise a wave takes one piece of all 64 rows.
-template <int DT, int NP, int MODE> struct Feat {
-    static constexpr int pieces = NP * NT / ROWS, LDC = pieces * AzElem<DT>::EP + AzElem<DT>::EP;
+template <int DT, int NP, int MODE, int NW = WAVES> struct Feat {                // NW: waves that take part
+    static constexpr int pieces = NP * NW, LDC = pieces * AzElem<DT>::EP + AzElem<DT>::EP;
     az_i4 v[NP];
     __device__ __forceinline__ void place(int i, int tid, int& row, int& p) const {
-        const int k = tid + i * NT;
+        const int k = tid + i * NW * 64;
         if constexpr (MODE == WHOLE_LAST) { row = k / pieces; p = k - row * pieces; }
-        else { row = tid & (ROWS - 1); p = __builtin_amdgcn_readfirstlane(tid / ROWS) + i * WAVES; }
+        else { row = tid & (ROWS - 1); p = __builtin_amdgcn_readfirstlane(tid / ROWS) + i * NW; }
     }
     __device__ __forceinline__ void load(const PolicyDev& a, const Step& st, int tid) {
         constexpr int EP = AzElem<DT>::EP;
@@ -584,34 +585,19 @@ template <int LD> __device__ __forceinline__ void scatter_targets(const PolicyDe
 // channels a wave, kept in registers over all of a workgroup's steps).  16-bit features: dz goes to LDS as hi + lo of the
 // type, hi alone feeds dh (whose result is rounded to that type anyway), both feed dw (an fp32 sum over all rows: one
 // rounding to 16 bits of each term would stay in it).
-//
-// The LDS port bounds the step (128 bytes a cycle for operands that the matrix units eat at 1 KB per 16 cycles and SIMD),
-// so 16-bit kernels of up to 128 channels (LEAN) hold their shares of w in registers in both roles, 72 of a wave's 256
-// for 96 planes; the room that leaves in LDS takes a second buffer of features and each wave's own targets, and a step
-// has two barriers instead of five.
-template <int DT, int OT, int CB> struct GradCfg {
+// (16-bit features of up to 128 channels and 96 planes have a kernel of their own below.)
+template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT, 2) az_policy_grad_kernel(PolicyDev a) {
     typedef Lay<DT, OT, CB> L;
-    static constexpr bool LEAN = DT != 0 && CB == 1;
-    static constexpr bool WLDS = !LEAN && w_in_lds<DT, OT, CB>();
-    static constexpr int OTH = (OT + 1) / 2, HBUF = LEAN ? 2 : 1, LDP = OTH * 16 + 4;   // LDP: a wave's own targets [16][LDP]
-    static constexpr size_t own = (size_t)16 * LDP * 4;
-    static constexpr int WAVES_EU = LEAN && OT <= 2 ? 4 : 2;
-    static size_t zb(const PolicyDev& a) { return L::z_bytes + (LEAN && a.counts ? WAVES * own : 0); }
-};
-template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT, (GradCfg<DT, OT, CB>::WAVES_EU)) az_policy_grad_kernel(PolicyDev a) {
-    typedef Lay<DT, OT, CB> L;
-    typedef GradCfg<DT, OT, CB> G;
     typedef typename AzElem<DT>::T T;
-    constexpr int NP = CB * 128 / L::EP * ROWS / NT, OTH = G::OTH, KO = L::OP / L::KS, KT = CB * 128 / L::KS;
+    constexpr int NP = CB * 128 / L::EP * ROWS / NT, OTH = (OT + 1) / 2, KO = L::OP / L::KS, KT = CB * 128 / L::KS;
     constexpr int OG = OT > 1 ? 2 : 1, CG = 8 / OG, OTN = OT / OG, CTN = CB * 8 / CG;   // dw: groups of planes and channels, tiles of a wave
-    constexpr bool LEAN = G::LEAN, WLDS = G::WLDS;
+    constexpr bool WLDS = w_in_lds<DT, OT, CB>();
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr int Cp = L::CP, ldc = L::LDC;
-    const Smem<DT, OT, CB, G::HBUF, WLDS> m(smem, a, L::z_bytes + (LEAN && a.counts ? WAVES * G::own : 0));
+    const Smem<DT, OT, CB, 1, WLDS> m(smem, a, L::z_bytes);
     T* zhi = (T*)m.t;
     T* zlo = zhi + ROWS * L::LDO;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, rt = wave & 3, half = wave >> 2;
-    float* own = (float*)((unsigned char*)m.t + L::z_bytes + wave * G::own);
     const int s_lo = (int)((long long)blockIdx.x * a.steps / gridDim.x), s_hi = (int)((long long)(blockIdx.x + 1) * a.steps / gridDim.x);
     const int og = OG == 2 ? wave & 1 : 0, cg = OG == 2 ? wave >> 1 : wave, pair = wave & 1, cq = wave >> 1;
     az_f4 dw[CTN][OTN];
@@ -627,29 +613,8 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
     f.load(a, st, tid);
     for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
     init_words(a, m.b, tid);
-    // this wave's shares of w: rows of its planes for the logits, columns of its channels for dh
-    az_i4 wr[LEAN ? OTH : 1][LEAN ? KT : 1], wc[LEAN ? CB * 2 : 1][LEAN ? KO : 1];
     if constexpr (WLDS) stage_w<DT, OT, CB>(a, m.w, tid);
-    if constexpr (LEAN) {
-        // through the features' and dz' room
-        unsigned char* w = m.h;
-        static_assert(L::w_bytes <= 2 * L::h_bytes, "w fits where the two feature buffers lie");
-        stage_w<DT, OT, CB>(a, w, tid);
-        __syncthreads();
-        #pragma unroll
-        for (int j = 0; j < OTH; ++j)
-            #pragma unroll
-            for (int k = 0; k < KT; ++k) {
-                const int ot = min(half * OTH + j, OT - 1);
-                wr[j][k] = az_row_frag<DT>(w, ldc, ot * 16, k * L::KS, lane);
-            }
-        #pragma unroll
-        for (int j = 0; j < CB * 2; ++j)
-            #pragma unroll
-            for (int k = 0; k < KO; ++k) wc[j][k] = az_col_frag<DT>(w, ldc, k * L::KS, (cq + 4 * j) * 16, lane);
-        __syncthreads();
-    }
-    if (a.C < Cp) for (int i = tid; i < G::HBUF * ROWS * ldc; i += NT) ((T*)m.h)[i] = (T)0.f;
+    if (a.C < Cp) for (int i = tid; i < ROWS * ldc; i += NT) ((T*)m.h)[i] = (T)0.f;
     // fp16: dz is r_b (a mean over the batch: 1 / B) times probabilities that may be 1e-5, below what fp16 resolves.  The
     // workgroup's dz carry a power of two that puts the largest r_b T_b of its boards at 2^9 .. 2^10; it comes off the
     // fp32 sums again.
@@ -693,28 +658,19 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         // dz of the step
         const int rl = rt * 16 + (lane & 15);
         const bool live = rl < st.rows;
-        const int bb = live && a.nb > 1 ? (int)((unsigned)rl * a.mag_s >> 16) : 0, b = st.b0 + bb, s = live ? st.cell0 + rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
+        const int bb = live && a.nb > 1 ? (int)((unsigned)rl * a.mag_s >> 16) : 0, s = live ? st.cell0 + rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
         const unsigned bit = live ? 1u << (s - y * a.N) : 0u;
         const unsigned* words = m.b.words + (bb * a.N + y) * (OT * 16) + half * OTH * 16 + q * 4;
         const az_f4 bst = m.b.stat[bb];                              // {lse, r T, r, is there a target that is not allowed}
         const float rs = up * bst[2];
         if (a.counts) {
-            if constexpr (LEAN) {                                    // the wave's own rows and planes, by itself
-                #pragma unroll
-                for (int i = 0; i < (int)(G::own / 16 + 63) / 64; ++i)
-                    if (i * 64 + lane < (int)(G::own / 16)) ((az_f4*)own)[i * 64 + lane] = az_f4{0.f, 0.f, 0.f, 0.f};
-                scatter_targets<G::LDP>(a, m.b, own, st, rt, half * OTH * 16, OTH * 16, lane);
-                #pragma unroll
-                for (int j = 0; j < OTH; ++j) tv[j] = *(const az_f4*)(own + (lane & 15) * G::LDP + j * 16 + q * 4);
-            } else {
-                float* t = m.t + rt * 16 * L::LDT;                   // where dz will lie: the waves clear and read it together
-                for (int i = tid; i < ROWS * L::LDT / 4; i += NT) ((az_f4*)m.t)[i] = az_f4{0.f, 0.f, 0.f, 0.f};
-                __syncthreads();
-                scatter_targets<L::LDT>(a, m.b, t + half * OTH * 16, st, rt, half * OTH * 16, OTH * 16, lane);
-                #pragma unroll
-                for (int j = 0; j < OTH; ++j) tv[j] = half * OTH + j < OT ? *(const az_f4*)(t + (lane & 15) * L::LDT + (half * OTH + j) * 16 + q * 4) : az_f4{0.f, 0.f, 0.f, 0.f};
-                __syncthreads();
-            }
+            float* t = m.t + rt * 16 * L::LDT;                   // where dz will lie: the waves clear and read it together
+            for (int i = tid; i < ROWS * L::LDT / 4; i += NT) ((az_f4*)m.t)[i] = az_f4{0.f, 0.f, 0.f, 0.f};
+            __syncthreads();
+            scatter_targets<L::LDT>(a, m.b, t + half * OTH * 16, st, rt, half * OTH * 16, OTH * 16, lane);
+            #pragma unroll
+            for (int j = 0; j < OTH; ++j) tv[j] = half * OTH + j < OT ? *(const az_f4*)(t + (lane & 15) * L::LDT + (half * OTH + j) * 16 + q * 4) : az_f4{0.f, 0.f, 0.f, 0.f};
+            __syncthreads();
         }
         az_f4 acc[OTH];
         #pragma unroll
@@ -728,12 +684,11 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             #pragma unroll
             for (int j = 0; j < OTH; ++j) {
                 const int ot = min(half * OTH + j, OT - 1);
-                if constexpr (LEAN) w[j] = wr[j][k];
-                else if constexpr (WLDS) w[j] = az_row_frag<DT>(m.w, ldc, ot * 16, k * L::KS, lane);
+                if constexpr (WLDS) w[j] = az_row_frag<DT>(m.w, ldc, ot * 16, k * L::KS, lane);
                 else w[j] = az_row_frag<DT>(a.wpad, Cp, ot * 16, k * L::KS, lane);
             }
         };
-        product<KT, L::KS, OTH, !LEAN && !WLDS>(a.C, fetch, step);
+        product<KT, L::KS, OTH, !WLDS>(a.C, fetch, step);
         const float rT = up * bst[1], lse2 = bst[0] * LOG2E;
         // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
         const bool bias_counts = a.O > 1 || bst[3] != 0.f;
@@ -761,15 +716,9 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             }
         }
         __syncthreads();
-        const T* hcur = h;
-        if constexpr (LEAN) {                                        // the next step's features into the other buffer, the one after it on its way
-            h = (T*)m.h + ((it + 1 - s_lo) & 1) * ROWS * ldc;
-            if (it + 1 < s_hi) f.store(a, nx, h, tid);
-        }
         Step after = nx;
         if (it + 2 < s_hi) after.next(a);
         if (!a.counts && it + 1 < s_hi) targets(a, nx);
-        if constexpr (LEAN) if (it + 2 < s_hi) f.load(a, after, tid);
         // dh: rows of a tile are channels, columns are cells
         {
             az_i4 zf[2][KO];
@@ -785,8 +734,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                 #pragma unroll
                 for (int k = 0; k < KO; ++k) {
                     az_i4 wa;
-                    if constexpr (LEAN) wa = wc[j][k];
-                    else if constexpr (WLDS) wa = az_col_frag<DT>(m.w, ldc, k * L::KS, ct * 16, lane);
+                    if constexpr (WLDS) wa = az_col_frag<DT>(m.w, ldc, k * L::KS, ct * 16, lane);
                     else wa = az_row_frag<DT>(a.wpadt, L::OP, ct * 16, k * L::KS, lane);
                     d[0] = az_mma<DT>(wa, zf[0][k], d[0]);
                     d[1] = az_mma<DT>(wa, zf[1][k], d[1]);
@@ -826,7 +774,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             for (int i = 0; i < CTN; ++i) {
                 const int ct = cg + CG * i;
                 if (ct * 16 >= a.C) continue;
-                const az_i4 hb = az_col_frag<DT>(hcur, ldc, k, ct * 16, lane);
+                const az_i4 hb = az_col_frag<DT>(h, ldc, k, ct * 16, lane);
                 #pragma unroll
                 for (int j = 0; j < OTN; ++j) {
                     dw[i][j] = az_mma<DT>(zf[j][0], hb, dw[i][j]);
@@ -835,12 +783,11 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             }
         }
         __syncthreads();                                             // everything of this step has been read
-        if constexpr (!LEAN)
-            if (it + 1 < s_hi) {
-                f.store(a, nx, h, tid);
-                if (it + 2 < s_hi) f.load(a, after, tid);
-                if (nx.b0 == st.b0) __syncthreads();                 // (else the boards' staging ends in one)
-            }
+        if (it + 1 < s_hi) {
+            f.store(a, nx, h, tid);
+            if (it + 2 < s_hi) f.load(a, after, tid);
+            if (nx.b0 == st.b0) __syncthreads();                     // (else the boards' staging ends in one)
+        }
         if (it + 1 < s_hi && nx.b0 != st.b0) stage_boards<true>(a, m.b, nx.b0, tid);
         st = nx;
         nx = after;
@@ -872,32 +819,285 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
     for (int o = tid; o < a.O; o += NT) out[(size_t)a.O * a.C + o] = ((red[o] + red[OT * 16 + o]) + (red[2 * OT * 16 + o] + red[3 * OT * 16 + o])) * down;
 }
 
-template <int DT, int OT, int CB, int MODE> hipError_t launch_products(const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
-    typedef GradCfg<DT, OT, CB> G;
-    const size_t lds = grad ? Smem<DT, OT, CB, G::HBUF, G::WLDS>::bytes(a, G::zb(a))
-                            : Smem<DT, OT, CB, 0, w_in_lds<DT, OT, CB>()>::bytes(a, a.counts ? WAVES * LossTile<OT>::bytes : 0);
-    const void* fn = grad ? (const void*)az_policy_grad_kernel<DT, OT, CB, MODE> : (const void*)az_policy_loss_kernel<DT, OT, CB, MODE>;
+// Gradients, 16-bit features of up to 128 channels and 96 planes.  Four waves make dz of step t (a row tile each, all planes: mostly
+// vector instructions) while the other four multiply dz of step t - 1 both ways (mostly matrix instructions), one of
+// either kind on each SIMD, one barrier a step; each kind holds its shares of w in registers.  Done by the same waves one
+// after the other, neither the vector nor the matrix pipes nor the LDS port were busy half of the time.  LDS: features of
+// three steps, dz (hi and lo) of two, the sparse targets of each row tile.
+template <int DT, int OT> struct PairCfg {
+    typedef Lay<DT, OT, 1> L;
+    static constexpr int LDP = OT * 16 + 4;
+    static constexpr size_t own = (size_t)16 * LDP * 4, z = (size_t)2 * ROWS * L::LDO * 2;    // a row tile's targets; a step's dz
+    static size_t zb(const PolicyDev& a) { return 2 * z + (a.counts ? 4 * own : 0); }
+};
+template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT <= 2 ? 4 : 2) az_policy_grad16_kernel(PolicyDev a) {
+    typedef Lay<DT, OT, 1> L;
+    typedef PairCfg<DT, OT> G;
+    typedef typename AzElem<DT>::T T;
+    constexpr int KT = 128 / L::KS, KO = L::OP / L::KS, ldc = L::LDC;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const Smem<DT, OT, 1, 3, false> m(smem, a, 2 * G::z + (a.counts ? 4 * G::own : 0));
+    T* const hbuf = (T*)m.h;
+    T* const zbuf = (T*)m.t;                                         // [2][hi, lo][ROWS][LDO]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
+    const int s_lo = (int)((long long)blockIdx.x * a.steps / gridDim.x), steps = (int)((long long)(blockIdx.x + 1) * a.steps / gridDim.x) - s_lo;
+    Step st(a, s_lo);
+    for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
+    init_words(a, m.b, tid);
+    // fp16: dz is r_b (a mean over the batch: 1 / B) times probabilities that may be 1e-5, below what fp16 resolves.  The
+    // workgroup's dz carry a power of two that puts the largest r_b T_b of its boards at 2^9 .. 2^10; it comes off the
+    // fp32 sums again.
+    float up = 1.f, down = 1.f;
+    if constexpr (DT == 1) {
+        const Step last(a, s_lo + steps - 1);
+        const int b1 = min(last.b0 + a.nb, a.B);
+        float mx = 0.f;
+        for (int b = st.b0 + tid; b < b1; b += NT) mx = fmaxf(mx, fabsf(a.scale * (a.row_scale ? a.row_scale[b] : 1.f) * a.stats[b][1]));
+        mx = wave_max(mx);
+        if (lane == 0) m.t[wave] = mx;
+        __syncthreads();
+        for (int w = 0; w < 8; ++w) mx = fmaxf(mx, m.t[w]);
+        if (mx > 0.f && mx < INFINITY) {
+            const int e = min(max(10 - (ilogbf(mx) + 1), -100), 100);
+            up = ldexpf(1.f, e);
+            down = ldexpf(1.f, -e);
+        }
+    }
+    static_assert(L::w_bytes <= 3 * L::h_bytes, "w passes through the features' room");
+    stage_w<DT, OT, 1>(a, m.h, tid);
+    __syncthreads();
+    float* const out = a.partial + (size_t)blockIdx.x * ((size_t)a.O * a.C + a.O);
+    if (wave < 4) {
+        az_i4 wr[OT][KT];
+        #pragma unroll
+        for (int j = 0; j < OT; ++j)
+            #pragma unroll
+            for (int k = 0; k < KT; ++k) wr[j][k] = az_row_frag<DT>(m.h, ldc, j * 16, k * L::KS, lane);
+        az_f4 db[OT];
+        #pragma unroll
+        for (int j = 0; j < OT; ++j) db[j] = az_f4{0.f, 0.f, 0.f, 0.f};
+        __syncthreads();                                             // w has been read
+        if (a.C < L::CP) for (int i = tid; i < 3 * ROWS * ldc; i += NT / 2) hbuf[i] = (T)0.f;
+        Feat<DT, 4, MODE, 4> f;
+        f.load(a, st, tid);
+        __syncthreads();
+        f.store(a, st, hbuf, tid);
+        stage_boards<true>(a, m.b, st.b0, tid);
+        float* const own = (float*)((unsigned char*)m.t + 2 * G::z + wave * G::own);
+        const int rl = wave * 16 + (lane & 15);
+        // dense targets of a step: asked for during the step before, ahead of the features (loads return in order)
+        az_f4 tv[OT];
+        const auto targets = [&](const PolicyDev& a, const Step& st) __attribute__((always_inline)) {
+            const int row = min(rl, st.rows - 1), bb = a.nb > 1 ? (int)((unsigned)row * a.mag_s >> 16) : 0, s = st.cell0 + row - bb * a.S;
+            const float* dense = a.dense + (size_t)st.b0 * a.O * a.S;
+            const int at = (bb * a.O + q * 4) * a.S + s, last = ((bb + 1) * a.O - 1) * a.S + s;
+            #pragma unroll
+            for (int j = 0; j < OT; ++j)
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) tv[j][i] = dense[min(at + (j * 16 + i) * a.S, last)];   // (dropped where no action stands for it)
+        };
+        if (!a.counts) targets(a, st);
+        Step nx = st;
+        if (steps > 1) { nx.next(a); f.load(a, nx, tid); }
+        #pragma unroll 1
+        for (int t = 0; t < steps; ++t) {
+            const PolicyDev a = arguments();
+            if (t && st.blk == 0) stage_boards<true>(a, m.b, st.b0, tid);    // (the first step's were staged above)
+            if (t + 1 < steps) f.store(a, nx, hbuf + (t + 1) % 3 * ROWS * ldc, tid);
+            Step after = nx;
+            if (t + 2 < steps) after.next(a);
+            const T* h = hbuf + t % 3 * ROWS * ldc;
+            T* const zhi = zbuf + (t & 1) * 2 * ROWS * L::LDO;
+            T* const zlo = zhi + ROWS * L::LDO;
+            const bool live = rl < st.rows;
+            const int bb = live && a.nb > 1 ? (int)((unsigned)rl * a.mag_s >> 16) : 0, s = live ? st.cell0 + rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
+            const unsigned bit = live ? 1u << (s - y * a.N) : 0u;
+            const unsigned* words = m.b.words + (bb * a.N + y) * (OT * 16) + q * 4;
+            const az_f4 bst = m.b.stat[bb];                          // {lse, r T, r, is there a target that is not allowed}
+            if (a.counts) {                                          // the wave's own rows, by itself
+                #pragma unroll
+                for (int i = 0; i < (int)(G::own / 16 + 63) / 64; ++i)
+                    if (i * 64 + lane < (int)(G::own / 16)) ((az_f4*)own)[i * 64 + lane] = az_f4{0.f, 0.f, 0.f, 0.f};
+                scatter_targets<G::LDP>(a, m.b, own, st, wave, 0, OT * 16, lane);
+                #pragma unroll
+                for (int j = 0; j < OT; ++j) tv[j] = *(const az_f4*)(own + (lane & 15) * G::LDP + j * 16 + q * 4);
+            }
+            az_f4 acc[OT];
+            #pragma unroll
+            for (int j = 0; j < OT; ++j) acc[j] = *(const az_f4*)(m.bias + j * 16 + q * 4);
+            #pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                const az_i4 hb = az_row_frag<DT>(h, ldc, wave * 16, k * L::KS, lane);
+                #pragma unroll
+                for (int j = 0; j < OT; ++j) acc[j] = az_mma<DT>(wr[j][k], hb, acc[j]);
+            }
+            const float rs = up * bst[2], rT = up * bst[1], lse2 = bst[0] * LOG2E;
+            // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
+            const bool bias_counts = a.O > 1 || bst[3] != 0.f;
+            #pragma unroll
+            for (int j = 0; j < OT; ++j) {
+                az_f4 dz;
+                const az_i4 w = *(const az_i4*)(words + j * 16);
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float v = rT * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -lse2)) - rs * tv[j][i];
+                    dz[i] = (unsigned)w[i] & bit ? v : 0.f;
+                }
+                if (bias_counts) db[j] += dz;
+                az_s4 hi, lo;
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) { hi[i] = az_to16<DT>(dz[i]); lo[i] = az_to16<DT>(dz[i] - az_from16<DT>(hi[i])); }
+                *(az_s4*)((short*)zhi + rl * L::LDO + j * 16 + q * 4) = hi;
+                *(az_s4*)((short*)zlo + rl * L::LDO + j * 16 + q * 4) = lo;
+            }
+            if constexpr (OT == 1) {                                 // planes 16 .. 31 of the contraction: zero
+                *(az_s4*)((short*)zhi + rl * L::LDO + 16 + q * 4) = az_s4{0, 0, 0, 0};
+                *(az_s4*)((short*)zlo + rl * L::LDO + 16 + q * 4) = az_s4{0, 0, 0, 0};
+            }
+            if (!a.counts && t + 1 < steps) targets(a, nx);
+            if (t + 2 < steps) f.load(a, after, tid);
+            st = nx;
+            nx = after;
+            __syncthreads();
+        }
+        float* const r4 = (float*)(hbuf + steps % 3 * ROWS * ldc);   // (the other waves still read the features of step steps - 1)
+        #pragma unroll
+        for (int j = 0; j < OT; ++j)
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v = db[j][i];
+                for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d, 64);
+                if ((lane & 15) == 0) r4[wave * OT * 16 + j * 16 + q * 4 + i] = v;
+            }
+        __syncthreads();
+        for (int o = tid; o < a.O; o += NT / 2) out[(size_t)a.O * a.C + o] = ((r4[o] + r4[OT * 16 + o]) + (r4[2 * OT * 16 + o] + r4[3 * OT * 16 + o])) * down;
+    } else {
+        const int cq = wave - 4;                                     // channels 16 cq .. and 64 + 16 cq ..
+        az_i4 wc[2][KO];
+        #pragma unroll
+        for (int j = 0; j < 2; ++j)
+            #pragma unroll
+            for (int k = 0; k < KO; ++k) wc[j][k] = az_col_frag<DT>(m.h, ldc, k * L::KS, (cq + 4 * j) * 16, lane);
+        az_f4 dw[2][OT];
+        #pragma unroll
+        for (int i = 0; i < 2; ++i)
+            #pragma unroll
+            for (int j = 0; j < OT; ++j) dw[i][j] = az_f4{0.f, 0.f, 0.f, 0.f};
+        __syncthreads();
+        __syncthreads();
+        stage_boards<true>(a, m.b, st.b0, tid);
+        Step nx = st;
+        if (steps > 1) nx.next(a);
+        __syncthreads();                                             // dz of step 0
+        #pragma unroll 1
+        for (int t = 0; t < steps; ++t) {
+            const PolicyDev a = arguments();
+            Step after = nx;
+            if (t + 2 < steps) after.next(a);
+            if (t + 1 < steps && nx.blk == 0) stage_boards<true>(a, m.b, nx.b0, tid);   // (with the other waves, ahead of their step t + 1)
+            const T* h = hbuf + t % 3 * ROWS * ldc;
+            const T* const zhi = zbuf + (t & 1) * 2 * ROWS * L::LDO;
+            const T* const zlo = zhi + ROWS * L::LDO;
+            // dh: rows of a tile are channels, columns are cells
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (e * 16 >= st.rows) break;
+                az_f4 d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                #pragma unroll
+                for (int k = 0; k < KO; ++k) {
+                    const az_i4 zf = az_row_frag<DT>(zhi, L::LDO, e * 16, k * L::KS, lane);
+                    d[0] = az_mma<DT>(wc[0][k], zf, d[0]);
+                    d[1] = az_mma<DT>(wc[1][k], zf, d[1]);
+                }
+                const int row = e * 16 + (lane & 15);
+                #pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int c = (cq + 4 * j) * 16 + q * 4;
+                    if (row >= st.rows || c >= a.C) continue;
+                    if constexpr (DT == 1) d[j] *= down;
+                    if (MODE == WHOLE_LAST || (MODE == ANY && !a.nchw)) {
+                        T* dst = (T*)a.dh + ((size_t)st.b0 * a.S + st.cell0) * a.C + (row * a.C + c);
+                        if (MODE == WHOLE_LAST || c + 4 <= a.C) *(az_s4_u*)dst = az_s4{az_to16<DT>(d[j][0]), az_to16<DT>(d[j][1]), az_to16<DT>(d[j][2]), az_to16<DT>(d[j][3])};
+                        else for (int i = 0; i < 4; ++i) if (c + i < a.C) az_store<DT>(dst, i, d[j][i]);
+                    } else {
+                        const int b2 = a.nb > 1 ? (int)((unsigned)row * a.mag_s >> 16) : 0, s2 = st.cell0 + row - b2 * a.S;
+                        T* dst = (T*)a.dh + (size_t)st.b0 * a.C * a.S + ((b2 * a.C + c) * a.S + s2);
+                        for (int i = 0; i < 4; ++i) if (MODE == WHOLE_FIRST || c + i < a.C) az_store<DT>(dst, (size_t)i * a.S, d[j][i]);
+                    }
+                }
+            }
+            // dw: rows of a tile are planes, columns are channels, the contraction runs over the step's rows (rows beyond the
+            // step have dz = 0 and features of 0)
+            #pragma unroll
+            for (int k = 0; k < ROWS; k += L::KS) {
+                if (k >= st.rows) break;
+                const az_i4 hb0 = az_col_frag<DT>(h, ldc, k, cq * 16, lane), hb1 = az_col_frag<DT>(h, ldc, k, (cq + 4) * 16, lane);
+                #pragma unroll
+                for (int j = 0; j < OT; ++j) {
+                    const az_i4 z1 = az_col_frag<DT>(zhi, L::LDO, k, j * 16, lane), z2 = az_col_frag<DT>(zlo, L::LDO, k, j * 16, lane);
+                    dw[0][j] = az_mma<DT>(z1, hb0, dw[0][j]);
+                    dw[1][j] = az_mma<DT>(z1, hb1, dw[1][j]);
+                    dw[0][j] = az_mma<DT>(z2, hb0, dw[0][j]);
+                    dw[1][j] = az_mma<DT>(z2, hb1, dw[1][j]);
+                }
+            }
+            st = nx;
+            nx = after;
+            if (t + 1 < steps) __syncthreads();
+        }
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = (cq + 4 * i) * 16 + (lane & 15);
+            #pragma unroll
+            for (int j = 0; j < OT; ++j)
+                #pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int o = j * 16 + q * 4 + e;
+                    if (o < a.O && c < a.C) out[(size_t)o * a.C + c] = dw[i][j][e] * down;
+                }
+        }
+        __syncthreads();
+    }
+}
+
+template <int DT, int OT, int CB, int MODE> hipError_t launch_products(const PolicyDev& a, bool grad, int& groups, hipStream_t stream) {
+    constexpr bool PAIR = DT != 0 && CB == 1 && OT <= 6;              // (more planes: w's shares do not fit the registers)
+    size_t lds;
+    const void* fn;
+    if (!grad) {
+        lds = Smem<DT, OT, CB, 0, w_in_lds<DT, OT, CB>()>::bytes(a, a.counts ? WAVES * LossTile<OT>::bytes : 0);
+        fn = (const void*)az_policy_loss_kernel<DT, OT, CB, MODE>;
+    } else if constexpr (PAIR) {
+        lds = Smem<DT, OT, 1, 3, false>::bytes(a, PairCfg<DT, OT>::zb(a));
+        fn = (const void*)az_policy_grad16_kernel<DT, OT, MODE>;
+    } else {
+        lds = Smem<DT, OT, CB, 1, w_in_lds<DT, OT, CB>()>::bytes(a, Lay<DT, OT, CB>::z_bytes);
+        fn = (const void*)az_policy_grad_kernel<DT, OT, CB, MODE>;
+    }
     if (lds > 32 * 1024) {
         const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    if (grad) az_policy_grad_kernel<DT, OT, CB, MODE><<<groups, NT, lds, stream>>>(a);
-    else {
+    if (!grad) {
         // as many workgroups as the chip holds at once, the boards in even shares
         const int per_cu = loss_waves<DT, OT, CB>() * 4 / WAVES >= 2 && (lds + 4 * ROWS * 16) * 2 <= LDS_BYTES ? 2 : 1;
         const int work = (a.B + a.nb - 1) / a.nb, room = CUS * per_cu, rounds = (work + room - 1) / room;
         az_policy_loss_kernel<DT, OT, CB, MODE><<<(work + rounds - 1) / rounds, NT, lds, stream>>>(a, work);
+    } else {
+        if (lds * 2 > LDS_BYTES && groups > CUS) groups = CUS;       // one workgroup a CU
+        if constexpr (PAIR) az_policy_grad16_kernel<DT, OT, MODE><<<groups, NT, lds, stream>>>(a);
+        else az_policy_grad_kernel<DT, OT, CB, MODE><<<groups, NT, lds, stream>>>(a);
     }
     return hipGetLastError();
 }
-template <int DT, int OT, int CB> hipError_t launch_mode(const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
+template <int DT, int OT, int CB> hipError_t launch_mode(const PolicyDev& a, bool grad, int& groups, hipStream_t stream) {
     if (a.C % AzElem<DT>::KS) return launch_products<DT, OT, CB, ANY>(a, grad, groups, stream);
     return a.nchw ? launch_products<DT, OT, CB, WHOLE_FIRST>(a, grad, groups, stream) : launch_products<DT, OT, CB, WHOLE_LAST>(a, grad, groups, stream);
 }
-template <int DT, int OT> hipError_t launch_c(const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
+template <int DT, int OT> hipError_t launch_c(const PolicyDev& a, bool grad, int& groups, hipStream_t stream) {
     return a.C <= 128 ? launch_mode<DT, OT, 1>(a, grad, groups, stream) : launch_mode<DT, OT, 2>(a, grad, groups, stream);
 }
-template <int DT> hipError_t launch_o(const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
+template <int DT> hipError_t launch_o(const PolicyDev& a, bool grad, int& groups, hipStream_t stream) {
     if (a.O <= 16) return launch_c<DT, 1>(a, grad, groups, stream);
     if (a.O <= 32) return launch_c<DT, 2>(a, grad, groups, stream);
     if (a.O <= 64) return launch_c<DT, 4>(a, grad, groups, stream);

@@ -43,6 +43,6 @@ struct PolicyDev {
 };
 
 // the two product kernels of one element type (policy_f32.hip, policy_f16.hip, policy_bf16.hip)
-hipError_t az_policy_launch_f32(const PolicyDev& a, bool grad, int groups, hipStream_t stream);
-hipError_t az_policy_launch_f16(const PolicyDev& a, bool grad, int groups, hipStream_t stream);
-hipError_t az_policy_launch_bf16(const PolicyDev& a, bool grad, int groups, hipStream_t stream);
+hipError_t az_policy_launch_f32(const PolicyDev& a, bool grad, int& groups, hipStream_t stream);
+hipError_t az_policy_launch_f16(const PolicyDev& a, bool grad, int& groups, hipStream_t stream);
+hipError_t az_policy_launch_bf16(const PolicyDev& a, bool grad, int& groups, hipStream_t stream);

@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(512) az_policy_reduce_kernel(const float* part
     }
 }
 
-hipError_t launch_dt(int dtype, const PolicyDev& a, bool grad, int groups, hipStream_t stream) {
+hipError_t launch_dt(int dtype, const PolicyDev& a, bool grad, int& groups, hipStream_t stream) {
     if (dtype == AZ_F32) return az_policy_launch_f32(a, grad, groups, stream);
     if (dtype == AZ_F16) return az_policy_launch_f16(a, grad, groups, stream);
     return az_policy_launch_bf16(a, grad, groups, stream);
@@ -128,7 +128,7 @@ extern "C" int az_policy_loss_dev(const az_policy_loss_args* p, void* workspace,
     float* pad = (float*)ws;
     if (pads) { a.wpad = pad; a.wpadt = pad + PAD_BYTES / 4; ws += 2 * PAD_BYTES; }
     a.partial = (float*)ws;
-    const int groups = groups_of(a.steps);
+    int groups = groups_of(a.steps);                                 // (the launch may take fewer)
     hipError_t e = hipSuccess;
     if (a.B > 0 && pads) {
         az_policy_pad_weight_kernel<<<64, 256, 0, st>>>((const float*)p->weight, pad, pad + PAD_BYTES / 4, a.O, a.C, a.O <= 64 ? 64 : a.O <= 96 ? 96 : 128, 256);
