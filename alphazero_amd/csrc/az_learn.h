@@ -62,8 +62,10 @@ template <int DT> __device__ __forceinline__ az_i4 az_row_frag(const void* m, in
 }
 // Fragment whose contraction runs down a column: column n0 + l % 16, rows k0 + EP * (l / 16) ..  For 16-bit elements the
 // LDS read transposes: in each group of 16 lanes, lane i's address names 4 elements of row i / 4 and the lane gets
-// column i of the 4 x 16 block.
-template <int DT> __device__ __forceinline__ az_i4 az_col_frag(const void* m, int ld, int k0, int n0, int lane) {
+// column i of the 4 x 16 block.  BANKS: group g of lanes takes rows 4 g .. + 3 and 16 more behind, instead of 8 g .. + 7 --
+// for products both of whose operands are read this way; with rows an odd multiple of 32 bytes apart the 8 rows of a half
+// wave then lie in different banks.
+template <int DT, bool BANKS = false> __device__ __forceinline__ az_i4 az_col_frag(const void* m, int ld, int k0, int n0, int lane) {
     if constexpr (DT == 0) {
         const float* p = (const float*)m + (k0 + 4 * (lane >> 4)) * ld + n0 + (lane & 15);
         az_f4 v;
@@ -71,9 +73,9 @@ template <int DT> __device__ __forceinline__ az_i4 az_col_frag(const void* m, in
         return __builtin_bit_cast(az_i4, v);
     } else {
         typedef __attribute__((address_space(3))) az_s4* lds_s4;
-        const short* p = (const short*)m + (k0 + 8 * (lane >> 4) + ((lane & 15) >> 2)) * ld + n0 + (lane & 3) * 4;
+        const short* p = (const short*)m + (k0 + (BANKS ? 4 : 8) * (lane >> 4) + ((lane & 15) >> 2)) * ld + n0 + (lane & 3) * 4;
         const az_s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p);
-        const az_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 4 * ld));
+        const az_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + (BANKS ? 16 : 4) * ld));
         return __builtin_bit_cast(az_i4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 }

@@ -9,10 +9,10 @@ namespace {
 template <int DT, int OT, int CB> struct Lay {
     static constexpr int EP = AzElem<DT>::EP, KS = AzElem<DT>::KS, SZ = 16 / EP;
     static constexpr int OP = (OT * 16 + KS - 1) / KS * KS;          // planes, padded to a step of the contraction over them
-    static constexpr int LDT = OT * 16 + 4, LDO = OP + EP;
-    // channels are padded to what the kernel is built for (every LDS address is then a base and a constant), rows by 16
-    // bytes more, so that they start in different banks
-    static constexpr int CP = CB * 128, LDC = CP + EP, PIECES = CP / EP;
+    static constexpr int PAD = DT == 0 ? 4 : 16;                     // 16-bit rows: odd multiples of 32 bytes (az_col_frag), fp32: 16 bytes more
+    static constexpr int LDT = OT * 16 + 4, LDO = OP + PAD;
+    // channels are padded to what the kernel is built for: every LDS address is then a base and a constant
+    static constexpr int CP = CB * 128, LDC = CP + PAD, PIECES = CP / EP;
     static constexpr size_t w_bytes = (size_t)OP * LDC * SZ, h_bytes = (size_t)ROWS * LDC * SZ;
     static constexpr size_t z_bytes = (size_t)ROWS * (LDO > LDT ? LDO : LDT) * 4;
 };
@@ -82,14 +82,15 @@ template <int DT, int OT, int CB> __device__ __forceinline__ void stage_w(const 
 }
 
 // What a workgroup's boards need beside the features, brought to LDS when the board changes: the legal-move words as
-// [board, row][plane], and the sparse targets sorted by tile as {row of the boards * 256 + plane, value}.
+// [board, row][plane], and the sparse targets sorted by blocks of 64 rows as {row of the boards * 256 + plane, value}.
+constexpr int BLOCKS = 16;                                           // blocks of 64 rows: boards of 32 x 32
 struct BoardLds {
     unsigned* words;                                                 // bit 0 = no action stands for the entry: a plane beyond the last, or not allowed
     int planes;                                                      // words of a line: the planes, padded to 16
     int* key;
     float* val;
-    int* cnt;                                                        // [64-entry chunk][64 tiles]
-    int* start;                                                      // [65]: a tile's first entry
+    int* cnt;                                                        // [64-entry chunk][BLOCKS]
+    int* start;                                                      // [BLOCKS + 1]: a block's first entry
     az_f4* stat;                                                     // [MAX_BOARDS] of the gradients: {lse, r T, r, is there a target that is not allowed}
     bool listed;                                                     // the entries fit
 };
@@ -114,13 +115,16 @@ __device__ __forceinline__ void init_words(const PolicyDev& a, const BoardLds& l
 }
 
 // One group's words and entries: a thread's first loads go out together.
-struct BoardLoads {
+template <bool GRAD> struct BoardLoads {
     static constexpr int W = 4, E = ENTRIES / NT;
     unsigned w[W];
     int act[E], cnt[E];
     float val[E];
+    az_f4 st;
+    float r;
     __device__ __forceinline__ void load(const PolicyDev& a, const BoardLds& l, int b0, int tid) {
-        const int boards = min(a.nb, a.B - b0);
+        const int boards = min(a.nb, a.B - b0), b = b0 + min(tid, boards - 1);
+        if (GRAD) { st = a.stats[b]; r = a.row_scale ? a.row_scale[b] : 1.f; }
         if (a.legal) {
             const int n = boards * a.O * a.N;
             const unsigned* src = a.legal + (size_t)b0 * a.O * a.N;
@@ -143,12 +147,11 @@ struct BoardLoads {
         l.words[(bb * a.N + y) * l.planes + bo - bb * a.O] = v;
     }
     // every thread; ends in a barrier
-    template <bool GRAD> __device__ __forceinline__ void store(const PolicyDev& a, const BoardLds& l, int b0, int tid) const {
+    __device__ __forceinline__ void store(const PolicyDev& a, const BoardLds& l, int b0, int tid) const {
         const int boards = min(a.nb, a.B - b0), lane = tid & 63, wave = tid >> 6;
         if (GRAD && tid < boards) {
-            const az_f4 st = a.stats[b0 + tid];
-            const float r = a.scale * (a.row_scale ? a.row_scale[b0 + tid] : 1.f);
-            l.stat[tid] = az_f4{st[0], r * st[1], r, st[2]};
+            const float rs = a.scale * r;
+            l.stat[tid] = az_f4{st[0], rs * st[1], rs, st[2]};
         }
         if (a.legal) {
             const int n = boards * a.O * a.N;
@@ -158,8 +161,8 @@ struct BoardLoads {
             for (int i = tid + W * NT; i < n; i += NT) put_word(a, l, i, src[i]);
         }
         if (l.listed) {
-            // a stable counting sort by tile: the entries of a tile keep their order, whatever the waves' timing
-            const int n = boards * a.cap, chunks = (n + 63) / 64, tiles = (boards * a.S + 15) / 16;
+            // a stable counting sort by block: the entries of a block keep their order, whatever the waves' timing
+            const int n = boards * a.cap, chunks = (n + 63) / 64, blocks = (boards * a.S + 63) / 64;
             int key[E], rank[E];
             #pragma unroll
             for (int u = 0; u < E; ++u) {
@@ -167,44 +170,60 @@ struct BoardLoads {
                 const int bb = a.nb > 1 ? min(e, n - 1) / a.cap : 0;
                 key[u] = e < n && e - bb * a.cap < cnt[u] ? entry_key(a, act[u], bb) : -1;
                 if (chunk >= chunks) continue;
-                const int tile = key[u] < 0 ? -1 : key[u] >> 12;
+                const int block = key[u] < 0 ? -1 : key[u] >> 14;
                 int mine = 0;
-                for (int t = 0; t < tiles; ++t) {
-                    const unsigned long long m = __ballot(tile == t);
-                    if (tile == t) rank[u] = __popcll(m & ((1ull << lane) - 1));
+                for (int t = 0; t < blocks; ++t) {
+                    const unsigned long long m = __ballot(block == t);
+                    if (block == t) rank[u] = __popcll(m & ((1ull << lane) - 1));
                     if (lane == t) mine = __popcll(m);
                 }
-                l.cnt[chunk * 64 + lane] = mine;
+                if (lane < BLOCKS) l.cnt[chunk * BLOCKS + lane] = mine;
             }
             __syncthreads();
-            if (wave == 0) {
-                int sum = 0;
-                for (int c = 0; c < chunks; ++c) sum += l.cnt[c * 64 + lane];
-                int incl = sum;
-                for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
-                int at = incl - sum;
-                l.start[lane] = at;
-                if (lane == 63) l.start[64] = incl;
-                for (int c = 0; c < chunks; ++c) { const int k = l.cnt[c * 64 + lane]; l.cnt[c * 64 + lane] = at; at += k; }
+            // lane t of every wave: where block t starts, and within it this wave's chunks
+            int sum = 0, before[E] = {};
+            for (int c = 0; c < chunks; ++c) {
+                const int k = lane < BLOCKS ? l.cnt[c * BLOCKS + lane] : 0;
+                #pragma unroll
+                for (int u = 0; u < E; ++u) before[u] += c < wave + u * WAVES ? k : 0;
+                sum += k;
             }
-            __syncthreads();
+            int incl = sum;
+            for (int d = 1; d < BLOCKS; d <<= 1) { const int o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
+            if (wave == 0 && lane < BLOCKS) { l.start[lane] = incl - sum; if (lane == BLOCKS - 1) l.start[BLOCKS] = incl; }
             #pragma unroll
-            for (int u = 0; u < E; ++u)
+            for (int u = 0; u < E; ++u) {
+                const int at = __shfl(incl - sum + before[u], key[u] < 0 ? 0 : key[u] >> 14, 64) + rank[u];
                 if (key[u] >= 0) {
-                    const int at = l.cnt[(wave + u * WAVES) * 64 + (key[u] >> 12)] + rank[u];
                     l.key[at] = key[u];
                     l.val[at] = val[u];
                 }
+            }
         }
         __syncthreads();
     }
 };
 
 template <bool GRAD> __device__ __forceinline__ void stage_boards(const PolicyDev& a, const BoardLds& l, int b0, int tid) {
-    BoardLoads x;
+    BoardLoads<GRAD> x;
     x.load(a, l, b0, tid);
-    x.store<GRAD>(a, l, b0, tid);
+    x.store(a, l, b0, tid);
 }
+
+// The gradient kernel's boards in turn; the loads of the one to come wait in registers.
+struct BoardQueue {
+    BoardLoads<true> x;
+    // first: any board; next: the one behind, which is on its way
+    __device__ __forceinline__ void first(const PolicyDev& a, const BoardLds& l, int b0, int tid) {
+        x.load(a, l, b0, tid);
+        x.store(a, l, b0, tid);
+        if (b0 + a.nb < a.B) x.load(a, l, b0 + a.nb, tid);
+    }
+    __device__ __forceinline__ void next(const PolicyDev& a, const BoardLds& l, int b0, int tid) {
+        x.store(a, l, b0, tid);
+        if (b0 + a.nb < a.B) x.load(a, l, b0 + a.nb, tid);
+    }
+};
 
 // LDS of the product kernels, in this order; zb: bytes of the kernel's own tile (logits or dz)
 template <int DT, int OT, int CB, int HBUF, bool WBUF> struct Smem {
@@ -224,13 +243,13 @@ template <int DT, int OT, int CB, int HBUF, bool WBUF> struct Smem {
         b.listed = room > 0;
         b.key = (int*)p; p += (size_t)room * 4;
         b.val = (float*)p; p += (size_t)room * 4;
-        b.start = (int*)p; p += 65 * 4;
+        b.start = (int*)p; p += (BLOCKS + 1) * 4;
         b.cnt = (int*)p;
     }
     static size_t bytes(const PolicyDev& a, size_t zb) {
         const size_t room = a.counts ? (size_t)entry_room(a.nb, a.cap) : 0;
         return (WBUF ? L::w_bytes : 0) + HBUF * L::h_bytes + zb + OT * 16 * 4 + MAX_BOARDS * 16 + (size_t)a.nb * a.N * OT * 16 * 4 +
-               (room ? room * 8 + 65 * 4 + (room + 63) / 64 * 256 : 0);
+               (room ? room * 8 + (BLOCKS + 1) * 4 + (room + 63) / 64 * BLOCKS * 4 : 0);
     }
 };
 
@@ -369,7 +388,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             const unsigned bit = live ? 1u << (s - y * a.N) : 0u;
             const unsigned* words = m.b.words + ((live ? bb : 0) * a.N + y) * (OT * 16) + q * 4;
             const float* dense = a.dense + (size_t)b0 * a.O * a.S;
-            const int hi = min(r0 + 16, rows), e0 = m.b.listed ? m.b.start[r0 >> 4] : 0, e1 = m.b.listed ? m.b.start[(r0 >> 4) + 1] : min(a.nb, a.B - b0) * a.cap;
+            const int hi = min(r0 + 16, rows), e0 = m.b.listed ? m.b.start[r0 >> 6] : 0, e1 = m.b.listed ? m.b.start[(r0 >> 6) + 1] : min(a.nb, a.B - b0) * a.cap;
             int key0 = -1;
             float val0 = 0.f;
             if (m.b.listed && e0 + lane < e1) { key0 = m.b.key[e0 + lane]; val0 = m.b.val[e0 + lane]; }
@@ -507,7 +526,7 @@ struct Step {
 // The 16-byte pieces of a step's features that a thread carries from memory to LDS.  WHOLE_LAST: consecutive threads take
 // consecutive pieces of a row; otherwise a wave takes one piece of all 64 rows.
 template <int DT, int NP, int MODE, int NW = WAVES> struct Feat {                // NW: waves that take part
-    static constexpr int pieces = NP * NW, LDC = pieces * AzElem<DT>::EP + AzElem<DT>::EP;
+    static constexpr int pieces = NP * NW, LDC = pieces * AzElem<DT>::EP + (DT == 0 ? 4 : 16);
     az_i4 v[NP];
     __device__ __forceinline__ void place(int i, int tid, int& row, int& p) const {
         const int k = tid + i * NW * 64;
@@ -562,20 +581,25 @@ template <int DT, int NP, int MODE, int NW = WAVES> struct Feat {               
 // The sparse targets of 16 rows (tile rt of the step) and planes o0 .. o0 + n - 1 into t [16][LD], cleared before: one
 // wave, the entries in their order (an LDS add takes a wave's lanes in theirs), so an action that is named more than once
 // is summed in one order.
-template <int LD> __device__ __forceinline__ void scatter_targets(const PolicyDev& a, const BoardLds& l, float* t, const Step& st, int rt, int o0, int n, int lane) {
-    const int row0 = st.cell0 + rt * 16, tile = min(row0 >> 4, 63);
-    const int e0 = l.listed ? l.start[tile] : 0, e1 = l.listed ? l.start[tile + 1] : min(a.nb, a.B - st.b0) * a.cap;
+// key0, val0: the lane's entry of the step's first 64 (e0 ..).
+template <int LD> __device__ __forceinline__ void scatter_targets(const PolicyDev& a, const BoardLds& l, float* t, const Step& st, int rt, int e0, int e1, int key0, float val0, int lane,
+                                                                  int o0 = 0, int n = 128) {
+    const int row0 = st.cell0 + rt * 16;
+    const auto put = [&](int key, float v) __attribute__((always_inline)) {
+        const int o = (key & 255) - o0, row = (key >> 8) - row0;
+        if (key >= 0 && (unsigned)o < (unsigned)n && (unsigned)row < 16u) __hip_atomic_fetch_add(t + row * LD + o, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    };
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    for (int e = e0 + lane; e < e1; e += 64) {
-        int key;
-        float v = 0.f;
-        if (l.listed) { key = l.key[e]; v = l.val[e]; }
-        else key = entry_at(a, st.b0, e, v);
-        const int o = (key & 255) - o0, row = (key >> 8) - row0;
-        if (key >= 0 && (unsigned)o < (unsigned)n && (unsigned)row < 16u)
-            __hip_atomic_fetch_add(t + row * LD + o, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-    }
+    if (l.listed) {
+        put(key0, val0);
+        for (int e = e0 + 64 + lane; e < e1; e += 64) put(l.key[e], l.val[e]);
+    } else
+        for (int e = lane; e < min(a.nb, a.B - st.b0) * a.cap; e += 64) {
+            float v = 0.f;
+            const int key = entry_at(a, st.b0, e, v);
+            put(key, v);
+        }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
@@ -667,7 +691,9 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             float* t = m.t + rt * 16 * L::LDT;                   // where dz will lie: the waves clear and read it together
             for (int i = tid; i < ROWS * L::LDT / 4; i += NT) ((az_f4*)m.t)[i] = az_f4{0.f, 0.f, 0.f, 0.f};
             __syncthreads();
-            scatter_targets<L::LDT>(a, m.b, t + half * OTH * 16, st, rt, half * OTH * 16, OTH * 16, lane);
+            const int e0 = m.b.listed ? m.b.start[st.blk] : 0, e1 = m.b.listed ? m.b.start[st.blk + 1] : 0;
+            const bool first = e0 + lane < e1;
+            scatter_targets<L::LDT>(a, m.b, t + half * OTH * 16, st, rt, e0, e1, first ? m.b.key[e0 + lane] : -1, first ? m.b.val[e0 + lane] : 0.f, lane, half * OTH * 16, OTH * 16);
             #pragma unroll
             for (int j = 0; j < OTH; ++j) tv[j] = half * OTH + j < OT ? *(const az_f4*)(t + (lane & 15) * L::LDT + (half * OTH + j) * 16 + q * 4) : az_f4{0.f, 0.f, 0.f, 0.f};
             __syncthreads();
@@ -726,7 +752,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             for (int k = 0; k < KO; ++k)
                 #pragma unroll
                 for (int e = 0; e < 2; ++e) zf[e][k] = az_row_frag<DT>(zhi, L::LDO, (pair * 2 + e) * 16, k * L::KS, lane);
-            #pragma unroll
+            #pragma unroll 1
             for (int j = 0; j < CB * 2; ++j) {
                 const int ct = cq + 4 * j;
                 if (ct * 16 >= a.C) continue;
@@ -767,14 +793,14 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             az_i4 zf[OTN][DT == 0 ? 1 : 2];
             #pragma unroll
             for (int j = 0; j < OTN; ++j) {
-                zf[j][0] = az_col_frag<DT>(zhi, L::LDO, k, (og * OTN + j) * 16, lane);
-                if constexpr (DT != 0) zf[j][1] = az_col_frag<DT>(zlo, L::LDO, k, (og * OTN + j) * 16, lane);
+                zf[j][0] = az_col_frag<DT, true>(zhi, L::LDO, k, (og * OTN + j) * 16, lane);
+                if constexpr (DT != 0) zf[j][1] = az_col_frag<DT, true>(zlo, L::LDO, k, (og * OTN + j) * 16, lane);
             }
             #pragma unroll
             for (int i = 0; i < CTN; ++i) {
                 const int ct = cg + CG * i;
                 if (ct * 16 >= a.C) continue;
-                const az_i4 hb = az_col_frag<DT>(h, ldc, k, ct * 16, lane);
+                const az_i4 hb = az_col_frag<DT, true>(h, ldc, k, ct * 16, lane);
                 #pragma unroll
                 for (int j = 0; j < OTN; ++j) {
                     dw[i][j] = az_mma<DT>(zf[j][0], hb, dw[i][j]);
@@ -830,7 +856,16 @@ template <int DT, int OT> struct PairCfg {
     static constexpr size_t own = (size_t)16 * LDP * 4, z = (size_t)2 * ROWS * L::LDO * 2;    // a row tile's targets; a step's dz
     static size_t zb(const PolicyDev& a) { return 2 * z + (a.counts ? 4 * own : 0); }
 };
-template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT <= 2 ? 4 : 2) az_policy_grad16_kernel(PolicyDev a) {
+// az_col_frag of 16 columns that are not neighbours: four from n0, four from n0 + 8, ...
+__device__ __forceinline__ az_i4 pair_col_frag(const void* m, int ld, int k0, int n0, int lane) {
+    typedef __attribute__((address_space(3))) az_s4* lds_s4;
+    const short* p = (const short*)m + (k0 + 8 * (lane >> 4) + ((lane & 15) >> 2)) * ld + n0 + (lane & 3) * 8;
+    const az_s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p);
+    const az_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 4 * ld));
+    return __builtin_bit_cast(az_i4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 1 ? 4 : 2) az_policy_grad16_kernel(PolicyDev a) {
     typedef Lay<DT, OT, 1> L;
     typedef PairCfg<DT, OT> G;
     typedef typename AzElem<DT>::T T;
@@ -842,7 +877,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT <= 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
     const int s_lo = (int)((long long)blockIdx.x * a.steps / gridDim.x), steps = (int)((long long)(blockIdx.x + 1) * a.steps / gridDim.x) - s_lo;
     Step st(a, s_lo);
-    for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
+    for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : -INFINITY;   // (planes there are not: dz = 0)
     init_words(a, m.b, tid);
     // fp16: dz is r_b (a mean over the batch: 1 / B) times probabilities that may be 1e-5, below what fp16 resolves.  The
     // workgroup's dz carry a power of two that puts the largest r_b T_b of its boards at 2^9 .. 2^10; it comes off the
@@ -867,6 +902,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT <= 
     stage_w<DT, OT, 1>(a, m.h, tid);
     __syncthreads();
     float* const out = a.partial + (size_t)blockIdx.x * ((size_t)a.O * a.C + a.O);
+    BoardQueue boards;
     if (wave < 4) {
         az_i4 wr[OT][KT];
         #pragma unroll
@@ -878,15 +914,18 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT <= 
         for (int j = 0; j < OT; ++j) db[j] = az_f4{0.f, 0.f, 0.f, 0.f};
         __syncthreads();                                             // w has been read
         if (a.C < L::CP) for (int i = tid; i < 3 * ROWS * ldc; i += NT / 2) hbuf[i] = (T)0.f;
-        Feat<DT, 4, MODE, 4> f;
-        f.load(a, st, tid);
         __syncthreads();
-        f.store(a, st, hbuf, tid);
-        stage_boards<true>(a, m.b, st.b0, tid);
+        boards.first(a, m.b, st.b0, tid);
         float* const own = (float*)((unsigned char*)m.t + 2 * G::z + wave * G::own);
         const int rl = wave * 16 + (lane & 15);
+        const auto clear_own = [&]() __attribute__((always_inline)) {
+            #pragma unroll
+            for (int i = 0; i < (int)(G::own / 16 + 63) / 64; ++i)
+                if (i * 64 + lane < (int)(G::own / 16)) ((az_f4*)own)[i * 64 + lane] = az_f4{0.f, 0.f, 0.f, 0.f};
+        };
+        if (a.counts) clear_own();
         // dense targets of a step: asked for during the step before, ahead of the features (loads return in order)
-        az_f4 tv[OT];
+        az_f4 tv[OT] = {};
         const auto targets = [&](const PolicyDev& a, const Step& st) __attribute__((always_inline)) {
             const int row = min(rl, st.rows - 1), bb = a.nb > 1 ? (int)((unsigned)row * a.mag_s >> 16) : 0, s = st.cell0 + row - bb * a.S;
             const float* dense = a.dense + (size_t)st.b0 * a.O * a.S;
@@ -894,18 +933,19 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT <= 
             #pragma unroll
             for (int j = 0; j < OT; ++j)
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) tv[j][i] = dense[min(at + (j * 16 + i) * a.S, last)];   // (dropped where no action stands for it)
+                for (int i = 0; i < 4; ++i) { const float v = dense[min(at + (j * 16 + i) * a.S, last)]; tv[j][i] = j * 16 + q * 4 + i < a.O ? v : 0.f; }
         };
         if (!a.counts) targets(a, st);
         Step nx = st;
-        if (steps > 1) { nx.next(a); f.load(a, nx, tid); }
+        if (steps > 1) nx.next(a);
         #pragma unroll 1
         for (int t = 0; t < steps; ++t) {
             const PolicyDev a = arguments();
-            if (t && st.blk == 0) stage_boards<true>(a, m.b, st.b0, tid);    // (the first step's were staged above)
-            if (t + 1 < steps) f.store(a, nx, hbuf + (t + 1) % 3 * ROWS * ldc, tid);
-            Step after = nx;
-            if (t + 2 < steps) after.next(a);
+            if (t && st.blk == 0) boards.next(a, m.b, st.b0, tid);
+            const int e0 = m.b.listed ? m.b.start[st.blk] : 0, e1 = m.b.listed ? m.b.start[st.blk + 1] : 0;
+            int key0 = -1;
+            float val0 = 0.f;
+            if (e0 + lane < e1) { key0 = m.b.key[e0 + lane]; val0 = m.b.val[e0 + lane]; }
             const T* h = hbuf + t % 3 * ROWS * ldc;
             T* const zhi = zbuf + (t & 1) * 2 * ROWS * L::LDO;
             T* const zlo = zhi + ROWS * L::LDO;
@@ -914,50 +954,54 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT <= 
             const unsigned bit = live ? 1u << (s - y * a.N) : 0u;
             const unsigned* words = m.b.words + (bb * a.N + y) * (OT * 16) + q * 4;
             const az_f4 bst = m.b.stat[bb];                          // {lse, r T, r, is there a target that is not allowed}
-            if (a.counts) {                                          // the wave's own rows, by itself
-                #pragma unroll
-                for (int i = 0; i < (int)(G::own / 16 + 63) / 64; ++i)
-                    if (i * 64 + lane < (int)(G::own / 16)) ((az_f4*)own)[i * 64 + lane] = az_f4{0.f, 0.f, 0.f, 0.f};
-                scatter_targets<G::LDP>(a, m.b, own, st, wave, 0, OT * 16, lane);
-                #pragma unroll
-                for (int j = 0; j < OT; ++j) tv[j] = *(const az_f4*)(own + (lane & 15) * G::LDP + j * 16 + q * 4);
-            }
-            az_f4 acc[OT];
-            #pragma unroll
-            for (int j = 0; j < OT; ++j) acc[j] = *(const az_f4*)(m.bias + j * 16 + q * 4);
-            #pragma unroll
-            for (int k = 0; k < KT; ++k) {
-                const az_i4 hb = az_row_frag<DT>(h, ldc, wave * 16, k * L::KS, lane);
-                #pragma unroll
-                for (int j = 0; j < OT; ++j) acc[j] = az_mma<DT>(wr[j][k], hb, acc[j]);
-            }
-            const float rs = up * bst[2], rT = up * bst[1], lse2 = bst[0] * LOG2E;
+            if (a.counts) scatter_targets<G::LDP>(a, m.b, own, st, wave, e0, e1, key0, val0, lane);
+            const float rs = live ? up * bst[2] : 0.f, rT = live ? up * bst[1] : 0.f, lse2 = bst[0] * LOG2E;
             // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
             const bool bias_counts = a.O > 1 || bst[3] != 0.f;
+            constexpr int OH = OT > 2 ? OT / 2 : OT;                 // planes in two halves: fewer registers
             #pragma unroll
-            for (int j = 0; j < OT; ++j) {
-                az_f4 dz;
-                const az_i4 w = *(const az_i4*)(words + j * 16);
+            for (int j0 = 0; j0 < OT; j0 += OH) {
+                az_f4 acc[OH];
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float v = rT * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -lse2)) - rs * tv[j][i];
-                    dz[i] = (unsigned)w[i] & bit ? v : 0.f;
+                for (int j = 0; j < OH; ++j) acc[j] = *(const az_f4*)(m.bias + (j0 + j) * 16 + q * 4);
+                #pragma unroll
+                for (int k = 0; k < KT; ++k) {
+                    const az_i4 hb = az_row_frag<DT>(h, ldc, wave * 16, k * L::KS, lane);
+                    #pragma unroll
+                    for (int j = 0; j < OH; ++j) acc[j] = az_mma<DT>(wr[j0 + j][k], hb, acc[j]);
                 }
-                if (bias_counts) db[j] += dz;
-                az_s4 hi, lo;
+                if (a.counts) {
+                    #pragma unroll
+                    for (int j = 0; j < OH; ++j) tv[j0 + j] = *(const az_f4*)(own + (lane & 15) * G::LDP + (j0 + j) * 16 + q * 4);
+                }
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) { hi[i] = az_to16<DT>(dz[i]); lo[i] = az_to16<DT>(dz[i] - az_from16<DT>(hi[i])); }
-                *(az_s4*)((short*)zhi + rl * L::LDO + j * 16 + q * 4) = hi;
-                *(az_s4*)((short*)zlo + rl * L::LDO + j * 16 + q * 4) = lo;
+                for (int j = 0; j < OH; ++j) {
+                    const int o = (j0 + j) * 16 + q * 4;
+                    az_f4 dz;
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) dz[i] = __builtin_fmaf(rT, __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -lse2)), -rs * tv[j0 + j][i]);
+                    if (a.legal) {
+                        const az_i4 w = *(const az_i4*)(words + (j0 + j) * 16);
+                        #pragma unroll
+                        for (int i = 0; i < 4; ++i) dz[i] = (unsigned)w[i] & bit ? dz[i] : 0.f;
+                    }
+                    if (bias_counts) db[j0 + j] += dz;
+                    az_s4 hi, lo;
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) { hi[i] = az_to16<DT>(dz[i]); lo[i] = az_to16<DT>(dz[i] - az_from16<DT>(hi[i])); }
+                    *(az_s4*)((short*)zhi + rl * L::LDO + o) = hi;
+                    *(az_s4*)((short*)zlo + rl * L::LDO + o) = lo;
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (OT == 1) {                                 // planes 16 .. 31 of the contraction: zero
                 *(az_s4*)((short*)zhi + rl * L::LDO + 16 + q * 4) = az_s4{0, 0, 0, 0};
                 *(az_s4*)((short*)zlo + rl * L::LDO + 16 + q * 4) = az_s4{0, 0, 0, 0};
             }
+            if (a.counts) clear_own();
             if (!a.counts && t + 1 < steps) targets(a, nx);
-            if (t + 2 < steps) f.load(a, after, tid);
             st = nx;
-            nx = after;
+            if (t + 2 < steps) nx.next(a);
             __syncthreads();
         }
         float* const r4 = (float*)(hbuf + steps % 3 * ROWS * ldc);   // (the other waves still read the features of step steps - 1)
@@ -972,29 +1016,42 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT <= 
         __syncthreads();
         for (int o = tid; o < a.O; o += NT / 2) out[(size_t)a.O * a.C + o] = ((r4[o] + r4[OT * 16 + o]) + (r4[2 * OT * 16 + o] + r4[3 * OT * 16 + o])) * down;
     } else {
-        const int cq = wave - 4;                                     // channels 16 cq .. and 64 + 16 cq ..
+        const int cq = wave - 4, tb = tid - NT / 2;                  // channels 32 cq .. + 31
         az_i4 wc[2][KO];
         #pragma unroll
         for (int j = 0; j < 2; ++j)
             #pragma unroll
-            for (int k = 0; k < KO; ++k) wc[j][k] = az_col_frag<DT>(m.h, ldc, k * L::KS, (cq + 4 * j) * 16, lane);
+            for (int k = 0; k < KO; ++k) wc[j][k] = pair_col_frag(m.h, ldc, k * L::KS, cq * 32 + 4 * j, lane);
         az_f4 dw[2][OT];
         #pragma unroll
         for (int i = 0; i < 2; ++i)
             #pragma unroll
             for (int j = 0; j < OT; ++j) dw[i][j] = az_f4{0.f, 0.f, 0.f, 0.f};
+        // features: step t + 1 goes to LDS at the start of interval t (in which dz of step t are made and those of step t - 1
+        // multiplied), t + 2 and t + 3 are on their way
+        Feat<DT, 4, MODE, 4> f[2];
+        Step s0 = st, s1 = st, s2 = st;                              // steps t - 1 .. t + 1; s3: t + 2
+        f[0].load(a, st, tb);
+        if (steps > 1) { s1.next(a); f[1].load(a, s1, tb); }
+        s2 = s1;
+        if (steps > 2) s2.next(a);
         __syncthreads();
-        __syncthreads();
-        stage_boards<true>(a, m.b, st.b0, tid);
-        Step nx = st;
-        if (steps > 1) nx.next(a);
+        __syncthreads();                                             // w has been read, the padding cleared
+        f[0].store(a, st, hbuf, tb);
+        if (steps > 2) f[0].load(a, s2, tb);
+        boards.first(a, m.b, st.b0, tid);
+        // interval 0
+        if (steps > 1) f[1].store(a, s1, hbuf + ROWS * ldc, tb);
+        Step s3 = s2;
+        if (steps > 3) { s3.next(a); f[1].load(a, s3, tb); }
         __syncthreads();                                             // dz of step 0
-        #pragma unroll 1
-        for (int t = 0; t < steps; ++t) {
+        const auto interval = [&](int t, Feat<DT, 4, MODE, 4>& f) __attribute__((always_inline)) {   // multiplies step t; interval t + 1
             const PolicyDev a = arguments();
-            Step after = nx;
-            if (t + 2 < steps) after.next(a);
-            if (t + 1 < steps && nx.blk == 0) stage_boards<true>(a, m.b, nx.b0, tid);   // (with the other waves, ahead of their step t + 1)
+            const Step st = s0;
+            if (t + 1 < steps && s1.blk == 0) boards.next(a, m.b, s1.b0, tid);   // (with the other waves, ahead of their step t + 1)
+            if (t + 2 < steps) f.store(a, s2, hbuf + (t + 2) % 3 * ROWS * ldc, tb);
+            s0 = s1; s1 = s2; s2 = s3;
+            if (t + 4 < steps) { s3.next(a); f.load(a, s3, tb); }
             const T* h = hbuf + t % 3 * ROWS * ldc;
             const T* const zhi = zbuf + (t & 1) * 2 * ROWS * L::LDO;
             const T* const zlo = zhi + ROWS * L::LDO;
@@ -1009,21 +1066,24 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT <= 
                     d[0] = az_mma<DT>(wc[0][k], zf, d[0]);
                     d[1] = az_mma<DT>(wc[1][k], zf, d[1]);
                 }
-                const int row = e * 16 + (lane & 15);
+                const int row = e * 16 + (lane & 15), c = cq * 32 + q * 8;       // the two tiles hold 8 channels of the row in turn
+                if (row >= st.rows || c >= a.C) continue;
+                if constexpr (DT == 1) { d[0] *= down; d[1] *= down; }
+                az_s8 o;
                 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int c = (cq + 4 * j) * 16 + q * 4;
-                    if (row >= st.rows || c >= a.C) continue;
-                    if constexpr (DT == 1) d[j] *= down;
-                    if (MODE == WHOLE_LAST || (MODE == ANY && !a.nchw)) {
-                        T* dst = (T*)a.dh + ((size_t)st.b0 * a.S + st.cell0) * a.C + (row * a.C + c);
-                        if (MODE == WHOLE_LAST || c + 4 <= a.C) *(az_s4_u*)dst = az_s4{az_to16<DT>(d[j][0]), az_to16<DT>(d[j][1]), az_to16<DT>(d[j][2]), az_to16<DT>(d[j][3])};
-                        else for (int i = 0; i < 4; ++i) if (c + i < a.C) az_store<DT>(dst, i, d[j][i]);
-                    } else {
-                        const int b2 = a.nb > 1 ? (int)((unsigned)row * a.mag_s >> 16) : 0, s2 = st.cell0 + row - b2 * a.S;
-                        T* dst = (T*)a.dh + (size_t)st.b0 * a.C * a.S + ((b2 * a.C + c) * a.S + s2);
-                        for (int i = 0; i < 4; ++i) if (MODE == WHOLE_FIRST || c + i < a.C) az_store<DT>(dst, (size_t)i * a.S, d[j][i]);
+                for (int i = 0; i < 8; ++i) o[i] = az_to16<DT>(d[i >> 2][i & 3]);
+                if (MODE == WHOLE_LAST || (MODE == ANY && !a.nchw)) {
+                    short* dst = (short*)a.dh + ((size_t)st.b0 * a.S + st.cell0) * a.C + (row * a.C + c);
+                    if (MODE == WHOLE_LAST || c + 8 <= a.C) *(az_s8_u*)dst = o;
+                    else {
+                        #pragma unroll
+                        for (int i = 0; i < 8; ++i) if (c + i < a.C) dst[i] = o[i];
                     }
+                } else {
+                    const int b2 = a.nb > 1 ? (int)((unsigned)row * a.mag_s >> 16) : 0;
+                    short* dst = (short*)a.dh + (size_t)st.b0 * a.C * a.S + ((b2 * a.C + c) * a.S + st.cell0 + row - b2 * a.S);
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i) if (MODE == WHOLE_FIRST || c + i < a.C) dst[(size_t)i * a.S] = o[i];
                 }
             }
             // dw: rows of a tile are planes, columns are channels, the contraction runs over the step's rows (rows beyond the
@@ -1031,23 +1091,26 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT <= 
             #pragma unroll
             for (int k = 0; k < ROWS; k += L::KS) {
                 if (k >= st.rows) break;
-                const az_i4 hb0 = az_col_frag<DT>(h, ldc, k, cq * 16, lane), hb1 = az_col_frag<DT>(h, ldc, k, (cq + 4) * 16, lane);
+                const az_i4 hb0 = az_col_frag<DT, true>(h, ldc, k, cq * 32, lane), hb1 = az_col_frag<DT, true>(h, ldc, k, cq * 32 + 16, lane);
                 #pragma unroll
                 for (int j = 0; j < OT; ++j) {
-                    const az_i4 z1 = az_col_frag<DT>(zhi, L::LDO, k, j * 16, lane), z2 = az_col_frag<DT>(zlo, L::LDO, k, j * 16, lane);
+                    const az_i4 z1 = az_col_frag<DT, true>(zhi, L::LDO, k, j * 16, lane), z2 = az_col_frag<DT, true>(zlo, L::LDO, k, j * 16, lane);
                     dw[0][j] = az_mma<DT>(z1, hb0, dw[0][j]);
                     dw[1][j] = az_mma<DT>(z1, hb1, dw[1][j]);
                     dw[0][j] = az_mma<DT>(z2, hb0, dw[0][j]);
                     dw[1][j] = az_mma<DT>(z2, hb1, dw[1][j]);
                 }
             }
-            st = nx;
-            nx = after;
             if (t + 1 < steps) __syncthreads();
+        };
+        #pragma unroll 1
+        for (int t = 0; t < steps; t += 2) {
+            interval(t, f[0]);
+            if (t + 1 < steps) interval(t + 1, f[1]);
         }
         #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int c = (cq + 4 * i) * 16 + (lane & 15);
+            const int c = cq * 32 + i * 16 + (lane & 15);
             #pragma unroll
             for (int j = 0; j < OT; ++j)
                 #pragma unroll
