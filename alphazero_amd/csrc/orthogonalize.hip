@@ -9,8 +9,9 @@
 // so the long dimension is touched twice, for A0 and for Q X0, and what lies between are r x r products: 4 r^3 k-free
 // products a step instead of 2 r^2 k + r^3.  The price is that a singular value is carried as its square: one that is
 // small against the largest keeps the absolute precision of A's arithmetic, and the steps enlarge that error as they
-// enlarge the value (a^2 each).  So the products run on pairs of fp16 values, x = hi + lo / 2048 (22 bits; three MFMA a
-// product, fp32 sums), and for fp32 results X is formed anew after `stage` steps and A from it.
+// enlarge the value (a^2 each).  So the products run on pairs of fp16 values, s x = hi + lo (22 bits, s a power of two that
+// keeps lo out of fp16's subnormals where it matters; three MFMA a product, fp32 sums), and for fp32 results X is formed
+// anew after three steps and A from it.
 #include "../../include/az_hip.h"
 #include "az_learn.h"
 
@@ -26,9 +27,9 @@ int ofail(int code, const char* fmt, ...) {
     return az_internal_fail(code, buf);
 }
 
-constexpr float LO = 2048.f;                  // scale of a pair's second value
+constexpr float SA = 256.f, SQ = 16.f;        // scales of the pairs: A, P and A P (at most about 4), Q (a^5 = 485)
 constexpr int KSTEP = 32;                     // contraction of one step of a tile product
-constexpr int MAX_SLICES = 64;                // pieces of a matrix whose squares are summed apart
+constexpr int MAX_SLICES = 256;               // pieces of a matrix whose squares are summed apart
 constexpr int SRC_PAIR = 3;                   // operand kinds: AZ_F32, AZ_F16, AZ_BF16, or pairs
 
 enum { GRAM_WIDE, GRAM_TALL, APPLY_WIDE, APPLY_TALL, SYM };          // what a tile product computes
@@ -55,31 +56,68 @@ struct OrthoDev {
     float keep;
 };
 
-// |U|_F of matrix z, and the power of two under which its elements are split into pairs (root mean square near 1)
+// |U|_F of matrix z, and the power of two under which its elements are split into pairs (root mean square near 4).  Every
+// wave by itself, in one order.
 __device__ __forceinline__ void norm_of(const OrthoDev& d, int z, int& e, float& back) {
     if (!d.sq) { e = d.scale_exp; back = ldexpf(1.f, -e); return; }
     double s = 0.0;
-    for (int i = 0; i < d.slices; ++i) s += d.sq[(size_t)z * d.slices + i];
+    for (int i = threadIdx.x & 63; i < d.slices; i += 64) s += d.sq[(size_t)z * d.slices + i];
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     const double norm = sqrt(s);
     e = 0;
-    if (norm > 0.0 && norm < 1e300) e = min(max(ilogb(sqrt((double)d.r * d.k) / norm), -120), 120);
+    if (norm > 0.0 && norm < 1e300) e = min(max(ilogb(sqrt((double)d.r * d.k) / norm) + 2, -120), 120);
     back = (float)ldexp(1.0 / (norm + (double)d.eps), -e);
 }
 
-// sums of squares of a matrix's slices; with mom the update itself: m' = beta m + g, u = nesterov ? g + beta m' : m'
-template <int DT> __global__ void __launch_bounds__(256) az_ortho_norm_kernel(const void* g, size_t g_stride, int count, int slices, double* sq,
-                                                                          const float* mom, size_t m_stride, float* mom_out, size_t mo_stride, float* u, float beta, int nesterov) {
+// sums of squares of a matrix's slices; with mom the update itself: m' = beta m + g, u = nesterov ? g + beta m' : m'.  Four
+// elements a thread and load, four loads in flight; what a slice leaves over (and whatever is not there) is dropped.
+template <int DT> __device__ __forceinline__ az_f4 load4(const void* p, size_t i) {
+    if constexpr (DT == 0) return *(const az_f4_u*)((const float*)p + i);
+    else {
+        const az_s4 x = *(const az_s4_u*)((const short*)p + i);
+        return az_f4{az_from16<DT>(x[0]), az_from16<DT>(x[1]), az_from16<DT>(x[2]), az_from16<DT>(x[3])};
+    }
+}
+template <int DT, bool MOM> __global__ void __launch_bounds__(256) az_ortho_norm_kernel(const void* g, size_t g_stride, int count, int slices, double* sq,
+                                                                                     const float* mom, size_t m_stride, float* mom_out, size_t mo_stride, float* u, float beta, int nesterov) {
     __shared__ double red[4];
-    const int z = blockIdx.y, sl = blockIdx.x;
-    const long long lo = (long long)count * sl / slices, hi = (long long)count * (sl + 1) / slices;
+    const int z = blockIdx.y, sl = blockIdx.x, quads = count / 4;
+    const int lo = (int)((long long)quads * sl / slices), hi = (int)((long long)quads * (sl + 1) / slices);
+    const size_t go = z * g_stride, mo = z * m_stride, oo = z * mo_stride, uo = (size_t)z * count;
     double s = 0.0;
-    for (long long i = lo + threadIdx.x; i < hi; i += 256) {
-        float v = az_load<DT>(g, z * g_stride + i);
-        if (mom) {
-            const float m = beta * mom[z * m_stride + i] + v;
-            v = nesterov ? v + beta * m : m;
-            mom_out[z * mo_stride + i] = m;
-            u[(size_t)z * count + i] = v;
+    const auto one = [&](float v, float m) __attribute__((always_inline)) { return beta * m + v; };
+    constexpr int U = 4;
+    for (int base = lo + threadIdx.x; base < hi; base += 256 * U) {
+        az_f4 v[U], m[U];
+        #pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const size_t i = (size_t)min(base + k * 256, hi - 1) * 4;
+            v[k] = load4<DT>(g, go + i);
+            if (MOM) m[k] = *(const az_f4_u*)(mom + mo + i);
+        }
+        #pragma unroll
+        for (int k = 0; k < U; ++k) {
+            if (base + k * 256 >= hi) break;
+            const size_t i = (size_t)(base + k * 256) * 4;
+            if (MOM) {
+                az_f4 n;
+                #pragma unroll
+                for (int e = 0; e < 4; ++e) { n[e] = one(v[k][e], m[k][e]); v[k][e] = nesterov ? v[k][e] + beta * n[e] : n[e]; }
+                *(az_f4_u*)(mom_out + oo + i) = n;
+                *(az_f4_u*)(u + uo + i) = v[k];
+            }
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) s += (double)v[k][e] * v[k][e];
+        }
+    }
+    if (sl == slices - 1 && (int)threadIdx.x < count - quads * 4) {
+        const size_t i = (size_t)quads * 4 + threadIdx.x;
+        float v = az_load<DT>(g, go + i);
+        if (MOM) {
+            const float n = one(v, mom[mo + i]);
+            v = nesterov ? v + beta * n : n;
+            mom_out[oo + i] = n;
+            u[uo + i] = v;
         }
         s += (double)v * v;
     }
@@ -89,62 +127,91 @@ template <int DT> __global__ void __launch_bounds__(256) az_ortho_norm_kernel(co
     if (threadIdx.x == 0) sq[(size_t)z * slices + sl] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// 8 elements of a line: hi (and lo) halves.  Lines and positions beyond the matrix are zero.
-template <int SRC> __device__ __forceinline__ void load8(const void* p, const void* plo, size_t ld, int line, int pos, int nlines, int npos, float up, az_s8& hi, az_s8& lo) {
-    if constexpr (SRC == SRC_PAIR) {
-        hi = *(const az_s8*)((const short*)p + (size_t)line * ld + pos);
-        lo = *(const az_s8*)((const short*)plo + (size_t)line * ld + pos);
-    } else {
-        float v[8];
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.f;
-        if (line < nlines && pos < npos) {
-            const size_t at = (size_t)line * ld + pos;
-            if (pos + 8 <= npos) {
-                if constexpr (SRC == 0) {
-                    const az_f4 x = *(const az_f4_u*)((const float*)p + at), y = *(const az_f4_u*)((const float*)p + at + 4);
-                    for (int j = 0; j < 4; ++j) { v[j] = x[j]; v[4 + j] = y[j]; }
-                } else {
-                    const az_s8 x = *(const az_s8_u*)((const short*)p + at);
-                    #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = az_from16<SRC>(x[j]);
-                }
-            } else {
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) if (pos + j < npos) v[j] = az_load<SRC>(p, at + j);
-            }
-        }
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float x = v[j] * up;
-            hi[j] = az_to16<1>(x);
-            if constexpr (SRC == 0) lo[j] = az_to16<1>((x - az_from16<1>(hi[j])) * LO);
-        }
-    }
-}
+__device__ __forceinline__ void split(float x, short& hi, short& lo) { hi = az_to16<1>(x); lo = az_to16<1>(x - az_from16<1>(hi)); }
 
-// One operand of a tile product: TILE lines-or-columns by KSTEP.  Along: the contraction runs along a line (LDS rows are
-// the tile's rows); otherwise lines are the contraction (LDS rows are its steps, read transposed).
+// One operand of a tile product: TILE lines-or-columns by KSTEP.  ALONG: the contraction runs along a line of memory (LDS
+// rows are the tile's rows); otherwise lines are the contraction (LDS rows are its steps, read transposed).  A thread
+// carries pieces of 8 elements of a line, as they lie in memory (the loads are unconditional, clamped into the matrix, and
+// stay in flight over a step's products), and splits them into hi (and lo) halves on their way to LDS.
 template <int TILE, int SRC, bool ALONG> struct Operand {
-    static constexpr int PARTS = SRC == 0 || SRC == SRC_PAIR ? 2 : 1;
+    static constexpr int PARTS = SRC == 0 || SRC == SRC_PAIR ? 2 : 1, RAW = PARTS;
     static constexpr int LD = ALONG ? KSTEP + 8 : TILE + 16;
     static constexpr int LINES = ALONG ? TILE : KSTEP, PER = (ALONG ? KSTEP : TILE) / 8;
     static constexpr int NP = LINES * PER / 256;                     // pieces a thread
     static constexpr int HALVES = LINES * LD;                        // of one part
-    az_s8 hi[NP], lo[NP];
-    __device__ __forceinline__ void load(const void* p, const void* plo, size_t ld, int t0, int k0, int nlines, int npos, float up, int tid) {
+    az_i4 raw[NP][RAW];
+    static __device__ __forceinline__ void place(int i, int tid, int& line, int& pos) { const int w = tid + i * 256; line = w / PER; pos = w % PER * 8; }
+    // p (and plo, a pair's lo plane): the matrix; t0, k0: the tile's corner; nlines x npos: the matrix as stored
+    __device__ __forceinline__ void load(const void* p, const void* plo, int ld, int t0, int k0, int nlines, int npos, int tid) {
         #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const int w = tid + i * 256, line = w / PER, pos = w % PER * 8;
-            load8<SRC>(p, plo, ld, (ALONG ? t0 : k0) + line, (ALONG ? k0 : t0) + pos, nlines, npos, up, hi[i], lo[i]);
+            int line, pos;
+            place(i, tid, line, pos);
+            line += ALONG ? t0 : k0;
+            pos += ALONG ? k0 : t0;
+            if constexpr (SRC == SRC_PAIR) {
+                raw[i][0] = *(const az_i4*)((const short*)p + (size_t)line * ld + pos);
+                raw[i][1] = *(const az_i4*)((const short*)plo + (size_t)line * ld + pos);
+            } else {
+                line = min(line, nlines - 1);
+                if (npos >= 8) {
+                    // a piece that hangs over the line's end is the line's last 8 elements
+                    const size_t at = (size_t)line * ld + min(pos, npos - 8);
+                    if constexpr (SRC == 0) {
+                        raw[i][0] = __builtin_bit_cast(az_i4, *(const az_f4_u*)((const float*)p + at));
+                        raw[i][1] = __builtin_bit_cast(az_i4, *(const az_f4_u*)((const float*)p + at + 4));
+                    } else raw[i][0] = __builtin_bit_cast(az_i4, *(const az_s8_u*)((const short*)p + at));
+                } else {                                             // short lines: an element a load
+                    #pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const size_t at = (size_t)line * ld + min(pos + e, npos - 1);
+                        if constexpr (SRC == 0) raw[i][e >> 2][e & 3] = ((const int*)p)[at];
+                        else {
+                            const int v = ((const unsigned short*)p)[at];
+                            raw[i][0][e >> 1] = e & 1 ? raw[i][0][e >> 1] | v << 16 : v;
+                        }
+                    }
+                }
+            }
         }
     }
-    __device__ __forceinline__ void store(short* s, int tid) const {
+    __device__ __forceinline__ void store(short* s, int t0, int k0, int nlines, int npos, float up, int tid) const {
         #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const int w = tid + i * 256, at = w / PER * LD + w % PER * 8;
-            *(az_s8*)(s + at) = hi[i];
-            if constexpr (PARTS == 2) *(az_s8*)(s + HALVES + at) = lo[i];
+            int line, pos;
+            place(i, tid, line, pos);
+            short* dst = s + line * LD + pos;
+            if constexpr (SRC == SRC_PAIR) {
+                *(az_i4*)dst = raw[i][0];
+                *(az_i4*)(dst + HALVES) = raw[i][1];
+            } else {
+                line += ALONG ? t0 : k0;
+                pos += ALONG ? k0 : t0;
+                az_s8 hi, lo;
+                #pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float x;
+                    if constexpr (SRC == 0) x = __int_as_float(raw[i][e >> 2][e & 3]);
+                    else x = az_from16<SRC>((short)(raw[i][0][e >> 1] >> (e & 1) * 16));
+                    x *= up;
+                    hi[e] = az_to16<1>(x);
+                    lo[e] = SRC == 0 ? az_to16<1>(x - az_from16<1>(hi[e])) : (short)0;
+                }
+                if (line < nlines && pos + 8 <= npos) {
+                    *(az_s8*)dst = hi;
+                    if constexpr (PARTS == 2) *(az_s8*)(dst + HALVES) = lo;
+                } else {                                             // the matrix's edge: what lies beyond is zero
+                    const int first = npos >= 8 ? min(pos, npos - 8) : pos;      // of the piece as loaded
+                    #pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (line >= nlines || pos + e >= npos) { dst[e] = 0; if constexpr (PARTS == 2) dst[HALVES + e] = 0; }
+                    #pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int at = first + e - pos;
+                        if (line < nlines && at >= 0 && pos + at < npos) { dst[at] = hi[e]; if constexpr (PARTS == 2) dst[HALVES + at] = lo[e]; }
+                    }
+                }
+            }
         }
     }
     static __device__ __forceinline__ az_i4 frag(const short* s, int part, int t, int lane) {
@@ -166,8 +233,8 @@ __device__ __forceinline__ void lower_tile(int i, int& ti, int& tj) {
 //   SYM         M = rows of a symmetric matrix, N = rows of another that commutes with it: their product, lower triangle
 //   GRAM_*      M = N = rows of X: lower triangle
 //   APPLY_WIDE  M = columns of X, N = rows of Q;   APPLY_TALL  M = rows of Q, N = rows of X as stored (columns of X)
-template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256) az_ortho_product_kernel(OrthoDev d, const short* ma, const short* na, short* res,
-                                                                                                 const short* ma2, const short* na2, short* res2, int epi, int n) {
+template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256, 2) az_ortho_product_kernel(OrthoDev d, const short* ma, const short* na, short* res,
+                                                                                                 const short* ma2, const short* na2, short* res2, int epi, float sr, float sr2) {
     constexpr bool GRAM = MODE == GRAM_WIDE || MODE == GRAM_TALL;
     constexpr int MS = MODE == SYM || MODE == APPLY_TALL ? SRC_PAIR : DT, NS = MODE == SYM || MODE == APPLY_WIDE ? SRC_PAIR : DT;
     constexpr bool MA = !(MODE == GRAM_TALL || MODE == APPLY_WIDE), NA = MODE != GRAM_TALL;
@@ -190,8 +257,8 @@ template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256) az_
             k_lo = steps * sp / d.split * KSTEP;
             k_hi = steps * (sp + 1) / d.split * KSTEP;
         } else {
-            if (blockIdx.y) { ma = ma2; na = na2; res = res2; epi = EPI_PAIR; }   // a second product of the same launch
-            k_hi = d.rp;
+            if (blockIdx.y) { ma = ma2; na = na2; res = res2; epi = EPI_PAIR; sr = sr2; }   // a second product of the same launch
+            k_hi = (d.r + TILE - 1) / TILE * TILE;                  // (what lies behind, up to rp, is never written)
         }
     } else {
         // APPLY: x runs over the long side
@@ -203,32 +270,33 @@ template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256) az_
     float back = 1.f, up = 1.f;
     if constexpr (MODE != SYM) { norm_of(d, z, e, back); up = ldexpf(1.f, e); }
     const void *mp, *mlo = nullptr, *np, *nlo = nullptr;
-    size_t mld, nld;
+    int mld, nld;
     const size_t esz = DT == 0 ? 4 : 2;
     if constexpr (MS == SRC_PAIR) { mp = ma + (size_t)z * 2 * plane; mlo = ma + (size_t)z * 2 * plane + plane; mld = d.rp; }
     else { mp = (const char*)d.x + z * d.x_stride * esz; mld = d.cols; }
     if constexpr (NS == SRC_PAIR) { np = na + (size_t)z * 2 * plane; nlo = na + (size_t)z * 2 * plane + plane; nld = d.rp; }
     else { np = (const char*)d.x + z * d.x_stride * esz; nld = d.cols; }
-    az_f4 hh[WT][WT], cross[WT][WT];
+    az_f4 acc[WT][WT];
     #pragma unroll
     for (int i = 0; i < WT; ++i)
-        for (int j = 0; j < WT; ++j) { hh[i][j] = az_f4{0.f, 0.f, 0.f, 0.f}; cross[i][j] = az_f4{0.f, 0.f, 0.f, 0.f}; }
+        for (int j = 0; j < WT; ++j) acc[i][j] = az_f4{0.f, 0.f, 0.f, 0.f};
     OM om;
     ON on;
-    om.load(mp, mlo, mld, m0, k_lo, d.rows, d.cols, up, tid);
-    on.load(np, nlo, nld, n0, k_lo, d.rows, d.cols, up, tid);
+    om.load(mp, mlo, mld, m0, k_lo, d.rows, d.cols, tid);
+    on.load(np, nlo, nld, n0, k_lo, d.rows, d.cols, tid);
     int buf = 0;
     const int mw = (wave & 1) * TILE / 2, nw = (wave >> 1) * TILE / 2;
+    #pragma unroll 1
     for (int k = k_lo; k < k_hi; k += KSTEP, buf ^= 1) {
         short* sm = lds + buf * STAGE;
         short* sn = sm + OM::PARTS * OM::HALVES;
-        om.store(sm, tid);
-        on.store(sn, tid);
-        __syncthreads();                                             // (the other stage was last read before this barrier)
+        om.store(sm, m0, k, d.rows, d.cols, up, tid);
+        on.store(sn, n0, k, d.rows, d.cols, up, tid);
         if (k + KSTEP < k_hi) {
-            om.load(mp, mlo, mld, m0, k + KSTEP, d.rows, d.cols, up, tid);
-            on.load(np, nlo, nld, n0, k + KSTEP, d.rows, d.cols, up, tid);
+            om.load(mp, mlo, mld, m0, k + KSTEP, d.rows, d.cols, tid);
+            on.load(np, nlo, nld, n0, k + KSTEP, d.rows, d.cols, tid);
         }
+        __syncthreads();                                             // (the other stage was last read before this barrier)
         az_i4 mf[WT][OM::PARTS];
         #pragma unroll
         for (int i = 0; i < WT; ++i)
@@ -240,9 +308,9 @@ template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256) az_
             for (int p = 0; p < ON::PARTS; ++p) nf[p] = ON::frag(sn, p, nw + j * 16, lane);
             #pragma unroll
             for (int i = 0; i < WT; ++i) {
-                hh[i][j] = az_mma<1>(mf[i][0], nf[0], hh[i][j]);
-                if constexpr (ON::PARTS == 2) cross[i][j] = az_mma<1>(mf[i][0], nf[1], cross[i][j]);
-                if constexpr (OM::PARTS == 2) cross[i][j] = az_mma<1>(mf[i][1], nf[0], cross[i][j]);
+                acc[i][j] = az_mma<1>(mf[i][0], nf[0], acc[i][j]);
+                if constexpr (ON::PARTS == 2) acc[i][j] = az_mma<1>(mf[i][0], nf[1], acc[i][j]);
+                if constexpr (OM::PARTS == 2) acc[i][j] = az_mma<1>(mf[i][1], nf[0], acc[i][j]);
             }
         }
     }
@@ -250,22 +318,25 @@ template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256) az_
     for (int i = 0; i < WT; ++i)
         #pragma unroll
         for (int j = 0; j < WT; ++j) {
-            az_f4 v = hh[i][j] + cross[i][j] * (1.f / LO);
+            az_f4 v = acc[i][j];
             const int m = m0 + mw + i * 16 + q * 4, nn = n0 + nw + j * 16 + (lane & 15);
             if constexpr (MODE == SYM || GRAM) {
-                if constexpr (GRAM) v *= back * back;
+                // sr: from the operands' scales to the result's (a partial sum has none)
+                if constexpr (GRAM) v *= back * back * (epi == EPI_PARTIAL ? 1.f : SA);
+                else v *= sr;
                 if (GRAM && epi == EPI_PARTIAL) { *(az_f4*)(d.partial + ((size_t)z * d.split + sp) * plane + (size_t)nn * d.rp + m) = v; continue; }
                 short* hi = res + (size_t)z * 2 * plane;
                 short* lo = hi + plane;
                 if (MODE == SYM && epi == EPI_POLY) {                 // P = a I + b A + c A A
                     const az_s4 ah = *(const az_s4*)(ma + (size_t)z * 2 * plane + (size_t)nn * d.rp + m);
                     const az_s4 al = *(const az_s4*)(ma + (size_t)z * 2 * plane + plane + (size_t)nn * d.rp + m);
+                    const float res_scale = sr * SA * SA;
                     #pragma unroll
-                    for (int t = 0; t < 4; ++t) v[t] = (m + t == nn ? d.a : 0.f) + d.b * (az_from16<1>(ah[t]) + az_from16<1>(al[t]) * (1.f / LO)) + d.c * v[t];
+                    for (int t = 0; t < 4; ++t) v[t] = (m + t == nn ? d.a * res_scale : 0.f) + d.b * (res_scale / SA) * (az_from16<1>(ah[t]) + az_from16<1>(al[t])) + d.c * v[t];
                 }
                 az_s4 h, l;
                 #pragma unroll
-                for (int t = 0; t < 4; ++t) { h[t] = az_to16<1>(v[t]); l[t] = az_to16<1>((v[t] - az_from16<1>(h[t])) * LO); }
+                for (int t = 0; t < 4; ++t) { short x, y; split(v[t], x, y); h[t] = x; l[t] = y; }
                 *(az_s4*)(hi + (size_t)nn * d.rp + m) = h;
                 *(az_s4*)(lo + (size_t)nn * d.rp + m) = l;
                 if (m0 != n0)
@@ -274,7 +345,7 @@ template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256) az_
                 // the result's line and position in memory: the positions m .. m + 3 of line nn
                 const int nl = d.rows, np_ = d.cols;
                 if (nn >= nl || m >= np_) continue;
-                const float f = back * d.scale;
+                const float f = back * (1.f / SQ) * d.scale;
                 const size_t at = (size_t)nn * d.cols + m;
                 if (d.w) {
                     const float* w = d.w + z * d.w_stride + at;
@@ -309,7 +380,8 @@ __global__ void __launch_bounds__(256) az_ortho_join_kernel(OrthoDev d, int tile
         const int nn = ti * tile + i / tile, m = tj * tile + i % tile;
         float v = 0.f;
         for (int s = 0; s < d.split; ++s) v += d.partial[((size_t)z * d.split + s) * plane + (size_t)nn * d.rp + m];
-        const short h = az_to16<1>(v), l = az_to16<1>((v - az_from16<1>(h)) * LO);
+        short h, l;
+        split(v * SA, h, l);
         hi[(size_t)nn * d.rp + m] = h; lo[(size_t)nn * d.rp + m] = l;
         if (ti != tj) { hi[(size_t)m * d.rp + nn] = h; lo[(size_t)m * d.rp + nn] = l; }
     }
@@ -320,11 +392,11 @@ __global__ void __launch_bounds__(256) az_ortho_identity_kernel(short* Q, int rp
     const size_t plane = (size_t)rp * rp;
     short* q = Q + (size_t)blockIdx.y * 2 * plane;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < 2 * plane; i += (size_t)gridDim.x * 256)
-        q[i] = i < plane && i / rp == i % rp ? az_to16<1>(1.f) : (short)0;
+        q[i] = i < plane && i / rp == i % rp ? az_to16<1>(SQ) : (short)0;
 }
 
 struct Plan {
-    int n, rows, cols, r, k, rp, tile, tiles, low, slices, split, stage;
+    int n, rows, cols, r, k, rp, tile, apply_tile, tiles, low, slices, split, stage;
     bool muon, restart;
     size_t off_sq, off_u, off_x1, off_mat, off_partial, bytes;
     size_t pair_bytes;
@@ -332,21 +404,38 @@ struct Plan {
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-Plan make_plan(int n, int rows, int cols, int dtype, int steps, bool muon) {
+// largest |a + b y + c y^2| for y = x^2 of singular values up to 1.2
+float largest_factor(float a, float b, float c) {
+    float m = 0.f;
+    for (int i = 0; i <= 150; ++i) { const float y = i * 0.01f; m = std::fmax(m, std::fabs(a + b * y + c * y * y)); }
+    return m;
+}
+
+Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b, float c, bool muon) {
     Plan p = {};
     p.n = n; p.rows = rows; p.cols = cols; p.muon = muon;
     p.r = rows < cols ? rows : cols;
     p.k = rows < cols ? cols : rows;
-    p.tile = p.r <= 64 ? 64 : 128;
+    // Tiles of 128 x 128 move half the LDS bytes a product of tiles of 64 x 64, but there are a quarter as many: taken where
+    // they fill the chip's 256 CUs.
+    const auto low = [&](int tile) { const long long t = (p.r + tile - 1) / tile; return t * (t + 1) / 2; };
+    p.tile = low(128) * n >= 256 ? 128 : 64;
+    p.rp = (p.r + 127) / 128 * 128;
+    if (p.r <= 64) p.rp = 64;
     p.tiles = (p.r + p.tile - 1) / p.tile;
-    p.rp = p.tiles * p.tile;
-    p.low = p.tiles * (p.tiles + 1) / 2;
+    p.low = (int)low(p.tile);
+    p.apply_tile = p.rp % 128 == 0 && (long long)((p.k + 127) / 128) * ((p.r + 127) / 128) * n >= 256 ? 128 : 64;
     const long long count = (long long)rows * cols;
     p.slices = (int)(count / 4096 < 1 ? 1 : count / 4096 > MAX_SLICES ? MAX_SLICES : count / 4096);
+    while (p.slices > 64 && (long long)p.slices * n > 2048) p.slices /= 2;
     const int ksteps = (p.k + KSTEP - 1) / KSTEP;
     p.split = 1;
     while (p.split < 16 && (long long)p.low * n * p.split < 256 && ksteps / (p.split * 2) >= 4) p.split *= 2;
+    // Steps between two formations of X.  fp32 results: three (comment at the top); 16-bit results: five, their own rounding
+    // is larger; fewer where the coefficients would take Q out of fp16's range.
     p.stage = dtype == AZ_F32 || muon ? 3 : 5;
+    const float f = largest_factor(a, b, c);
+    while (p.stage > 1 && std::pow(f, (float)p.stage) * SQ > 30000.f) --p.stage;
     p.restart = steps > p.stage;
     p.pair_bytes = up256((size_t)n * 2 * p.rp * p.rp * 2);
     size_t o = 0;
@@ -359,8 +448,8 @@ Plan make_plan(int n, int rows, int cols, int dtype, int steps, bool muon) {
     return p;
 }
 
-template <int TILE, int DT, int MODE> hipError_t product(const OrthoDev& d, dim3 grid, const short* ma, const short* na, short* res, const short* ma2, const short* na2, short* res2,
-                                                         int epi, int n, hipStream_t st) {
+struct Pairs { const short *m, *n; short* out; float scale; };       // one product: operands, result, scale (of EPI_PAIR / EPI_POLY)
+template <int TILE, int DT, int MODE> hipError_t product(const OrthoDev& d, dim3 grid, Pairs one, Pairs two, int epi, hipStream_t st) {
     constexpr int MS = MODE == SYM || MODE == APPLY_TALL ? SRC_PAIR : DT, NS = MODE == SYM || MODE == APPLY_WIDE ? SRC_PAIR : DT;
     typedef Operand<TILE, MS, !(MODE == GRAM_TALL || MODE == APPLY_WIDE)> OM;
     typedef Operand<TILE, NS, MODE != GRAM_TALL> ON;
@@ -369,15 +458,15 @@ template <int TILE, int DT, int MODE> hipError_t product(const OrthoDev& d, dim3
         const hipError_t e = hipFuncSetAttribute((const void*)az_ortho_product_kernel<TILE, DT, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    az_ortho_product_kernel<TILE, DT, MODE><<<grid, 256, lds, st>>>(d, ma, na, res, ma2, na2, res2, epi, n);
+    az_ortho_product_kernel<TILE, DT, MODE><<<grid, 256, lds, st>>>(d, one.m, one.n, one.out, two.m, two.n, two.out, epi, one.scale, two.scale);
     return hipGetLastError();
 }
 
 template <int TILE, int DT> hipError_t gram(const Plan& p, const OrthoDev& d, hipStream_t st) {
     const dim3 grid(p.low, p.split, p.n);
     const int epi = p.split > 1 ? EPI_PARTIAL : EPI_PAIR;
-    hipError_t e = p.rows <= p.cols ? product<TILE, DT, GRAM_WIDE>(d, grid, nullptr, nullptr, d.A, nullptr, nullptr, nullptr, epi, p.n, st)
-                                    : product<TILE, DT, GRAM_TALL>(d, grid, nullptr, nullptr, d.A, nullptr, nullptr, nullptr, epi, p.n, st);
+    const Pairs x = {nullptr, nullptr, d.A, 1.f};
+    hipError_t e = p.rows <= p.cols ? product<TILE, DT, GRAM_WIDE>(d, grid, x, Pairs{}, epi, st) : product<TILE, DT, GRAM_TALL>(d, grid, x, Pairs{}, epi, st);
     if (e == hipSuccess && p.split > 1) {
         az_ortho_join_kernel<<<dim3(p.low, TILE * TILE / 1024, p.n), 256, 0, st>>>(d, TILE);
         e = hipGetLastError();
@@ -385,9 +474,9 @@ template <int TILE, int DT> hipError_t gram(const Plan& p, const OrthoDev& d, hi
     return e;
 }
 template <int TILE, int DT> hipError_t apply(const Plan& p, const OrthoDev& d, hipStream_t st) {
-    const dim3 grid((p.k + TILE - 1) / TILE, p.tiles, p.n);
-    return p.rows <= p.cols ? product<TILE, DT, APPLY_WIDE>(d, grid, nullptr, d.Q, nullptr, nullptr, nullptr, nullptr, 0, p.n, st)
-                            : product<TILE, DT, APPLY_TALL>(d, grid, d.Q, nullptr, nullptr, nullptr, nullptr, nullptr, 0, p.n, st);
+    const dim3 grid((p.k + TILE - 1) / TILE, (p.r + TILE - 1) / TILE, p.n);
+    return p.rows <= p.cols ? product<TILE, DT, APPLY_WIDE>(d, grid, Pairs{nullptr, d.Q, nullptr, 1.f}, Pairs{}, 0, st)
+                            : product<TILE, DT, APPLY_TALL>(d, grid, Pairs{d.Q, nullptr, nullptr, 1.f}, Pairs{}, 0, st);
 }
 template <int TILE> hipError_t gram_dt(int dt, const Plan& p, const OrthoDev& d, hipStream_t st) {
     return dt == AZ_F32 ? gram<TILE, 0>(p, d, st) : dt == AZ_F16 ? gram<TILE, 1>(p, d, st) : gram<TILE, 2>(p, d, st);
@@ -399,25 +488,27 @@ template <int TILE> hipError_t apply_dt(int dt, const Plan& p, const OrthoDev& d
 // `m` steps on A: leaves Q
 template <int TILE> hipError_t iterate(const Plan& p, OrthoDev& d, int m, hipStream_t st) {
     const dim3 one(p.low, 1, p.n), two(p.low, 2, p.n);
+    const float aa = 1.f / SA, aq = SQ / (SA * SA), qq = 1.f / SA;   // A-kind x A-kind -> A-kind, -> Q, Q x A-kind -> Q
     hipError_t e = hipSuccess;
 #define RUN(call) do { if (e == hipSuccess) e = (call); } while (0)
     if (m == 0) { az_ortho_identity_kernel<<<dim3(64, p.n), 256, 0, st>>>(d.Q, p.rp); return hipGetLastError(); }
     for (int i = 0; i < m; ++i) {
         const bool first = i == 0, last = i + 1 == m;
-        RUN((product<TILE, 0, SYM>(d, one, d.A, d.A, first ? d.Q : d.P, nullptr, nullptr, nullptr, EPI_POLY, p.n, st)));
-        short* P = first ? d.Q : d.P;                                // the first step's Q is its P
+        // the first step's Q is its P, at Q's scale: written where it is wanted
+        if (first) RUN((product<TILE, 0, SYM>(d, one, Pairs{d.A, d.A, d.Q, aq}, Pairs{}, EPI_POLY, st)));
+        if (!first || !last) RUN((product<TILE, 0, SYM>(d, one, Pairs{d.A, d.A, d.P, aa}, Pairs{}, EPI_POLY, st)));
         if (!last) {
-            if (first) RUN((product<TILE, 0, SYM>(d, one, d.A, P, d.T, nullptr, nullptr, nullptr, EPI_PAIR, p.n, st)));
-            else RUN((product<TILE, 0, SYM>(d, two, d.A, P, d.T, d.Q, P, d.Q2, EPI_PAIR, p.n, st)));
-            RUN((product<TILE, 0, SYM>(d, one, d.T, P, d.A, nullptr, nullptr, nullptr, EPI_PAIR, p.n, st)));
-        } else if (!first) RUN((product<TILE, 0, SYM>(d, one, d.Q, P, d.Q2, nullptr, nullptr, nullptr, EPI_PAIR, p.n, st)));
+            if (first) RUN((product<TILE, 0, SYM>(d, one, Pairs{d.A, d.P, d.T, aa}, Pairs{}, EPI_PAIR, st)));
+            else RUN((product<TILE, 0, SYM>(d, two, Pairs{d.A, d.P, d.T, aa}, Pairs{d.Q, d.P, d.Q2, qq}, EPI_PAIR, st)));
+            RUN((product<TILE, 0, SYM>(d, one, Pairs{d.T, d.P, d.A, aa}, Pairs{}, EPI_PAIR, st)));
+        } else if (!first) RUN((product<TILE, 0, SYM>(d, one, Pairs{d.Q, d.P, d.Q2, qq}, Pairs{}, EPI_PAIR, st)));
         if (!first) { short* t = d.Q; d.Q = d.Q2; d.Q2 = t; }
     }
 #undef RUN
     return e;
 }
 
-template <int TILE> hipError_t run_plan(const Plan& p, OrthoDev d, int dtype, int steps, unsigned char* ws, hipStream_t st) {
+hipError_t run_plan(const Plan& p, OrthoDev d, int dtype, int steps, unsigned char* ws, hipStream_t st) {
     const OrthoDev fin = d;                                          // result pointers of the last application
     const size_t count = (size_t)p.rows * p.cols;
     float* x1[2] = {(float*)(ws + p.off_x1), (float*)(ws + p.off_x1 + up256((size_t)p.n * count * 4))};
@@ -428,13 +519,14 @@ template <int TILE> hipError_t run_plan(const Plan& p, OrthoDev d, int dtype, in
         // stage starts far below 1 (|X0|_F = 1 spread over the singular values) and the later ones near 1
         const int left = steps - done, m = left < p.stage ? left : p.stage;
         done += m;
-        if (m > 0) e = gram_dt<TILE>(dtype, p, d, st);
-        if (e == hipSuccess) e = iterate<TILE>(p, d, m, st);
+        if (m > 0) e = p.tile == 64 ? gram_dt<64>(dtype, p, d, st) : gram_dt<128>(dtype, p, d, st);
+        if (e == hipSuccess) e = p.tile == 64 ? iterate<64>(p, d, m, st) : iterate<128>(p, d, m, st);
         if (done < steps) { d.out = x1[which]; d.out_stride = count; d.out_dtype = AZ_F32; d.scale = 1.f; d.w = nullptr; }
         else { d.out = fin.out; d.out_stride = fin.out_stride; d.out_dtype = fin.out_dtype; d.scale = fin.scale; d.w = fin.w; }
-        if (e == hipSuccess) e = apply_dt<TILE>(dtype, p, d, st);
+        if (e == hipSuccess) e = p.apply_tile == 64 ? apply_dt<64>(dtype, p, d, st) : apply_dt<128>(dtype, p, d, st);
         d.x = x1[which]; d.x_stride = count; dtype = AZ_F32; d.sq = nullptr;
-        d.scale_exp = ilogb(std::sqrt((double)p.k));                 // an iterate's elements: about 1 / sqrt(k)
+        const int se = std::ilogb(std::sqrt((double)p.k)) + 2;       // an iterate's elements: about 1 / sqrt(k)
+        d.scale_exp = se < 13 ? se : 13;
         which ^= 1;
     } while (e == hipSuccess && done < steps);
     return e;
@@ -491,7 +583,7 @@ int run(const Plan& p, OrthoDev d, int dtype, int steps, unsigned char* ws, hipS
     short** m[5] = {&d.A, &d.P, &d.T, &d.Q, &d.Q2};
     for (int i = 0; i < 5; ++i) *m[i] = (short*)(ws + p.off_mat + i * p.pair_bytes);
     d.partial = (float*)(ws + p.off_partial);
-    const hipError_t e = p.tile == 64 ? run_plan<64>(p, d, dtype, steps, ws, st) : run_plan<128>(p, d, dtype, steps, ws, st);
+    const hipError_t e = run_plan(p, d, dtype, steps, ws, st);
     if (e != hipSuccess) return ofail(AZ_E_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
     return AZ_OK;
 }
@@ -500,11 +592,11 @@ int run(const Plan& p, OrthoDev d, int dtype, int steps, unsigned char* ws, hipS
 
 extern "C" size_t az_orthogonalize_workspace(const az_orthogonalize_args* p) {
     if (check_ortho(p) != AZ_OK) return 0;
-    return make_plan(p->n, p->rows, p->cols, p->dtype, p->steps, false).bytes + 256;
+    return make_plan(p->n, p->rows, p->cols, p->dtype, p->steps, p->a, p->b, p->c, false).bytes + 256;
 }
 extern "C" size_t az_muon_step_workspace(const az_muon_step_args* p) {
     if (check_muon(p) != AZ_OK) return 0;
-    return make_plan(p->n, p->rows, p->cols, AZ_F32, p->steps, true).bytes + 256;
+    return make_plan(p->n, p->rows, p->cols, AZ_F32, p->steps, p->a, p->b, p->c, true).bytes + 256;
 }
 
 extern "C" int az_orthogonalize_dev(const az_orthogonalize_args* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -519,7 +611,7 @@ extern "C" int az_orthogonalize_dev(const az_orthogonalize_args* p, void* worksp
     // (a tile of the result is written while other workgroups still read the update)
     if (meet(span_of(p->update, p->update_stride, p->n, p->rows, p->cols, esz), span_of(p->out, p->out_stride, p->n, p->rows, p->cols, esz)))
         return ofail(AZ_E_ARG, "out overlaps update");
-    const Plan plan = make_plan(p->n, p->rows, p->cols, p->dtype, p->steps, false);
+    const Plan plan = make_plan(p->n, p->rows, p->cols, p->dtype, p->steps, p->a, p->b, p->c, false);
     if ((rc = check_ws(workspace, workspace_bytes, plan.bytes + 256)) != AZ_OK) return rc;
     AzDeviceGuard dev(p->device);
     if (!dev.ok) return ofail(AZ_E_HIP, "device %d cannot be used (no HIP device: libazhip has no CPU fallback)", p->device);
@@ -528,9 +620,9 @@ extern "C" int az_orthogonalize_dev(const az_orthogonalize_args* p, void* worksp
     double* sq = (double*)(ws + plan.off_sq);
     const dim3 grid(plan.slices, p->n);
     const int count = p->rows * p->cols;
-    if (p->dtype == AZ_F32) az_ortho_norm_kernel<0><<<grid, 256, 0, st>>>(p->update, p->update_stride, count, plan.slices, sq, nullptr, 0, nullptr, 0, nullptr, 0.f, 0);
-    else if (p->dtype == AZ_F16) az_ortho_norm_kernel<1><<<grid, 256, 0, st>>>(p->update, p->update_stride, count, plan.slices, sq, nullptr, 0, nullptr, 0, nullptr, 0.f, 0);
-    else az_ortho_norm_kernel<2><<<grid, 256, 0, st>>>(p->update, p->update_stride, count, plan.slices, sq, nullptr, 0, nullptr, 0, nullptr, 0.f, 0);
+    if (p->dtype == AZ_F32) az_ortho_norm_kernel<0, false><<<grid, 256, 0, st>>>(p->update, p->update_stride, count, plan.slices, sq, nullptr, 0, nullptr, 0, nullptr, 0.f, 0);
+    else if (p->dtype == AZ_F16) az_ortho_norm_kernel<1, false><<<grid, 256, 0, st>>>(p->update, p->update_stride, count, plan.slices, sq, nullptr, 0, nullptr, 0, nullptr, 0.f, 0);
+    else az_ortho_norm_kernel<2, false><<<grid, 256, 0, st>>>(p->update, p->update_stride, count, plan.slices, sq, nullptr, 0, nullptr, 0, nullptr, 0.f, 0);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return ofail(AZ_E_HIP, "az_orthogonalize_dev: launch failed: %s", hipGetErrorString(e));
     OrthoDev d = {};
@@ -559,7 +651,7 @@ extern "C" int az_muon_step_dev(const az_muon_step_args* p, void* workspace, siz
     const Span wo = span_of(p->weight_out, p->weight_out_stride, p->n, p->rows, p->cols, 4), mo = span_of(p->momentum_out, p->momentum_out_stride, p->n, p->rows, p->cols, 4);
     if ((meet(w, wo) && !same(w, wo)) || (meet(m, mo) && !same(m, mo)) || meet(wo, mo) || meet(wo, m) || meet(mo, w) || meet(g, wo) || meet(g, mo))
         return ofail(AZ_E_ARG, "an output overlaps another tensor (in place means the same address and stride)");
-    const Plan plan = make_plan(p->n, p->rows, p->cols, AZ_F32, p->steps, true);
+    const Plan plan = make_plan(p->n, p->rows, p->cols, AZ_F32, p->steps, p->a, p->b, p->c, true);
     if ((rc = check_ws(workspace, workspace_bytes, plan.bytes + 256)) != AZ_OK) return rc;
     AzDeviceGuard dev(p->device);
     if (!dev.ok) return ofail(AZ_E_HIP, "device %d cannot be used (no HIP device: libazhip has no CPU fallback)", p->device);
@@ -569,7 +661,7 @@ extern "C" int az_muon_step_dev(const az_muon_step_args* p, void* workspace, siz
     float* u = (float*)(ws + plan.off_u);
     const dim3 grid(plan.slices, p->n);
     const int count = p->rows * p->cols;
-#define NORM(DT) az_ortho_norm_kernel<DT><<<grid, 256, 0, st>>>(p->grad, p->grad_stride, count, plan.slices, sq, p->momentum, p->momentum_stride, \
+#define NORM(DT) az_ortho_norm_kernel<DT, true><<<grid, 256, 0, st>>>(p->grad, p->grad_stride, count, plan.slices, sq, p->momentum, p->momentum_stride, \
                                                                 p->momentum_out, p->momentum_out_stride, u, p->beta, p->nesterov)
     if (p->grad_dtype == AZ_F32) NORM(0);
     else if (p->grad_dtype == AZ_F16) NORM(1);
