@@ -28,7 +28,9 @@ int ofail(int code, const char* fmt, ...) {
 }
 
 constexpr float SA = 256.f, SQ = 16.f;        // scales of the pairs: A, P and A P (at most about 4), Q (a^5 = 485)
-constexpr int KSTEP = 32;                     // contraction of one step of a tile product
+// Contraction of one step of a tile product: 64 halves are a whole 128-byte line of a row; tiles of 128 would then leave
+// LDS for one workgroup a CU.
+template <int TILE> constexpr int kstep() { return TILE == 64 ? 64 : 32; }
 constexpr int MAX_SLICES = 256;               // pieces of a matrix whose squares are summed apart
 constexpr int SRC_PAIR = 3;                   // operand kinds: AZ_F32, AZ_F16, AZ_BF16, or pairs
 
@@ -134,6 +136,7 @@ __device__ __forceinline__ void split(float x, short& hi, short& lo) { hi = az_t
 // carries pieces of 8 elements of a line, as they lie in memory (the loads are unconditional, clamped into the matrix, and
 // stay in flight over a step's products), and splits them into hi (and lo) halves on their way to LDS.
 template <int TILE, int SRC, bool ALONG> struct Operand {
+    static constexpr int KSTEP = kstep<TILE>();
     static constexpr int PARTS = SRC == 0 || SRC == SRC_PAIR ? 2 : 1, RAW = PARTS;
     static constexpr int LD = ALONG ? KSTEP + 8 : TILE + 16;
     static constexpr int LINES = ALONG ? TILE : KSTEP, PER = (ALONG ? KSTEP : TILE) / 8;
@@ -214,9 +217,9 @@ template <int TILE, int SRC, bool ALONG> struct Operand {
             }
         }
     }
-    static __device__ __forceinline__ az_i4 frag(const short* s, int part, int t, int lane) {
-        if constexpr (ALONG) return az_row_frag<1>(s + part * HALVES, LD, t, 0, lane);
-        else return az_col_frag<1>(s + part * HALVES, LD, 0, t, lane);
+    static __device__ __forceinline__ az_i4 frag(const short* s, int part, int t, int k, int lane) {
+        if constexpr (ALONG) return az_row_frag<1>(s + part * HALVES, LD, t, k, lane);
+        else return az_col_frag<1>(s + part * HALVES, LD, k, t, lane);
     }
 };
 
@@ -234,22 +237,28 @@ __device__ __forceinline__ void lower_tile(int i, int& ti, int& tj) {
 //   GRAM_*      M = N = rows of X: lower triangle
 //   APPLY_WIDE  M = columns of X, N = rows of Q;   APPLY_TALL  M = rows of Q, N = rows of X as stored (columns of X)
 template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256, 2) az_ortho_product_kernel(OrthoDev d, const short* ma, const short* na, short* res,
-                                                                                                 const short* ma2, const short* na2, short* res2, int epi, float sr, float sr2) {
+                                                                                                 const short* ma2, const short* na2, short* res2, int epi, float sr, float sr2, int n) {                                      // n: tiles of a matrix
     constexpr bool GRAM = MODE == GRAM_WIDE || MODE == GRAM_TALL;
     constexpr int MS = MODE == SYM || MODE == APPLY_TALL ? SRC_PAIR : DT, NS = MODE == SYM || MODE == APPLY_WIDE ? SRC_PAIR : DT;
     constexpr bool MA = !(MODE == GRAM_TALL || MODE == APPLY_WIDE), NA = MODE != GRAM_TALL;
     typedef Operand<TILE, MS, MA> OM;
     typedef Operand<TILE, NS, NA> ON;
+    constexpr int KSTEP = kstep<TILE>();
     constexpr int WT = TILE / 2 / 16;                                // 16 x 16 tiles of a wave, each way
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr int STAGE = OM::PARTS * OM::HALVES + ON::PARTS * ON::HALVES;
     short* lds = (short*)smem;                                       // two stages
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
-    int z = blockIdx.z, m0, n0, k_lo = 0, k_hi, sp = 0;
+    // Workgroups go to the 8 XCDs in turn; each XCD gets a run of tiles, so that the panels that neighbouring tiles (and
+    // the next launch's products of the same matrix) read are in its own L2.
+    const int total = gridDim.x, run = total / 8, rest = total % 8, xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+    const int tile = xcd * run + min(xcd, rest) + at;
+    int z, m0, n0, k_lo = 0, k_hi, sp = 0;
     const size_t plane = (size_t)d.rp * d.rp;
     if constexpr (MODE == SYM || GRAM) {
         int ti, tj;
-        lower_tile(blockIdx.x, ti, tj);
+        z = tile / n;
+        lower_tile(tile - z * n, ti, tj);
         m0 = tj * TILE; n0 = ti * TILE;
         if constexpr (GRAM) {
             sp = blockIdx.y;
@@ -261,9 +270,12 @@ template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256, 2) 
             k_hi = (d.r + TILE - 1) / TILE * TILE;                  // (what lies behind, up to rp, is never written)
         }
     } else {
-        // APPLY: x runs over the long side
-        m0 = (MODE == APPLY_WIDE ? blockIdx.x : blockIdx.y) * TILE;
-        n0 = (MODE == APPLY_WIDE ? blockIdx.y : blockIdx.x) * TILE;
+        // APPLY: neighbours differ in the rows of Q and share the piece of X
+        const int sides = (d.r + TILE - 1) / TILE;
+        z = tile / n;
+        const int t = tile - z * n, l = t / sides, o = t - l * sides;
+        m0 = (MODE == APPLY_WIDE ? l : o) * TILE;
+        n0 = (MODE == APPLY_WIDE ? o : l) * TILE;
         k_hi = (d.r + KSTEP - 1) / KSTEP * KSTEP;
     }
     int e = 0;
@@ -280,39 +292,53 @@ template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256, 2) 
     #pragma unroll
     for (int i = 0; i < WT; ++i)
         for (int j = 0; j < WT; ++j) acc[i][j] = az_f4{0.f, 0.f, 0.f, 0.f};
-    OM om;
-    ON on;
-    om.load(mp, mlo, mld, m0, k_lo, d.rows, d.cols, tid);
-    on.load(np, nlo, nld, n0, k_lo, d.rows, d.cols, tid);
-    int buf = 0;
+    // AHEAD steps of operands wait in registers: a step's products take a few hundred cycles, a load a few thousand
+    constexpr int AHEAD = 2;
+    OM om[AHEAD];
+    ON on[AHEAD];
+    #pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+        if (k_lo + u * KSTEP < k_hi) {
+            om[u].load(mp, mlo, mld, m0, k_lo + u * KSTEP, d.rows, d.cols, tid);
+            on[u].load(np, nlo, nld, n0, k_lo + u * KSTEP, d.rows, d.cols, tid);
+        }
     const int mw = (wave & 1) * TILE / 2, nw = (wave >> 1) * TILE / 2;
-    #pragma unroll 1
-    for (int k = k_lo; k < k_hi; k += KSTEP, buf ^= 1) {
+    const auto step = [&](int k, OM& om, ON& on, int buf) __attribute__((always_inline)) {
         short* sm = lds + buf * STAGE;
         short* sn = sm + OM::PARTS * OM::HALVES;
         om.store(sm, m0, k, d.rows, d.cols, up, tid);
         on.store(sn, n0, k, d.rows, d.cols, up, tid);
-        if (k + KSTEP < k_hi) {
-            om.load(mp, mlo, mld, m0, k + KSTEP, d.rows, d.cols, tid);
-            on.load(np, nlo, nld, n0, k + KSTEP, d.rows, d.cols, tid);
+        if (k + AHEAD * KSTEP < k_hi) {
+            om.load(mp, mlo, mld, m0, k + AHEAD * KSTEP, d.rows, d.cols, tid);
+            on.load(np, nlo, nld, n0, k + AHEAD * KSTEP, d.rows, d.cols, tid);
         }
         __syncthreads();                                             // (the other stage was last read before this barrier)
-        az_i4 mf[WT][OM::PARTS];
         #pragma unroll
-        for (int i = 0; i < WT; ++i)
-            for (int p = 0; p < OM::PARTS; ++p) mf[i][p] = OM::frag(sm, p, mw + i * 16, lane);
-        #pragma unroll
-        for (int j = 0; j < WT; ++j) {
-            az_i4 nf[ON::PARTS];
+        for (int kk = 0; kk < KSTEP; kk += 32) {
+            az_i4 mf[WT][OM::PARTS];
             #pragma unroll
-            for (int p = 0; p < ON::PARTS; ++p) nf[p] = ON::frag(sn, p, nw + j * 16, lane);
+            for (int i = 0; i < WT; ++i)
+                #pragma unroll
+                for (int p = 0; p < OM::PARTS; ++p) mf[i][p] = OM::frag(sm, p, mw + i * 16, kk, lane);
             #pragma unroll
-            for (int i = 0; i < WT; ++i) {
-                acc[i][j] = az_mma<1>(mf[i][0], nf[0], acc[i][j]);
-                if constexpr (ON::PARTS == 2) acc[i][j] = az_mma<1>(mf[i][0], nf[1], acc[i][j]);
-                if constexpr (OM::PARTS == 2) acc[i][j] = az_mma<1>(mf[i][1], nf[0], acc[i][j]);
+            for (int j = 0; j < WT; ++j) {
+                az_i4 nf[ON::PARTS];
+                #pragma unroll
+                for (int p = 0; p < ON::PARTS; ++p) nf[p] = ON::frag(sn, p, nw + j * 16, kk, lane);
+                #pragma unroll
+                for (int i = 0; i < WT; ++i) {
+                    acc[i][j] = az_mma<1>(mf[i][0], nf[0], acc[i][j]);
+                    if constexpr (ON::PARTS == 2) acc[i][j] = az_mma<1>(mf[i][0], nf[1], acc[i][j]);
+                    if constexpr (OM::PARTS == 2) acc[i][j] = az_mma<1>(mf[i][1], nf[0], acc[i][j]);
+                }
             }
         }
+    };
+    #pragma unroll 1
+    for (int k = k_lo; k < k_hi; k += AHEAD * KSTEP) {
+        #pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (k + u * KSTEP < k_hi) step(k + u * KSTEP, om[u], on[u], u & 1);
     }
     #pragma unroll
     for (int i = 0; i < WT; ++i)
@@ -368,23 +394,28 @@ template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256, 2) 
         }
 }
 
-// The slices of a contraction that was split, added in their order: A as pairs, both triangles.
+// The slices of a contraction that was split, added in their order: A as pairs, both triangles.  Four entries of a row a
+// thread, all slices' loads in flight.
 __global__ void __launch_bounds__(256) az_ortho_join_kernel(OrthoDev d, int tile) {
     int ti, tj;
     lower_tile(blockIdx.x, ti, tj);
-    const int z = blockIdx.z;
+    const int z = blockIdx.z, i = (blockIdx.y * 256 + threadIdx.x) * 4;
     const size_t plane = (size_t)d.rp * d.rp;
     short* hi = d.A + (size_t)z * 2 * plane;
     short* lo = hi + plane;
-    for (int i = threadIdx.x + blockIdx.y * 256; i < tile * tile; i += 256 * gridDim.y) {
-        const int nn = ti * tile + i / tile, m = tj * tile + i % tile;
-        float v = 0.f;
-        for (int s = 0; s < d.split; ++s) v += d.partial[((size_t)z * d.split + s) * plane + (size_t)nn * d.rp + m];
-        short h, l;
-        split(v * SA, h, l);
-        hi[(size_t)nn * d.rp + m] = h; lo[(size_t)nn * d.rp + m] = l;
-        if (ti != tj) { hi[(size_t)m * d.rp + nn] = h; lo[(size_t)m * d.rp + nn] = l; }
-    }
+    const int nn = ti * tile + i / tile, m = tj * tile + i % tile;
+    const float* p = d.partial + (size_t)z * d.split * plane + (size_t)nn * d.rp + m;
+    az_f4 v = {0.f, 0.f, 0.f, 0.f};
+    #pragma unroll 8
+    for (int s = 0; s < d.split; ++s) v += *(const az_f4*)(p + s * plane);
+    az_s4 h, l;
+    #pragma unroll
+    for (int t = 0; t < 4; ++t) { short x, y; split(v[t] * SA, x, y); h[t] = x; l[t] = y; }
+    *(az_s4*)(hi + (size_t)nn * d.rp + m) = h;
+    *(az_s4*)(lo + (size_t)nn * d.rp + m) = l;
+    if (ti != tj)
+        #pragma unroll
+        for (int t = 0; t < 4; ++t) { hi[(size_t)(m + t) * d.rp + nn] = h[t]; lo[(size_t)(m + t) * d.rp + nn] = l[t]; }
 }
 
 // no step at all: Q = I
@@ -428,9 +459,9 @@ Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b
     const long long count = (long long)rows * cols;
     p.slices = (int)(count / 4096 < 1 ? 1 : count / 4096 > MAX_SLICES ? MAX_SLICES : count / 4096);
     while (p.slices > 64 && (long long)p.slices * n > 2048) p.slices /= 2;
-    const int ksteps = (p.k + KSTEP - 1) / KSTEP;
+    const int ksteps = (p.k + 63) / 64;
     p.split = 1;
-    while (p.split < 16 && (long long)p.low * n * p.split < 256 && ksteps / (p.split * 2) >= 4) p.split *= 2;
+    while (p.split < 16 && (long long)p.low * n * p.split < 512 && ksteps / (p.split * 2) >= 4) p.split *= 2;
     // Steps between two formations of X.  fp32 results: three (comment at the top); 16-bit results: five, their own rounding
     // is larger; fewer where the coefficients would take Q out of fp16's range.
     p.stage = dtype == AZ_F32 || muon ? 3 : 5;
@@ -449,6 +480,7 @@ Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b
 }
 
 struct Pairs { const short *m, *n; short* out; float scale; };       // one product: operands, result, scale (of EPI_PAIR / EPI_POLY)
+// grid x: tiles of a matrix, z: matrices (one dimension of the launch), y: slices or products
 template <int TILE, int DT, int MODE> hipError_t product(const OrthoDev& d, dim3 grid, Pairs one, Pairs two, int epi, hipStream_t st) {
     constexpr int MS = MODE == SYM || MODE == APPLY_TALL ? SRC_PAIR : DT, NS = MODE == SYM || MODE == APPLY_WIDE ? SRC_PAIR : DT;
     typedef Operand<TILE, MS, !(MODE == GRAM_TALL || MODE == APPLY_WIDE)> OM;
@@ -458,7 +490,7 @@ template <int TILE, int DT, int MODE> hipError_t product(const OrthoDev& d, dim3
         const hipError_t e = hipFuncSetAttribute((const void*)az_ortho_product_kernel<TILE, DT, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    az_ortho_product_kernel<TILE, DT, MODE><<<grid, 256, lds, st>>>(d, one.m, one.n, one.out, two.m, two.n, two.out, epi, one.scale, two.scale);
+    az_ortho_product_kernel<TILE, DT, MODE><<<dim3(grid.x * grid.z, grid.y), 256, lds, st>>>(d, one.m, one.n, one.out, two.m, two.n, two.out, epi, one.scale, two.scale, (int)grid.x);
     return hipGetLastError();
 }
 
@@ -474,7 +506,7 @@ template <int TILE, int DT> hipError_t gram(const Plan& p, const OrthoDev& d, hi
     return e;
 }
 template <int TILE, int DT> hipError_t apply(const Plan& p, const OrthoDev& d, hipStream_t st) {
-    const dim3 grid((p.k + TILE - 1) / TILE, (p.r + TILE - 1) / TILE, p.n);
+    const dim3 grid((p.k + TILE - 1) / TILE * ((p.r + TILE - 1) / TILE), 1, p.n);
     return p.rows <= p.cols ? product<TILE, DT, APPLY_WIDE>(d, grid, Pairs{nullptr, d.Q, nullptr, 1.f}, Pairs{}, 0, st)
                             : product<TILE, DT, APPLY_TALL>(d, grid, Pairs{d.Q, nullptr, nullptr, 1.f}, Pairs{}, 0, st);
 }
