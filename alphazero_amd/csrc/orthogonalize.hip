@@ -426,6 +426,156 @@ __global__ void __launch_bounds__(256) az_ortho_identity_kernel(short* Q, int rp
         q[i] = i < plane && i / rp == i % rp ? az_to16<1>(SQ) : (short)0;
 }
 
+// All of a stage's steps for matrices of up to R = 64 or 128 rows, one workgroup a matrix: A and P lie in LDS as pairs, Q in
+// registers, A P takes A's place.  Launched one product at a time these cost a launch and a trip to L2 each (5 us) for
+// 1 to 2 us of matrix instructions.  A wave holds 16 columns of Q as operands: the product P Q leaves rows 4 g .. 4 g + 3 of
+// the tiles 2 s, 2 s + 1 in lane group g, which is a fragment of step s whose contraction runs over those rows in that order,
+// and P's rows are read in the same order.
+template <int R> __global__ void __launch_bounds__(R * 4) az_ortho_iterate_kernel(OrthoDev d, int m) {
+    constexpr int LD = R + 8, PLANE = R * LD, KS = R / 32, MT = R / 16, WM = R / 32, WN = 2, NTH = R * 4;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    short* const A = (short*)smem;                                   // [hi, lo][R][LD]
+    short* const P = A + 2 * PLANE;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, z = blockIdx.x;
+    const size_t plane = (size_t)d.rp * d.rp;
+    {
+        const short* src = d.A + (size_t)z * 2 * plane;
+        constexpr int PIECES = 2 * R * R / 8 / NTH;
+        az_i4 v[PIECES];
+        #pragma unroll
+        for (int i = 0; i < PIECES; ++i) v[i] = ((const az_i4*)src)[tid + i * NTH];          // rp = R: both planes in one run
+        #pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int e = (tid + i * NTH) * 8, part = e / (R * R), row = e % (R * R) / R;
+            *(az_i4*)(A + part * PLANE + row * LD + e % R) = v[i];
+        }
+    }
+    const int m0 = (wave & 1) * (R / 2), n0 = (wave >> 1) * 32;      // a wave's block of a product: R / 2 rows (M) by 32 (N)
+    az_i4 qf[KS][2];                                                 // Q's columns 16 wave .. as operands
+    az_f4 acc[WM][WN], qa[MT];
+    const auto square = [&](const short* M, const short* N) __attribute__((always_inline)) {
+        #pragma unroll
+        for (int i = 0; i < WM; ++i)
+            #pragma unroll
+            for (int j = 0; j < WN; ++j) acc[i][j] = az_f4{0.f, 0.f, 0.f, 0.f};
+        #pragma unroll
+        for (int k = 0; k < R; k += 32) {
+            az_i4 mf[WM][2], nf[WN][2];
+            #pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                #pragma unroll
+                for (int i = 0; i < WM; ++i) mf[i][p] = az_row_frag<1>(M + p * PLANE, LD, m0 + i * 16, k, lane);
+                #pragma unroll
+                for (int j = 0; j < WN; ++j) nf[j][p] = az_row_frag<1>(N + p * PLANE, LD, n0 + j * 16, k, lane);
+            }
+            #pragma unroll
+            for (int i = 0; i < WM; ++i)
+                #pragma unroll
+                for (int j = 0; j < WN; ++j) {
+                    acc[i][j] = az_mma<1>(mf[i][0], nf[j][0], acc[i][j]);
+                    acc[i][j] = az_mma<1>(mf[i][0], nf[j][1], acc[i][j]);
+                    acc[i][j] = az_mma<1>(mf[i][1], nf[j][0], acc[i][j]);
+                }
+        }
+    };
+    // entry (n, m .. m + 3) of the symmetric result
+    const auto put = [&](short* D, int i, int j, az_f4 v) __attribute__((always_inline)) {
+        az_s4 h, l;
+        #pragma unroll
+        for (int t = 0; t < 4; ++t) { short x, y; split(v[t], x, y); h[t] = x; l[t] = y; }
+        short* at = D + (n0 + j * 16 + (lane & 15)) * LD + m0 + i * 16 + q * 4;
+        *(az_s4*)at = h;
+        *(az_s4*)(at + PLANE) = l;
+    };
+    const auto put_all = [&](short* D, float scale) __attribute__((always_inline)) {
+        #pragma unroll
+        for (int i = 0; i < WM; ++i)
+            #pragma unroll
+            for (int j = 0; j < WN; ++j) put(D, i, j, acc[i][j] * scale);
+    };
+    #pragma unroll 1
+    for (int step = 0; step < m; ++step) {
+        __syncthreads();                                             // A is there
+        square(A, A);
+        #pragma unroll
+        for (int i = 0; i < WM; ++i)
+            #pragma unroll
+            for (int j = 0; j < WN; ++j) {                           // P = a I + b A + c A A at scale SA
+                const int nn = n0 + j * 16 + (lane & 15), mm = m0 + i * 16 + q * 4;
+                const az_s4 h = *(const az_s4*)(A + nn * LD + mm), l = *(const az_s4*)(A + PLANE + nn * LD + mm);
+                az_f4 v;
+                #pragma unroll
+                for (int t = 0; t < 4; ++t) v[t] = (mm + t == nn ? d.a * SA : 0.f) + d.b * (az_from16<1>(h[t]) + az_from16<1>(l[t])) + d.c * (acc[i][j][t] * (1.f / SA));
+                put(P, i, j, v);
+            }
+        __syncthreads();
+        // Q <- P Q (columns 16 wave ..); the first step's Q is P itself
+        #pragma unroll
+        for (int i = 0; i < MT; ++i) qa[i] = az_f4{0.f, 0.f, 0.f, 0.f};
+        if (step == 0) {
+            #pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const short* at = P + (wave * 16 + (lane & 15)) * LD + i * 16 + q * 4;
+                const az_s4 h = *(const az_s4*)at, l = *(const az_s4*)(at + PLANE);
+                #pragma unroll
+                for (int t = 0; t < 4; ++t) qa[i][t] = (az_from16<1>(h[t]) + az_from16<1>(l[t])) * (SQ / SA);
+            }
+        } else {
+            #pragma unroll
+            for (int k = 0; k < KS; ++k)
+                #pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    az_i4 pf[2];
+                    #pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const short* at = P + p * PLANE + (i * 16 + (lane & 15)) * LD + k * 32 + q * 4;
+                        pf[p] = __builtin_bit_cast(az_i4, __builtin_shufflevector(*(const az_s4*)at, *(const az_s4*)(at + 16), 0, 1, 2, 3, 4, 5, 6, 7));
+                    }
+                    qa[i] = az_mma<1>(pf[0], qf[k][0], qa[i]);
+                    qa[i] = az_mma<1>(pf[0], qf[k][1], qa[i]);
+                    qa[i] = az_mma<1>(pf[1], qf[k][0], qa[i]);
+                }
+            #pragma unroll
+            for (int i = 0; i < MT; ++i) qa[i] *= 1.f / SA;
+        }
+        #pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            az_s8 h, l;
+            #pragma unroll
+            for (int t = 0; t < 8; ++t) { short x, y; split(qa[2 * k + (t >> 2)][t & 3], x, y); h[t] = x; l[t] = y; }
+            qf[k][0] = __builtin_bit_cast(az_i4, h);
+            qf[k][1] = __builtin_bit_cast(az_i4, l);
+        }
+        if (step + 1 < m) {
+            square(A, P);                                            // A P
+            __syncthreads();
+            put_all(A, 1.f / SA);
+            __syncthreads();
+            square(A, P);                                            // A P P
+            __syncthreads();
+            put_all(A, 1.f / SA);
+        }
+    }
+    short* out = d.Q + (size_t)z * 2 * plane + (size_t)(wave * 16 + (lane & 15)) * d.rp + q * 4;
+    #pragma unroll
+    for (int k = 0; k < KS; ++k)
+        #pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const az_s8 v = __builtin_bit_cast(az_s8, qf[k][p]);
+            *(az_s4*)(out + p * plane + k * 32) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+            *(az_s4*)(out + p * plane + k * 32 + 16) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+        }
+}
+template <int R> hipError_t iterate_in_lds(const OrthoDev& d, int n, int m, hipStream_t st) {
+    constexpr size_t lds = (size_t)4 * R * (R + 8) * 2;
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void*)az_ortho_iterate_kernel<R>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    az_ortho_iterate_kernel<R><<<n, R * 4, lds, st>>>(d, m);
+    return hipGetLastError();
+}
+
 struct Plan {
     int n, rows, cols, r, k, rp, tile, apply_tile, tiles, low, slices, split, stage;
     bool muon, restart;
@@ -524,6 +674,8 @@ template <int TILE> hipError_t iterate(const Plan& p, OrthoDev& d, int m, hipStr
     hipError_t e = hipSuccess;
 #define RUN(call) do { if (e == hipSuccess) e = (call); } while (0)
     if (m == 0) { az_ortho_identity_kernel<<<dim3(64, p.n), 256, 0, st>>>(d.Q, p.rp); return hipGetLastError(); }
+    if (p.rp == 64) return iterate_in_lds<64>(d, p.n, m, st);
+    if (p.rp == 128) return iterate_in_lds<128>(d, p.n, m, st);
     for (int i = 0; i < m; ++i) {
         const bool first = i == 0, last = i + 1 == m;
         // the first step's Q is its P, at Q's scale: written where it is wanted
