@@ -12,8 +12,9 @@ template <int DT, int OT, int CB> struct Lay {
     static constexpr int PAD = DT == 0 ? 4 : 16;                     // 16-bit rows: odd multiples of 32 bytes (az_col_frag), fp32: 16 bytes more
     static constexpr int LDT = OT * 16 + 4, LDO = OP + PAD;
     // channels are padded to what the kernel is built for: every LDS address is then a base and a constant
-    static constexpr int CP = CB * 128, LDC = CP + PAD, PIECES = CP / EP;
-    static constexpr size_t w_bytes = (size_t)OP * LDC * SZ, h_bytes = (size_t)ROWS * LDC * SZ;
+    // LDW: rows of w, read along only, 16 in one go: an odd multiple of 16 bytes
+    static constexpr int CP = CB * 128, LDC = CP + PAD, LDW = CP + EP, PIECES = CP / EP;
+    static constexpr size_t w_bytes = (size_t)OP * LDW * SZ, h_bytes = (size_t)ROWS * LDC * SZ;
     static constexpr size_t z_bytes = (size_t)ROWS * (LDO > LDT ? LDO : LDT) * 4;
 };
 
@@ -76,7 +77,7 @@ template <int DT, int OT, int CB> __device__ __forceinline__ void stage_w(const 
         #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = base + u * NT, o = i / per, c = (i - o * per) * EP;
-            if (i < total) *(az_i4*)((char*)wl + ((size_t)o * L::LDC + c) * L::SZ) = o < a.O && c < a.C ? v[u] : az_i4{0, 0, 0, 0};
+            if (i < total) *(az_i4*)((char*)wl + ((size_t)o * L::LDW + c) * L::SZ) = o < a.O && c < a.C ? v[u] : az_i4{0, 0, 0, 0};
         }
     }
 }
@@ -364,7 +365,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
     constexpr bool WLDS = w_in_lds<DT, OT, CB>();
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ az_f4 red[4 * ROWS];
-    constexpr int Cp = L::CP, ldc = L::LDC;
+    constexpr int Cp = L::CP;
     const Smem<DT, OT, CB, 0, WLDS> m(smem, a, a.counts ? WAVES * R::bytes : 0);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
     float* zt = m.t + wave * (R::bytes / 4);
@@ -413,7 +414,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                 };
                 const auto fetch = [&](int k, az_i4* w) __attribute__((always_inline)) {
                     #pragma unroll
-                    for (int j = 0; j < R::OTP; ++j) w[j] = WLDS ? az_row_frag<DT>(m.w, ldc, o0 + j * 16, k * L::KS, lane) : az_row_frag<DT>(a.wpad, Cp, o0 + j * 16, k * L::KS, lane);
+                    for (int j = 0; j < R::OTP; ++j) w[j] = WLDS ? az_row_frag<DT>(m.w, L::LDW, o0 + j * 16, k * L::KS, lane) : az_row_frag<DT>(a.wpad, Cp, o0 + j * 16, k * L::KS, lane);
                 };
                 product<KT, L::KS, R::OTP, !WLDS>(a.C, fetch, step);
                 // the wave's next tile: of this group, or the first of the next one (which the barriers between do not touch)
@@ -632,6 +633,9 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
     az_f4 db[OTH];
     #pragma unroll
     for (int j = 0; j < OTH; ++j) db[j] = az_f4{0.f, 0.f, 0.f, 0.f};
+    // fp32, more than 128 channels: a step's features are 32 registers a thread that the products need; they are asked for
+    // when the step before is done (on their way earlier they went through scratch memory, a load at a time)
+    constexpr bool EARLY = !(DT == 0 && CB == 2);
     Step st(a, s_lo);
     Feat<DT, NP, MODE> f;
     f.load(a, st, tid);
@@ -675,7 +679,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
     };
     if (!a.counts) targets(a, st);
     Step nx = st;
-    if (s_lo + 1 < s_hi) { nx.next(a); f.load(a, nx, tid); }
+    if (s_lo + 1 < s_hi) { nx.next(a); if (EARLY) f.load(a, nx, tid); }
     #pragma unroll 1
     for (int it = s_lo; it < s_hi; ++it) {
         const PolicyDev a = arguments();
@@ -710,11 +714,13 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             #pragma unroll
             for (int j = 0; j < OTH; ++j) {
                 const int ot = min(half * OTH + j, OT - 1);
-                if constexpr (WLDS) w[j] = az_row_frag<DT>(m.w, ldc, ot * 16, k * L::KS, lane);
+                if constexpr (WLDS) w[j] = az_row_frag<DT>(m.w, L::LDW, ot * 16, k * L::KS, lane);
                 else w[j] = az_row_frag<DT>(a.wpad, Cp, ot * 16, k * L::KS, lane);
             }
         };
+        __builtin_amdgcn_sched_barrier(0);                           // (phases apart: mixed, they want more registers than there are)
         product<KT, L::KS, OTH, !WLDS>(a.C, fetch, step);
+        __builtin_amdgcn_sched_barrier(0);
         const float rT = up * bst[1], lse2 = bst[0] * LOG2E;
         // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
         const bool bias_counts = a.O > 1 || bst[3] != 0.f;
@@ -747,11 +753,16 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         if (!a.counts && it + 1 < s_hi) targets(a, nx);
         // dh: rows of a tile are channels, columns are cells
         {
-            az_i4 zf[2][KO];
-            #pragma unroll
-            for (int k = 0; k < KO; ++k)
+            // (fp32: dz is read again for every tile of channels -- the LDS port is idle behind the fp32 matrix instructions,
+            // and the fragments of both row tiles would take 48 registers)
+            constexpr bool KEEP = DT != 0;
+            az_i4 zf[2][KEEP ? KO : 1];
+            if constexpr (KEEP) {
                 #pragma unroll
-                for (int e = 0; e < 2; ++e) zf[e][k] = az_row_frag<DT>(zhi, L::LDO, (pair * 2 + e) * 16, k * L::KS, lane);
+                for (int k = 0; k < KO; ++k)
+                    #pragma unroll
+                    for (int e = 0; e < 2; ++e) zf[e][k] = az_row_frag<DT>(zhi, L::LDO, (pair * 2 + e) * 16, k * L::KS, lane);
+            }
             #pragma unroll 1
             for (int j = 0; j < CB * 2; ++j) {
                 const int ct = cq + 4 * j;
@@ -760,10 +771,10 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                 #pragma unroll
                 for (int k = 0; k < KO; ++k) {
                     az_i4 wa;
-                    if constexpr (WLDS) wa = az_col_frag<DT>(m.w, ldc, k * L::KS, ct * 16, lane);
+                    if constexpr (WLDS) wa = az_col_frag<DT>(m.w, L::LDW, k * L::KS, ct * 16, lane);
                     else wa = az_row_frag<DT>(a.wpadt, L::OP, ct * 16, k * L::KS, lane);
-                    d[0] = az_mma<DT>(wa, zf[0][k], d[0]);
-                    d[1] = az_mma<DT>(wa, zf[1][k], d[1]);
+                    d[0] = az_mma<DT>(wa, KEEP ? zf[0][KEEP ? k : 0] : az_row_frag<DT>(zhi, L::LDO, pair * 32, k * L::KS, lane), d[0]);
+                    d[1] = az_mma<DT>(wa, KEEP ? zf[1][KEEP ? k : 0] : az_row_frag<DT>(zhi, L::LDO, pair * 32 + 16, k * L::KS, lane), d[1]);
                 }
                 const int c = ct * 16 + q * 4;
                 #pragma unroll
@@ -790,6 +801,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         #pragma unroll
         for (int k = 0; k < ROWS; k += L::KS) {
             if (k >= st.rows) break;
+            __builtin_amdgcn_sched_barrier(0);
             az_i4 zf[OTN][DT == 0 ? 1 : 2];
             #pragma unroll
             for (int j = 0; j < OTN; ++j) {
@@ -810,8 +822,9 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         }
         __syncthreads();                                             // everything of this step has been read
         if (it + 1 < s_hi) {
+            if (!EARLY) f.load(a, nx, tid);
             f.store(a, nx, h, tid);
-            if (it + 2 < s_hi) f.load(a, after, tid);
+            if (EARLY && it + 2 < s_hi) f.load(a, after, tid);
             if (nx.b0 == st.b0) __syncthreads();                     // (else the boards' staging ends in one)
         }
         if (it + 1 < s_hi && nx.b0 != st.b0) stage_boards<true>(a, m.b, nx.b0, tid);
@@ -908,7 +921,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
         #pragma unroll
         for (int j = 0; j < OT; ++j)
             #pragma unroll
-            for (int k = 0; k < KT; ++k) wr[j][k] = az_row_frag<DT>(m.h, ldc, j * 16, k * L::KS, lane);
+            for (int k = 0; k < KT; ++k) wr[j][k] = az_row_frag<DT>(m.h, L::LDW, j * 16, k * L::KS, lane);
         az_f4 db[OT];
         #pragma unroll
         for (int j = 0; j < OT; ++j) db[j] = az_f4{0.f, 0.f, 0.f, 0.f};
@@ -1021,7 +1034,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
         #pragma unroll
         for (int j = 0; j < 2; ++j)
             #pragma unroll
-            for (int k = 0; k < KO; ++k) wc[j][k] = pair_col_frag(m.h, ldc, k * L::KS, cq * 32 + 4 * j, lane);
+            for (int k = 0; k < KO; ++k) wc[j][k] = pair_col_frag(m.h, L::LDW, k * L::KS, cq * 32 + 4 * j, lane);
         az_f4 dw[2][OT];
         #pragma unroll
         for (int i = 0; i < 2; ++i)
