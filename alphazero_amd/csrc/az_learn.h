@@ -89,6 +89,7 @@ struct AzDeviceGuard {
     explicit AzDeviceGuard(int device) {
         if (hipGetDevice(&before) != hipSuccess) before = -1;
         ok = before == device || hipSetDevice(device) == hipSuccess;
+        if (!ok) (void)hipGetLastError();
     }
     ~AzDeviceGuard() { if (before >= 0) (void)hipSetDevice(before); }
 };

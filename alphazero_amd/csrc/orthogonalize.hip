@@ -799,6 +799,7 @@ extern "C" int az_orthogonalize_dev(const az_orthogonalize_args* p, void* worksp
     if ((rc = check_ws(workspace, workspace_bytes, plan.bytes + 256)) != AZ_OK) return rc;
     AzDeviceGuard dev(p->device);
     if (!dev.ok) return ofail(AZ_E_HIP, "device %d cannot be used (no HIP device: libazhip has no CPU fallback)", p->device);
+    (void)hipGetLastError();                                         // (an earlier call's error is not this one's)
     unsigned char* ws = (unsigned char*)workspace;
     hipStream_t st = (hipStream_t)stream;
     double* sq = (double*)(ws + plan.off_sq);
@@ -839,6 +840,7 @@ extern "C" int az_muon_step_dev(const az_muon_step_args* p, void* workspace, siz
     if ((rc = check_ws(workspace, workspace_bytes, plan.bytes + 256)) != AZ_OK) return rc;
     AzDeviceGuard dev(p->device);
     if (!dev.ok) return ofail(AZ_E_HIP, "device %d cannot be used (no HIP device: libazhip has no CPU fallback)", p->device);
+    (void)hipGetLastError();                                         // (an earlier call's error is not this one's)
     unsigned char* ws = (unsigned char*)workspace;
     hipStream_t st = (hipStream_t)stream;
     double* sq = (double*)(ws + plan.off_sq);

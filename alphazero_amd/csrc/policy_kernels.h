@@ -95,7 +95,6 @@ struct BoardLds {
     az_f4* stat;                                                     // [MAX_BOARDS] of the gradients: {lse, r T, r, is there a target that is not allowed}
     bool listed;                                                     // the entries fit
 };
-__host__ __device__ inline int entry_room(int nb, int cap) { return (long long)nb * cap <= ENTRIES ? nb * cap : 0; }
 // entries outside the board's actions: -1
 __device__ __forceinline__ int entry_key(const PolicyDev& a, int act, int bb) {
     if ((unsigned)act >= (unsigned)(a.O * a.S)) return -1;
@@ -240,7 +239,7 @@ template <int DT, int OT, int CB, int HBUF, bool WBUF> struct Smem {
         b.stat = (az_f4*)p; p += MAX_BOARDS * 16;
         b.words = (unsigned*)p; p += (size_t)a.nb * a.N * OT * 16 * 4;
         b.planes = OT * 16;
-        const int room = a.counts ? entry_room(a.nb, a.cap) : 0;
+        const int room = a.room;
         b.listed = room > 0;
         b.key = (int*)p; p += (size_t)room * 4;
         b.val = (float*)p; p += (size_t)room * 4;
@@ -248,7 +247,7 @@ template <int DT, int OT, int CB, int HBUF, bool WBUF> struct Smem {
         b.cnt = (int*)p;
     }
     static size_t bytes(const PolicyDev& a, size_t zb) {
-        const size_t room = a.counts ? (size_t)entry_room(a.nb, a.cap) : 0;
+        const size_t room = a.room;
         return (WBUF ? L::w_bytes : 0) + HBUF * L::h_bytes + zb + OT * 16 * 4 + MAX_BOARDS * 16 + (size_t)a.nb * a.N * OT * 16 * 4 +
                (room ? room * 8 + (BLOCKS + 1) * 4 + (room + 63) / 64 * BLOCKS * 4 : 0);
     }
@@ -385,9 +384,9 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             const PolicyDev a = arguments();
             const int rl = r0 + (lane & 15);
             const bool live = rl < rows;
-            const int bb = a.nb > 1 ? (int)((unsigned)min(rl, ROWS - 1) * a.mag_s >> 16) : 0, s = live ? rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
+            const int bb = live && a.nb > 1 ? (int)((unsigned)rl * a.mag_s >> 16) : 0, s = live ? rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
             const unsigned bit = live ? 1u << (s - y * a.N) : 0u;
-            const unsigned* words = m.b.words + ((live ? bb : 0) * a.N + y) * (OT * 16) + q * 4;
+            const unsigned* words = m.b.words + (bb * a.N + y) * (OT * 16) + q * 4;
             const float* dense = a.dense + (size_t)b0 * a.O * a.S;
             const int hi = min(r0 + 16, rows), e0 = m.b.listed ? m.b.start[r0 >> 6] : 0, e1 = m.b.listed ? m.b.start[(r0 >> 6) + 1] : min(a.nb, a.B - b0) * a.cap;
             int key0 = -1;
@@ -1136,29 +1135,29 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
     }
 }
 
-template <int DT, int OT, int CB, int MODE> hipError_t launch_products(const PolicyDev& a, bool grad, int& groups, hipStream_t stream) {
+template <int DT, int OT, int CB, int MODE> hipError_t launch_products(PolicyDev a, bool grad, int& groups, hipStream_t stream) {
     constexpr bool PAIR = DT != 0 && CB == 1 && OT <= 6;              // (more planes: w's shares do not fit the registers)
-    size_t lds;
+    const auto bytes = [&]() -> size_t {
+        if (!grad) return Smem<DT, OT, CB, 0, w_in_lds<DT, OT, CB>()>::bytes(a, a.counts ? WAVES * LossTile<OT>::bytes : 0) + 4 * ROWS * 16;   // (and the kernel's `red`)
+        if constexpr (PAIR) return Smem<DT, OT, 1, 3, false>::bytes(a, PairCfg<DT, OT>::zb(a));
+        else return Smem<DT, OT, CB, 1, w_in_lds<DT, OT, CB>()>::bytes(a, Lay<DT, OT, CB>::z_bytes);
+    };
+    size_t lds = bytes();
+    if (lds > LDS_BYTES) { a.room = 0; lds = bytes(); }              // the longest lists with the largest boards and heads: targets read from memory
+    if (lds > LDS_BYTES) return hipErrorInvalidConfiguration;
     const void* fn;
-    if (!grad) {
-        lds = Smem<DT, OT, CB, 0, w_in_lds<DT, OT, CB>()>::bytes(a, a.counts ? WAVES * LossTile<OT>::bytes : 0);
-        fn = (const void*)az_policy_loss_kernel<DT, OT, CB, MODE>;
-    } else if constexpr (PAIR) {
-        lds = Smem<DT, OT, 1, 3, false>::bytes(a, PairCfg<DT, OT>::zb(a));
-        fn = (const void*)az_policy_grad16_kernel<DT, OT, MODE>;
-    } else {
-        lds = Smem<DT, OT, CB, 1, w_in_lds<DT, OT, CB>()>::bytes(a, Lay<DT, OT, CB>::z_bytes);
-        fn = (const void*)az_policy_grad_kernel<DT, OT, CB, MODE>;
-    }
+    if (!grad) fn = (const void*)az_policy_loss_kernel<DT, OT, CB, MODE>;
+    else if constexpr (PAIR) fn = (const void*)az_policy_grad16_kernel<DT, OT, MODE>;
+    else fn = (const void*)az_policy_grad_kernel<DT, OT, CB, MODE>;
     if (lds > 32 * 1024) {
         const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
     if (!grad) {
         // as many workgroups as the chip holds at once, the boards in even shares
-        const int per_cu = loss_waves<DT, OT, CB>() * 4 / WAVES >= 2 && (lds + 4 * ROWS * 16) * 2 <= LDS_BYTES ? 2 : 1;
+        const int per_cu = loss_waves<DT, OT, CB>() * 4 / WAVES >= 2 && lds * 2 <= LDS_BYTES ? 2 : 1;
         const int work = (a.B + a.nb - 1) / a.nb, room = CUS * per_cu, rounds = (work + room - 1) / room;
-        az_policy_loss_kernel<DT, OT, CB, MODE><<<(work + rounds - 1) / rounds, NT, lds, stream>>>(a, work);
+        az_policy_loss_kernel<DT, OT, CB, MODE><<<(work + rounds - 1) / rounds, NT, lds - 4 * ROWS * 16, stream>>>(a, work);
     } else {
         if (lds * 2 > LDS_BYTES && groups > CUS) groups = CUS;       // one workgroup a CU
         if constexpr (PAIR) az_policy_grad16_kernel<DT, OT, MODE><<<groups, NT, lds, stream>>>(a);

@@ -37,6 +37,7 @@ struct PolicyDev {
     const float *wpad, *wpadt;               // fp32 weights that do not fit LDS: padded copies
     void* dh;
     int B, N, S, C, O, cap, nchw;
+    int room;                                // sparse targets that LDS has room for: those of a workgroup's boards, or 0 = read from memory
     int nb, blocks;                          // boards a workgroup takes at once (blocks = 1), or steps a board is cut into (nb = 1)
     int steps;                               // of the gradient kernel
     unsigned mag_n, mag_s, mag_w;            // x / N = x * mag_n >> 16 for x < 1024 = x * mag_w >> 20 for x < 4096, x / S = x * mag_s >> 16 for x < 64

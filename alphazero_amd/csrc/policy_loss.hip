@@ -107,12 +107,18 @@ extern "C" int az_policy_loss_dev(const az_policy_loss_args* p, void* workspace,
              (size_t)p->d_weight | (size_t)p->d_bias) % 4) return lfail(AZ_E_ARG, "a tensor is not aligned to its element type");
     }
     if ((size_t)p->stats % 16) return lfail(AZ_E_ARG, "stats needs 16-byte alignment");
+    if (p->B > 0 && p->d_features) {                                 // (features are read while gradients of other boards are written)
+        const size_t n = (size_t)p->B * p->N * p->N * p->C * (p->dtype == AZ_F32 ? 4 : 2);
+        const char *f = (const char*)p->features, *d = (const char*)p->d_features;
+        if (f < d + n && d < f + n) return lfail(AZ_E_ARG, "d_features overlaps features");
+    }
     const size_t need = az_policy_loss_workspace(p);
     if (!workspace) return lfail(AZ_E_ARG, "null argument: workspace");
     if ((size_t)workspace % 256) return lfail(AZ_E_ARG, "workspace needs 256-byte alignment");
     if (workspace_bytes < need) return lfail(AZ_E_CAPACITY, "workspace has %zu bytes, az_policy_loss_workspace asks for %zu", workspace_bytes, need);
     AzDeviceGuard dev(p->device);
     if (!dev.ok) return lfail(AZ_E_HIP, "device %d cannot be used (no HIP device: libazhip has no CPU fallback)", p->device);
+    (void)hipGetLastError();                                         // (an earlier call's error is not this one's)
     hipStream_t st = (hipStream_t)stream;
     PolicyDev a = {};
     a.h = p->features; a.w = p->weight; a.bias = p->bias; a.dense = p->target; a.counts = p->counts; a.actions = p->actions; a.probs = p->probs;
@@ -121,6 +127,7 @@ extern "C" int az_policy_loss_dev(const az_policy_loss_args* p, void* workspace,
     long long steps;
     geometry(p->B, p->N, a.nb, a.blocks, steps);
     a.steps = (int)steps;
+    a.room = a.counts && (long long)a.nb * a.cap <= ENTRIES ? a.nb * a.cap : 0;
     a.mag_n = (65536 + a.N - 1) / a.N; a.mag_s = (65536 + a.S - 1) / a.S; a.mag_w = ((1u << 20) + a.N - 1) / a.N;
     unsigned char* ws = (unsigned char*)workspace;
     a.stats = p->stats ? (az_f4*)p->stats : (az_f4*)ws; ws += up256((size_t)a.B * sizeof(az_f4));

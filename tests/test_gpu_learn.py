@@ -215,3 +215,273 @@ def test_optimiser_step_matches_the_formula(shape, nesterov, gdtype):
     w2, m3 = torch.empty_like(wg), torch.empty_like(mg)
     learn.muon_step(w.cuda(), mom.cuda(), grad.cuda(), lr=lr, beta=beta, nesterov=nesterov, weight_decay=wd, scale=scale, weight_out=w2, momentum_out=m3)
     assert torch.equal(w2, wg) and torch.equal(m3, mg)                                                        # in place and apart: the same bits
+
+
+# ---- the calls around the products: edges, streams, graphs, sizes -----------------------------------------------------------
+
+def _grad(p, scale=1.0, **kw):
+    x, w, b, tgt, words = _cuda(p)
+    return learn.policy_loss_grad(x, w, b, kw.get("tgt", tgt), row_scale=scale, legal=kw.get("words", words))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("N", [3, 9])
+def test_boards_without_targets_or_without_allowed_actions(N, dtype):
+    """No target: loss 0, no gradient.  No allowed action and no target: the same.  A target on an action that is not
+    allowed: loss inf, the gradient still finite and 0 at that entry."""
+    B, C, O = 6, 32, 3
+    p = _rows(B, N, C, O, dtype, legal=0.5, seed=5, empty=(1,))
+    p["ok"][2] = False                                    # nothing allowed, targets there: inf
+    p["ok"][3] = False
+    p["t"][3] = 0                                         # nothing allowed, no target
+    p["tgt"].view(B, -1)[3] = 0
+    p["ok"][4, 7] = False
+    p["t"][4, 7] = 0.25                                   # one target outside
+    p["tgt"].view(B, -1)[4, 7] = 0.25
+    bits = (p["ok"].view(B, O * N, N).long() << torch.arange(N)).sum(2)
+    p["words"] = bits.to(torch.int32)
+    loss, dx, dw, db = [v.cpu().double() for v in _grad(p)]
+    assert loss[1] == 0 and loss[3] == 0 and math.isinf(loss[2]) and math.isinf(loss[4]) and torch.isfinite(loss[[0, 5]]).all()
+    assert (dx[[1, 2, 3]] == 0).all()
+    assert torch.isfinite(dx).all() and torch.isfinite(dw).all() and torch.isfinite(db).all()
+    _check(p, _grad(p), torch.ones(B, dtype=torch.float64))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("layout", ["nchw", "nhwc"])
+def test_what_lies_behind_a_mask_does_not_matter_for_the_loss(layout, dtype):
+    """NaN and inf in the features of cells none of whose actions is allowed: the loss and the other cells' feature gradients
+    are those of a clean board."""
+    B, N, C, O = 3, 8, 64, 2
+    p = _rows(B, N, C, O, dtype, layout, legal=0.6, seed=9)
+    ok = p["ok"].view(B, O, N, N)
+    ok[:, :, 2, 3] = False
+    ok[:, :, 7, 7] = False
+    p["t"] = (p["t"].view(B, O, N, N) * ok).view(B, -1)
+    p["tgt"] = p["t"].float().view(B, O, N, N).contiguous()
+    p["words"] = (ok.reshape(B, O * N, N).long() << torch.arange(N)).sum(2).to(torch.int32)
+    clean = [v.cpu() for v in _grad(p)]
+    p["x"][:, :, 2, 3] = float("nan")
+    p["x"][:, :, 7, 7] = float("inf")
+    dirty = [v.cpu() for v in _grad(p)]
+    assert torch.equal(clean[0], dirty[0])
+    keep = torch.ones(N, N, dtype=torch.bool)
+    keep[2, 3] = keep[7, 7] = False
+    assert torch.equal(clean[1][:, :, keep], dirty[1][:, :, keep]) and (dirty[1][:, :, ~keep] == 0).all()
+
+
+def test_the_same_action_twice_entries_outside_and_counts_beyond_the_list():
+    B, N, C, O = 5, 9, 48, 4
+    A = O * N * N
+    p = _rows(B, N, C, O, "f32", "nhwc", sparse=True, seed=3, cap=12)
+    counts, acts, probs = p["tgt"]
+    counts[:] = torch.tensor([12, 12, 0, 99, -4], dtype=torch.int32)
+    acts[0, :6] = 17                                      # six times the same
+    acts[1, 3] = -1
+    acts[1, 4] = A
+    acts[1, 5] = 2 ** 31 - 1
+    acts[1, 6] = -2 ** 31
+    p["t"] = torch.zeros(B, A, dtype=torch.float64)
+    for r in range(B):
+        for e in range(max(0, min(int(counts[r]), 12))):
+            if 0 <= int(acts[r, e]) < A:
+                p["t"][r, acts[r, e]] += float(probs[r, e])
+    got = _grad(p)
+    _check(p, got, torch.ones(B, dtype=torch.float64))
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(got, _grad(p)))
+
+
+@pytest.mark.parametrize("case", [(2, 32, 256, 128, 1024, "f16"), (2, 32, 128, 128, 1024, "f32"), (1, 20, 128, 91, 5000, "bf16"), (3, 32, 128, 96, 1024, "bf16"),
+                                  (40, 2, 16, 5, 30, "f32"), (2, 4, 256, 128, 2048, "f16")], ids=lambda c: "b%d-n%d-c%d-o%d-cap%d-%s" % c)
+def test_long_target_lists_and_the_largest_heads(case):
+    B, N, C, O, cap, dtype = case
+    p = _rows(B, N, C, O, dtype, "nhwc", sparse=True, legal=0.3, seed=cap, cap=min(cap, 5000))
+    _check(p, _grad(p), torch.ones(B, dtype=torch.float64))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_tensors_at_odd_addresses(dtype):
+    """Views that are aligned to their element type only."""
+    B, N, C, O = 3, 7, 64, 5
+    p = _rows(B, N, C, O, dtype, "nhwc", seed=1)
+    x, w, b, tgt, _ = _cuda(p)
+
+    def shift(t):
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        buf[1:] = t.flatten()
+        return buf[1:].view(t.shape)
+    xs = shift(x.permute(0, 2, 3, 1).contiguous()).permute(0, 3, 1, 2)
+    got = learn.policy_loss_grad(xs, shift(w), shift(b), shift(tgt))
+    want = learn.policy_loss_grad(x, w, b, tgt)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    u = _mats(2, 33, 70, dtype).cuda()
+    assert torch.equal(learn.orthogonalize(shift(u)), learn.orthogonalize(u))
+
+
+def test_empty_batches():
+    x, w, b = torch.empty(0, 8, 5, 5, device="cuda"), torch.randn(2, 8, device="cuda"), torch.zeros(2, device="cuda")
+    t = torch.empty(0, 2, 5, 5, device="cuda")
+    assert learn.policy_loss(x, w, b, t).shape == (0,)
+    loss, dx, dw, db = learn.policy_loss_grad(x, w, b, t)
+    assert loss.shape == (0,) and dx.shape == x.shape and (dw == 0).all() and (db == 0).all()
+    assert learn.orthogonalize(torch.empty(0, 4, 6, device="cuda")).shape == (0, 4, 6)
+
+
+def test_autograd_gives_the_same_gradients_and_checks_its_inputs():
+    p = _rows(4, 9, 40, 3, "f32", legal=0.7, seed=8)
+    x, w, b, tgt, words = _cuda(p)
+    xr, wr, br = x.clone().requires_grad_(), w.view(3, 40, 1, 1).clone().requires_grad_(), b.clone().requires_grad_()
+    g = torch.tensor([0.5, -1.0, 2.0, 0.0], device="cuda")
+    (learn.policy_loss(xr, wr, br, tgt, legal=words) * g).sum().backward()
+    _, dx, dw, db = learn.policy_loss_grad(x, w, b, tgt, row_scale=g, legal=words)
+    assert torch.equal(xr.grad, dx) and torch.equal(wr.grad.view(3, 40), dw) and torch.equal(br.grad, db)
+    learn.policy_loss(xr, wr, br, tgt, legal=words).mean().backward()        # an expanded gradient
+    loss = learn.policy_loss(xr, wr, br, tgt, legal=words)
+    with torch.no_grad():
+        wr.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()
+
+
+def test_gradients_against_differences():
+    """d/dx and d/dw of the summed loss along random directions, central differences of the 64-bit loss."""
+    p = _rows(2, 5, 20, 3, "f32", seed=4)
+    _, dx, dw, db = [v.cpu().double() for v in _grad(p)]
+    r = torch.ones(2, dtype=torch.float64)
+    g = torch.Generator().manual_seed(0)
+    for key, d in (("x", dx), ("w", dw), ("b", db)):
+        v = torch.randn(p[key].shape, generator=g, dtype=torch.float64)
+        base, h, side = p[key], 1e-5, []
+        for s in (1, -1):
+            q = dict(p)
+            q[key] = base.double() + s * h * v
+            side.append(float(_exact(q, r)[0].sum()))
+        num = (side[0] - side[1]) / (2 * h)
+        assert abs(num - float((d * v).sum())) <= 1e-5 * float((d * v).abs().sum()) + 1e-7
+
+
+def test_another_stream_than_the_default_one():
+    p = _rows(32, 15, 128, 1, "bf16", "nhwc", seed=2)
+    want = _grad(p)
+    x, w, b, tgt, words = _cuda(p)
+    u = _mats(3, 100, 300, "f32").cuda()
+    o = learn.orthogonalize(u)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        xs = x * 1.0                                      # made on this stream: the call has to be ordered behind it
+        got = learn.policy_loss_grad(xs, w, b, tgt)
+        o2 = learn.orthogonalize(u * 1.0)
+    s.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(want, got)) and torch.equal(o, o2)
+
+
+def test_two_captured_steps_replayed_between_eager_ones():
+    """Forward, gradients and the optimiser step of two heads, each captured into a graph of its own, replayed several times
+    with other inputs, eager calls and synchronisations between the replays: every replay against the eager result."""
+    ps = [_rows(8, 9, 64, 3, "bf16", "nhwc", sparse=True, seed=s) for s in (1, 2)]
+    static, graphs = [], []
+    for p in ps:
+        x, w, b, tgt, _ = _cuda(p)
+        wm, mm = torch.randn(3, 64, device="cuda"), torch.zeros(3, 64, device="cuda")
+        st = dict(x=x, w=w, b=b, tgt=tgt, wm=wm, mm=mm)
+
+        def step(st=st):
+            st["loss"], st["dx"], st["dw"], st["db"] = learn.policy_loss_grad(st["x"], st["w"], st["b"], st["tgt"], row_scale=1.0 / 8)
+            st["wm2"], st["mm2"] = learn.muon_step(st["wm"], st["mm"], st["dw"], lr=0.1, weight_out=torch.empty_like(st["wm"]), momentum_out=torch.empty_like(st["mm"]))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step()
+        static.append(st)
+        graphs.append(g)
+    for rep in range(4):
+        for st in static:
+            st["x"].copy_((torch.randn(st["x"].shape, device="cuda") + rep).relu())
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for st in static:
+            loss, dx, dw, db = learn.policy_loss_grad(st["x"], st["w"], st["b"], st["tgt"], row_scale=1.0 / 8)
+            wm, mm = learn.muon_step(st["wm"].clone(), st["mm"].clone(), dw, lr=0.1)
+            for a, c in ((loss, st["loss"]), (dx, st["dx"]), (dw, st["dw"]), (db, st["db"]), (wm, st["wm2"]), (mm, st["mm2"])):
+                assert torch.equal(a, c)
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 features: the last boards of a large batch come out as alone."""
+    B, N, C = 21100, 20, 256
+    x = torch.zeros(B, N, N, C, dtype=torch.float16, device="cuda").permute(0, 3, 1, 2)
+    assert x.numel() > 2 ** 31
+    g = torch.Generator().manual_seed(0)
+    tail = torch.randn(3, C, N, N, generator=g).relu().half().cuda().contiguous(memory_format=torch.channels_last)
+    x[-3:] = tail
+    w, b = (torch.randn(1, C, generator=g) / 8).half().cuda(), torch.zeros(1, dtype=torch.float16, device="cuda")
+    t = torch.zeros(B, 1, N, N, device="cuda")
+    t[:, 0, 3, 4] = 1.0
+    loss, dx, _, _ = learn.policy_loss_grad(x, w, b, t)
+    l3, d3, _, _ = learn.policy_loss_grad(tail, w, b, t[-3:].contiguous())
+    assert torch.equal(loss[-3:], l3) and torch.equal(dx[-3:], d3)
+    assert torch.allclose(loss[:5], torch.full((5,), math.log(400.0), device="cuda"), rtol=1e-6)
+
+
+def test_weight_blob_in_place():
+    """The convolutions of all blocks as strided batches of a flat blob: one call each for conv1 and conv2, everything else in the
+    blob left as it was; the result is taken by az_load_weights_dev."""
+    from alphazero_amd import synth
+    N, Cs = 9, [64] * 4
+    blob = torch.from_numpy(synth.make_blob(N, 3, Cs, 5)).cuda()
+    before = blob.clone()
+    layout, at, off = synth.blob_layout(N, 3, Cs), 0, {}
+    for name, shape in layout:
+        off[name] = at
+        at += int(np.prod(shape))
+    stride = off["RBlock_1.conv1.weight"] - off["RBlock_0.conv1.weight"]
+    assert stride == off["RBlock_2.conv2.weight"] - off["RBlock_1.conv2.weight"]
+    grad, mom = torch.randn(at, generator=torch.Generator().manual_seed(1)).cuda() * 1e-3, torch.zeros(at, device="cuda")
+    touched = torch.zeros(at, dtype=torch.bool)
+    for conv in ("conv1", "conv2"):
+        o = off["RBlock_0.%s.weight" % conv]
+        view = lambda t: t.as_strided((3, 64, 64, 3, 3), (stride, 64 * 9, 9, 3, 1), o)                          # noqa: E731
+        want_w, want_m = learn.muon_step(view(blob).contiguous(), view(mom).contiguous(), view(grad).contiguous(), lr=0.02)
+        learn.muon_step(view(blob), view(mom), view(grad), lr=0.02)
+        assert torch.equal(view(blob), want_w) and torch.equal(view(mom), want_m)
+        for i in range(3):
+            touched[o + i * stride:o + i * stride + 64 * 64 * 9] = True
+    same = (blob == before).cpu()
+    assert same[~touched].all() and not same[touched].all() and (mom.cpu()[~touched] == 0).all()
+    eng = capi.Engine(N, 5, 2, Cs=Cs)
+    eng.load_weights_dev(blob.data_ptr(), blob.numel())
+    eng.sync()
+    eng.close()
+
+
+def test_zero_and_nonfinite_updates():
+    z = torch.zeros(2, 20, 50, device="cuda")
+    assert (learn.orthogonalize(z) == 0).all()
+    z[1, 3, 4] = float("nan")
+    z[0, 0, 0] = 2.0
+    out = learn.orthogonalize(z)
+    assert torch.isfinite(out[0]).all() and torch.isnan(out[1]).all()
+    for s in (1e-30, 1e30):                               # far from 1: the norm is taken in 64 bits
+        u = _mats(1, 40, 90, "f32", 5)
+        a, b = learn.orthogonalize((u * s).cuda(), eps=0.0), learn.orthogonalize(u.cuda(), eps=0.0)
+        assert torch.allclose(a, b, atol=1e-5)
+
+
+@pytest.mark.parametrize("steps", [0, 1, 2, 4, 7, 12])
+@pytest.mark.parametrize("shape", [(2, 50, 130), (1, 140, 90), (1, 300, 200)], ids=lambda s: "%dx%dx%d" % s)
+def test_any_number_of_steps(shape, steps):
+    n, R, K = shape
+    u = _mats(n, R, K, "f32", 11)
+    coef = (1.875, -1.25, 0.375)                          # converges: every number of steps stays bounded
+    want = _matrix_exact(u, steps, coef)
+    got = learn.orthogonalize(u.cuda(), steps=steps, coefficients=coef).cpu().double()
+    for i in range(n):
+        # as above: 3e-5 of the norm for up to three steps after the last formation of X, and what the earlier ones left
+        assert torch.linalg.matrix_norm(got[i] - want[i], 2) <= 4e-5 * max(1.0, float(torch.linalg.matrix_norm(want[i], 2)))
