@@ -576,9 +576,215 @@ template <int R> hipError_t iterate_in_lds(const OrthoDev& d, int n, int m, hipS
     return hipGetLastError();
 }
 
+// A whole call for matrices that fit one workgroup's LDS (up to 64 rows, 480 columns): momentum, norm, all steps, result.
+// The long dimension is as cheap to multiply here as the short one, so the steps are the plain ones, X <- P X, on X as
+// pairs; a wave owns its columns of X and replaces them in place.  Launched one product at a time the same call is 10 to 13
+// launches of 4 to 5 us each.
+constexpr int SMALL_R = 64, SMALL_K = 480, SMALL_NT = 512;
+struct SmallDev {
+    const void* g;
+    size_t g_stride;
+    const float* mom;         // optimiser step: u = g + beta m' or m', m' = beta m + g
+    float* mom_out;
+    size_t m_stride, mo_stride;
+    float beta;
+    int nesterov, steps;
+};
+template <int DT, bool MOM> __global__ void __launch_bounds__(SMALL_NT, 2) az_ortho_small_kernel(OrthoDev d, SmallDev s) {
+    constexpr int LD = SMALL_R + 8, PLANE = SMALL_R * LD;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    __shared__ double red[SMALL_NT / 64];
+    short* const A = (short*)smem;                                   // [hi, lo][64][LD]
+    short* const P = A + 2 * PLANE;
+    short* const X = P + 2 * PLANE;                                  // [hi, lo][64][ldx], rows of k
+    const int kp = (d.k + 31) / 32 * 32, ldx = kp + 8, xplane = SMALL_R * ldx;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, z = blockIdx.x, count = d.rows * d.cols;
+    const bool wide = d.rows <= d.cols;
+    // The update is read twice, 32 elements a thread in flight: for its norm (and the momentum, which the second time is
+    // read as written), and scaled into pairs.  Straight code that kept it in registers took longer: it runs once, at the
+    // pace of instruction fetches.
+    for (int i = tid; i < 2 * xplane / 8; i += SMALL_NT) ((az_i4*)X)[i] = az_i4{0, 0, 0, 0};
+    constexpr int U = 8;                                             // quads
+    const size_t go = z * s.g_stride, mo = z * s.m_stride, oo = z * s.mo_stride;
+    const int quads = count / 4, left = count - quads * 4;
+    const auto momentum = [&](float m, float v) __attribute__((always_inline)) { return s.beta * m + v; };
+    const auto update = [&](float m, float v) __attribute__((always_inline)) { return s.nesterov ? v + s.beta * m : m; };
+    double sum = 0.0;
+    #pragma unroll 1
+    for (int base = tid; base < quads; base += SMALL_NT * U) {
+        az_f4 v[U], m[U];
+        #pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const size_t i = (size_t)min(base + u * SMALL_NT, quads - 1) * 4;
+            v[u] = load4<DT>(s.g, go + i);
+            if (MOM) m[u] = *(const az_f4_u*)(s.mom + mo + i);
+        }
+        #pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (base + u * SMALL_NT < quads) {
+                #pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (MOM) { m[u][e] = momentum(m[u][e], v[u][e]); v[u][e] = update(m[u][e], v[u][e]); }
+                    sum += (double)v[u][e] * v[u][e];
+                }
+                if (MOM) *(az_f4_u*)(s.mom_out + oo + (size_t)(base + u * SMALL_NT) * 4) = m[u];
+            }
+    }
+    float last = 0.f;                                                // the up to three elements behind the last quad
+    if (tid < left) {
+        const size_t i = (size_t)quads * 4 + tid;
+        last = az_load<DT>(s.g, go + i);
+        if (MOM) {
+            const float m = momentum(s.mom[mo + i], last);
+            s.mom_out[oo + i] = m;
+            last = update(m, last);
+        }
+        sum += (double)last * last;
+    }
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) red[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < SMALL_NT / 64; ++w) sum += red[w];
+    const float up = ldexpf(1.f, d.scale_exp), down = ldexpf(1.f, -d.scale_exp);
+    const double inv = (double)up / (sqrt(sum) + (double)d.eps);
+    {
+        const auto place = [&](int line, int pos, float v) __attribute__((always_inline)) {
+            short* at = X + (wide ? line * ldx + pos : pos * ldx + line);
+            split((float)(v * inv), at[0], at[xplane]);
+        };
+        int line = tid * 4 / d.cols, pos = tid * 4 - line * d.cols;
+        const int dl = SMALL_NT * 4 / d.cols, dp = SMALL_NT * 4 - dl * d.cols;
+        #pragma unroll 1
+        for (int base = tid; base < quads; base += SMALL_NT * U) {
+            az_f4 v[U], m[U];
+            #pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const size_t i = (size_t)min(base + u * SMALL_NT, quads - 1) * 4;
+                v[u] = load4<DT>(s.g, go + i);
+                if (MOM) m[u] = *(const az_f4_u*)(s.mom_out + oo + i);
+            }
+            #pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (base + u * SMALL_NT < quads) {                   // (the momentum of other elements is other threads')
+                    int l = line, p = pos;
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        place(l, p, MOM ? update(m[u][e], v[u][e]) : v[u][e]);
+                        if (++p == d.cols) { p = 0; ++l; }
+                    }
+                }
+                line += dl; pos += dp;
+                if (pos >= d.cols) { pos -= d.cols; ++line; }
+            }
+        }
+        if (tid < left) { const int i = quads * 4 + tid, l = i / d.cols; place(l, i - l * d.cols, last); }
+    }
+    const int m0 = (wave & 3) * 16, n0 = (wave >> 2) * 32;           // a wave's 16 x 32 of A and P
+    const auto pairs = [&](az_f4& acc, const az_i4* m, const az_i4* n) __attribute__((always_inline)) {
+        acc = az_mma<1>(m[0], n[0], acc);
+        acc = az_mma<1>(m[0], n[1], acc);
+        acc = az_mma<1>(m[1], n[0], acc);
+    };
+    const auto rows_product = [&](az_f4* acc, const short* M, int ld, int plane, int len) __attribute__((always_inline)) {
+        acc[0] = acc[1] = az_f4{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < len; k += 32) {
+            az_i4 mf[2], nf[2][2];
+            #pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                mf[p] = az_row_frag<1>(M + p * plane, ld, m0, k, lane);
+                #pragma unroll
+                for (int j = 0; j < 2; ++j) nf[j][p] = az_row_frag<1>(M + p * plane, ld, n0 + j * 16, k, lane);
+            }
+            #pragma unroll
+            for (int j = 0; j < 2; ++j) pairs(acc[j], mf, nf[j]);
+        }
+    };
+    const auto put = [&](short* at, int plane, az_f4 x) __attribute__((always_inline)) {
+        az_s4 h, l;
+        #pragma unroll
+        for (int t = 0; t < 4; ++t) { short a, b; split(x[t], a, b); h[t] = a; l[t] = b; }
+        *(az_s4*)at = h;
+        *(az_s4*)(at + plane) = l;
+    };
+    #pragma unroll 1
+    for (int step = 0; step < s.steps; ++step) {
+        az_f4 acc[2], a[2];
+        __syncthreads();                                             // X is there
+        rows_product(a, X, ldx, xplane, kp);
+        const float f = SA * down * down;
+        #pragma unroll
+        for (int j = 0; j < 2; ++j) { a[j] *= f; put(A + (n0 + j * 16 + (lane & 15)) * LD + m0 + q * 4, PLANE, a[j]); }
+        __syncthreads();
+        rows_product(acc, A, LD, PLANE, SMALL_R);
+        #pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int nn = n0 + j * 16 + (lane & 15), mm = m0 + q * 4;
+            #pragma unroll
+            for (int t = 0; t < 4; ++t) acc[j][t] = (mm + t == nn ? d.a * SA : 0.f) + d.b * a[j][t] + d.c * (acc[j][t] * (1.f / SA));
+            put(P + nn * LD + mm, PLANE, acc[j]);
+        }
+        __syncthreads();
+        // X <- P X, 16 columns at a time; the last step's go to the result
+        az_i4 pf[4][2][2];
+        #pragma unroll
+        for (int j = 0; j < 4; ++j)
+            #pragma unroll
+            for (int k = 0; k < 2; ++k)
+                #pragma unroll
+                for (int p = 0; p < 2; ++p) pf[j][k][p] = az_row_frag<1>(P + p * PLANE, LD, j * 16, k * 32, lane);
+        #pragma unroll 1
+        for (int c = wave * 16; c < kp; c += SMALL_NT / 64 * 16) {
+            az_f4 x[4];
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = az_f4{0.f, 0.f, 0.f, 0.f};
+            #pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                az_i4 xf[2];
+                #pragma unroll
+                for (int p = 0; p < 2; ++p) xf[p] = az_col_frag<1>(X + p * xplane, ldx, k * 32, c, lane);
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) pairs(x[j], xf, pf[j][k]);
+            }
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int row = j * 16 + (lane & 15), col = c + q * 4;
+                if (step + 1 < s.steps) { put(X + row * ldx + col, xplane, x[j] * (1.f / SA)); continue; }
+                if (row >= d.r) continue;
+                const az_f4 y = x[j] * (down * (1.f / SA) * d.scale);
+                if (wide && col + 4 <= d.k) {
+                    const size_t at = (size_t)row * d.cols + col;
+                    if (MOM) *(az_f4_u*)((float*)d.out + z * d.out_stride + at) = *(const az_f4_u*)(d.w + z * d.w_stride + at) * d.keep + y;
+                    else if constexpr (DT == 0) *(az_f4_u*)((float*)d.out + z * d.out_stride + at) = y;
+                    else *(az_s4_u*)((short*)d.out + z * d.out_stride + at) = az_s4{az_to16<DT>(y[0]), az_to16<DT>(y[1]), az_to16<DT>(y[2]), az_to16<DT>(y[3])};
+                    continue;
+                }
+                #pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    if (col + t >= d.k) continue;
+                    const size_t at = wide ? (size_t)row * d.cols + col + t : (size_t)(col + t) * d.cols + row;
+                    if (MOM) ((float*)d.out)[z * d.out_stride + at] = d.w[z * d.w_stride + at] * d.keep + y[t];
+                    else az_store<DT>(d.out, z * d.out_stride + at, y[t]);
+                }
+            }
+        }
+    }
+}
+bool fits_small(int r, int k, int steps) { return r <= SMALL_R && k <= SMALL_K && steps > 0; }
+template <int DT, bool MOM> hipError_t small(OrthoDev d, const SmallDev& s, int n, hipStream_t st) {
+    d.scale_exp = std::ilogb(std::sqrt((double)d.k)) + 2;            // an iterate's elements: about 1 / sqrt(k)
+    const size_t lds = (size_t)2 * SMALL_R * ((d.k + 31) / 32 * 32 + 8) * 2 + (size_t)4 * SMALL_R * (SMALL_R + 8) * 2;
+    if (lds > 60 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void*)az_ortho_small_kernel<DT, MOM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    az_ortho_small_kernel<DT, MOM><<<n, SMALL_NT, lds, st>>>(d, s);
+    return hipGetLastError();
+}
+
 struct Plan {
     int n, rows, cols, r, k, rp, tile, apply_tile, tiles, low, slices, split, stage;
-    bool muon, restart;
+    bool muon, restart, small;
     size_t off_sq, off_u, off_x1, off_mat, off_partial, bytes;
     size_t pair_bytes;
 };
@@ -612,13 +818,15 @@ Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b
     const int ksteps = (p.k + 63) / 64;
     p.split = 1;
     while (p.split < 16 && (long long)p.low * n * p.split < 512 && ksteps / (p.split * 2) >= 4) p.split *= 2;
-    // Steps between two formations of X.  fp32 results: three (comment at the top); 16-bit results: five, their own rounding
-    // is larger; fewer where the coefficients would take Q out of fp16's range.
-    p.stage = dtype == AZ_F32 || muon ? 3 : 5;
+    // Steps between two formations of X.  fp32 results: two (comment at the top); the optimiser step, whose weights take
+    // lr times the result: three; 16-bit results: five, their own rounding is larger.  Fewer where the coefficients would
+    // take Q out of fp16's range.
+    p.stage = muon ? 3 : dtype == AZ_F32 ? 2 : 5;
     const float f = largest_factor(a, b, c);
     while (p.stage > 1 && std::pow(f, (float)p.stage) * SQ > 30000.f) --p.stage;
     p.restart = steps > p.stage;
     p.pair_bytes = up256((size_t)n * 2 * p.rp * p.rp * 2);
+    if ((p.small = fits_small(p.r, p.k, steps))) return p;           // (no workspace)
     size_t o = 0;
     p.off_sq = o; o += up256((size_t)n * p.slices * 8);
     p.off_u = o; if (muon) o += up256((size_t)n * count * 4);
@@ -802,6 +1010,16 @@ extern "C" int az_orthogonalize_dev(const az_orthogonalize_args* p, void* worksp
     (void)hipGetLastError();                                         // (an earlier call's error is not this one's)
     unsigned char* ws = (unsigned char*)workspace;
     hipStream_t st = (hipStream_t)stream;
+    OrthoDev d = {};
+    d.x = p->update; d.x_stride = p->update_stride;
+    d.eps = p->eps; d.a = p->a; d.b = p->b; d.c = p->c;
+    d.out = p->out; d.out_stride = p->out_stride; d.out_dtype = p->dtype; d.scale = p->scale;
+    if (plan.small) {
+        const SmallDev s = {p->update, (size_t)p->update_stride, nullptr, nullptr, 0, 0, 0.f, 0, p->steps};
+        d.rows = plan.rows; d.cols = plan.cols; d.r = plan.r; d.k = plan.k;
+        const hipError_t e = p->dtype == AZ_F32 ? small<0, false>(d, s, p->n, st) : p->dtype == AZ_F16 ? small<1, false>(d, s, p->n, st) : small<2, false>(d, s, p->n, st);
+        return e == hipSuccess ? AZ_OK : ofail(AZ_E_HIP, "az_orthogonalize_dev: launch failed: %s", hipGetErrorString(e));
+    }
     double* sq = (double*)(ws + plan.off_sq);
     const dim3 grid(plan.slices, p->n);
     const int count = p->rows * p->cols;
@@ -810,10 +1028,6 @@ extern "C" int az_orthogonalize_dev(const az_orthogonalize_args* p, void* worksp
     else az_ortho_norm_kernel<2, false><<<grid, 256, 0, st>>>(p->update, p->update_stride, count, plan.slices, sq, nullptr, 0, nullptr, 0, nullptr, 0.f, 0);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return ofail(AZ_E_HIP, "az_orthogonalize_dev: launch failed: %s", hipGetErrorString(e));
-    OrthoDev d = {};
-    d.x = p->update; d.x_stride = p->update_stride;
-    d.eps = p->eps; d.a = p->a; d.b = p->b; d.c = p->c;
-    d.out = p->out; d.out_stride = p->out_stride; d.out_dtype = p->dtype; d.scale = p->scale;
     return run(plan, d, p->dtype, p->steps, ws, st, "az_orthogonalize_dev");
 }
 
@@ -843,6 +1057,16 @@ extern "C" int az_muon_step_dev(const az_muon_step_args* p, void* workspace, siz
     (void)hipGetLastError();                                         // (an earlier call's error is not this one's)
     unsigned char* ws = (unsigned char*)workspace;
     hipStream_t st = (hipStream_t)stream;
+    OrthoDev d = {};
+    d.eps = p->eps; d.a = p->a; d.b = p->b; d.c = p->c;
+    d.out = p->weight_out; d.out_stride = p->weight_out_stride; d.out_dtype = AZ_F32; d.scale = -p->lr * p->scale;
+    d.w = p->weight; d.w_stride = p->weight_stride; d.keep = 1.f - p->lr * p->weight_decay;
+    if (plan.small) {
+        const SmallDev s = {p->grad, (size_t)p->grad_stride, p->momentum, p->momentum_out, (size_t)p->momentum_stride, (size_t)p->momentum_out_stride, p->beta, p->nesterov, p->steps};
+        d.rows = plan.rows; d.cols = plan.cols; d.r = plan.r; d.k = plan.k;
+        const hipError_t e = p->grad_dtype == AZ_F32 ? small<0, true>(d, s, p->n, st) : p->grad_dtype == AZ_F16 ? small<1, true>(d, s, p->n, st) : small<2, true>(d, s, p->n, st);
+        return e == hipSuccess ? AZ_OK : ofail(AZ_E_HIP, "az_muon_step_dev: launch failed: %s", hipGetErrorString(e));
+    }
     double* sq = (double*)(ws + plan.off_sq);
     float* u = (float*)(ws + plan.off_u);
     const dim3 grid(plan.slices, p->n);
@@ -855,10 +1079,6 @@ extern "C" int az_muon_step_dev(const az_muon_step_args* p, void* workspace, siz
 #undef NORM
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return ofail(AZ_E_HIP, "az_muon_step_dev: launch failed: %s", hipGetErrorString(e));
-    OrthoDev d = {};
     d.x = u; d.x_stride = count;
-    d.eps = p->eps; d.a = p->a; d.b = p->b; d.c = p->c;
-    d.out = p->weight_out; d.out_stride = p->weight_out_stride; d.out_dtype = AZ_F32; d.scale = -p->lr * p->scale;
-    d.w = p->weight; d.w_stride = p->weight_stride; d.keep = 1.f - p->lr * p->weight_decay;
     return run(plan, d, AZ_F32, p->steps, ws, st, "az_muon_step_dev");
 }

@@ -92,7 +92,7 @@ struct BoardLds {
     float* val;
     int* cnt;                                                        // [64-entry chunk][BLOCKS]
     int* start;                                                      // [BLOCKS + 1]: a block's first entry
-    az_f4* stat;                                                     // [MAX_BOARDS] of the gradients: {lse, r T, r, is there a target that is not allowed}
+    az_f4* stat;                                                     // [MAX_BOARDS] of the gradients: {log2 e max, r T / sum of exp, r, is the loss infinite}
     bool listed;                                                     // the entries fit
 };
 // entries outside the board's actions: -1
@@ -151,7 +151,7 @@ template <bool GRAD> struct BoardLoads {
         const int boards = min(a.nb, a.B - b0), lane = tid & 63, wave = tid >> 6;
         if (GRAD && tid < boards) {
             const float rs = a.scale * r;
-            l.stat[tid] = az_f4{st[0], rs * st[1], rs, st[2]};
+            l.stat[tid] = az_f4{st[0], rs * st[1] * st[2], rs, st[3] == INFINITY ? 1.f : 0.f};
         }
         if (a.legal) {
             const int n = boards * a.O * a.N;
@@ -265,7 +265,10 @@ __device__ __forceinline__ void finish_board(const PolicyDev& a, int b, float m,
     const float lse = m == -INFINITY ? (l == l ? -INFINITY : l) : m + logf(l);
     const bool masked = tz == -INFINITY;                             // a target on an action that is not allowed
     const float loss = masked ? INFINITY : (tm != 0.f ? tm * lse : 0.f) - tz;
-    a.stats[b] = az_f4{lse, tm, masked ? 1.f : 0.f, loss};
+    // The gradients take probabilities as exp2(log2 e z - log2 e max) / l: an lse rounded to 32 bits, off by up to 2^-22
+    // where it is about 5, would move all of a board's probabilities one way, and where one plane's sum to the targets' sum
+    // that is what is left of the products with features of one sign.
+    a.stats[b] = az_f4{m == -INFINITY ? 0.f : m * LOG2E, tm, l == 0.f ? 0.f : 1.f / l, loss};
     if (a.loss) a.loss[b] = loss;
 }
 
@@ -688,7 +691,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         const int bb = live && a.nb > 1 ? (int)((unsigned)rl * a.mag_s >> 16) : 0, s = live ? st.cell0 + rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
         const unsigned bit = live ? 1u << (s - y * a.N) : 0u;
         const unsigned* words = m.b.words + (bb * a.N + y) * (OT * 16) + half * OTH * 16 + q * 4;
-        const az_f4 bst = m.b.stat[bb];                              // {lse, r T, r, is there a target that is not allowed}
+        const az_f4 bst = m.b.stat[bb];
         const float rs = up * bst[2];
         if (a.counts) {
             float* t = m.t + rt * 16 * L::LDT;                   // where dz will lie: the waves clear and read it together
@@ -720,7 +723,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         __builtin_amdgcn_sched_barrier(0);                           // (phases apart: mixed, they want more registers than there are)
         product<KT, L::KS, OTH, !WLDS>(a.C, fetch, step);
         __builtin_amdgcn_sched_barrier(0);
-        const float rT = up * bst[1], lse2 = bst[0] * LOG2E;
+        const float rp = up * bst[1], m2 = bst[0];
         // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
         const bool bias_counts = a.O > 1 || bst[3] != 0.f;
         #pragma unroll
@@ -732,7 +735,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                 const az_i4 w = *(const az_i4*)(words + j * 16);
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float v = rT * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -lse2)) - rs * tv[j][i];
+                    const float v = rp * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -m2)) - rs * tv[j][i];
                     dz[i] = (unsigned)w[i] & bit ? v : 0.f;
                 }
             }
@@ -965,9 +968,9 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
             const int bb = live && a.nb > 1 ? (int)((unsigned)rl * a.mag_s >> 16) : 0, s = live ? st.cell0 + rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
             const unsigned bit = live ? 1u << (s - y * a.N) : 0u;
             const unsigned* words = m.b.words + (bb * a.N + y) * (OT * 16) + q * 4;
-            const az_f4 bst = m.b.stat[bb];                          // {lse, r T, r, is there a target that is not allowed}
+            const az_f4 bst = m.b.stat[bb];
             if (a.counts) scatter_targets<G::LDP>(a, m.b, own, st, wave, e0, e1, key0, val0, lane);
-            const float rs = live ? up * bst[2] : 0.f, rT = live ? up * bst[1] : 0.f, lse2 = bst[0] * LOG2E;
+            const float rs = live ? up * bst[2] : 0.f, rp = live ? up * bst[1] : 0.f, m2 = bst[0];
             // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
             const bool bias_counts = a.O > 1 || bst[3] != 0.f;
             constexpr int OH = OT > 2 ? OT / 2 : OT;                 // planes in two halves: fewer registers
@@ -991,7 +994,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
                     const int o = (j0 + j) * 16 + q * 4;
                     az_f4 dz;
                     #pragma unroll
-                    for (int i = 0; i < 4; ++i) dz[i] = __builtin_fmaf(rT, __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -lse2)), -rs * tv[j0 + j][i]);
+                    for (int i = 0; i < 4; ++i) dz[i] = __builtin_fmaf(rp, __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -m2)), -rs * tv[j0 + j][i]);
                     if (a.legal) {
                         const az_i4 w = *(const az_i4*)(words + (j0 + j) * 16);
                         #pragma unroll

@@ -448,7 +448,7 @@ typedef struct az_policy_loss_args {
     float scale;
     const float* row_scale;        /* f32 [B] or NULL = 1 */
     float* loss;                   /* out f32 [B] or NULL */
-    float* stats;                  /* f32 [B, 4] or NULL, 16-byte aligned: {lse, sum of targets, internal, loss}.  Out, unless
+    float* stats;                  /* f32 [B, 4] or NULL, 16-byte aligned: what the gradients need of the losses.  Out, unless
                                       stats_given: then in, as an earlier call without it left them for the same inputs, and
                                       only the gradients are computed */
     int   stats_given;
