@@ -46,6 +46,13 @@ template <int DT> __device__ __forceinline__ float az_from16(short v) {
     if constexpr (DT == 1) return (float)__builtin_bit_cast(_Float16, v);
     else return __uint_as_float((unsigned)(unsigned short)v << 16);
 }
+// x as hi + lo.  x is fixed to its 32 bits first: where it is a product or a sum of products, the compiler may round it to
+// hi in one instruction with them, in another place in two, and lo would then belong to another hi than the one stored.
+template <int DT> __device__ __forceinline__ void az_split(float x, short& hi, short& lo) {
+    asm("" : "+v"(x));
+    hi = az_to16<DT>(x);
+    lo = az_to16<DT>(x - az_from16<DT>(hi));
+}
 template <int DT> __device__ __forceinline__ float az_load(const void* p, size_t i) {
     if constexpr (DT == 0) return ((const float*)p)[i];
     else return az_from16<DT>(((const short*)p)[i]);

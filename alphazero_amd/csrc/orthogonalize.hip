@@ -42,12 +42,16 @@ struct OrthoDev {
     size_t x_stride;          // elements from matrix to matrix
     int rows, cols, r, k, rp; // as stored; r = min, k = max; rp = r padded to the tile
     int slices;
-    const double* sq;         // [n][slices] sums of squares, or null: X is an iterate, scale_exp its power of two
-    int scale_exp;
+    const double* sq;         // [n][slices] sums of squares, or null: X is an iterate
+    int scale_exp;            // an iterate's power of two
     float eps, a, b, c;
     short *A, *P, *T, *Q, *Q2;// [n][2][rp][rp]: hi plane, lo plane
     float* partial;           // [n][split][rp][rp]
     int split;
+    const short* xp;          // an iterate as pairs: [n][2][lines][xld], both sides padded and zero there
+    short* xo;                // where the result goes as such pairs (null: the call's own result)
+    int xld;
+    size_t xplane;
     // result
     void* out;
     size_t out_stride;
@@ -129,7 +133,7 @@ template <int DT, bool MOM> __global__ void __launch_bounds__(256) az_ortho_norm
     if (threadIdx.x == 0) sq[(size_t)z * slices + sl] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-__device__ __forceinline__ void split(float x, short& hi, short& lo) { hi = az_to16<1>(x); lo = az_to16<1>(x - az_from16<1>(hi)); }
+__device__ __forceinline__ void split(float x, short& hi, short& lo) { az_split<1>(x, hi, lo); }
 
 // One operand of a tile product: TILE lines-or-columns by KSTEP.  ALONG: the contraction runs along a line of memory (LDS
 // rows are the tile's rows); otherwise lines are the contraction (LDS rows are its steps, read transposed).  A thread
@@ -231,13 +235,27 @@ __device__ __forceinline__ void lower_tile(int i, int& ti, int& tj) {
     tj = i - ti * (ti + 1) / 2;
 }
 
+// entries (nn, m .. m + 3) of a symmetric result as pairs, v at its scale; mirror: and (m .. m + 3, nn)
+__device__ __forceinline__ void put_symmetric(const OrthoDev& d, short* res, int z, int m, int nn, bool mirror, az_f4 v) {
+    short* hi = res + (size_t)z * 2 * d.rp * d.rp;
+    short* lo = hi + (size_t)d.rp * d.rp;
+    az_s4 h, l;
+    #pragma unroll
+    for (int t = 0; t < 4; ++t) { short x, y; split(v[t], x, y); h[t] = x; l[t] = y; }
+    *(az_s4*)(hi + (size_t)nn * d.rp + m) = h;
+    *(az_s4*)(lo + (size_t)nn * d.rp + m) = l;
+    if (mirror)
+        #pragma unroll
+        for (int t = 0; t < 4; ++t) { hi[(size_t)(m + t) * d.rp + nn] = h[t]; lo[(size_t)(m + t) * d.rp + nn] = l[t]; }
+}
+
 // D[m][n] = sum over the contraction, 4 waves of TILE/2 x TILE/2.  Lane l of a 16 x 16 tile holds rows 4 (l / 16) .. + 3 of
 // column l % 16, so M is the side along which the result is contiguous in memory.
 //   SYM         M = rows of a symmetric matrix, N = rows of another that commutes with it: their product, lower triangle
 //   GRAM_*      M = N = rows of X: lower triangle
 //   APPLY_WIDE  M = columns of X, N = rows of Q;   APPLY_TALL  M = rows of Q, N = rows of X as stored (columns of X)
 template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256, 2) az_ortho_product_kernel(OrthoDev d, const short* ma, const short* na, short* res,
-                                                                                                 const short* ma2, const short* na2, short* res2, int epi, float sr, float sr2, int n) {                                      // n: tiles of a matrix
+                                                                                                 const short* ma2, const short* na2, short* res2, int epi, int n) {                                      // n: tiles of a matrix
     constexpr bool GRAM = MODE == GRAM_WIDE || MODE == GRAM_TALL;
     constexpr int MS = MODE == SYM || MODE == APPLY_TALL ? SRC_PAIR : DT, NS = MODE == SYM || MODE == APPLY_WIDE ? SRC_PAIR : DT;
     constexpr bool MA = !(MODE == GRAM_TALL || MODE == APPLY_WIDE), NA = MODE != GRAM_TALL;
@@ -266,12 +284,12 @@ template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256, 2) 
             k_lo = steps * sp / d.split * KSTEP;
             k_hi = steps * (sp + 1) / d.split * KSTEP;
         } else {
-            if (blockIdx.y) { ma = ma2; na = na2; res = res2; epi = EPI_PAIR; sr = sr2; }   // a second product of the same launch
+            if (blockIdx.y) { ma = ma2; na = na2; res = res2; }      // a second product of the same launch
             k_hi = (d.r + TILE - 1) / TILE * TILE;                  // (what lies behind, up to rp, is never written)
         }
     } else {
         // APPLY: neighbours differ in the rows of Q and share the piece of X
-        const int sides = (d.r + TILE - 1) / TILE;
+        const int sides = d.xo ? d.rp / TILE : (d.r + TILE - 1) / TILE;
         z = tile / n;
         const int t = tile - z * n, l = t / sides, o = t - l * sides;
         m0 = (MODE == APPLY_WIDE ? l : o) * TILE;
@@ -284,10 +302,12 @@ template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256, 2) 
     const void *mp, *mlo = nullptr, *np, *nlo = nullptr;
     int mld, nld;
     const size_t esz = DT == 0 ? 4 : 2;
-    if constexpr (MS == SRC_PAIR) { mp = ma + (size_t)z * 2 * plane; mlo = ma + (size_t)z * 2 * plane + plane; mld = d.rp; }
-    else { mp = (const char*)d.x + z * d.x_stride * esz; mld = d.cols; }
-    if constexpr (NS == SRC_PAIR) { np = na + (size_t)z * 2 * plane; nlo = na + (size_t)z * 2 * plane + plane; nld = d.rp; }
-    else { np = (const char*)d.x + z * d.x_stride * esz; nld = d.cols; }
+    if constexpr (DT == SRC_PAIR && MODE != SYM) { mp = np = d.xp + z * 2 * d.xplane; mlo = nlo = d.xp + z * 2 * d.xplane + d.xplane; mld = nld = d.xld; }
+    constexpr bool MQ = MODE == SYM || MODE == APPLY_TALL, NQ = MODE == SYM || MODE == APPLY_WIDE;      // a symmetric matrix
+    if constexpr (MQ) { mp = ma + (size_t)z * 2 * plane; mlo = ma + (size_t)z * 2 * plane + plane; mld = d.rp; }
+    else if constexpr (DT != SRC_PAIR) { mp = (const char*)d.x + z * d.x_stride * esz; mld = d.cols; }
+    if constexpr (NQ) { np = na + (size_t)z * 2 * plane; nlo = na + (size_t)z * 2 * plane + plane; nld = d.rp; }
+    else if constexpr (DT != SRC_PAIR) { np = (const char*)d.x + z * d.x_stride * esz; nld = d.cols; }
     az_f4 acc[WT][WT];
     #pragma unroll
     for (int i = 0; i < WT; ++i)
@@ -347,28 +367,29 @@ template <int TILE, int DT, int MODE> __global__ void __launch_bounds__(256, 2) 
             az_f4 v = acc[i][j];
             const int m = m0 + mw + i * 16 + q * 4, nn = n0 + nw + j * 16 + (lane & 15);
             if constexpr (MODE == SYM || GRAM) {
-                // sr: from the operands' scales to the result's (a partial sum has none)
                 if constexpr (GRAM) v *= back * back * (epi == EPI_PARTIAL ? 1.f : SA);
-                else v *= sr;
+                else v *= 1.f / SA;                                  // (one factor is at scale SA: the result is at the other's)
                 if (GRAM && epi == EPI_PARTIAL) { *(az_f4*)(d.partial + ((size_t)z * d.split + sp) * plane + (size_t)nn * d.rp + m) = v; continue; }
-                short* hi = res + (size_t)z * 2 * plane;
-                short* lo = hi + plane;
-                if (MODE == SYM && epi == EPI_POLY) {                 // P = a I + b A + c A A
+                if (MODE == SYM && epi == EPI_POLY) {                 // P = a I + b A + c A A at scale SA, and at SQ where it is Q
                     const az_s4 ah = *(const az_s4*)(ma + (size_t)z * 2 * plane + (size_t)nn * d.rp + m);
                     const az_s4 al = *(const az_s4*)(ma + (size_t)z * 2 * plane + plane + (size_t)nn * d.rp + m);
-                    const float res_scale = sr * SA * SA;
                     #pragma unroll
-                    for (int t = 0; t < 4; ++t) v[t] = (m + t == nn ? d.a * res_scale : 0.f) + d.b * (res_scale / SA) * (az_from16<1>(ah[t]) + az_from16<1>(al[t])) + d.c * v[t];
+                    for (int t = 0; t < 4; ++t) v[t] = (m + t == nn ? d.a * SA : 0.f) + d.b * (az_from16<1>(ah[t]) + az_from16<1>(al[t])) + d.c * v[t];
+                    if (res2) put_symmetric(d, res2, z, m, nn, m0 != n0, v * (SQ / SA));
                 }
-                az_s4 h, l;
-                #pragma unroll
-                for (int t = 0; t < 4; ++t) { short x, y; split(v[t], x, y); h[t] = x; l[t] = y; }
-                *(az_s4*)(hi + (size_t)nn * d.rp + m) = h;
-                *(az_s4*)(lo + (size_t)nn * d.rp + m) = l;
-                if (m0 != n0)
-                    for (int t = 0; t < 4; ++t) { hi[(size_t)(m + t) * d.rp + nn] = h[t]; lo[(size_t)(m + t) * d.rp + nn] = l[t]; }
+                if (res) put_symmetric(d, res, z, m, nn, m0 != n0, v);
             } else {
                 // the result's line and position in memory: the positions m .. m + 3 of line nn
+                if (d.xo) {                                          // (zero where the matrix is padded)
+                    const float f = back * (1.f / SQ) * ldexpf(1.f, d.scale_exp);
+                    short* hi = d.xo + z * 2 * d.xplane + (size_t)nn * d.xld + m;
+                    az_s4 h, l;
+                    #pragma unroll
+                    for (int t = 0; t < 4; ++t) { short a, b; split(v[t] * f, a, b); h[t] = a; l[t] = b; }
+                    *(az_s4*)hi = h;
+                    *(az_s4*)(hi + d.xplane) = l;
+                    continue;
+                }
                 const int nl = d.rows, np_ = d.cols;
                 if (nn >= nl || m >= np_) continue;
                 const float f = back * (1.f / SQ) * d.scale;
@@ -783,10 +804,10 @@ template <int DT, bool MOM> hipError_t small(OrthoDev d, const SmallDev& s, int 
 }
 
 struct Plan {
-    int n, rows, cols, r, k, rp, tile, apply_tile, tiles, low, slices, split, stage;
+    int n, rows, cols, r, k, rp, kp, tile, apply_tile, tiles, low, slices, split, stage;
     bool muon, restart, small;
     size_t off_sq, off_u, off_x1, off_mat, off_partial, bytes;
-    size_t pair_bytes;
+    size_t pair_bytes, iter_bytes;
 };
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -806,9 +827,9 @@ Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b
     // Tiles of 128 x 128 move half the LDS bytes a product of tiles of 64 x 64, but there are a quarter as many: taken where
     // they fill the chip's 256 CUs.
     const auto low = [&](int tile) { const long long t = (p.r + tile - 1) / tile; return t * (t + 1) / 2; };
-    p.tile = low(128) * n >= 256 ? 128 : 64;
-    p.rp = (p.r + 127) / 128 * 128;
-    if (p.r <= 64) p.rp = 64;
+    p.rp = p.r <= 64 ? 64 : (p.r + 127) / 128 * 128;
+    p.kp = (p.k + 127) / 128 * 128;
+    p.tile = p.rp % 128 == 0 && low(128) * n >= 256 ? 128 : 64;
     p.tiles = (p.r + p.tile - 1) / p.tile;
     p.low = (int)low(p.tile);
     p.apply_tile = p.rp % 128 == 0 && (long long)((p.k + 127) / 128) * ((p.r + 127) / 128) * n >= 256 ? 128 : 64;
@@ -830,14 +851,14 @@ Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b
     size_t o = 0;
     p.off_sq = o; o += up256((size_t)n * p.slices * 8);
     p.off_u = o; if (muon) o += up256((size_t)n * count * 4);
-    p.off_x1 = o; if (p.restart) o += 2 * up256((size_t)n * count * 4);   // iterates: read one, write the other
+    p.off_x1 = o; if (p.restart) o += 2 * (p.iter_bytes = up256((size_t)n * 2 * p.rp * p.kp * 2));   // iterates: read one, write the other
     p.off_mat = o; o += 5 * p.pair_bytes;
     p.off_partial = o; if (p.split > 1) o += up256((size_t)n * p.split * p.rp * p.rp * 4);
     p.bytes = o;
     return p;
 }
 
-struct Pairs { const short *m, *n; short* out; float scale; };       // one product: operands, result, scale (of EPI_PAIR / EPI_POLY)
+struct Pairs { const short *m, *n; short* out; };                    // one product: operands, result
 // grid x: tiles of a matrix, z: matrices (one dimension of the launch), y: slices or products
 template <int TILE, int DT, int MODE> hipError_t product(const OrthoDev& d, dim3 grid, Pairs one, Pairs two, int epi, hipStream_t st) {
     constexpr int MS = MODE == SYM || MODE == APPLY_TALL ? SRC_PAIR : DT, NS = MODE == SYM || MODE == APPLY_WIDE ? SRC_PAIR : DT;
@@ -848,14 +869,14 @@ template <int TILE, int DT, int MODE> hipError_t product(const OrthoDev& d, dim3
         const hipError_t e = hipFuncSetAttribute((const void*)az_ortho_product_kernel<TILE, DT, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    az_ortho_product_kernel<TILE, DT, MODE><<<dim3(grid.x * grid.z, grid.y), 256, lds, st>>>(d, one.m, one.n, one.out, two.m, two.n, two.out, epi, one.scale, two.scale, (int)grid.x);
+    az_ortho_product_kernel<TILE, DT, MODE><<<dim3(grid.x * grid.z, grid.y), 256, lds, st>>>(d, one.m, one.n, one.out, two.m, two.n, two.out, epi, (int)grid.x);
     return hipGetLastError();
 }
 
 template <int TILE, int DT> hipError_t gram(const Plan& p, const OrthoDev& d, hipStream_t st) {
     const dim3 grid(p.low, p.split, p.n);
     const int epi = p.split > 1 ? EPI_PARTIAL : EPI_PAIR;
-    const Pairs x = {nullptr, nullptr, d.A, 1.f};
+    const Pairs x = {nullptr, nullptr, d.A};
     hipError_t e = p.rows <= p.cols ? product<TILE, DT, GRAM_WIDE>(d, grid, x, Pairs{}, epi, st) : product<TILE, DT, GRAM_TALL>(d, grid, x, Pairs{}, epi, st);
     if (e == hipSuccess && p.split > 1) {
         az_ortho_join_kernel<<<dim3(p.low, TILE * TILE / 1024, p.n), 256, 0, st>>>(d, TILE);
@@ -864,21 +885,20 @@ template <int TILE, int DT> hipError_t gram(const Plan& p, const OrthoDev& d, hi
     return e;
 }
 template <int TILE, int DT> hipError_t apply(const Plan& p, const OrthoDev& d, hipStream_t st) {
-    const dim3 grid((p.k + TILE - 1) / TILE * ((p.r + TILE - 1) / TILE), 1, p.n);
-    return p.rows <= p.cols ? product<TILE, DT, APPLY_WIDE>(d, grid, Pairs{nullptr, d.Q, nullptr, 1.f}, Pairs{}, 0, st)
-                            : product<TILE, DT, APPLY_TALL>(d, grid, Pairs{d.Q, nullptr, nullptr, 1.f}, Pairs{}, 0, st);
+    const dim3 grid(d.xo ? p.kp / TILE * (p.rp / TILE) : (p.k + TILE - 1) / TILE * ((p.r + TILE - 1) / TILE), 1, p.n);
+    return p.rows <= p.cols ? product<TILE, DT, APPLY_WIDE>(d, grid, Pairs{nullptr, d.Q, nullptr}, Pairs{}, 0, st)
+                            : product<TILE, DT, APPLY_TALL>(d, grid, Pairs{d.Q, nullptr, nullptr}, Pairs{}, 0, st);
 }
 template <int TILE> hipError_t gram_dt(int dt, const Plan& p, const OrthoDev& d, hipStream_t st) {
-    return dt == AZ_F32 ? gram<TILE, 0>(p, d, st) : dt == AZ_F16 ? gram<TILE, 1>(p, d, st) : gram<TILE, 2>(p, d, st);
+    return dt == SRC_PAIR ? gram<TILE, SRC_PAIR>(p, d, st) : dt == AZ_F32 ? gram<TILE, 0>(p, d, st) : dt == AZ_F16 ? gram<TILE, 1>(p, d, st) : gram<TILE, 2>(p, d, st);
 }
 template <int TILE> hipError_t apply_dt(int dt, const Plan& p, const OrthoDev& d, hipStream_t st) {
-    return dt == AZ_F32 ? apply<TILE, 0>(p, d, st) : dt == AZ_F16 ? apply<TILE, 1>(p, d, st) : apply<TILE, 2>(p, d, st);
+    return dt == SRC_PAIR ? apply<TILE, SRC_PAIR>(p, d, st) : dt == AZ_F32 ? apply<TILE, 0>(p, d, st) : dt == AZ_F16 ? apply<TILE, 1>(p, d, st) : apply<TILE, 2>(p, d, st);
 }
 
 // `m` steps on A: leaves Q
 template <int TILE> hipError_t iterate(const Plan& p, OrthoDev& d, int m, hipStream_t st) {
     const dim3 one(p.low, 1, p.n), two(p.low, 2, p.n);
-    const float aa = 1.f / SA, aq = SQ / (SA * SA), qq = 1.f / SA;   // A-kind x A-kind -> A-kind, -> Q, Q x A-kind -> Q
     hipError_t e = hipSuccess;
 #define RUN(call) do { if (e == hipSuccess) e = (call); } while (0)
     if (m == 0) { az_ortho_identity_kernel<<<dim3(64, p.n), 256, 0, st>>>(d.Q, p.rp); return hipGetLastError(); }
@@ -886,14 +906,13 @@ template <int TILE> hipError_t iterate(const Plan& p, OrthoDev& d, int m, hipStr
     if (p.rp == 128) return iterate_in_lds<128>(d, p.n, m, st);
     for (int i = 0; i < m; ++i) {
         const bool first = i == 0, last = i + 1 == m;
-        // the first step's Q is its P, at Q's scale: written where it is wanted
-        if (first) RUN((product<TILE, 0, SYM>(d, one, Pairs{d.A, d.A, d.Q, aq}, Pairs{}, EPI_POLY, st)));
-        if (!first || !last) RUN((product<TILE, 0, SYM>(d, one, Pairs{d.A, d.A, d.P, aa}, Pairs{}, EPI_POLY, st)));
+        // P; the first step's is Q too
+        RUN((product<TILE, 0, SYM>(d, one, Pairs{d.A, d.A, first && last ? nullptr : d.P}, Pairs{nullptr, nullptr, first ? d.Q : nullptr}, EPI_POLY, st)));
+        const Pairs q = {d.Q, d.P, d.Q2};
         if (!last) {
-            if (first) RUN((product<TILE, 0, SYM>(d, one, Pairs{d.A, d.P, d.T, aa}, Pairs{}, EPI_PAIR, st)));
-            else RUN((product<TILE, 0, SYM>(d, two, Pairs{d.A, d.P, d.T, aa}, Pairs{d.Q, d.P, d.Q2, qq}, EPI_PAIR, st)));
-            RUN((product<TILE, 0, SYM>(d, one, Pairs{d.T, d.P, d.A, aa}, Pairs{}, EPI_PAIR, st)));
-        } else if (!first) RUN((product<TILE, 0, SYM>(d, one, Pairs{d.Q, d.P, d.Q2, qq}, Pairs{}, EPI_PAIR, st)));
+            RUN((product<TILE, 0, SYM>(d, first ? one : two, Pairs{d.A, d.P, d.T}, first ? Pairs{} : q, EPI_PAIR, st)));
+            RUN((product<TILE, 0, SYM>(d, one, Pairs{d.T, d.P, d.A}, Pairs{}, EPI_PAIR, st)));
+        } else if (!first) RUN((product<TILE, 0, SYM>(d, one, q, Pairs{}, EPI_PAIR, st)));
         if (!first) { short* t = d.Q; d.Q = d.Q2; d.Q2 = t; }
     }
 #undef RUN
@@ -901,9 +920,12 @@ template <int TILE> hipError_t iterate(const Plan& p, OrthoDev& d, int m, hipStr
 }
 
 hipError_t run_plan(const Plan& p, OrthoDev d, int dtype, int steps, unsigned char* ws, hipStream_t st) {
-    const OrthoDev fin = d;                                          // result pointers of the last application
-    const size_t count = (size_t)p.rows * p.cols;
-    float* x1[2] = {(float*)(ws + p.off_x1), (float*)(ws + p.off_x1 + up256((size_t)p.n * count * 4))};
+    short* const x[2] = {(short*)(ws + p.off_x1), (short*)(ws + p.off_x1 + p.iter_bytes)};
+    const bool wide = p.rows <= p.cols;
+    d.xld = wide ? p.kp : p.rp;
+    d.xplane = (size_t)p.rp * p.kp;
+    const int se = std::ilogb(std::sqrt((double)p.k)) + 2;           // an iterate's elements: about 1 / sqrt(k)
+    d.scale_exp = se < 13 ? se : 13;
     hipError_t e = hipSuccess;
     int done = 0, which = 0;
     do {
@@ -913,12 +935,9 @@ hipError_t run_plan(const Plan& p, OrthoDev d, int dtype, int steps, unsigned ch
         done += m;
         if (m > 0) e = p.tile == 64 ? gram_dt<64>(dtype, p, d, st) : gram_dt<128>(dtype, p, d, st);
         if (e == hipSuccess) e = p.tile == 64 ? iterate<64>(p, d, m, st) : iterate<128>(p, d, m, st);
-        if (done < steps) { d.out = x1[which]; d.out_stride = count; d.out_dtype = AZ_F32; d.scale = 1.f; d.w = nullptr; }
-        else { d.out = fin.out; d.out_stride = fin.out_stride; d.out_dtype = fin.out_dtype; d.scale = fin.scale; d.w = fin.w; }
+        d.xo = done < steps ? x[which] : nullptr;
         if (e == hipSuccess) e = p.apply_tile == 64 ? apply_dt<64>(dtype, p, d, st) : apply_dt<128>(dtype, p, d, st);
-        d.x = x1[which]; d.x_stride = count; dtype = AZ_F32; d.sq = nullptr;
-        const int se = std::ilogb(std::sqrt((double)p.k)) + 2;       // an iterate's elements: about 1 / sqrt(k)
-        d.scale_exp = se < 13 ? se : 13;
+        d.xp = x[which]; dtype = SRC_PAIR; d.sq = nullptr;
         which ^= 1;
     } while (e == hipSuccess && done < steps);
     return e;

@@ -744,7 +744,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             else {
                 az_s4 hi, lo;
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) { hi[i] = az_to16<DT>(dz[i]); lo[i] = az_to16<DT>(dz[i] - az_from16<DT>(hi[i])); }
+                for (int i = 0; i < 4; ++i) { short x, y; az_split<DT>(dz[i], x, y); hi[i] = x; lo[i] = y; }
                 *(az_s4*)((short*)zhi + rl * L::LDO + ot * 16 + q * 4) = hi;
                 *(az_s4*)((short*)zlo + rl * L::LDO + ot * 16 + q * 4) = lo;
             }
@@ -1003,7 +1003,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
                     if (bias_counts) db[j0 + j] += dz;
                     az_s4 hi, lo;
                     #pragma unroll
-                    for (int i = 0; i < 4; ++i) { hi[i] = az_to16<DT>(dz[i]); lo[i] = az_to16<DT>(dz[i] - az_from16<DT>(hi[i])); }
+                    for (int i = 0; i < 4; ++i) { short x, y; az_split<DT>(dz[i], x, y); hi[i] = x; lo[i] = y; }
                     *(az_s4*)((short*)zhi + rl * L::LDO + o) = hi;
                     *(az_s4*)((short*)zlo + rl * L::LDO + o) = lo;
                 }

@@ -485,3 +485,18 @@ def test_any_number_of_steps(shape, steps):
     for i in range(n):
         # as above: 3e-5 of the norm for up to three steps after the last formation of X, and what the earlier ones left
         assert torch.linalg.matrix_norm(got[i] - want[i], 2) <= 4e-5 * max(1.0, float(torch.linalg.matrix_norm(want[i], 2)))
+
+
+@pytest.mark.parametrize("shape", [(260, 40, 500), (300, 600, 64), (90, 200, 200), (3, 65, 64), (2, 64, 481)], ids=lambda s: "%dx%dx%d" % s)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_matrices(shape, dtype):
+    """Batches that fill the chip with large tiles, shapes at the borders between the kernels; a few matrices against 64 bits."""
+    n, R, K = shape
+    u = _mats(n, R, K, dtype, 21)
+    got = learn.orthogonalize(u.cuda())
+    half = 0.0 if dtype == "f32" else torch.finfo(DT[dtype]).eps / 2
+    for i in sorted({0, 1, n // 2, n - 1}):
+        want = _matrix_exact(u[i:i + 1])[0]
+        err = got[i].cpu().double() - want
+        # as above, and the rounding of the result: each element by half a step
+        assert torch.linalg.matrix_norm(err, 2) <= 4e-5 * max(1.0, float(torch.linalg.matrix_norm(want, 2))) + half * float(want.norm())
