@@ -948,6 +948,7 @@ int check_common(int n, int rows, int cols, int steps, float a, float b, float c
     if (n > 65535) return ofail(AZ_E_ARG, "%d matrices are too many for one call (65535)", n);
     if (rows < 1 || cols < 1) return ofail(AZ_E_ARG, "matrix %d x %d", rows, cols);
     if ((long long)rows * cols > 0x7fffffffll) return ofail(AZ_E_ARG, "matrix %d x %d has too many elements", rows, cols);
+    if ((rows < cols ? cols : rows) > 1 << 24) return ofail(AZ_E_ARG, "the longer side of %d x %d is beyond 2^24", rows, cols);
     if ((rows < cols ? rows : cols) > 8192) return ofail(AZ_E_ARG, "the shorter side of %d x %d is beyond 8192", rows, cols);
     if (steps < 0 || steps > 100) return ofail(AZ_E_ARG, "%d steps (0..100)", steps);
     if (!(std::fabs(a) + std::fabs(b) + std::fabs(c) <= 32.f)) return ofail(AZ_E_ARG, "coefficients %g, %g, %g: their magnitudes sum beyond 32", a, b, c);

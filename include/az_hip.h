@@ -466,7 +466,7 @@ int az_policy_loss_dev(const az_policy_loss_args*, void* workspace, size_t works
  * ResBlocks straight out of the weight blob (az_load_weights).  out may not overlap update. */
 typedef struct az_orthogonalize_args {
     int   device;
-    int   n, rows, cols;           /* n may be 0; the shorter side at most 8192 */
+    int   n, rows, cols;           /* n may be 0; the shorter side at most 8192, the longer 2^24 */
     int   dtype;                   /* of update and out */
     int   steps;                   /* 0..100 */
     float a, b, c, eps, scale;     /* |a| + |b| + |c| <= 32 */

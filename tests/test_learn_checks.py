@@ -67,7 +67,7 @@ def test_policy_loss_refuses(kw, word):
 
 @pytest.mark.parametrize("kw,word", [
     (dict(n=-1), "-1 matrices"), (dict(n=65536), "too many"), (dict(rows=0), "matrix 0"), (dict(cols=0), "x 0"), (dict(rows=1 << 16, cols=1 << 16), "too many elements"),
-    (dict(rows=8193, cols=8193, update_stride=1 << 40, out_stride=1 << 40), "8192"), (dict(steps=-1), "steps"), (dict(steps=101), "steps"), (dict(a=40.0), "coefficients"),
+    (dict(rows=8193, cols=8193, update_stride=1 << 40, out_stride=1 << 40), "8192"), (dict(rows=(1 << 24) + 1, cols=1, update_stride=1 << 40, out_stride=1 << 40), "2^24"), (dict(steps=-1), "steps"), (dict(steps=101), "steps"), (dict(a=40.0), "coefficients"),
     (dict(b=float("nan")), "coefficients"), (dict(eps=-1.0), "eps"), (dict(eps=float("inf")), "eps"), (dict(eps=float("nan")), "eps"), (dict(dtype=7), "element type"),
     (dict(update=None), "update"), (dict(out=None), "out"), (dict(update=P + 2), "aligned"), (dict(update_stride=10), "stride"), (dict(out_stride=0), "stride"),
     (dict(out=P), "overlaps"), (dict(out=P + 64 * 225 * 4), "overlaps"),
@@ -139,8 +139,8 @@ def test_kernels_hold_no_packed_fp32_and_no_write_behind_a_wide_store(tmp_path):
         subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                         "--cuda-device-only", "-S", os.path.join(ROOT, "alphazero_amd", "csrc", src), "-o", out], check=True, capture_output=True, timeout=900)
         return out
-    with concurrent.futures.ThreadPoolExecutor(2) as pool:
-        files = list(pool.map(asm, ["policy_loss.hip", "orthogonalize.hip"]))
+    with concurrent.futures.ThreadPoolExecutor(5) as pool:
+        files = list(pool.map(asm, ["policy_f32.hip", "policy_f16.hip", "policy_bf16.hip", "orthogonalize.hip", "policy_loss.hip"]))
     for f in files:
         text = open(f).read()
         assert not any("v_pk_%s_f32" % op in text for op in ("add", "mul", "fma"))
