@@ -804,7 +804,7 @@ template <int DT, bool MOM> hipError_t small(OrthoDev d, const SmallDev& s, int 
 }
 
 struct Plan {
-    int n, rows, cols, r, k, rp, kp, tile, apply_tile, tiles, low, slices, split, stage;
+    int n, rows, cols, r, k, rp, kp, apply_tile, low, slices, split, stage;
     bool muon, restart, small;
     size_t off_sq, off_u, off_x1, off_mat, off_partial, bytes;
     size_t pair_bytes, iter_bytes;
@@ -819,26 +819,35 @@ float largest_factor(float a, float b, float c) {
     return m;
 }
 
+// Slices of the contraction of X X^T.  In steps of 64 (1.4 us where a workgroup has its CU to itself; two take 1.7 times as
+// long): what the fullest CU does, two more to begin a workgroup, five for the launch that joins the slices, and the slices'
+// traffic (16 KB a tile written and read).  2 x 4096 x 1024 (272 tiles on 256 CUs, 64 steps): a slice 696 us a call, two 677,
+// four 653; 40 x 256 x 2304 (400 tiles, 36 steps): one 503, two 535; 18 x 128 x 1152 (54 tiles, 18 steps): one 88, four 83.
+int split_of(long long tiles, int steps) {
+    int best = 1;
+    double cost = 0.0;
+    for (int s = 1; s <= 64 && s <= steps; s *= 2) {
+        const long long w = (tiles * s + 255) / 256;
+        const double t = ((double)(w / 2) * 1.7 + (double)(w % 2)) * ((steps + s - 1) / s + 2) + (s > 1 ? 5.0 + (double)tiles * s * 0.0047 : 0.0);
+        if (s == 1 || t < cost) { cost = t; best = s; }
+    }
+    return best;
+}
+
 Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b, float c, bool muon) {
     Plan p = {};
     p.n = n; p.rows = rows; p.cols = cols; p.muon = muon;
     p.r = rows < cols ? rows : cols;
     p.k = rows < cols ? cols : rows;
-    // Tiles of 128 x 128 move half the LDS bytes a product of tiles of 64 x 64, but there are a quarter as many: taken where
-    // they fill the chip's 256 CUs.
-    const auto low = [&](int tile) { const long long t = (p.r + tile - 1) / tile; return t * (t + 1) / 2; };
+    const int t = (p.r + 63) / 64;
+    p.low = t * (t + 1) / 2;
     p.rp = p.r <= 64 ? 64 : (p.r + 127) / 128 * 128;
     p.kp = (p.k + 127) / 128 * 128;
-    p.tile = p.rp % 128 == 0 && low(128) * n >= 256 ? 128 : 64;
-    p.tiles = (p.r + p.tile - 1) / p.tile;
-    p.low = (int)low(p.tile);
     p.apply_tile = p.rp % 128 == 0 && (long long)((p.k + 127) / 128) * ((p.r + 127) / 128) * n >= 256 ? 128 : 64;
     const long long count = (long long)rows * cols;
     p.slices = (int)(count / 4096 < 1 ? 1 : count / 4096 > MAX_SLICES ? MAX_SLICES : count / 4096);
     while (p.slices > 64 && (long long)p.slices * n > 2048) p.slices /= 2;
-    const int ksteps = (p.k + 63) / 64;
-    p.split = 1;
-    while (p.split < 16 && (long long)p.low * n * p.split < 512 && ksteps / (p.split * 2) >= 4) p.split *= 2;
+    p.split = split_of((long long)p.low * n, (p.k + 63) / 64);
     // Steps between two formations of X.  fp32 results: two (comment at the top); the optimiser step, whose weights take
     // lr times the result: three; 16-bit results: five, their own rounding is larger.  Fewer where the coefficients would
     // take Q out of fp16's range.
@@ -889,15 +898,15 @@ template <int TILE, int DT> hipError_t apply(const Plan& p, const OrthoDev& d, h
     return p.rows <= p.cols ? product<TILE, DT, APPLY_WIDE>(d, grid, Pairs{nullptr, d.Q, nullptr}, Pairs{}, 0, st)
                             : product<TILE, DT, APPLY_TALL>(d, grid, Pairs{d.Q, nullptr, nullptr}, Pairs{}, 0, st);
 }
-template <int TILE> hipError_t gram_dt(int dt, const Plan& p, const OrthoDev& d, hipStream_t st) {
-    return dt == SRC_PAIR ? gram<TILE, SRC_PAIR>(p, d, st) : dt == AZ_F32 ? gram<TILE, 0>(p, d, st) : dt == AZ_F16 ? gram<TILE, 1>(p, d, st) : gram<TILE, 2>(p, d, st);
+hipError_t gram_dt(int dt, const Plan& p, const OrthoDev& d, hipStream_t st) {
+    return dt == SRC_PAIR ? gram<64, SRC_PAIR>(p, d, st) : dt == AZ_F32 ? gram<64, 0>(p, d, st) : dt == AZ_F16 ? gram<64, 1>(p, d, st) : gram<64, 2>(p, d, st);
 }
 template <int TILE> hipError_t apply_dt(int dt, const Plan& p, const OrthoDev& d, hipStream_t st) {
     return dt == SRC_PAIR ? apply<TILE, SRC_PAIR>(p, d, st) : dt == AZ_F32 ? apply<TILE, 0>(p, d, st) : dt == AZ_F16 ? apply<TILE, 1>(p, d, st) : apply<TILE, 2>(p, d, st);
 }
 
 // `m` steps on A: leaves Q
-template <int TILE> hipError_t iterate(const Plan& p, OrthoDev& d, int m, hipStream_t st) {
+hipError_t iterate(const Plan& p, OrthoDev& d, int m, hipStream_t st) {
     const dim3 one(p.low, 1, p.n), two(p.low, 2, p.n);
     hipError_t e = hipSuccess;
 #define RUN(call) do { if (e == hipSuccess) e = (call); } while (0)
@@ -907,12 +916,12 @@ template <int TILE> hipError_t iterate(const Plan& p, OrthoDev& d, int m, hipStr
     for (int i = 0; i < m; ++i) {
         const bool first = i == 0, last = i + 1 == m;
         // P; the first step's is Q too
-        RUN((product<TILE, 0, SYM>(d, one, Pairs{d.A, d.A, first && last ? nullptr : d.P}, Pairs{nullptr, nullptr, first ? d.Q : nullptr}, EPI_POLY, st)));
+        RUN((product<64, 0, SYM>(d, one, Pairs{d.A, d.A, first && last ? nullptr : d.P}, Pairs{nullptr, nullptr, first ? d.Q : nullptr}, EPI_POLY, st)));
         const Pairs q = {d.Q, d.P, d.Q2};
         if (!last) {
-            RUN((product<TILE, 0, SYM>(d, first ? one : two, Pairs{d.A, d.P, d.T}, first ? Pairs{} : q, EPI_PAIR, st)));
-            RUN((product<TILE, 0, SYM>(d, one, Pairs{d.T, d.P, d.A}, Pairs{}, EPI_PAIR, st)));
-        } else if (!first) RUN((product<TILE, 0, SYM>(d, one, q, Pairs{}, EPI_PAIR, st)));
+            RUN((product<64, 0, SYM>(d, first ? one : two, Pairs{d.A, d.P, d.T}, first ? Pairs{} : q, EPI_PAIR, st)));
+            RUN((product<64, 0, SYM>(d, one, Pairs{d.T, d.P, d.A}, Pairs{}, EPI_PAIR, st)));
+        } else if (!first) RUN((product<64, 0, SYM>(d, one, q, Pairs{}, EPI_PAIR, st)));
         if (!first) { short* t = d.Q; d.Q = d.Q2; d.Q2 = t; }
     }
 #undef RUN
@@ -933,8 +942,8 @@ hipError_t run_plan(const Plan& p, OrthoDev d, int dtype, int steps, unsigned ch
         // stage starts far below 1 (|X0|_F = 1 spread over the singular values) and the later ones near 1
         const int left = steps - done, m = left < p.stage ? left : p.stage;
         done += m;
-        if (m > 0) e = p.tile == 64 ? gram_dt<64>(dtype, p, d, st) : gram_dt<128>(dtype, p, d, st);
-        if (e == hipSuccess) e = p.tile == 64 ? iterate<64>(p, d, m, st) : iterate<128>(p, d, m, st);
+        if (m > 0) e = gram_dt(dtype, p, d, st);
+        if (e == hipSuccess) e = iterate(p, d, m, st);
         d.xo = done < steps ? x[which] : nullptr;
         if (e == hipSuccess) e = p.apply_tile == 64 ? apply_dt<64>(dtype, p, d, st) : apply_dt<128>(dtype, p, d, st);
         d.xp = x[which]; dtype = SRC_PAIR; d.sq = nullptr;

@@ -1139,19 +1139,23 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
 }
 
 template <int DT, int OT, int CB, int MODE> hipError_t launch_products(PolicyDev a, bool grad, int& groups, hipStream_t stream) {
-    constexpr bool PAIR = DT != 0 && CB == 1 && OT <= 6;              // (more planes: w's shares do not fit the registers)
+    // az_policy_grad16_kernel: 16-bit features of up to 128 channels and 96 planes (with more, w's shares do not fit the
+    // registers), where a workgroup has more than a step.  20 x 20, 91 planes bf16: 2048 boards 228 us a call, with
+    // az_policy_grad_kernel 334; 36 boards (252 steps) 37.7 against 36.6, and 9 x 9, 3 planes fp16 24.7 against 19.8.
+    constexpr bool PAIR = DT != 0 && CB == 1 && OT <= 6;
+    const bool pair = PAIR && a.steps > CUS;
     const auto bytes = [&]() -> size_t {
         if (!grad) return Smem<DT, OT, CB, 0, w_in_lds<DT, OT, CB>()>::bytes(a, a.counts ? WAVES * LossTile<OT>::bytes : 0) + 4 * ROWS * 16;   // (and the kernel's `red`)
-        if constexpr (PAIR) return Smem<DT, OT, 1, 3, false>::bytes(a, PairCfg<DT, OT>::zb(a));
-        else return Smem<DT, OT, CB, 1, w_in_lds<DT, OT, CB>()>::bytes(a, Lay<DT, OT, CB>::z_bytes);
+        if constexpr (PAIR) if (pair) return Smem<DT, OT, 1, 3, false>::bytes(a, PairCfg<DT, OT>::zb(a));
+        return Smem<DT, OT, CB, 1, w_in_lds<DT, OT, CB>()>::bytes(a, Lay<DT, OT, CB>::z_bytes);
     };
     size_t lds = bytes();
     if (lds > LDS_BYTES) { a.room = 0; lds = bytes(); }              // the longest lists with the largest boards and heads: targets read from memory
     if (lds > LDS_BYTES) return hipErrorInvalidConfiguration;
     const void* fn;
     if (!grad) fn = (const void*)az_policy_loss_kernel<DT, OT, CB, MODE>;
-    else if constexpr (PAIR) fn = (const void*)az_policy_grad16_kernel<DT, OT, MODE>;
     else fn = (const void*)az_policy_grad_kernel<DT, OT, CB, MODE>;
+    if constexpr (PAIR) if (grad && pair) fn = (const void*)az_policy_grad16_kernel<DT, OT, MODE>;
     if (lds > 32 * 1024) {
         const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
@@ -1163,8 +1167,8 @@ template <int DT, int OT, int CB, int MODE> hipError_t launch_products(PolicyDev
         az_policy_loss_kernel<DT, OT, CB, MODE><<<(work + rounds - 1) / rounds, NT, lds - 4 * ROWS * 16, stream>>>(a, work);
     } else {
         if (lds * 2 > LDS_BYTES && groups > CUS) groups = CUS;       // one workgroup a CU
-        if constexpr (PAIR) az_policy_grad16_kernel<DT, OT, MODE><<<groups, NT, lds, stream>>>(a);
-        else az_policy_grad_kernel<DT, OT, CB, MODE><<<groups, NT, lds, stream>>>(a);
+        if constexpr (PAIR) if (pair) { az_policy_grad16_kernel<DT, OT, MODE><<<groups, NT, lds, stream>>>(a); return hipGetLastError(); }
+        az_policy_grad_kernel<DT, OT, CB, MODE><<<groups, NT, lds, stream>>>(a);
     }
     return hipGetLastError();
 }

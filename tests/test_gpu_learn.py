@@ -500,3 +500,16 @@ def test_many_matrices(shape, dtype):
         err = got[i].cpu().double() - want
         # as above, and the rounding of the result: each element by half a step
         assert torch.linalg.matrix_norm(err, 2) <= 4e-5 * max(1.0, float(torch.linalg.matrix_norm(want, 2))) + half * float(want.norm())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("layout", ["nchw", "nhwc"])
+@pytest.mark.parametrize("case", [(90, 15, 128, 1, False, 0.0), (150, 9, 100, 3, False, 0.5), (300, 7, 48, 17, True, 0.3), (2000, 3, 40, 65, True, 0.0),
+                                  (2200, 3, 33, 2, False, 0.6), (40, 20, 128, 91, True, 0.02), (38, 20, 64, 40, False, 0.0), (5000, 1, 31, 7, True, 0.0), (17, 32, 96, 33, True, 0.2)],
+                         ids=lambda c: "b%d-n%d-c%d-o%d%s%s" % (c[0], c[1], c[2], c[3], "-sparse" if c[4] else "", "-legal" if c[5] else ""))
+def test_gradients_of_more_than_a_step_a_workgroup(case, layout, dtype):
+    B, N, C, O, sparse, legal = case
+    p = _rows(B, N, C, O, dtype, layout, sparse, legal, seed=B + N, empty=(0, B - 1))
+    r = torch.linspace(0.5, -1.5, B, dtype=torch.float64)
+    r = r.float()
+    _check(p, _grad(p, r.cuda()), r.double())
