@@ -11,7 +11,14 @@
 // small against the largest keeps the absolute precision of A's arithmetic, and the steps enlarge that error as they
 // enlarge the value (a^2 each).  So the products run on pairs of fp16 values, s x = hi + lo (22 bits, s a power of two that
 // keeps lo out of fp16's subnormals where it matters; three MFMA a product, fp32 sums), and for fp32 results X is formed
-// anew after three steps and A from it.
+// anew after two steps and A from it: for matrices whose largest singular value stands for most of the norm three steps
+// leave 6 times fp32's error (64 x 225 with 8 strong directions: 6e-6, two steps 1.1e-6, products in fp32 1.1e-6), two steps
+// at most fp32's.  fp32 matrix instructions would run at 154 TFLOP/s, three fp16 ones at 1.1 / 3 PFLOP/s.
+//
+// Measured on an MI355X that copies 4.9 TB/s and multiplies 1.1 PFLOP/s (fp16): 2 x 4096 x 1024 fp32 655 us (eleven
+// r x r launches of 25 us, X X^T 86 + 59 + 59 us, Q X 70 + 64 + 64 us; the Gram form's operations are 276 us at the rate of
+// a large product); optimiser step of 40 x 256 x 2304 513 us (momentum and norm 65 us at 5.7 TB/s, X X^T 68 + 50, r x r 13
+// launches of 12, Q X 78 + 95 us, the last with weights read and written).  18 x 128 x 1152 bf16 84 us.
 #include "../../include/az_hip.h"
 #include "az_learn.h"
 
@@ -249,6 +256,11 @@ __device__ __forceinline__ void put_symmetric(const OrthoDev& d, short* res, int
         for (int t = 0; t < 4; ++t) { hi[(size_t)(m + t) * d.rp + nn] = h[t]; lo[(size_t)(m + t) * d.rp + nn] = l[t]; }
 }
 
+// One tile of a product.  Bound by a workgroup's own chain -- loads, LDS, products, barrier: 1.4 us a step of 64 where it
+// has its CU to itself, against 0.2 us of matrix instructions.  X X^T and the r x r products take tiles of 64:
+// 2 x 4096 x 1024 674 us a call, in tiles of 128 803, 16 x 4096 x 1024 3.6 ms either way, 300 x 128 x 1152 bf16 227 and 241 us.  An
+// r x r product of 2 x 1024 rows 25 us; its operands straight from memory to fragments, without LDS, 39.
+// Q X: tiles of 128 where those fill the chip (16 x 4096 x 1024: 3.6 ms a call, in tiles of 64 4.2 ms; 7 x 512 x 512: 244 and 223 us).
 // D[m][n] = sum over the contraction, 4 waves of TILE/2 x TILE/2.  Lane l of a 16 x 16 tile holds rows 4 (l / 16) .. + 3 of
 // column l % 16, so M is the side along which the result is contiguous in memory.
 //   SYM         M = rows of a symmetric matrix, N = rows of another that commutes with it: their product, lower triangle
@@ -449,7 +461,8 @@ __global__ void __launch_bounds__(256) az_ortho_identity_kernel(short* Q, int rp
 
 // All of a stage's steps for matrices of up to R = 64 or 128 rows, one workgroup a matrix: A and P lie in LDS as pairs, Q in
 // registers, A P takes A's place.  Launched one product at a time these cost a launch and a trip to L2 each (5 us) for
-// 1 to 2 us of matrix instructions.  A wave holds 16 columns of Q as operands: the product P Q leaves rows 4 g .. 4 g + 3 of
+// 1 to 2 us of matrix instructions.  18 matrices of 128 rows, five steps: 58 us, bound by the chain of products of one
+// workgroup and its LDS reads (rows 16 halves longer instead of 8, a two-way conflict: 73 us).  A wave holds 16 columns of Q as operands: the product P Q leaves rows 4 g .. 4 g + 3 of
 // the tiles 2 s, 2 s + 1 in lane group g, which is a fragment of step s whose contraction runs over those rows in that order,
 // and P's rows are read in the same order.
 template <int R> __global__ void __launch_bounds__(R * 4) az_ortho_iterate_kernel(OrthoDev d, int m) {
@@ -600,7 +613,8 @@ template <int R> hipError_t iterate_in_lds(const OrthoDev& d, int n, int m, hipS
 // A whole call for matrices that fit one workgroup's LDS (up to 64 rows, 480 columns): momentum, norm, all steps, result.
 // The long dimension is as cheap to multiply here as the short one, so the steps are the plain ones, X <- P X, on X as
 // pairs; a wave owns its columns of X and replaces them in place.  Launched one product at a time the same call is 10 to 13
-// launches of 4 to 5 us each.
+// launches of 4 to 5 us each: 64 x 225 fp32 63 us, here 32; 64 x 480 69 and 53 (one step: 24 and 24); 1000 x 64 x 480 547 and
+// 234; 1000 x 27 x 128 231 and 78.  Bound by the chain of a step, 2 us and 2 more for 256 columns.
 constexpr int SMALL_R = 64, SMALL_K = 480, SMALL_NT = 512;
 struct SmallDev {
     const void* g;
@@ -843,6 +857,7 @@ Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b
     p.low = t * (t + 1) / 2;
     p.rp = p.r <= 64 ? 64 : (p.r + 127) / 128 * 128;
     p.kp = (p.k + 127) / 128 * 128;
+    // Q X in tiles of 128 where they fill the chip (figures at az_ortho_product_kernel)
     p.apply_tile = p.rp % 128 == 0 && (long long)((p.k + 127) / 128) * ((p.r + 127) / 128) * n >= 256 ? 128 : 64;
     const long long count = (long long)rows * cols;
     p.slices = (int)(count / 4096 < 1 ? 1 : count / 4096 > MAX_SLICES ? MAX_SLICES : count / 4096);
@@ -938,7 +953,7 @@ hipError_t run_plan(const Plan& p, OrthoDev d, int dtype, int steps, unsigned ch
     hipError_t e = hipSuccess;
     int done = 0, which = 0;
     do {
-        // stages of p.stage steps, the shorter one last: A's error is relative to its largest eigenvalue, which the first
+        // stages of p.stage steps, a shorter one last: A's error is relative to its largest eigenvalue, which the first
         // stage starts far below 1 (|X0|_F = 1 spread over the singular values) and the later ones near 1
         const int left = steps - done, m = left < p.stage ? left : p.stage;
         done += m;

@@ -352,9 +352,13 @@ template <int KT, int KS, int W, bool AHEAD, class F, class S> __device__ __forc
 
 // Losses.  A workgroup takes a board (or nb small ones) at a time, its waves the tiles of 16 rows in turn, all planes.  The
 // features go from memory to fragments (no other wave wants these rows), the next tile's while this one is worked on; the
-// waves meet only where the board changes.  Planes are taken half at a time where there are many (all at
-// once leaves a wave too few registers for four waves a SIMD).  Sparse targets: the logits pass through LDS, and lanes
+// waves meet only where the board changes.  Planes are taken half at a time from 64 on (all at
+// once leaves a wave too few registers for four waves a SIMD: 512 boards of 20 x 20, 128 planes bf16 76 us, in halves 40;
+// 91 planes 33 and 30, 64 planes 23.5 and 24).  Sparse targets: the logits pass through LDS, and lanes
 // pick out those that the tile's entries name.
+// 2048 boards of 20 x 20, 128 channels, 91 planes fp16, legal actions only: 86 us, 2.7 TB/s of the features (43 us of copying);
+// bound by the vector instructions of 36 400 exponentials and masks a board.  4096 boards of 15 x 15, one plane bf16: 61 us,
+// 3.9 TB/s, bound by memory.  256 boards of 20 x 20, 256 channels fp32: 91 us, 52 TFLOP/s.
 template <int OT> struct LossTile {
     static constexpr int PASSES = OT >= 4 ? 2 : 1, OTP = OT / PASSES, LDZ = OTP * 16 + 4;
     static constexpr size_t bytes = (size_t)16 * LDZ * 4;            // of one wave
@@ -612,7 +616,10 @@ template <int LD> __device__ __forceinline__ void scatter_targets(const PolicyDe
 // channels a wave, kept in registers over all of a workgroup's steps).  16-bit features: dz goes to LDS as hi + lo of the
 // type, hi alone feeds dh (whose result is rounded to that type anyway), both feed dw (an fp32 sum over all rows: one
 // rounding to 16 bits of each term would stay in it).
-// (16-bit features of up to 128 channels and 96 planes have a kernel of their own below.)
+// (16-bit features of up to 128 channels and 96 planes have a kernel of their own below for all but the smallest batches.)
+// fp32: bound by the matrix instructions, 32 cycles for the 16 x 16 x 4: 256 boards of 20 x 20, 256 channels, 91 planes
+// 225 us, 64 TFLOP/s (three products: 93 us at the rate of a large one).  256 channels leave no registers to ask for the next
+// step's features early: kept in flight they went to scratch memory and back (367 us).
 template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT, 2) az_policy_grad_kernel(PolicyDev a) {
     typedef Lay<DT, OT, CB> L;
     typedef typename AzElem<DT>::T T;
@@ -865,6 +872,9 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
 // either kind on each SIMD, one barrier a step; each kind holds its shares of w in registers.  Done by the same waves one
 // after the other, neither the vector nor the matrix pipes nor the LDS port were busy half of the time.  LDS: features of
 // three steps, dz (hi and lo) of two, the sparse targets of each row tile.
+// 2048 boards of 20 x 20, 128 channels, 91 planes bf16: 158 us, 361 TFLOP/s of useful products (two of dw's halves counted
+// once), 2.7 TB/s of features and their gradients (86 us of copying); what bounds it is the step's chain of logits, exponentials,
+// LDS and products between two barriers with one workgroup a CU.  4096 boards of 15 x 15, one plane: 93 us, 5.1 TB/s: memory.
 template <int DT, int OT> struct PairCfg {
     typedef Lay<DT, OT, 1> L;
     static constexpr int LDP = OT * 16 + 4;

@@ -12,6 +12,9 @@
 // sum t} over them.  az_policy_grad_kernel forms the same logits again, 64 rows a step -- 2 C flop an entry against 8 bytes
 // of a kept fp32 logit written and read -- turns them into dz in LDS and multiplies it both ways; az_policy_reduce_kernel
 // adds the workgroups' dw and dbias in a fixed order.
+//
+// The features are read twice, once for the losses and once for the gradients: a board's lse is not known before all of its
+// logits are.  Times are those of an MI355X that copies 4.9 TB/s and multiplies 1.1 PFLOP/s (16 bits) / 154 TFLOP/s (fp32).
 #pragma once
 #include "../../include/az_hip.h"
 #include "az_learn.h"
