@@ -86,12 +86,14 @@ def _loss_args(features, weight, bias, targets, legal):
     return a
 
 
-def _loss(features, weight, bias, targets, legal):
+def _loss(features, weight, bias, targets, legal, keep=False):
     a = _loss_args(features, weight, bias, targets, legal)
     loss = torch.empty(a.B, dtype=torch.float32, device=features.device)
-    stats = torch.empty(a.B, 4, dtype=torch.float32, device=features.device)
+    stats = torch.empty(a.B, 4, dtype=torch.float32, device=features.device) if keep else None
     if a.B:
-        a.loss, a.stats = loss.data_ptr(), stats.data_ptr()
+        a.loss = loss.data_ptr()
+        if keep:
+            a.stats = stats.data_ptr()
         _run("policy_loss", a, features.device)
     return loss, stats
 
@@ -121,7 +123,7 @@ class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, features, weight, bias, legal, *targets):
         tgt = targets[0] if len(targets) == 1 else targets
-        loss, stats = _loss(features, weight, bias, tgt, legal)
+        loss, stats = _loss(features, weight, bias, tgt, legal, keep=True)
         ctx.save_for_backward(features, weight, bias, legal, stats, *targets)
         return loss
 
@@ -149,6 +151,7 @@ def policy_loss(features, weight, bias, targets, legal=None):
     """
     tgt = (targets,) if isinstance(targets, torch.Tensor) else tuple(targets)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (features, weight, bias)):
+        _need(not torch.cuda.is_current_stream_capturing(), "policy_loss with gradients cannot be captured into a graph: policy_loss_grad can")
         return _PolicyLoss.apply(features, weight, bias, legal, *tgt)
     return _loss(features, weight, bias, targets, legal)[0]
 
@@ -165,16 +168,15 @@ def _batch(t, what):
     """(n, rows, cols, stride) of a matrix [R, K], a batch [n, R, K], a convolution's weight [O, I, kh, kw] (as O x I kh kw)
     or a batch of those."""
     _need(isinstance(t, torch.Tensor) and t.is_cuda and 2 <= t.dim() <= 5, "%s: a matrix or a batch of matrices on the GPU", what)
-    lead = t.dim() in (3, 5)
-    n = t.shape[0] if lead else 1
-    stride = t.stride(0) if lead else t.numel()
-    m = t[0] if lead and n else t
-    _need(n == 0 or m.is_contiguous(), "%s: every matrix has to be contiguous (strides %s)", what, t.stride())
-    shape = t.shape[1:] if lead else t.shape
-    cols = 1
-    for s in shape[1:]:
-        cols *= s
-    return n, shape[0], cols, stride
+    shape, strides = t.shape, t.stride()
+    lead = len(shape) & 1
+    want = 1
+    for d in range(len(shape) - 1, lead, -1):
+        _need(strides[d] == want or shape[d] == 1 or 0 in shape, "%s: every matrix has to be contiguous (strides %s)", what, strides)
+        want *= shape[d]
+    rows = shape[lead]
+    _need(strides[lead] == want or rows == 1 or 0 in shape, "%s: every matrix has to be contiguous (strides %s)", what, strides)
+    return (shape[0], rows, want, strides[0]) if lead else (1, rows, want, rows * want)
 
 
 def _coef(a, coefficients, eps, steps):
@@ -218,7 +220,7 @@ def muon_step(weight, momentum, grad, lr, beta=0.95, nesterov=True, weight_decay
     m_out = momentum if momentum_out is None else momentum_out
     for t, what in ((momentum, "momentum"), (grad, "grad"), (w_out, "weight_out"), (m_out, "momentum_out")):
         _on(t, weight.device, what)
-        _need(t.shape == weight.shape, "%s: shape %s is not the weight's %s", what, tuple(t.shape), tuple(weight.shape))
+        _need(t.shape == weight.shape, "%s: shape %s is not the weight's %s", what, t.shape, weight.shape)
     for t, what in ((weight, "weight"), (momentum, "momentum"), (w_out, "weight_out"), (m_out, "momentum_out")):
         _need(t.dtype == torch.float32, "%s: %s (float32)", what, t.dtype)
     _need(grad.dtype in _DTYPES, "grad: %s (float32, float16 or bfloat16)", grad.dtype)

@@ -513,3 +513,32 @@ def test_gradients_of_more_than_a_step_a_workgroup(case, layout, dtype):
     r = torch.linspace(0.5, -1.5, B, dtype=torch.float64)
     r = r.float()
     _check(p, _grad(p, r.cuda()), r.double())
+
+
+def test_gradients_through_autograd_are_refused_under_capture():
+    p = _rows(2, 5, 16, 1, "f32", seed=1)
+    x, w, b, tgt, _ = _cuda(p)
+    xr = x.clone().requires_grad_()
+    policy = learn.policy_loss(xr, w, b, tgt)             # an eager graph of the same leaf lives
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        with pytest.raises(capi.AzError, match="policy_loss_grad"):
+            learn.policy_loss(xr, w, b, tgt)
+        out = learn.policy_loss(x, w, b, tgt)             # without gradients it can be captured
+    for _ in range(3):
+        x.copy_(torch.randn_like(x).relu())
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, learn.policy_loss(x, w, b, tgt))
+    policy.sum().backward()
+    assert torch.isfinite(xr.grad).all()
+
+
+def test_matrices_that_are_not_contiguous_are_refused():
+    u = torch.randn(4, 12, 20, device="cuda")
+    for bad in (u.transpose(1, 2), u[:, :, ::2], u[:, ::2], torch.randn(2, 8, 3, 3, 4, device="cuda").permute(0, 1, 4, 2, 3)):
+        with pytest.raises(capi.AzError, match="contiguous"):
+            learn.orthogonalize(bad)
+    for good in (u[::2], u[1:2, :, :], u[:, :1], u.view(4, 12, 5, 4)[0], u[0], u.view(4, 12, 5, 2, 2)[::3], u[:, 3:7]):
+        assert torch.equal(learn.orthogonalize(good), learn.orthogonalize(good.contiguous()))
