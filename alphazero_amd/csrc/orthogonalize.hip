@@ -45,7 +45,7 @@ enum { GRAM_WIDE, GRAM_TALL, APPLY_WIDE, APPLY_TALL, SYM };          // what a t
 enum { EPI_PAIR, EPI_PARTIAL, EPI_POLY };                             // what SYM / GRAM leave
 
 struct OrthoDev {
-    const void* x;            // operand X: the update or a formed iterate
+    const void* x;            // operand X: the update
     size_t x_stride;          // elements from matrix to matrix
     int rows, cols, r, k, rp; // as stored; r = min, k = max; rp = r padded to the tile
     int slices;

@@ -261,10 +261,22 @@ __device__ __forceinline__ void join(float& m, float& l, float om, float ol) {
     l = l * rescale(m, to) + ol * rescale(om, to);
     m = to;
 }
-__device__ __forceinline__ void finish_board(const PolicyDev& a, int b, float m, float l, float tz, float tm) {
+// A whole wave.  Where a NaN made the targets' sum one, the loss takes the sum of the others, read once more.
+__device__ __forceinline__ void finish_board(const PolicyDev& a, int b, float m, float l, float tz, float tm, int lane) {
+    float tl = tm;
+    if (tm != tm) {
+        tl = 0.f;
+        const int n = a.counts ? min(a.counts[b], a.cap) : a.O * a.S;
+        for (int i = lane; i < n; i += 64) {
+            const float v = a.counts ? a.probs[(size_t)b * a.cap + i] : a.dense[(size_t)b * a.O * a.S + i];
+            if (__builtin_islessgreater(v, 0.f) && (!a.counts || (unsigned)a.actions[(size_t)b * a.cap + i] < (unsigned)(a.O * a.S))) tl += v;
+        }
+        for (int o = 32; o > 0; o >>= 1) tl += __shfl_xor(tl, o, 64);
+    }
+    if (lane != 0) return;
     const float lse = m == -INFINITY ? (l == l ? -INFINITY : l) : m + logf(l);
     const bool masked = tz == -INFINITY;                             // a target on an action that is not allowed
-    const float loss = masked ? INFINITY : (tm != 0.f ? tm * lse : 0.f) - tz;
+    const float loss = masked ? INFINITY : (tl != 0.f ? tl * lse : 0.f) - tz;
     // The gradients take probabilities as exp2(log2 e z - log2 e max) / l: an lse rounded to 32 bits, off by up to 2^-22
     // where it is about 5, would move all of a board's probabilities one way, and where one plane's sum to the targets' sum
     // that is what is left of the products with features of one sign.
@@ -435,14 +447,14 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                     for (int i = 0; i < 4; ++i) acc[j][i] = (unsigned)w[i] & bit ? acc[j][i] : -INFINITY;
                 }
                 // (an entry without a target does not count, whatever its logit; one with a target whose action is not
-                // allowed gives -inf)
+                // allowed gives -inf; a NaN is no target for the loss: finish_board)
                 if (!a.counts) {
                     #pragma unroll
                     for (int j = 0; j < R::OTP; ++j)
                         #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float v = live && o0 + j * 16 + q * 4 + i < a.O ? tv[j][i] : 0.f;
-                            tz += v != 0.f ? v * acc[j][i] : 0.f;
+                            tz += __builtin_islessgreater(v, 0.f) ? v * acc[j][i] : 0.f;
                             tm += v;
                         }
                 } else {
@@ -453,7 +465,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                     const auto take = [&](int k, float v) __attribute__((always_inline)) {
                         const int row = (k >> 8) - r0, o = (k & 255) - o0;
                         if ((unsigned)row < (unsigned)(hi - r0) && (unsigned)o < (unsigned)(R::OTP * 16)) {
-                            tz += v != 0.f ? v * zt[row * R::LDZ + o] : 0.f;
+                            tz += __builtin_islessgreater(v, 0.f) ? v * zt[row * R::LDZ + o] : 0.f;
                             tm += v;
                         }
                     };
@@ -492,11 +504,11 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         } else if (wave < 4) red[wave * 64 + (lane & 15) * 4 + q] = az_f4{mx, l, tz, tm};
         __syncthreads();
         if (a.nb == 1) {
-            if (tid == 0) {
+            if (wave == 0) {
                 az_f4 r = red[0];
                 float fm = r[0], fl = r[1], fz = r[2], ft = r[3];
                 for (int w = 1; w < WAVES; ++w) { r = red[w]; join(fm, fl, r[0], r[1]); fz += r[2]; ft += r[3]; }
-                finish_board(a, b0, fm, fl, fz, ft);
+                finish_board(a, b0, fm, fl, fz, ft, lane);
             }
         } else
             for (int bb = wave; bb * a.S < rows; bb += WAVES) {
@@ -507,7 +519,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                     fz += __shfl_xor(fz, d, 64);
                     ft += __shfl_xor(ft, d, 64);
                 }
-                if (lane == 0) finish_board(a, b0 + bb, fm, fl, fz, ft);
+                finish_board(a, b0 + bb, fm, fl, fz, ft, lane);
             }
     }
 }
@@ -1148,6 +1160,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
     }
 }
 
+constexpr size_t LOSS_STATIC = (size_t)4 * ROWS * 16;                // az_policy_loss_kernel's `red`
 template <int DT, int OT, int CB, int MODE> hipError_t launch_products(PolicyDev a, bool grad, int& groups, hipStream_t stream) {
     // az_policy_grad16_kernel: 16-bit features of up to 128 channels and 96 planes (with more, w's shares do not fit the
     // registers), where a workgroup has more than a step.  20 x 20, 91 planes bf16: 2048 boards 228 us a call, with
@@ -1155,7 +1168,7 @@ template <int DT, int OT, int CB, int MODE> hipError_t launch_products(PolicyDev
     constexpr bool PAIR = DT != 0 && CB == 1 && OT <= 6;
     const bool pair = PAIR && a.steps > CUS;
     const auto bytes = [&]() -> size_t {
-        if (!grad) return Smem<DT, OT, CB, 0, w_in_lds<DT, OT, CB>()>::bytes(a, a.counts ? WAVES * LossTile<OT>::bytes : 0) + 4 * ROWS * 16;   // (and the kernel's `red`)
+        if (!grad) return Smem<DT, OT, CB, 0, w_in_lds<DT, OT, CB>()>::bytes(a, a.counts ? WAVES * LossTile<OT>::bytes : 0) + LOSS_STATIC;
         if constexpr (PAIR) if (pair) return Smem<DT, OT, 1, 3, false>::bytes(a, PairCfg<DT, OT>::zb(a));
         return Smem<DT, OT, CB, 1, w_in_lds<DT, OT, CB>()>::bytes(a, Lay<DT, OT, CB>::z_bytes);
     };
@@ -1174,7 +1187,7 @@ template <int DT, int OT, int CB, int MODE> hipError_t launch_products(PolicyDev
         // as many workgroups as the chip holds at once, the boards in even shares
         const int per_cu = loss_waves<DT, OT, CB>() * 4 / WAVES >= 2 && lds * 2 <= LDS_BYTES ? 2 : 1;
         const int work = (a.B + a.nb - 1) / a.nb, room = CUS * per_cu, rounds = (work + room - 1) / room;
-        az_policy_loss_kernel<DT, OT, CB, MODE><<<(work + rounds - 1) / rounds, NT, lds - 4 * ROWS * 16, stream>>>(a, work);
+        az_policy_loss_kernel<DT, OT, CB, MODE><<<(work + rounds - 1) / rounds, NT, lds - LOSS_STATIC, stream>>>(a, work);
     } else {
         if (lds * 2 > LDS_BYTES && groups > CUS) groups = CUS;       // one workgroup a CU
         if constexpr (PAIR) if (pair) { az_policy_grad16_kernel<DT, OT, MODE><<<groups, NT, lds, stream>>>(a); return hipGetLastError(); }

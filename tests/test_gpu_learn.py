@@ -542,3 +542,28 @@ def test_matrices_that_are_not_contiguous_are_refused():
             learn.orthogonalize(bad)
     for good in (u[::2], u[1:2, :, :], u[:, :1], u.view(4, 12, 5, 4)[0], u[0], u.view(4, 12, 5, 2, 2)[::3], u[:, 3:7]):
         assert torch.equal(learn.orthogonalize(good), learn.orthogonalize(good.contiguous()))
+
+
+@pytest.mark.parametrize("sparse", [False, True], ids=["dense", "sparse"])
+@pytest.mark.parametrize("N", [3, 9, 20])
+def test_a_nan_target_counts_for_the_gradients_only(N, sparse):
+    B, C, O = 6, 24, 5
+    p = _rows(B, N, C, O, "f32", sparse=sparse, seed=N, cap=9)
+    if sparse:
+        p["tgt"][0][2] = 9
+        p["tgt"][2][2] = 0.1
+        p["tgt"][1][2] = torch.arange(9, dtype=torch.int32)
+        p["tgt"][2][2, 4] = float("nan")
+        p["t"][2] = 0
+        p["t"][2, :9] = 0.1
+        p["t"][2, 4] = 0
+        p["t"] = p["t"].float().double()
+    else:
+        p["tgt"].view(B, -1)[2, 4] = float("nan")
+        p["t"][2, 4] = 0
+    loss, dx, dw, db = _grad(p)
+    want = _exact(p, torch.ones(B, dtype=torch.float64))[0]
+    assert torch.allclose(loss.cpu().double(), want, rtol=1e-5, atol=1e-5)      # (sums of at most 2000 fp32 terms: 2^-13 of them at worst)
+    keep = torch.arange(B) != 2
+    assert torch.isnan(dx[2]).all() and torch.isfinite(dx.cpu()[keep]).all()
+    assert torch.isnan(dw).all() and torch.isnan(db).all()
