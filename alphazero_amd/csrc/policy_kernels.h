@@ -92,7 +92,7 @@ struct BoardLds {
     float* val;
     int* cnt;                                                        // [64-entry chunk][BLOCKS]
     int* start;                                                      // [BLOCKS + 1]: a block's first entry
-    az_f4* stat;                                                     // [MAX_BOARDS] of the gradients: {log2 e max, r T / sum of exp, r, is the loss infinite}
+    az_f4* stat;                                                     // [MAX_BOARDS] of the gradients: {max z, r T / sum of exp, r, is the loss infinite}
     bool listed;                                                     // the entries fit
 };
 // entries outside the board's actions: -1
@@ -277,10 +277,10 @@ __device__ __forceinline__ void finish_board(const PolicyDev& a, int b, float m,
     const float lse = m == -INFINITY ? (l == l ? -INFINITY : l) : m + logf(l);
     const bool masked = tz == -INFINITY;                             // a target on an action that is not allowed
     const float loss = masked ? INFINITY : (tl != 0.f ? tl * lse : 0.f) - tz;
-    // The gradients take probabilities as exp2(log2 e z - log2 e max) / l: an lse rounded to 32 bits, off by up to 2^-22
+    // The gradients take probabilities as exp2((z - max) log2 e) / l, which is exactly 1 where one action is allowed: an lse rounded to 32 bits, off by up to 2^-22
     // where it is about 5, would move all of a board's probabilities one way, and where one plane's sum to the targets' sum
     // that is what is left of the products with features of one sign.
-    a.stats[b] = az_f4{m == -INFINITY ? 0.f : m * LOG2E, tm, l == 0.f ? 0.f : 1.f / l, loss};
+    a.stats[b] = az_f4{m == -INFINITY ? 0.f : m, tm, l == 0.f ? 0.f : 1.f / l, loss};
     if (a.loss) a.loss[b] = loss;
 }
 
@@ -485,12 +485,12 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                 float to = mx;
                 #pragma unroll
                 for (int j = 0; j < R::OTP; ++j) to = fmaxf(to, fmaxf(fmaxf(acc[j][0], acc[j][1]), fmaxf(acc[j][2], acc[j][3])));
-                const float ml = to == -INFINITY ? 0.f : to * LOG2E;
+                const float ml = to == -INFINITY ? 0.f : to;
                 l *= rescale(mx, to);
                 #pragma unroll
                 for (int j = 0; j < R::OTP; ++j)
                     #pragma unroll
-                    for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -ml));
+                    for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f((acc[j][i] - ml) * LOG2E);
                 mx = to;
             }
         }
@@ -742,7 +742,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         __builtin_amdgcn_sched_barrier(0);                           // (phases apart: mixed, they want more registers than there are)
         product<KT, L::KS, OTH, !WLDS>(a.C, fetch, step);
         __builtin_amdgcn_sched_barrier(0);
-        const float rp = up * bst[1], m2 = bst[0];
+        const float rp = up * bst[1], mz = bst[0];
         // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
         const bool bias_counts = a.O > 1 || bst[3] != 0.f;
         #pragma unroll
@@ -754,7 +754,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                 const az_i4 w = *(const az_i4*)(words + j * 16);
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float v = rp * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -m2)) - rs * tv[j][i];
+                    const float v = __builtin_fmaf(rp, __builtin_amdgcn_exp2f((acc[j][i] - mz) * LOG2E), -rs * tv[j][i]);
                     dz[i] = (unsigned)w[i] & bit ? v : 0.f;
                 }
             }
@@ -992,7 +992,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
             const unsigned* words = m.b.words + (bb * a.N + y) * (OT * 16) + q * 4;
             const az_f4 bst = m.b.stat[bb];
             if (a.counts) scatter_targets<G::LDP>(a, m.b, own, st, wave, e0, e1, key0, val0, lane);
-            const float rs = live ? up * bst[2] : 0.f, rp = live ? up * bst[1] : 0.f, m2 = bst[0];
+            const float rs = live ? up * bst[2] : 0.f, rp = live ? up * bst[1] : 0.f, mz = bst[0];
             // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
             const bool bias_counts = a.O > 1 || bst[3] != 0.f;
             constexpr int OH = OT > 2 ? OT / 2 : OT;                 // planes in two halves: fewer registers
@@ -1016,7 +1016,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
                     const int o = (j0 + j) * 16 + q * 4;
                     az_f4 dz;
                     #pragma unroll
-                    for (int i = 0; i < 4; ++i) dz[i] = __builtin_fmaf(rp, __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][i], LOG2E, -m2)), -rs * tv[j0 + j][i]);
+                    for (int i = 0; i < 4; ++i) dz[i] = __builtin_fmaf(rp, __builtin_amdgcn_exp2f((acc[j][i] - mz) * LOG2E), -rs * tv[j0 + j][i]);
                     if (a.legal) {
                         const az_i4 w = *(const az_i4*)(words + (j0 + j) * 16);
                         #pragma unroll

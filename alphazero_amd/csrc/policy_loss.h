@@ -35,7 +35,7 @@ struct PolicyDev {
     const unsigned* legal;                   // [B, O * N] or null
     const float* row_scale;                  // [B] or null
     float scale;
-    az_f4* stats;                            // [B] {log2 e max z, T, 1 / sum of exp(z - max), loss}
+    az_f4* stats;                            // [B] {max z, T, 1 / sum of exp(z - max), loss}
     float *loss, *partial;
     const float *wpad, *wpadt;               // fp32 weights that do not fit LDS: padded copies
     void* dh;

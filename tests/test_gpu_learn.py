@@ -567,3 +567,18 @@ def test_a_nan_target_counts_for_the_gradients_only(N, sparse):
     keep = torch.arange(B) != 2
     assert torch.isnan(dx[2]).all() and torch.isfinite(dx.cpu()[keep]).all()
     assert torch.isnan(dw).all() and torch.isnan(db).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("case", [(5, 3, 20, 1), (200, 9, 64, 2), (3, 20, 200, 91), (40, 20, 128, 91)], ids=lambda c: "b%d-n%d-c%d-o%d" % c)
+def test_a_board_with_one_allowed_action_has_exactly_no_loss(case, dtype):
+    B, N, C, O = case
+    p = _rows(B, N, C, O, dtype, "nhwc", legal=0.5, seed=3)
+    A = O * N * N
+    at = torch.randint(0, A, (B,), generator=torch.Generator().manual_seed(1))
+    ok = torch.zeros(B, A, dtype=torch.bool)
+    ok[torch.arange(B), at] = True
+    p["tgt"] = ok.view(B, O, N, N).float() * torch.linspace(0.3, 1.0, B).view(B, 1, 1, 1)
+    p["words"] = (ok.view(B, O * N, N).long() << torch.arange(N)).sum(2).to(torch.int32)
+    loss, dx, dw, db = _grad(p, 1.0 / 3)
+    assert (loss == 0).all() and (dx == 0).all() and (dw == 0).all() and (db == 0).all()
