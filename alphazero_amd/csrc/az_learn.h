@@ -53,6 +53,14 @@ template <int DT> __device__ __forceinline__ void az_split(float x, short& hi, s
     hi = az_to16<DT>(x);
     lo = az_to16<DT>(x - az_from16<DT>(hi));
 }
+// and with a third part: all 24 bits of a bf16 triple
+template <int DT> __device__ __forceinline__ void az_split(float x, short& hi, short& lo, short& rest) {
+    asm("" : "+v"(x));
+    hi = az_to16<DT>(x);
+    const float r = x - az_from16<DT>(hi);
+    lo = az_to16<DT>(r);
+    rest = az_to16<DT>(r - az_from16<DT>(lo));
+}
 template <int DT> __device__ __forceinline__ float az_load(const void* p, size_t i) {
     if constexpr (DT == 0) return ((const float*)p)[i];
     else return az_from16<DT>(((const short*)p)[i]);

@@ -3,6 +3,8 @@
 #pragma once
 #include "policy_loss.h"
 
+#include <type_traits>
+
 namespace {
 
 // dynamic LDS of the two product kernels
@@ -627,7 +629,8 @@ template <int LD> __device__ __forceinline__ void scatter_targets(const PolicyDe
 // rows and a quarter of the channels a wave) and its product with the features (half of the planes and a quarter of the
 // channels a wave, kept in registers over all of a workgroup's steps).  16-bit features: dz goes to LDS as hi + lo of the
 // type, hi alone feeds dh (whose result is rounded to that type anyway), both feed dw (an fp32 sum over all rows: one
-// rounding to 16 bits of each term would stay in it).
+// rounding to 16 bits of each term would stay in it).  bf16: hi + lo are 16 bits, which shows in dw of small batches (up to
+// 5e-6 of it against 1e-7 in fp32); a third part takes hi's place once that has been read.
 // (16-bit features of up to 128 channels and 96 planes have a kernel of their own below for all but the smallest batches.)
 // fp32: bound by the matrix instructions, 32 cycles for the 16 x 16 x 4: 256 boards of 20 x 20, 256 channels, 91 planes
 // 225 us, 64 TFLOP/s (three products: 93 us at the rate of a large one).  256 channels leave no registers to ask for the next
@@ -637,7 +640,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
     typedef typename AzElem<DT>::T T;
     constexpr int NP = CB * 128 / L::EP * ROWS / NT, OTH = (OT + 1) / 2, KO = L::OP / L::KS, KT = CB * 128 / L::KS;
     constexpr int OG = OT > 1 ? 2 : 1, CG = 8 / OG, OTN = OT / OG, CTN = CB * 8 / CG;   // dw: groups of planes and channels, tiles of a wave
-    constexpr bool WLDS = w_in_lds<DT, OT, CB>();
+    constexpr bool WLDS = w_in_lds<DT, OT, CB>(), THIRD = DT == 2;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr int Cp = L::CP, ldc = L::LDC;
     const Smem<DT, OT, CB, 1, WLDS> m(smem, a, L::z_bytes);
@@ -745,6 +748,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         const float rp = up * bst[1], mz = bst[0];
         // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
         const bool bias_counts = a.O > 1 || bst[3] != 0.f;
+        az_s4 rest[THIRD ? OTH : 1];
         #pragma unroll
         for (int j = 0; j < OTH; ++j) {
             const int ot = half * OTH + j;
@@ -763,7 +767,13 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
             else {
                 az_s4 hi, lo;
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) { short x, y; az_split<DT>(dz[i], x, y); hi[i] = x; lo[i] = y; }
+                for (int i = 0; i < 4; ++i) {
+                    short x, y, z;
+                    if constexpr (THIRD) { az_split<DT>(dz[i], x, y, z); rest[j][i] = z; }
+                    else az_split<DT>(dz[i], x, y);
+                    hi[i] = x;
+                    lo[i] = y;
+                }
                 *(az_s4*)((short*)zhi + rl * L::LDO + ot * 16 + q * 4) = hi;
                 *(az_s4*)((short*)zlo + rl * L::LDO + ot * 16 + q * 4) = lo;
             }
@@ -819,27 +829,38 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         }
         // dw: rows of a tile are planes, columns are channels, the contraction runs over the step's rows (rows beyond the
         // step have dz = 0 and features of 0)
-        #pragma unroll
-        for (int k = 0; k < ROWS; k += L::KS) {
-            if (k >= st.rows) break;
-            __builtin_amdgcn_sched_barrier(0);
-            az_i4 zf[OTN][DT == 0 ? 1 : 2];
+        const auto times_features = [&](auto parts) __attribute__((always_inline)) {
+            constexpr int P = decltype(parts)::value;
             #pragma unroll
-            for (int j = 0; j < OTN; ++j) {
-                zf[j][0] = az_col_frag<DT, true>(zhi, L::LDO, k, (og * OTN + j) * 16, lane);
-                if constexpr (DT != 0) zf[j][1] = az_col_frag<DT, true>(zlo, L::LDO, k, (og * OTN + j) * 16, lane);
-            }
-            #pragma unroll
-            for (int i = 0; i < CTN; ++i) {
-                const int ct = cg + CG * i;
-                if (ct * 16 >= a.C) continue;
-                const az_i4 hb = az_col_frag<DT, true>(h, ldc, k, ct * 16, lane);
+            for (int k = 0; k < ROWS; k += L::KS) {
+                if (k >= st.rows) break;
+                __builtin_amdgcn_sched_barrier(0);
+                az_i4 zf[OTN][P];
                 #pragma unroll
                 for (int j = 0; j < OTN; ++j) {
-                    dw[i][j] = az_mma<DT>(zf[j][0], hb, dw[i][j]);
-                    if constexpr (DT != 0) dw[i][j] = az_mma<DT>(zf[j][1], hb, dw[i][j]);
+                    zf[j][0] = az_col_frag<DT, true>(zhi, L::LDO, k, (og * OTN + j) * 16, lane);
+                    if constexpr (P == 2) zf[j][1] = az_col_frag<DT, true>(zlo, L::LDO, k, (og * OTN + j) * 16, lane);
+                }
+                #pragma unroll
+                for (int i = 0; i < CTN; ++i) {
+                    const int ct = cg + CG * i;
+                    if (ct * 16 >= a.C) continue;
+                    const az_i4 hb = az_col_frag<DT, true>(h, ldc, k, ct * 16, lane);
+                    #pragma unroll
+                    for (int j = 0; j < OTN; ++j)
+                        #pragma unroll
+                        for (int p = 0; p < P; ++p) dw[i][j] = az_mma<DT>(zf[j][p], hb, dw[i][j]);
                 }
             }
+        };
+        times_features(std::integral_constant<int, DT == 0 ? 1 : 2>{});
+        if constexpr (THIRD) {
+            __syncthreads();                                         // hi has been read
+            #pragma unroll
+            for (int j = 0; j < OTH; ++j)
+                if ((half * OTH + j) * 16 < L::OP) *(az_s4*)((short*)zhi + rl * L::LDO + (half * OTH + j) * 16 + q * 4) = rest[j];
+            __syncthreads();
+            times_features(std::integral_constant<int, 1>{});
         }
         __syncthreads();                                             // everything of this step has been read
         if (it + 1 < s_hi) {
