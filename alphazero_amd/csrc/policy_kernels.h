@@ -911,7 +911,12 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
 template <int DT, int OT> struct PairCfg {
     typedef Lay<DT, OT, 1> L;
     static constexpr int LDP = OT * 16 + 4;
-    static constexpr size_t own = (size_t)16 * LDP * 4, z = (size_t)2 * ROWS * L::LDO * 2;    // a row tile's targets; a step's dz
+    // bf16, up to 16 planes: a third part of dz for dw, as in az_policy_grad_kernel (with more planes and this kernel's more than
+    // 256 steps d_weight is as exact as fp32 products' without it).  Parts that only dw reads need no padding to a step of
+    // the contraction over planes.
+    static constexpr bool THIRD = DT == 2 && OT == 1;
+    static constexpr int LDL = OT == 1 ? 16 : L::LDO;
+    static constexpr size_t own = (size_t)16 * LDP * 4, z = (size_t)ROWS * (L::LDO + (THIRD ? 2 : 1) * LDL) * 2;    // a row tile's targets; a step's dz
     static size_t zb(const PolicyDev& a) { return 2 * z + (a.counts ? 4 * own : 0); }
 };
 // az_col_frag of 16 columns that are not neighbours: four from n0, four from n0 + 8, ...
@@ -1005,7 +1010,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
             float val0 = 0.f;
             if (e0 + lane < e1) { key0 = m.b.key[e0 + lane]; val0 = m.b.val[e0 + lane]; }
             const T* h = hbuf + t % 3 * ROWS * ldc;
-            T* const zhi = zbuf + (t & 1) * 2 * ROWS * L::LDO;
+            T* const zhi = zbuf + (t & 1) * (G::z / 2);
             T* const zlo = zhi + ROWS * L::LDO;
             const bool live = rl < st.rows;
             const int bb = live && a.nb > 1 ? (int)((unsigned)rl * a.mag_s >> 16) : 0, s = live ? st.cell0 + rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
@@ -1044,17 +1049,23 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
                         for (int i = 0; i < 4; ++i) dz[i] = (unsigned)w[i] & bit ? dz[i] : 0.f;
                     }
                     if (bias_counts) db[j0 + j] += dz;
-                    az_s4 hi, lo;
+                    az_s4 hi, lo, rest;
                     #pragma unroll
-                    for (int i = 0; i < 4; ++i) { short x, y; az_split<DT>(dz[i], x, y); hi[i] = x; lo[i] = y; }
+                    for (int i = 0; i < 4; ++i) {
+                        short x, y, z;
+                        if constexpr (G::THIRD) { az_split<DT>(dz[i], x, y, z); rest[i] = z; }
+                        else az_split<DT>(dz[i], x, y);
+                        hi[i] = x;
+                        lo[i] = y;
+                    }
                     *(az_s4*)((short*)zhi + rl * L::LDO + o) = hi;
-                    *(az_s4*)((short*)zlo + rl * L::LDO + o) = lo;
+                    *(az_s4*)((short*)zlo + rl * G::LDL + o) = lo;
+                    if constexpr (G::THIRD) *(az_s4*)((short*)zlo + ROWS * G::LDL + rl * G::LDL + o) = rest;
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (OT == 1) {                                 // planes 16 .. 31 of the contraction: zero
                 *(az_s4*)((short*)zhi + rl * L::LDO + 16 + q * 4) = az_s4{0, 0, 0, 0};
-                *(az_s4*)((short*)zlo + rl * L::LDO + 16 + q * 4) = az_s4{0, 0, 0, 0};
             }
             if (a.counts) clear_own();
             if (!a.counts && t + 1 < steps) targets(a, nx);
@@ -1111,7 +1122,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
             s0 = s1; s1 = s2; s2 = s3;
             if (t + 4 < steps) { s3.next(a); f.load(a, s3, tb); }
             const T* h = hbuf + t % 3 * ROWS * ldc;
-            const T* const zhi = zbuf + (t & 1) * 2 * ROWS * L::LDO;
+            const T* const zhi = zbuf + (t & 1) * (G::z / 2);
             const T* const zlo = zhi + ROWS * L::LDO;
             // dh: rows of a tile are channels, columns are cells
             #pragma unroll
@@ -1152,11 +1163,16 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
                 const az_i4 hb0 = az_col_frag<DT, true>(h, ldc, k, cq * 32, lane), hb1 = az_col_frag<DT, true>(h, ldc, k, cq * 32 + 16, lane);
                 #pragma unroll
                 for (int j = 0; j < OT; ++j) {
-                    const az_i4 z1 = az_col_frag<DT, true>(zhi, L::LDO, k, j * 16, lane), z2 = az_col_frag<DT, true>(zlo, L::LDO, k, j * 16, lane);
+                    const az_i4 z1 = az_col_frag<DT, true>(zhi, L::LDO, k, j * 16, lane), z2 = az_col_frag<DT, true>(zlo, G::LDL, k, j * 16, lane);
                     dw[0][j] = az_mma<DT>(z1, hb0, dw[0][j]);
                     dw[1][j] = az_mma<DT>(z1, hb1, dw[1][j]);
                     dw[0][j] = az_mma<DT>(z2, hb0, dw[0][j]);
                     dw[1][j] = az_mma<DT>(z2, hb1, dw[1][j]);
+                    if constexpr (G::THIRD) {
+                        const az_i4 z3 = az_col_frag<DT, true>(zlo + ROWS * G::LDL, G::LDL, k, j * 16, lane);
+                        dw[0][j] = az_mma<DT>(z3, hb0, dw[0][j]);
+                        dw[1][j] = az_mma<DT>(z3, hb1, dw[1][j]);
+                    }
                 }
             }
             if (t + 1 < steps) __syncthreads();
