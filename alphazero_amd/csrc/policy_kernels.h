@@ -628,9 +628,10 @@ template <int LD> __device__ __forceinline__ void scatter_targets(const PolicyDe
 // Gradients.  Eight waves.  A step: dz of 64 rows (16 rows and half of the planes a wave), then its product with w (32
 // rows and a quarter of the channels a wave) and its product with the features (half of the planes and a quarter of the
 // channels a wave, kept in registers over all of a workgroup's steps).  16-bit features: dz goes to LDS as hi + lo of the
-// type, hi alone feeds dh (whose result is rounded to that type anyway), both feed dw (an fp32 sum over all rows: one
-// rounding to 16 bits of each term would stay in it).  bf16: hi + lo are 16 bits, which shows in dw of small batches (up to
-// 5e-6 of it against 1e-7 in fp32); a third part takes hi's place once that has been read.
+// type, and both feed both products: where planes cancel, hi alone (half a step of the type in each term) was off by up to a
+// third of an element of dh, and made its error 1.4 times its own rounding on the whole.  bf16: hi + lo are 16 bits, which shows
+// in dw of small batches (an fp32 sum over all rows: up to 5e-6 of it against 1e-7 in fp32); a third part takes hi's place
+// once that has been read.
 // (16-bit features of up to 128 channels and 96 planes have a kernel of their own below for all but the smallest batches.)
 // fp32: bound by the matrix instructions, 32 cycles for the 16 x 16 x 4: 256 boards of 20 x 20, 256 channels, 91 planes
 // 225 us, 64 TFLOP/s (three products: 93 us at the rate of a large one).  256 channels leave no registers to ask for the next
@@ -785,14 +786,19 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         // dh: rows of a tile are channels, columns are cells
         {
             // (fp32: dz is read again for every tile of channels -- the LDS port is idle behind the fp32 matrix instructions,
-            // and the fragments of both row tiles would take 48 registers)
-            constexpr bool KEEP = DT != 0;
-            az_i4 zf[2][KEEP ? KO : 1];
+            // and the fragments of both row tiles would take 48 registers; so it is where 16 bits' 64 registers do not fit
+            // beside the largest dw)
+            constexpr bool KEEP = DT != 0 && !(OT == 8 && CB == 2);
+            constexpr int PARTS = DT == 0 ? 1 : 2;
+            az_i4 zf[2][KEEP ? KO : 1][PARTS];                       // [row tile][step][hi, lo]
+            const auto dz_frag = [&](int e, int k, int p) __attribute__((always_inline)) { return az_row_frag<DT>(p ? zlo : zhi, L::LDO, (pair * 2 + e) * 16, k * L::KS, lane); };
             if constexpr (KEEP) {
                 #pragma unroll
                 for (int k = 0; k < KO; ++k)
                     #pragma unroll
-                    for (int e = 0; e < 2; ++e) zf[e][k] = az_row_frag<DT>(zhi, L::LDO, (pair * 2 + e) * 16, k * L::KS, lane);
+                    for (int e = 0; e < 2; ++e)
+                        #pragma unroll
+                        for (int p = 0; p < PARTS; ++p) zf[e][k][p] = dz_frag(e, k, p);
             }
             #pragma unroll 1
             for (int j = 0; j < CB * 2; ++j) {
@@ -804,8 +810,10 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                     az_i4 wa;
                     if constexpr (WLDS) wa = az_col_frag<DT>(m.w, L::LDW, k * L::KS, ct * 16, lane);
                     else wa = az_row_frag<DT>(a.wpadt, L::OP, ct * 16, k * L::KS, lane);
-                    d[0] = az_mma<DT>(wa, KEEP ? zf[0][KEEP ? k : 0] : az_row_frag<DT>(zhi, L::LDO, pair * 32, k * L::KS, lane), d[0]);
-                    d[1] = az_mma<DT>(wa, KEEP ? zf[1][KEEP ? k : 0] : az_row_frag<DT>(zhi, L::LDO, pair * 32 + 16, k * L::KS, lane), d[1]);
+                    #pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        #pragma unroll
+                        for (int p = 0; p < PARTS; ++p) d[e] = az_mma<DT>(wa, KEEP ? zf[e][KEEP ? k : 0][p] : dz_frag(e, k, p), d[e]);
                 }
                 const int c = ct * 16 + q * 4;
                 #pragma unroll
@@ -915,14 +923,16 @@ template <int DT, int OT> struct PairCfg {
     // 256 steps d_weight is as exact as fp32 products' without it).  Parts that only dw reads need no padding to a step of
     // the contraction over planes.
     static constexpr bool THIRD = DT == 2 && OT == 1;
-    static constexpr int LDL = OT == 1 ? 16 : L::LDO;
-    static constexpr size_t own = (size_t)16 * LDP * 4, z = (size_t)ROWS * (L::LDO + (THIRD ? 2 : 1) * LDL) * 2;    // a row tile's targets; a step's dz
+    // A row of dz: its parts side by side, PW planes each, rows an odd multiple of 32 bytes apart (az_col_frag).  Up to 16 planes:
+    // hi and lo are one step of the contraction over planes, against w's planes twice.
+    static constexpr int PW = OT * 16, LDZ = OT == 1 ? 48 : 2 * PW + 16;
+    static constexpr size_t own = (size_t)16 * LDP * 4, z = (size_t)ROWS * LDZ * 2;    // a row tile's targets; a step's dz
     static size_t zb(const PolicyDev& a) { return 2 * z + (a.counts ? 4 * own : 0); }
 };
-// az_col_frag of 16 columns that are not neighbours: four from n0, four from n0 + 8, ...
-__device__ __forceinline__ az_i4 pair_col_frag(const void* m, int ld, int k0, int n0, int lane) {
+// az_col_frag of 16 columns that are not neighbours: four from n0, four from n0 + 8, ...  TWICE: 16 rows, and the same again.
+template <bool TWICE> __device__ __forceinline__ az_i4 pair_col_frag(const void* m, int ld, int k0, int n0, int lane) {
     typedef __attribute__((address_space(3))) az_s4* lds_s4;
-    const short* p = (const short*)m + (k0 + 8 * (lane >> 4) + ((lane & 15) >> 2)) * ld + n0 + (lane & 3) * 8;
+    const short* p = (const short*)m + (k0 + 8 * (lane >> 4 & (TWICE ? 1 : 3)) + ((lane & 15) >> 2)) * ld + n0 + (lane & 3) * 8;
     const az_s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p);
     const az_s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 4 * ld));
     return __builtin_bit_cast(az_i4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -936,7 +946,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const Smem<DT, OT, 1, 3, false> m(smem, a, 2 * G::z + (a.counts ? 4 * G::own : 0));
     T* const hbuf = (T*)m.h;
-    T* const zbuf = (T*)m.t;                                         // [2][hi, lo][ROWS][LDO]
+    T* const zbuf = (T*)m.t;                                         // [2][ROWS][LDZ]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
     const int s_lo = (int)((long long)blockIdx.x * a.steps / gridDim.x), steps = (int)((long long)(blockIdx.x + 1) * a.steps / gridDim.x) - s_lo;
     Step st(a, s_lo);
@@ -1010,8 +1020,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
             float val0 = 0.f;
             if (e0 + lane < e1) { key0 = m.b.key[e0 + lane]; val0 = m.b.val[e0 + lane]; }
             const T* h = hbuf + t % 3 * ROWS * ldc;
-            T* const zhi = zbuf + (t & 1) * (G::z / 2);
-            T* const zlo = zhi + ROWS * L::LDO;
+            short* const dzr = (short*)zbuf + (t & 1) * (G::z / 2) + rl * G::LDZ;
             const bool live = rl < st.rows;
             const int bb = live && a.nb > 1 ? (int)((unsigned)rl * a.mag_s >> 16) : 0, s = live ? st.cell0 + rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
             const unsigned bit = live ? 1u << (s - y * a.N) : 0u;
@@ -1058,14 +1067,11 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
                         hi[i] = x;
                         lo[i] = y;
                     }
-                    *(az_s4*)((short*)zhi + rl * L::LDO + o) = hi;
-                    *(az_s4*)((short*)zlo + rl * G::LDL + o) = lo;
-                    if constexpr (G::THIRD) *(az_s4*)((short*)zlo + ROWS * G::LDL + rl * G::LDL + o) = rest;
+                    *(az_s4*)(dzr + o) = hi;
+                    *(az_s4*)(dzr + G::PW + o) = lo;
+                    if constexpr (G::THIRD) *(az_s4*)(dzr + 2 * G::PW + o) = rest;
                 }
                 __builtin_amdgcn_sched_barrier(0);
-            }
-            if constexpr (OT == 1) {                                 // planes 16 .. 31 of the contraction: zero
-                *(az_s4*)((short*)zhi + rl * L::LDO + 16 + q * 4) = az_s4{0, 0, 0, 0};
             }
             if (a.counts) clear_own();
             if (!a.counts && t + 1 < steps) targets(a, nx);
@@ -1090,7 +1096,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
         #pragma unroll
         for (int j = 0; j < 2; ++j)
             #pragma unroll
-            for (int k = 0; k < KO; ++k) wc[j][k] = pair_col_frag(m.h, L::LDW, k * L::KS, cq * 32 + 4 * j, lane);
+            for (int k = 0; k < KO; ++k) wc[j][k] = pair_col_frag<OT == 1>(m.h, L::LDW, k * L::KS, cq * 32 + 4 * j, lane);
         az_f4 dw[2][OT];
         #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -1122,8 +1128,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
             s0 = s1; s1 = s2; s2 = s3;
             if (t + 4 < steps) { s3.next(a); f.load(a, s3, tb); }
             const T* h = hbuf + t % 3 * ROWS * ldc;
-            const T* const zhi = zbuf + (t & 1) * (G::z / 2);
-            const T* const zlo = zhi + ROWS * L::LDO;
+            const T* const zt = zbuf + (t & 1) * (G::z / 2);
             // dh: rows of a tile are channels, columns are cells
             #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -1131,9 +1136,12 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
                 az_f4 d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
                 #pragma unroll
                 for (int k = 0; k < KO; ++k) {
-                    const az_i4 zf = az_row_frag<DT>(zhi, L::LDO, e * 16, k * L::KS, lane);
-                    d[0] = az_mma<DT>(wc[0][k], zf, d[0]);
-                    d[1] = az_mma<DT>(wc[1][k], zf, d[1]);
+                    #pragma unroll
+                    for (int part = 0; part < (OT == 1 ? 1 : 2); ++part) {       // (one plane tile: hi and lo in one)
+                        const az_i4 zf = az_row_frag<DT>(zt, G::LDZ, e * 16, part * G::PW + k * L::KS, lane);
+                        d[0] = az_mma<DT>(wc[0][k], zf, d[0]);
+                        d[1] = az_mma<DT>(wc[1][k], zf, d[1]);
+                    }
                 }
                 const int row = e * 16 + (lane & 15), c = cq * 32 + q * 8;       // the two tiles hold 8 channels of the row in turn
                 if (row >= st.rows || c >= a.C) continue;
@@ -1163,13 +1171,13 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
                 const az_i4 hb0 = az_col_frag<DT, true>(h, ldc, k, cq * 32, lane), hb1 = az_col_frag<DT, true>(h, ldc, k, cq * 32 + 16, lane);
                 #pragma unroll
                 for (int j = 0; j < OT; ++j) {
-                    const az_i4 z1 = az_col_frag<DT, true>(zhi, L::LDO, k, j * 16, lane), z2 = az_col_frag<DT, true>(zlo, G::LDL, k, j * 16, lane);
+                    const az_i4 z1 = az_col_frag<DT, true>(zt, G::LDZ, k, j * 16, lane), z2 = az_col_frag<DT, true>(zt, G::LDZ, k, G::PW + j * 16, lane);
                     dw[0][j] = az_mma<DT>(z1, hb0, dw[0][j]);
                     dw[1][j] = az_mma<DT>(z1, hb1, dw[1][j]);
                     dw[0][j] = az_mma<DT>(z2, hb0, dw[0][j]);
                     dw[1][j] = az_mma<DT>(z2, hb1, dw[1][j]);
                     if constexpr (G::THIRD) {
-                        const az_i4 z3 = az_col_frag<DT, true>(zlo + ROWS * G::LDL, G::LDL, k, j * 16, lane);
+                        const az_i4 z3 = az_col_frag<DT, true>(zt, G::LDZ, k, 2 * G::PW + j * 16, lane);
                         dw[0][j] = az_mma<DT>(z3, hb0, dw[0][j]);
                         dw[1][j] = az_mma<DT>(z3, hb1, dw[1][j]);
                     }
