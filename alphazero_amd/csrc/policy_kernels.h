@@ -919,15 +919,15 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
 template <int DT, int OT> struct PairCfg {
     typedef Lay<DT, OT, 1> L;
     static constexpr int LDP = OT * 16 + 4;
-    // bf16, up to 16 planes: a third part of dz for dw, as in az_policy_grad_kernel (with more planes and this kernel's more than
-    // 256 steps d_weight is as exact as fp32 products' without it).  Parts that only dw reads need no padding to a step of
-    // the contraction over planes.
-    static constexpr bool THIRD = DT == 2 && OT == 1;
+    // bf16: a third part of dz for dw, as in az_policy_grad_kernel.  Its room for 96 planes is that of the sparse targets' tiles:
+    // those lie in the rows that the wave's dz is about to take, and are all read before.
+    static constexpr bool THIRD = DT == 2, ALIAS = THIRD && OT == 6;
     // A row of dz: its parts side by side, PW planes each, rows an odd multiple of 32 bytes apart (az_col_frag).  Up to 16 planes:
     // hi and lo are one step of the contraction over planes, against w's planes twice.
-    static constexpr int PW = OT * 16, LDZ = OT == 1 ? 48 : 2 * PW + 16;
+    static constexpr int PW = OT * 16, LDZ = OT == 1 ? 48 : (THIRD ? 3 : 2) * PW + 16;
     static constexpr size_t own = (size_t)16 * LDP * 4, z = (size_t)ROWS * LDZ * 2;    // a row tile's targets; a step's dz
-    static size_t zb(const PolicyDev& a) { return 2 * z + (a.counts ? 4 * own : 0); }
+    static_assert(!ALIAS || own <= (size_t)16 * LDZ * 2, "a tile of targets lies in 16 rows of dz");
+    static __host__ __device__ size_t zb(const PolicyDev& a) { return 2 * z + (a.counts && !ALIAS ? 4 * own : 0); }
 };
 // az_col_frag of 16 columns that are not neighbours: four from n0, four from n0 + 8, ...  TWICE: 16 rows, and the same again.
 template <bool TWICE> __device__ __forceinline__ az_i4 pair_col_frag(const void* m, int ld, int k0, int n0, int lane) {
@@ -944,7 +944,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
     typedef typename AzElem<DT>::T T;
     constexpr int KT = 128 / L::KS, KO = L::OP / L::KS, ldc = L::LDC;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const Smem<DT, OT, 1, 3, false> m(smem, a, 2 * G::z + (a.counts ? 4 * G::own : 0));
+    const Smem<DT, OT, 1, 3, false> m(smem, a, G::zb(a));
     T* const hbuf = (T*)m.h;
     T* const zbuf = (T*)m.t;                                         // [2][ROWS][LDZ]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
@@ -989,14 +989,14 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
         if (a.C < L::CP) for (int i = tid; i < 3 * ROWS * ldc; i += NT / 2) hbuf[i] = (T)0.f;
         __syncthreads();
         boards.first(a, m.b, st.b0, tid);
-        float* const own = (float*)((unsigned char*)m.t + 2 * G::z + wave * G::own);
+        float* const apart = (float*)((unsigned char*)m.t + 2 * G::z + wave * G::own);
         const int rl = wave * 16 + (lane & 15);
-        const auto clear_own = [&]() __attribute__((always_inline)) {
+        const auto clear_own = [&](float* own) __attribute__((always_inline)) {
             #pragma unroll
             for (int i = 0; i < (int)(G::own / 16 + 63) / 64; ++i)
                 if (i * 64 + lane < (int)(G::own / 16)) ((az_f4*)own)[i * 64 + lane] = az_f4{0.f, 0.f, 0.f, 0.f};
         };
-        if (a.counts) clear_own();
+        if (a.counts && !G::ALIAS) clear_own(apart);
         // dense targets of a step: asked for during the step before, ahead of the features (loads return in order)
         az_f4 tv[OT] = {};
         const auto targets = [&](const PolicyDev& a, const Step& st) __attribute__((always_inline)) {
@@ -1021,12 +1021,22 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
             if (e0 + lane < e1) { key0 = m.b.key[e0 + lane]; val0 = m.b.val[e0 + lane]; }
             const T* h = hbuf + t % 3 * ROWS * ldc;
             short* const dzr = (short*)zbuf + (t & 1) * (G::z / 2) + rl * G::LDZ;
+            float* const own = G::ALIAS ? (float*)((short*)zbuf + (t & 1) * (G::z / 2) + wave * 16 * G::LDZ) : apart;
             const bool live = rl < st.rows;
             const int bb = live && a.nb > 1 ? (int)((unsigned)rl * a.mag_s >> 16) : 0, s = live ? st.cell0 + rl - bb * a.S : 0, y = (int)((unsigned)s * a.mag_n >> 16);
             const unsigned bit = live ? 1u << (s - y * a.N) : 0u;
             const unsigned* words = m.b.words + (bb * a.N + y) * (OT * 16) + q * 4;
             const az_f4 bst = m.b.stat[bb];
-            if (a.counts) scatter_targets<G::LDP>(a, m.b, own, st, wave, e0, e1, key0, val0, lane);
+            if (a.counts) {
+                if (G::ALIAS) clear_own(own);
+                scatter_targets<G::LDP>(a, m.b, own, st, wave, e0, e1, key0, val0, lane);
+                if (G::ALIAS) {
+                    #pragma unroll
+                    for (int j = 0; j < OT; ++j) tv[j] = *(const az_f4*)(own + (lane & 15) * G::LDP + j * 16 + q * 4);
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                }
+            }
             const float rs = live ? up * bst[2] : 0.f, rp = live ? up * bst[1] : 0.f, mz = bst[0];
             // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
             const bool bias_counts = a.O > 1 || bst[3] != 0.f;
@@ -1042,7 +1052,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
                     #pragma unroll
                     for (int j = 0; j < OH; ++j) acc[j] = az_mma<DT>(wr[j0 + j][k], hb, acc[j]);
                 }
-                if (a.counts) {
+                if (a.counts && !G::ALIAS) {
                     #pragma unroll
                     for (int j = 0; j < OH; ++j) tv[j0 + j] = *(const az_f4*)(own + (lane & 15) * G::LDP + (j0 + j) * 16 + q * 4);
                 }
@@ -1073,7 +1083,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (a.counts) clear_own();
+            if (a.counts && !G::ALIAS) clear_own(apart);
             if (!a.counts && t + 1 < steps) targets(a, nx);
             st = nx;
             if (t + 2 < steps) nx.next(a);

@@ -35,3 +35,34 @@ def test_gradient_of_16_bit_features_is_off_by_its_own_rounding(case, layout, dt
         before = before + 2.0 ** -34 * float((r.abs() * m["T"]).max()) * p["w"].double().abs().sum(0).view(1, C, 1, 1)
     tol = half * want.abs() + (1 + half) * before + (2.0 ** -25 if dtype == "f16" else 0.0)
     assert ((dx - want).abs() <= tol).all(), ((dx - want).abs() / tol).max()
+
+
+# d_weight where no error can average out: channel c is 1 in one cell of board c alone, so d_weight[o, c] is one dz, r T p.  The
+# weights are 0, so logits are the biases and p is known exactly.  Roundings, in F24 of the value: the sum of exponentials, at most
+# 62 additions one after another on the way (two tiles of 96 planes in a lane, 64 lanes, 8 waves); exp2 and its argument, 7 in
+# the sum and 7 in dz; products and the division, 6; parts of dz: the third one leaves 1 (bfloat16), two of fp16 4.  100 in all.
+# Two parts of bfloat16 would leave up to 128.  (fp16: steps of 2^-34 of the largest r T besides.)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("sparse", [False, True], ids=["dense", "sparse"])
+@pytest.mark.parametrize("N,O", [(5, 3), (5, 91), (5, 120), (15, 2), (15, 17), (15, 40), (15, 91), (15, 128)])
+def test_gradient_of_the_weight_holds_32_bits(N, O, sparse, dtype):
+    B = C = 128
+    S = N * N
+    g = torch.Generator().manual_seed(N + O)
+    at = torch.randint(0, S - 1, (B,), generator=g)
+    x = torch.zeros(B, C, S, dtype=DT[dtype])
+    x[torch.arange(B), torch.arange(B), at] = 1
+    w, b = torch.zeros(O, C, dtype=DT[dtype]), (torch.rand(O, generator=g) * 1.5).to(DT[dtype])
+    T, r = torch.rand(B, generator=g) + 0.5, torch.rand(B, generator=g) + 0.5
+    if sparse:
+        tgt = (torch.ones(B, dtype=torch.int32), torch.full((B, 3), S - 1, dtype=torch.int32), T.view(B, 1).repeat(1, 3))     # (plane 0, the last cell)
+    else:
+        tgt = torch.zeros(B, O, S)
+        tgt[:, 0, S - 1] = T
+        tgt = tgt.view(B, O, N, N)
+    tgt = tuple(t.cuda() for t in tgt) if sparse else tgt.cuda()
+    dw = learn.policy_loss_grad(x.view(B, C, N, N).cuda(), w.cuda(), b.cuda(), tgt, row_scale=r.cuda())[2].cpu().double()
+    p = torch.softmax(b.double(), 0) / S
+    want = p.view(O, 1) * (r.double() * T.double()).view(1, C)
+    tol = 100 * F24 * want + (2.0 ** -34 * float((r * T).max()) if dtype == "f16" else 0.0)
+    assert ((dw - want).abs() <= tol).all(), (((dw - want).abs() / want).max() / F24, dw.shape)
