@@ -18,7 +18,7 @@
 // Measured on an MI355X that copies 4.9 TB/s and multiplies 1.1 PFLOP/s (fp16): 2 x 4096 x 1024 fp32 655 us (eleven
 // r x r launches of 25 us, X X^T 86 + 59 + 59 us, Q X 70 + 64 + 64 us; the Gram form's operations are 276 us at the rate of
 // a large product); optimiser step of 40 x 256 x 2304 513 us (momentum and norm 65 us at 5.7 TB/s, X X^T 68 + 50, r x r 13
-// launches of 12, Q X 78 + 95 us, the last with weights read and written).  18 x 128 x 1152 bf16 84 us.
+// launches of 12, Q X 78 + 95 us, the last with weights read and written).  18 x 128 x 1152 bf16 109 us.
 #include "../../include/az_hip.h"
 #include "az_learn.h"
 
@@ -864,9 +864,11 @@ Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b
     while (p.slices > 64 && (long long)p.slices * n > 2048) p.slices /= 2;
     p.split = split_of((long long)p.low * n, (p.k + 63) / 64);
     // Steps between two formations of X.  fp32 results: two (comment at the top); the optimiser step, whose weights take
-    // lr times the result: three; 16-bit results: five, their own rounding is larger.  Fewer where the coefficients would
-    // take Q out of fp16's range.
-    p.stage = muon ? 3 : dtype == AZ_F32 ? 2 : 5;
+    // lr times the result: three.  16-bit results: three, off by at most 8e-5 where half a step of fp16 is 2e-4 and of bf16
+    // 1.7e-3 (relative norms over 128 x 1152 .. 600 x 200, one to eight strong directions a thousand to ten thousand times the
+    // rest, where fp32 products are off by as much); all five at once leave 1e-3 to 7e-3 there.  18 x 128 x 1152 bf16: five
+    // 86 us a call, three 109, two 131.  Fewer where the coefficients would take Q out of fp16's range.
+    p.stage = muon || dtype != AZ_F32 ? 3 : 2;
     const float f = largest_factor(a, b, c);
     while (p.stage > 1 && std::pow(f, (float)p.stage) * SQ > 30000.f) --p.stage;
     p.restart = steps > p.stage;

@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from alphazero_amd import learn
-from test_gpu_learn import DT, F24, _cuda, _exact, _rows
+from test_gpu_learn import DT, F24, _cuda, _exact, _matrix_exact, _rows
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,37 @@ def test_gradient_of_the_weight_holds_32_bits(N, O, sparse, dtype):
     want = p.view(O, 1) * (r.double() * T.double()).view(1, C)
     tol = 100 * F24 * want + (2.0 ** -34 * float((r * T).max()) if dtype == "f16" else 0.0)
     assert ((dw - want).abs() <= tol).all(), (((dw - want).abs() / want).max() / F24, dw.shape)
+
+
+def _values(n, R, K, s, seed):
+    """n matrices R x K with the singular values s"""
+    g = torch.Generator().manual_seed(seed)
+    r = min(R, K)
+    left, right = (torch.linalg.qr(torch.randn(n, m, r, generator=g, dtype=torch.float64))[0] for m in (R, K))
+    return (left * s) @ right.transpose(1, 2)
+
+
+# One direction that is most of the norm, the others far below: what A = X X^T holds of them it holds against the largest.
+# Three steps on one A leave up to 1e-4 of a value's own size, and two up to 1e-5 (test_gpu_learn.py); a step behind them
+# magnifies a relative error by |x f'(x) / f(x)|.  An element is off by that before it is rounded, and then by half a step of
+# the type.
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rest", [1e-3, 1e-4])
+@pytest.mark.parametrize("shape", [(2, 128, 1152), (1, 256, 600), (1, 600, 200), (2, 100, 300), (1, 64, 700)], ids=lambda s: "%dx%dx%d" % s)
+def test_orthogonalize_16_bits_with_one_strong_direction(shape, rest, dtype):
+    r = min(shape[1:])
+    s = torch.full((r,), rest, dtype=torch.float64)
+    s[0] = 1
+    u = (_values(*shape, s, seed=r) * 1e-2).to(DT[dtype])
+    want, got = _matrix_exact(u), learn.orthogonalize(u.cuda()).cpu().double()
+    x = torch.linalg.svdvals(u.double())
+    x, magnified = x / torch.linalg.vector_norm(x, dim=1, keepdim=True), 1.0
+    a, b, c = learn.NEWTON_SCHULZ
+    for step in range(5):
+        f = a + b * x ** 2 + c * x ** 4
+        if step >= 3:
+            magnified = magnified * ((a + 3 * b * x ** 2 + 5 * c * x ** 4) / f).abs().clamp_min(1.0)
+        x = (x * f).abs()
+    tol = torch.linalg.vector_norm(x * (1e-4 * magnified + 1e-5), dim=1)
+    over = ((got - want).abs() - torch.finfo(DT[dtype]).eps / 2 * want.abs() - (2.0 ** -25 if dtype == "f16" else 0.0)).clamp_min(0)
+    assert (torch.linalg.matrix_norm(over) <= tol).all(), torch.linalg.matrix_norm(over) / tol
