@@ -863,12 +863,12 @@ Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b
     p.slices = (int)(count / 4096 < 1 ? 1 : count / 4096 > MAX_SLICES ? MAX_SLICES : count / 4096);
     while (p.slices > 64 && (long long)p.slices * n > 2048) p.slices /= 2;
     p.split = split_of((long long)p.low * n, (p.k + 63) / 64);
-    // Steps between two formations of X.  fp32 results: two (comment at the top); the optimiser step, whose weights take
-    // lr times the result: three.  16-bit results: three, off by at most 8e-5 where half a step of fp16 is 2e-4 and of bf16
+    // Steps between two formations of X.  fp32 results and the optimiser step's weights: two (comment at the top; 40 x 256 x 2304
+    // with three 493 us a step, with two 579).  16-bit results: three, off by at most 8e-5 where half a step of fp16 is 2e-4 and of bf16
     // 1.7e-3 (relative norms over 128 x 1152 .. 600 x 200, one to eight strong directions a thousand to ten thousand times the
     // rest, where fp32 products are off by as much); all five at once leave 1e-3 to 7e-3 there.  18 x 128 x 1152 bf16: five
     // 86 us a call, three 109, two 131.  Fewer where the coefficients would take Q out of fp16's range.
-    p.stage = muon || dtype != AZ_F32 ? 3 : 2;
+    p.stage = dtype == AZ_F32 ? 2 : 3;
     const float f = largest_factor(a, b, c);
     while (p.stage > 1 && std::pow(f, (float)p.stage) * SQ > 30000.f) --p.stage;
     p.restart = steps > p.stage;

@@ -100,3 +100,13 @@ def test_orthogonalize_16_bits_with_one_strong_direction(shape, rest, dtype):
     tol = torch.linalg.vector_norm(x * (1e-4 * magnified + 1e-5), dim=1)
     over = ((got - want).abs() - torch.finfo(DT[dtype]).eps / 2 * want.abs() - (2.0 ** -25 if dtype == "f16" else 0.0)).clamp_min(0)
     assert (torch.linalg.matrix_norm(over) <= tol).all(), torch.linalg.matrix_norm(over) / tol
+
+
+@pytest.mark.parametrize("gdtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(3, 64, 225), (2, 100, 300), (2, 128, 1152), (1, 600, 200), (1, 256, 600)], ids=lambda s: "%dx%dx%d" % s)
+def test_optimiser_step_orthogonalises_as_exactly_as_orthogonalize(shape, gdtype):
+    """Weights 0, no momentum, lr 1: minus what orthogonalize makes of the gradient in fp32, bit for bit."""
+    s = torch.logspace(0, -3, min(shape[1:]), dtype=torch.float64)
+    grad = (_values(*shape, s, seed=3) * 1e-2).to(DT[gdtype]).cuda()
+    w, _ = learn.muon_step(torch.zeros(shape, device="cuda"), torch.zeros(shape, device="cuda"), grad, lr=1.0, beta=0.0)
+    assert torch.equal(-w, learn.orthogonalize(grad.float()))
