@@ -950,7 +950,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
     const int s_lo = (int)((long long)blockIdx.x * a.steps / gridDim.x), steps = (int)((long long)(blockIdx.x + 1) * a.steps / gridDim.x) - s_lo;
     Step st(a, s_lo);
-    for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : -INFINITY;   // (planes there are not: dz = 0)
+    for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
     init_words(a, m.b, tid);
     // fp16: dz is r_b (a mean over the batch: 1 / B) times probabilities that may be 1e-5, below what fp16 resolves.  The
     // workgroup's dz carry a power of two that puts the largest r_b T_b of its boards at 2^9 .. 2^10; it comes off the
@@ -1037,7 +1037,9 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
                     __builtin_amdgcn_wave_barrier();
                 }
             }
-            const float rs = live ? up * bst[2] : 0.f, rp = live ? up * bst[1] : 0.f, mz = bst[0];
+            // a row behind the board's last has the biases as its logits, which may lie far above the board's largest: its maximum
+            // is taken as infinite, its exponentials are 0
+            const float rs = live ? up * bst[2] : 0.f, rp = live ? up * bst[1] : 0.f, mz = live ? bst[0] : INFINITY;
             // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
             const bool bias_counts = a.O > 1 || bst[3] != 0.f;
             constexpr int OH = OT > 2 ? OT / 2 : OT;                 // planes in two halves: fewer registers
@@ -1066,6 +1068,10 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
                         const az_i4 w = *(const az_i4*)(words + (j0 + j) * 16);
                         #pragma unroll
                         for (int i = 0; i < 4; ++i) dz[i] = (unsigned)w[i] & bit ? dz[i] : 0.f;
+                    } else if (j0 + j >= (OT > 2 ? OT - 2 : OT - 1) && (j0 + j) * 16 + 16 > a.O) {
+                        // planes there are not: infinite features times weights of 0 (only the last tiles may have them)
+                        #pragma unroll
+                        for (int i = 0; i < 4; ++i) dz[i] = o + i < a.O ? dz[i] : 0.f;
                     }
                     if (bias_counts) db[j0 + j] += dz;
                     az_s4 hi, lo, rest;

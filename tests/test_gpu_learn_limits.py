@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from alphazero_amd import learn
-from test_gpu_learn import DT, F24, _cuda, _exact, _matrix_exact, _rows
+from test_gpu_learn import DT, F24, _check, _cuda, _exact, _matrix_exact, _rows
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +110,38 @@ def test_optimiser_step_orthogonalises_as_exactly_as_orthogonalize(shape, gdtype
     grad = (_values(*shape, s, seed=3) * 1e-2).to(DT[gdtype]).cuda()
     w, _ = learn.muon_step(torch.zeros(shape, device="cuda"), torch.zeros(shape, device="cuda"), grad, lr=1.0, beta=0.0)
     assert torch.equal(-w, learn.orthogonalize(grad.float()))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("sparse", [False, True], ids=["dense", "sparse"])
+@pytest.mark.parametrize("B,N,O", [(3, 9, 1), (5, 5, 7), (90, 15, 1), (90, 15, 3), (150, 9, 17), (2000, 5, 2), (40, 20, 91)])
+def test_logits_far_below_the_bias(B, N, O, sparse, dtype):
+    """Features of one sign against weights of the other: every logit is 128 below the bias, which is what a row beyond the board's last
+    would have.  All values are exact in the types: p = 1 / (S O)."""
+    C, S = 64, N * N
+    x = torch.ones(B, C, N, N, dtype=DT[dtype])
+    w, b = torch.full((O, C), -2.0, dtype=DT[dtype]), torch.zeros(O, dtype=DT[dtype])
+    if sparse:
+        tgt = (torch.ones(B, dtype=torch.int32), torch.full((B, 2), N + 1, dtype=torch.int32), torch.ones(B, 2))
+    else:
+        tgt = torch.zeros(B, O, N, N)
+        tgt[:, 0, 1, 1] = 1.0
+    p = dict(x=x, w=w, b=b, t=torch.zeros(B, O * S, dtype=torch.float64), ok=None, tgt=tgt, words=None, B=B, N=N, C=C, O=O, dtype=dtype, layout="nhwc")
+    p["t"][:, N + 1] = 1.0
+    xg, wg, bg, tg, _ = _cuda(p)
+    _check(p, learn.policy_loss_grad(xg, wg, bg, tg), torch.ones(B, dtype=torch.float64))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("B,O", [(2, 3), (90, 3), (90, 17), (90, 91)])
+def test_infinite_feature_whose_logits_are_all_minus_infinity(B, O, dtype):
+    """That cell's actions have probability 0 and the gradient of its features is 0, as anywhere (planes are padded inside)."""
+    N, C = 15, 64
+    x = torch.rand(B, C, N, N, generator=torch.Generator().manual_seed(1)).to(DT[dtype])
+    x[1, 5, 3, 3] = math.inf
+    w, b = torch.full((O, C), -0.125, dtype=DT[dtype]), torch.zeros(O, dtype=DT[dtype])
+    tgt = torch.zeros(B, O, N, N)
+    tgt[:, 0, 1, 1] = 1.0
+    loss, dx, _, db = [v.cpu() for v in learn.policy_loss_grad(x.cuda(), w.cuda(), b.cuda(), tgt.cuda())]
+    assert torch.isfinite(loss).all() and torch.isfinite(dx).all() and torch.isfinite(db).all()
+    assert (dx[1, :, 3, 3] == 0).all()
