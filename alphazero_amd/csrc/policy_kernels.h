@@ -153,7 +153,7 @@ template <bool GRAD> struct BoardLoads {
         const int boards = min(a.nb, a.B - b0), lane = tid & 63, wave = tid >> 6;
         if (GRAD && tid < boards) {
             const float rs = a.scale * r;
-            l.stat[tid] = az_f4{st[0], rs * st[1] * st[2], rs, st[3] == INFINITY ? 1.f : 0.f};
+            l.stat[tid] = az_f4{st[0], rs * st[1] * st[2], rs, st[3] < 0.f ? 1.f : 0.f};
         }
         if (a.legal) {
             const int n = boards * a.O * a.N;
@@ -263,26 +263,30 @@ __device__ __forceinline__ void join(float& m, float& l, float om, float ol) {
     l = l * rescale(m, to) + ol * rescale(om, to);
     m = to;
 }
-// A whole wave.  Where a NaN made the targets' sum one, the loss takes the sum of the others, read once more.
-__device__ __forceinline__ void finish_board(const PolicyDev& a, int b, float m, float l, float tz, float tm, int lane) {
-    float tl = tm;
-    if (tm != tm) {
-        tl = 0.f;
+// A whole wave.  Where a NaN made the targets' sum one, the loss takes the sum of the others; where one is negative (fp16), the
+// gradients need the sum of the magnitudes: the targets are read once more.
+template <int DT> __device__ __forceinline__ void finish_board(const PolicyDev& a, int b, float m, float l, float tz, float tm, bool negative, int lane) {
+    float tl = tm, ta = tm;
+    if (tm != tm || negative) {
+        float sum = 0.f, all = 0.f;
         const int n = a.counts ? min(a.counts[b], a.cap) : a.O * a.S;
         for (int i = lane; i < n; i += 64) {
             const float v = a.counts ? a.probs[(size_t)b * a.cap + i] : a.dense[(size_t)b * a.O * a.S + i];
-            if (__builtin_islessgreater(v, 0.f) && (!a.counts || (unsigned)a.actions[(size_t)b * a.cap + i] < (unsigned)(a.O * a.S))) tl += v;
+            if (__builtin_islessgreater(v, 0.f) && (!a.counts || (unsigned)a.actions[(size_t)b * a.cap + i] < (unsigned)(a.O * a.S))) { sum += v; all += fabsf(v); }
         }
-        for (int o = 32; o > 0; o >>= 1) tl += __shfl_xor(tl, o, 64);
+        for (int o = 32; o > 0; o >>= 1) { sum += __shfl_xor(sum, o, 64); all += __shfl_xor(all, o, 64); }
+        if (tm != tm) tl = sum;
+        ta = all;
     }
     if (lane != 0) return;
     const float lse = m == -INFINITY ? (l == l ? -INFINITY : l) : m + logf(l);
     const bool masked = tz == -INFINITY;                             // a target on an action that is not allowed
+    const float mag = DT == 1 ? ta : 1.f;
     const float loss = masked ? INFINITY : (tl != 0.f ? tl * lse : 0.f) - tz;
     // The gradients take probabilities as exp2((z - max) log2 e) / l, which is exactly 1 where one action is allowed: an lse rounded to 32 bits, off by up to 2^-22
     // where it is about 5, would move all of a board's probabilities one way, and where one plane's sum to the targets' sum
     // that is what is left of the products with features of one sign.
-    a.stats[b] = az_f4{m == -INFINITY ? 0.f : m, tm, l == 0.f ? 0.f : 1.f / l, loss};
+    a.stats[b] = az_f4{m == -INFINITY ? 0.f : m, tm, l == 0.f ? 0.f : 1.f / l, masked ? -mag : mag};
     if (a.loss) a.loss[b] = loss;
 }
 
@@ -385,6 +389,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
     constexpr bool WLDS = w_in_lds<DT, OT, CB>();
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ az_f4 red[4 * ROWS];
+    __shared__ int negative[MAX_BOARDS];                             // fp16: has the board a negative target
     constexpr int Cp = L::CP;
     const Smem<DT, OT, CB, 0, WLDS> m(smem, a, a.counts ? WAVES * R::bytes : 0);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4;
@@ -395,6 +400,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
     if (WLDS) stage_w<DT, OT, CB>(a, m.w, tid);
     for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
     init_words(a, m.b, tid);
+    if (tid < MAX_BOARDS) negative[tid] = 0;
     __syncthreads();
     for (int g = g_lo; g < g_hi; ++g) {
         const int b0 = g * a.nb, rows = min(a.nb, a.B - b0) * a.S;
@@ -451,6 +457,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                 // (an entry without a target does not count, whatever its logit; one with a target whose action is not
                 // allowed gives -inf; a NaN is no target for the loss: finish_board)
                 if (!a.counts) {
+                    float least = 0.f;
                     #pragma unroll
                     for (int j = 0; j < R::OTP; ++j)
                         #pragma unroll
@@ -458,7 +465,9 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                             const float v = live && o0 + j * 16 + q * 4 + i < a.O ? tv[j][i] : 0.f;
                             tz += __builtin_islessgreater(v, 0.f) ? v * acc[j][i] : 0.f;
                             tm += v;
+                            least = fminf(least, v);
                         }
+                    if (DT == 1 && least < 0.f) negative[bb] = 1;
                 } else {
                     #pragma unroll
                     for (int j = 0; j < R::OTP; ++j) *(az_f4*)(zt + (lane & 15) * R::LDZ + j * 16 + q * 4) = acc[j];
@@ -469,6 +478,7 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                         if ((unsigned)row < (unsigned)(hi - r0) && (unsigned)o < (unsigned)(R::OTP * 16)) {
                             tz += __builtin_islessgreater(v, 0.f) ? v * zt[row * R::LDZ + o] : 0.f;
                             tm += v;
+                            if (DT == 1 && v < 0.f) negative[bb] = 1;
                         }
                     };
                     if (m.b.listed && a.nb == 1) {                   // every lane takes an entry, whichever row it names
@@ -510,7 +520,9 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                 az_f4 r = red[0];
                 float fm = r[0], fl = r[1], fz = r[2], ft = r[3];
                 for (int w = 1; w < WAVES; ++w) { r = red[w]; join(fm, fl, r[0], r[1]); fz += r[2]; ft += r[3]; }
-                finish_board(a, b0, fm, fl, fz, ft, lane);
+                const bool neg = DT == 1 && negative[0];             // (nobody sets it again before the next board's barriers)
+                if (DT == 1 && lane == 0) negative[0] = 0;
+                finish_board<DT>(a, b0, fm, fl, fz, ft, neg, lane);
             }
         } else
             for (int bb = wave; bb * a.S < rows; bb += WAVES) {
@@ -521,7 +533,9 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
                     fz += __shfl_xor(fz, d, 64);
                     ft += __shfl_xor(ft, d, 64);
                 }
-                finish_board(a, b0 + bb, fm, fl, fz, ft, lane);
+                const bool neg = DT == 1 && negative[bb];
+                if (DT == 1 && lane == 0) negative[bb] = 0;
+                finish_board<DT>(a, b0 + bb, fm, fl, fz, ft, neg, lane);
             }
     }
 }
@@ -669,14 +683,14 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
     if constexpr (WLDS) stage_w<DT, OT, CB>(a, m.w, tid);
     if (a.C < Cp) for (int i = tid; i < ROWS * ldc; i += NT) ((T*)m.h)[i] = (T)0.f;
     // fp16: dz is r_b (a mean over the batch: 1 / B) times probabilities that may be 1e-5, below what fp16 resolves.  The
-    // workgroup's dz carry a power of two that puts the largest r_b T_b of its boards at 2^9 .. 2^10; it comes off the
-    // fp32 sums again.
+    // workgroup's dz carry a power of two that puts the largest of its boards' |r_b| sum |t|, which no dz exceeds, at 2^9 .. 2^10;
+    // it comes off the fp32 sums again.
     float up = 1.f, down = 1.f;
     if constexpr (DT == 1) {
         const Step last(a, s_hi - 1);
         const int b1 = min(last.b0 + a.nb, a.B);
         float mx = 0.f;
-        for (int b = st.b0 + tid; b < b1; b += NT) mx = fmaxf(mx, fabsf(a.scale * (a.row_scale ? a.row_scale[b] : 1.f) * a.stats[b][1]));
+        for (int b = st.b0 + tid; b < b1; b += NT) mx = fmaxf(mx, fabsf(a.scale * (a.row_scale ? a.row_scale[b] : 1.f) * a.stats[b][3]));
         mx = wave_max(mx);
         if (lane == 0) m.t[wave] = mx;
         __syncthreads();
@@ -953,14 +967,14 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
     for (int o = tid; o < OT * 16; o += NT) m.bias[o] = o < a.O ? az_load<DT>(a.bias, o) : 0.f;
     init_words(a, m.b, tid);
     // fp16: dz is r_b (a mean over the batch: 1 / B) times probabilities that may be 1e-5, below what fp16 resolves.  The
-    // workgroup's dz carry a power of two that puts the largest r_b T_b of its boards at 2^9 .. 2^10; it comes off the
-    // fp32 sums again.
+    // workgroup's dz carry a power of two that puts the largest of its boards' |r_b| sum |t|, which no dz exceeds, at 2^9 .. 2^10;
+    // it comes off the fp32 sums again.
     float up = 1.f, down = 1.f;
     if constexpr (DT == 1) {
         const Step last(a, s_lo + steps - 1);
         const int b1 = min(last.b0 + a.nb, a.B);
         float mx = 0.f;
-        for (int b = st.b0 + tid; b < b1; b += NT) mx = fmaxf(mx, fabsf(a.scale * (a.row_scale ? a.row_scale[b] : 1.f) * a.stats[b][1]));
+        for (int b = st.b0 + tid; b < b1; b += NT) mx = fmaxf(mx, fabsf(a.scale * (a.row_scale ? a.row_scale[b] : 1.f) * a.stats[b][3]));
         mx = wave_max(mx);
         if (lane == 0) m.t[wave] = mx;
         __syncthreads();
@@ -1221,7 +1235,7 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
     }
 }
 
-constexpr size_t LOSS_STATIC = (size_t)4 * ROWS * 16;                // az_policy_loss_kernel's `red`
+constexpr size_t LOSS_STATIC = (size_t)4 * ROWS * 16 + MAX_BOARDS * 4;           // az_policy_loss_kernel's `red` and `negative`
 template <int DT, int OT, int CB, int MODE> hipError_t launch_products(PolicyDev a, bool grad, int& groups, hipStream_t stream) {
     // az_policy_grad16_kernel: 16-bit features of up to 128 channels and 96 planes (with more, w's shares do not fit the
     // registers), where a workgroup has more than a step.  20 x 20, 91 planes bf16: 2048 boards 228 us a call, with

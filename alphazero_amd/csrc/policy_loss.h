@@ -35,7 +35,8 @@ struct PolicyDev {
     const unsigned* legal;                   // [B, O * N] or null
     const float* row_scale;                  // [B] or null
     float scale;
-    az_f4* stats;                            // [B] {max z, T, 1 / sum of exp(z - max), loss}
+    az_f4* stats;                            // [B] {max z, T, 1 / sum of exp(z - max), fp16: sum |t|, other types: 1}; the last negative
+                                             // where a target outside the allowed actions makes the loss infinite
     float *loss, *partial;
     const float *wpad, *wpadt;               // fp32 weights that do not fit LDS: padded copies
     void* dh;

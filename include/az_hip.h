@@ -423,7 +423,7 @@ int az_host_env_step(int N, int K, uint8_t* cells, int* to_move, int action, flo
 
 /* Cross entropy of the policy head over all c_out * N * N actions of a board, with its gradients; the logits are never
  * written.  z = weight . features + bias, loss[b] = sum t (lse_b - z) over the entries with a target, lse_b over the
- * allowed actions.  Targets need not sum to 1 (a search policy sums to (n - 1) / n, mcts.hpp:136-146).
+ * allowed actions.  Targets need not sum to 1 (a search policy sums to (n - 1) / n, mcts.hpp:136-146) and may be negative.
  * Gradients are those of sum_b r_b loss_b, r_b = scale * row_scale[b]: d_features in the features' type and layout,
  * d_weight and d_bias in fp32, written, not added to.
  * A board without a target has loss 0 and no gradient; so has one without an allowed action and without a target.  A

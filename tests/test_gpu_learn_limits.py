@@ -145,3 +145,44 @@ def test_infinite_feature_whose_logits_are_all_minus_infinity(B, O, dtype):
     loss, dx, _, db = [v.cpu() for v in learn.policy_loss_grad(x.cuda(), w.cuda(), b.cuda(), tgt.cuda())]
     assert torch.isfinite(loss).all() and torch.isfinite(dx).all() and torch.isfinite(db).all()
     assert (dx[1, :, 3, 3] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("sparse", [False, True], ids=["dense", "sparse"])
+@pytest.mark.parametrize("B,N,O", [(2, 15, 1), (6, 4, 3), (90, 15, 1), (2000, 4, 3), (90, 15, 17)])
+def test_targets_of_both_signs(B, N, O, sparse, dtype):
+    """Targets that nearly cancel: no sum of theirs bounds a gradient's terms, their magnitudes do."""
+    C = 48
+    p = _rows(B, N, C, O, dtype, "nhwc", sparse, seed=B + O, cap=8)
+    g = torch.Generator().manual_seed(1)
+    if sparse:
+        counts, acts, probs = p["tgt"]
+        counts[:] = 8
+        acts[:] = torch.stack([torch.randperm(O * N * N, generator=g)[:8] for _ in range(B)]).int()
+        probs[:, ::2] = 1.0
+        probs[:, 1::2] = -0.999
+        p["t"] = torch.zeros(B, O * N * N, dtype=torch.float64).scatter_(1, acts.long(), probs.double())
+    else:
+        t = torch.randn(B, O * N * N, generator=g)
+        t[:, 0] -= t.sum(1) - 1e-3
+        p["t"], p["tgt"] = t.double(), t.view(B, O, N, N).clone()
+    x, w, b, tgt, _ = _cuda(p)
+    loss, dx, dw, db = [v.cpu().double() for v in learn.policy_loss_grad(x, w, b, tgt, row_scale=1.0 / 32)]
+    r = torch.full((B,), 1.0 / 32, dtype=torch.float64)
+    eloss, edx, edw, edb, m = _exact(p, r)
+    # the sum of the targets in 32 bits: 64 F24 of their magnitudes, which reaches the loss with lse and a dz with its probability
+    S, half = N * N, torch.finfo(DT[dtype]).eps / 2 if dtype != "f32" else F24
+    h, wd = p["x"].double().reshape(B, C, S), p["w"].double()
+    z = (torch.matmul(wd, h) + p["b"].double().view(1, O, 1)).reshape(B, O * S)
+    tol = m["T"] * (2 * m["z"] + 64 * F24 * (torch.logsumexp(z, 1).abs() + z.abs().amax(1)))
+    assert ((loss - eloss).abs() <= tol).all(), ((loss - eloss).abs() / tol).max()
+    e = ((64 * F24 * m["T"].view(B, 1) * torch.softmax(z, 1) + 4 * F24 * p["t"].abs()) / 32).view(B, O, S)
+    if dtype == "f16":
+        e = e + 2.0 ** -34 / 32 * float(m["T"].max())
+    before = m["dxe"] + torch.matmul(wd.abs().t(), e).view(B, C, N, N) + (64 * F24 + half * half) * m["dx"]
+    tol = half * edx.abs() + (1 + half) * before + (2.0 ** -25 if dtype == "f16" else 0.0)
+    assert ((dx - edx).abs() <= tol).all(), ((dx - edx).abs() / tol).max()
+    tol = m["dwe"] + torch.matmul(e, h.transpose(1, 2)).sum(0) + (64 * F24 + half * half) * m["dw"]
+    assert ((dw - edw).abs() <= tol).all(), ((dw - edw).abs() / tol).max()
+    tol = m["dbe"] + e.sum((0, 2)) + 64 * F24 * m["db"]
+    assert (db == 0).all() if O == 1 else ((db - edb).abs() <= tol).all()
