@@ -264,23 +264,33 @@ __device__ __forceinline__ void join(float& m, float& l, float om, float ol) {
     m = to;
 }
 // A whole wave.  Where a NaN made the targets' sum one, the loss takes the sum of the others; where one is negative (fp16), the
-// gradients need the sum of the magnitudes: the targets are read once more.
+// gradients need the sum of the magnitudes: the targets are read once more.  So they are where a target outside the allowed
+// actions may be a negative one: tz is then +inf, or NaN beside a positive one, instead of -inf.
 template <int DT> __device__ __forceinline__ void finish_board(const PolicyDev& a, int b, float m, float l, float tz, float tm, bool negative, int lane) {
     float tl = tm, ta = tm;
-    if (tm != tm || negative) {
+    bool masked = tz == -INFINITY;                                   // a target on an action that is not allowed
+    const bool odd = a.legal && !masked && !(fabsf(tz) < INFINITY);
+    if (tm != tm || negative || odd) {
         float sum = 0.f, all = 0.f;
         const int n = a.counts ? min(a.counts[b], a.cap) : a.O * a.S;
         for (int i = lane; i < n; i += 64) {
             const float v = a.counts ? a.probs[(size_t)b * a.cap + i] : a.dense[(size_t)b * a.O * a.S + i];
-            if (__builtin_islessgreater(v, 0.f) && (!a.counts || (unsigned)a.actions[(size_t)b * a.cap + i] < (unsigned)(a.O * a.S))) { sum += v; all += fabsf(v); }
+            const int act = a.counts ? a.actions[(size_t)b * a.cap + i] : i;
+            if (!__builtin_islessgreater(v, 0.f) || (unsigned)act >= (unsigned)(a.O * a.S)) continue;
+            sum += v;
+            all += fabsf(v);
+            if (odd) {
+                const int line = act / a.N, x = act - line * a.N;    // (plane, row)
+                masked |= !(a.legal[(size_t)b * a.O * a.N + line] >> x & 1);
+            }
         }
+        masked = __ballot(masked) != 0;
         for (int o = 32; o > 0; o >>= 1) { sum += __shfl_xor(sum, o, 64); all += __shfl_xor(all, o, 64); }
         if (tm != tm) tl = sum;
         ta = all;
     }
     if (lane != 0) return;
     const float lse = m == -INFINITY ? (l == l ? -INFINITY : l) : m + logf(l);
-    const bool masked = tz == -INFINITY;                             // a target on an action that is not allowed
     const float mag = DT == 1 ? ta : 1.f;
     const float loss = masked ? INFINITY : (tl != 0.f ? tl * lse : 0.f) - tz;
     // The gradients take probabilities as exp2((z - max) log2 e) / l, which is exactly 1 where one action is allowed: an lse rounded to 32 bits, off by up to 2^-22

@@ -186,3 +186,42 @@ def test_targets_of_both_signs(B, N, O, sparse, dtype):
     assert ((dw - edw).abs() <= tol).all(), ((dw - edw).abs() / tol).max()
     tol = m["dbe"] + e.sum((0, 2)) + 64 * F24 * m["db"]
     assert (db == 0).all() if O == 1 else ((db - edb).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("sparse", [False, True], ids=["dense", "sparse"])
+@pytest.mark.parametrize("N", [3, 9])
+def test_any_target_outside_the_allowed_actions_makes_the_loss_infinite(N, sparse, dtype):
+    """Positive, negative, one of each; board 0 has none, board 4 negative ones on allowed actions only."""
+    B, C, O = 5, 32, 2
+    S = N * N
+    p = _rows(B, N, C, O, dtype, legal=0.5, seed=N)
+    ok = torch.ones(B, O * S, dtype=torch.bool)
+    ok[:, 4] = ok[:, S + 5] = False
+    acts = torch.tensor([0, 4, S + 5]).repeat(B, 1)
+    vals = torch.tensor([[0.5, 0.0, 0.0], [0.5, 0.25, 0.0], [0.5, 0.0, -0.25], [0.5, 0.25, -0.25], [0.5, 0.0, 0.0]])
+    acts[4], vals[4] = torch.tensor([0, 1, S]), torch.tensor([0.5, -0.25, -0.125])
+    t = torch.zeros(B, O * S).scatter_(1, acts, vals)
+    tgt = (torch.full((B,), 3, dtype=torch.int32), acts.int(), vals) if sparse else t.view(B, O, N, N)
+    words = (ok.view(B, O * N, N).long() << torch.arange(N)).sum(2).to(torch.int32).cuda()
+    p["t"], p["ok"] = t.double(), ok
+    tgt = tuple(v.cuda() for v in tgt) if sparse else tgt.cuda()
+    x, w, b, _, _ = _cuda(p)
+    loss, dx, dw, db = [v.cpu() for v in learn.policy_loss_grad(x, w, b, tgt, legal=words)]
+    assert loss[[1, 2, 3]].tolist() == [math.inf] * 3 and torch.isfinite(loss[[0, 4]]).all()
+    assert torch.isfinite(dx).all() and torch.isfinite(dw).all() and torch.isfinite(db).all()
+    assert torch.equal(learn.policy_loss(x, w, b, tgt, legal=words).cpu(), loss)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_one_plane_bias_gradient_with_a_target_outside_the_allowed_actions(sign):
+    """sum dz = r (T - the targets on allowed actions), not zero there."""
+    N, C = 5, 16
+    p = _rows(2, N, C, 1, "f32", seed=1)
+    t = torch.zeros(2, 1, N, N)
+    t[:, 0, 0, 0], t[1, 0, 1, 1] = 0.5, 0.25 * sign
+    words = torch.full((2, N), 31, dtype=torch.int32)
+    words[1, 1] = 31 - 2
+    x, w, b, _, _ = _cuda(p)
+    loss, _, _, db = learn.policy_loss_grad(x, w, b, t.cuda(), legal=words.cuda())
+    assert loss[1] == math.inf and abs(float(db) - 0.25 * sign) <= 64 * F24
