@@ -94,7 +94,7 @@ struct BoardLds {
     float* val;
     int* cnt;                                                        // [64-entry chunk][BLOCKS]
     int* start;                                                      // [BLOCKS + 1]: a block's first entry
-    az_f4* stat;                                                     // [MAX_BOARDS] of the gradients: {max z, r T / sum of exp, r, is the loss infinite}
+    az_f4* stat;                                                     // [MAX_BOARDS] of the gradients: {max z, r T / sum of exp, r, is the loss infinite or the gradient NaN}
     bool listed;                                                     // the entries fit
 };
 // entries outside the board's actions: -1
@@ -153,7 +153,8 @@ template <bool GRAD> struct BoardLoads {
         const int boards = min(a.nb, a.B - b0), lane = tid & 63, wave = tid >> 6;
         if (GRAD && tid < boards) {
             const float rs = a.scale * r;
-            l.stat[tid] = az_f4{st[0], rs * st[1] * st[2], rs, st[3] < 0.f ? 1.f : 0.f};
+            const float rp = rs * st[1] * st[2];
+            l.stat[tid] = az_f4{st[0], rp, rs, st[3] < 0.f || !(fabsf(rp) < INFINITY) ? 1.f : 0.f};
         }
         if (a.legal) {
             const int n = boards * a.O * a.N;
@@ -771,8 +772,9 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
         product<KT, L::KS, OTH, !WLDS>(a.C, fetch, step);
         __builtin_amdgcn_sched_barrier(0);
         const float rp = up * bst[1], mz = bst[0];
-        // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
-        const bool bias_counts = a.O > 1 || bst[3] != 0.f;
+        // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero (or NaN
+        // with all of the board's)
+        const bool bias_counts = OT > 1 || a.O > 1 || bst[3] != 0.f;
         az_s4 rest[THIRD ? OTH : 1];
         #pragma unroll
         for (int j = 0; j < OTH; ++j) {
@@ -1064,8 +1066,9 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
             // a row behind the board's last has the biases as its logits, which may lie far above the board's largest: its maximum
             // is taken as infinite, its exponentials are 0
             const float rs = live ? up * bst[2] : 0.f, rp = live ? up * bst[1] : 0.f, mz = live ? bst[0] : INFINITY;
-            // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero
-            const bool bias_counts = a.O > 1 || bst[3] != 0.f;
+            // one plane and no target outside the allowed actions: the bias moves every logit alike, its gradient is zero (or NaN
+            // with all of the board's)
+            const bool bias_counts = OT > 1 || a.O > 1 || bst[3] != 0.f;
             constexpr int OH = OT > 2 ? OT / 2 : OT;                 // planes in two halves: fewer registers
             #pragma unroll
             for (int j0 = 0; j0 < OT; j0 += OH) {

@@ -225,3 +225,20 @@ def test_one_plane_bias_gradient_with_a_target_outside_the_allowed_actions(sign)
     x, w, b, _, _ = _cuda(p)
     loss, _, _, db = learn.policy_loss_grad(x, w, b, t.cuda(), legal=words.cuda())
     assert loss[1] == math.inf and abs(float(db) - 0.25 * sign) <= 64 * F24
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("what", ["target", "feature"])
+@pytest.mark.parametrize("B,N", [(3, 4), (2, 15), (90, 15)])
+def test_one_plane_bias_gradient_of_a_nan(B, N, what, dtype):
+    """A NaN target, or a NaN logit, makes the board's gradients NaN: d_bias too, which is zero for one plane otherwise."""
+    p = _rows(B, N, 32, 1, dtype, "nhwc", seed=1)
+    if what == "target":
+        p["tgt"].view(B, -1)[1, 5] = float("nan")
+    else:
+        p["x"][1, 3, 2, 2] = float("nan")
+    x, w, b, tgt, _ = _cuda(p)
+    loss, dx, dw, db = [v.cpu() for v in learn.policy_loss_grad(x, w, b, tgt)]
+    keep = torch.arange(B) != 1
+    assert torch.isfinite(loss[keep]).all() and bool(torch.isnan(loss[1])) == (what == "feature")
+    assert torch.isnan(dx[1]).all() and torch.isfinite(dx[keep]).all() and torch.isnan(dw).all() and torch.isnan(db).all()
