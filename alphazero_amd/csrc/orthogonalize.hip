@@ -69,8 +69,9 @@ struct OrthoDev {
     float keep;
 };
 
-// |U|_F of matrix z, and the power of two under which its elements are split into pairs (root mean square near 4).  Every
-// wave by itself, in one order.
+// |U|_F of matrix z, and the power of two under which its elements are split into pairs: root mean square near 4, but the norm,
+// which one element may be most of, at most 2^15 (fp16 ends at 65504; matrices beyond 2^26 elements lose up to 3 of 22 bits to that).
+// Every wave by itself, in one order.
 __device__ __forceinline__ void norm_of(const OrthoDev& d, int z, int& e, float& back) {
     if (!d.sq) { e = d.scale_exp; back = ldexpf(1.f, -e); return; }
     double s = 0.0;
@@ -78,7 +79,7 @@ __device__ __forceinline__ void norm_of(const OrthoDev& d, int z, int& e, float&
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     const double norm = sqrt(s);
     e = 0;
-    if (norm > 0.0 && norm < 1e300) e = min(max(ilogb(sqrt((double)d.r * d.k) / norm) + 2, -120), 120);
+    if (norm > 0.0 && norm < 1e300) e = min(max(min(ilogb(sqrt((double)d.r * d.k) / norm) + 2, 14 - ilogb(norm)), -120), 120);
     back = (float)ldexp(1.0 / (norm + (double)d.eps), -e);
 }
 

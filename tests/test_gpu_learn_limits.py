@@ -242,3 +242,18 @@ def test_one_plane_bias_gradient_of_a_nan(B, N, what, dtype):
     keep = torch.arange(B) != 1
     assert torch.isfinite(loss[keep]).all() and bool(torch.isnan(loss[1])) == (what == "feature")
     assert torch.isnan(dx[1]).all() and torch.isfinite(dx[keep]).all() and torch.isnan(dw).all() and torch.isnan(db).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("shape", [(64, 1 << 22), (1 << 22, 64), (600, 1 << 19)], ids=lambda s: "%dx%d" % s)
+def test_one_element_of_a_large_matrix_is_all_of_its_norm(shape, dtype):
+    """2^28 and more elements: scaled by their root mean square the one would leave fp16.  Its result is the scalar iteration's."""
+    u = torch.zeros(shape, dtype=DT[dtype], device="cuda")
+    u[7, 33] = 1.0
+    got = learn.orthogonalize(u)
+    x = 1.0 / (1.0 + 1e-7)
+    a, b, c = learn.NEWTON_SCHULZ
+    for _ in range(5):
+        x = a * x + b * x ** 3 + c * x ** 5
+    assert abs(float(got[7, 33]) - x) <= 3e-5 + torch.finfo(DT[dtype]).eps * x     # (3e-5: test_gpu_learn.py)
+    assert int(torch.count_nonzero(got)) == 1
