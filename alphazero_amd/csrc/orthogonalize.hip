@@ -827,11 +827,27 @@ struct Plan {
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// largest |a + b y + c y^2| for y = x^2 of singular values up to 1.2
-float largest_factor(float a, float b, float c) {
-    float m = 0.f;
-    for (int i = 0; i <= 150; ++i) { const float y = i * 0.01f; m = std::fmax(m, std::fabs(a + b * y + c * y * y)); }
-    return m;
+// Largest |a + b y + c y^2| that the steps meet from singular values of up to 1 on, y their squares; negative where a value passes
+// MOST_ON_THE_WAY ahead of a step, or a factor MOST_FACTOR.  A step maps 0 .. x onto 0 .. the largest |t (a + b t^2 + c t^4)| for
+// t <= x, which lies at x or where the derivative is 0.  In that range, at the pairs' scales and in fp16 (65504): A <= 49 SA,
+// P <= 200 SA, P A (formed where another step follows) <= 49 SA, an iterate's elements <= 7 * 2^13; Q, a product of P's: make_plan.
+constexpr double MOST_ON_THE_WAY = 7.0, MOST_FACTOR = 200.0;
+double largest_factor(double a, double b, double c, int steps) {
+    const auto factor = [&](double y) { return std::fabs(a + y * (b + y * c)); };
+    double most = 1.0, largest = 0.0;
+    for (int i = 0; i < steps; ++i) {
+        if (most > MOST_ON_THE_WAY) return -1.0;
+        const double end = most * most, disc = 9.0 * b * b - 20.0 * a * c;
+        double at[3] = {end, 0.0, 0.0}, peak = 0.0;                  // derivatives: a + 3 b y + 5 c y^2, and b + 2 c y
+        if (c != 0.0) {
+            peak = -b / (2.0 * c);
+            if (disc >= 0.0) { at[1] = (-3.0 * b + std::sqrt(disc)) / (10.0 * c); at[2] = (-3.0 * b - std::sqrt(disc)) / (10.0 * c); }
+        } else if (b != 0.0) at[1] = -a / (3.0 * b);
+        most = 0.0;
+        for (const double y : at) if (y > 0.0 && y <= end) most = std::fmax(most, std::sqrt(y) * factor(y));
+        largest = std::fmax(largest, std::fmax(std::fabs(a), std::fmax(factor(end), peak > 0.0 && peak <= end ? factor(peak) : 0.0)));
+    }
+    return largest > MOST_FACTOR ? -1.0 : largest;
 }
 
 // Slices of the contraction of X X^T.  In steps of 64 (1.4 us where a workgroup has its CU to itself; two take 1.7 times as
@@ -870,8 +886,8 @@ Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b
     // rest, where fp32 products are off by as much); all five at once leave 1e-3 to 7e-3 there.  18 x 128 x 1152 bf16: five
     // 86 us a call, three 109, two 131.  Fewer where the coefficients would take Q out of fp16's range.
     p.stage = dtype == AZ_F32 ? 2 : 3;
-    const float f = largest_factor(a, b, c);
-    while (p.stage > 1 && std::pow(f, (float)p.stage) * SQ > 30000.f) --p.stage;
+    const double f = largest_factor(a, b, c, steps);
+    while (p.stage > 1 && std::pow(f, p.stage) * SQ > 30000.0) --p.stage;
     p.restart = steps > p.stage;
     p.pair_bytes = up256((size_t)n * 2 * p.rp * p.rp * 2);
     if ((p.small = fits_small(p.r, p.k, steps))) return p;           // (no workspace)
@@ -979,6 +995,7 @@ int check_common(int n, int rows, int cols, int steps, float a, float b, float c
     if ((rows < cols ? rows : cols) > 8192) return ofail(AZ_E_ARG, "the shorter side of %d x %d is beyond 8192", rows, cols);
     if (steps < 0 || steps > 100) return ofail(AZ_E_ARG, "%d steps (0..100)", steps);
     if (!(std::fabs(a) + std::fabs(b) + std::fabs(c) <= 32.f)) return ofail(AZ_E_ARG, "coefficients %g, %g, %g: their magnitudes sum beyond 32", a, b, c);
+    if (largest_factor(a, b, c, steps) < 0.0) return ofail(AZ_E_ARG, "coefficients %g, %g, %g: %d steps take singular values beyond %g or enlarge one more than %g times", a, b, c, steps, MOST_ON_THE_WAY, MOST_FACTOR);
     if (!(eps >= 0.f) || std::isinf(eps)) return ofail(AZ_E_ARG, "eps %g", eps);
     return AZ_OK;
 }

@@ -470,7 +470,8 @@ typedef struct az_orthogonalize_args {
     int   n, rows, cols;           /* n may be 0; the shorter side at most 8192, the longer 2^24 */
     int   dtype;                   /* of update and out */
     int   steps;                   /* 0..100 */
-    float a, b, c, eps, scale;     /* |a| + |b| + |c| <= 32 */
+    float a, b, c, eps, scale;     /* |a| + |b| + |c| <= 32; refused where a singular value of up to 1 would pass 7 ahead of a
+                                      step, or a step enlarge one more than 200 times */
     const void* update;
     int64_t update_stride;
     void* out;

@@ -257,3 +257,28 @@ def test_one_element_of_a_large_matrix_is_all_of_its_norm(shape, dtype):
         x = a * x + b * x ** 3 + c * x ** 5
     assert abs(float(got[7, 33]) - x) <= 3e-5 + torch.finfo(DT[dtype]).eps * x     # (3e-5: test_gpu_learn.py)
     assert int(torch.count_nonzero(got)) == 1
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("coef,steps", [((2.0, 0.0, 0.0), 3), ((-2.0, 0.0, 0.0), 3), ((4.0, 0.0, 0.0), 2), ((32.0, 0.0, 0.0), 1), ((0.0, 6.9, 0.0), 1), ((0.0, 1.5, 0.0), 2), ((20.0, -10.0, -2.0), 1),
+                                        ((6.9, 0.0, 0.0), 1), ((0.0, 0.0, 1.2), 3), ((0.0, 4.0, 0.0), 2)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 64, 225), (2, 100, 300), (1, 256, 256), (1, 300, 200)], ids=lambda s: "%dx%dx%d" % s)
+def test_coefficients_that_enlarge(shape, coef, steps, dtype):
+    """One singular value is the whole norm, in one element or spread over all, and grows to the borders of what is taken.  Its
+    result is the scalar iteration's: each step's 3e-5 of the value (test_gpu_learn.py), which two later steps may magnify by
+    |x f' / f| <= 5 each, and half a step of the type."""
+    x, most = 1.0, 1.0
+    f = [float(torch.tensor(v, dtype=torch.float32)) for v in coef]
+    for _ in range(steps):
+        x = f[0] * x + f[1] * x ** 3 + f[2] * x ** 5
+        most = max(most, abs(x))
+    g = torch.Generator().manual_seed(1)
+    n, R, K = shape
+    left, right = (torch.sign(torch.randn(n, m, generator=g)) for m in (R, K))
+    one = torch.zeros(shape)
+    one[:, R // 2, K // 3] = 1.0
+    half = 0.0 if dtype == "f32" else torch.finfo(DT[dtype]).eps / 2
+    for u, norm in ((left[:, :, None] * right[:, None, :], math.sqrt(R * K)), (one, 1.0)):    # exact in every type
+        got = learn.orthogonalize(u.to(DT[dtype]).cuda(), steps=steps, coefficients=coef).cpu().double()
+        err = torch.linalg.vector_norm((got - u.double() * (x / norm)).flatten(1), dim=1)
+        assert (err <= 25 * 3e-5 * most + half * abs(x)).all(), err

@@ -146,3 +146,21 @@ def test_kernels_hold_no_packed_fp32_and_no_write_behind_a_wide_store(tmp_path):
         assert not any("v_pk_%s_f32" % op in text for op in ("add", "mul", "fma"))
     r = subprocess.run([sys.executable, os.path.join(ROOT, "tools", "probe", "wide_store_overwrite_scan.py"), *files], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stdout[-3000:]
+
+
+@pytest.mark.parametrize("coef,steps,fine", [
+    ((2.0, 0.0, 0.0), 3, True), ((2.0, 0.0, 0.0), 4, False), ((2.0, 0.0, 0.0), 5, False), ((32.0, 0.0, 0.0), 1, True), ((32.0, 0.0, 0.0), 2, False),
+    ((-2.0, 0.0, 0.0), 5, False), ((0.0, 8.0, 0.0), 2, False), ((0.0, 6.9, 0.0), 2, False), ((0.0, 4.0, 0.0), 2, True), ((0.0, 0.0, 2.0), 2, True), ((0.0, 0.0, 2.0), 3, False), ((0.0, 0.0, 3.2), 2, False), ((7.0, 0.0, 0.0), 1, True), ((4.0, 0.0, 0.0), 2, True),
+    ((4.0, 0.0, 0.0), 3, False), ((0.0, 0.0, 1.0), 100, True), ((3.4445, -4.775, 2.0315), 100, True), ((1.875, -1.25, 0.375), 100, True), ((1.5, -0.5, 0.0), 100, True), ((0.0, 0.0, 0.0), 100, True),
+], ids=str)
+def test_coefficients_that_leave_the_arithmetics_range_are_refused(coef, steps, fine):
+    """Singular values of up to 1 may reach 7 ahead of a step, which may enlarge them 200 times: beyond that A = X X^T or its
+    products leave fp16.  Both sides of the rule, and the usual coefficients with any number of steps."""
+    L = capi.load()
+    for make, name in ((_ortho, "orthogonalize"), (_muon, "muon_step")):
+        a = make(a=coef[0], b=coef[1], c=coef[2], steps=steps)
+        size = getattr(L, "az_%s_workspace" % name)(C.byref(a))
+        assert (size > 0) == fine, L.az_last_error()
+        if not fine:
+            rc, msg = _call(name, a)
+            assert rc == capi.AZ_E_ARG and "singular values" in msg, msg
