@@ -203,6 +203,7 @@ def orthogonalize(update, scale=1.0, steps=5, coefficients=NEWTON_SCHULZ, eps=1e
     a.scale = scale
     a.update, a.update_stride, a.out, a.out_stride = update.data_ptr(), stride, out.data_ptr(), _batch(out, "out")[3]
     _run("orthogonalize", a, update.device)
+    torch.autograd.graph.increment_version(out)              # the kernels wrote where autograd cannot see
     return out
 
 
@@ -233,6 +234,6 @@ def muon_step(weight, momentum, grad, lr, beta=0.95, nesterov=True, weight_decay
     a.weight_out, a.weight_out_stride = w_out.data_ptr(), _batch(w_out, "weight_out")[3]
     a.momentum_out, a.momentum_out_stride = m_out.data_ptr(), _batch(m_out, "momentum_out")[3]
     _run("muon_step", a, weight.device)
-    torch.autograd.graph.increment_version(w_out)            # the kernels wrote where autograd cannot see
+    torch.autograd.graph.increment_version(w_out)
     torch.autograd.graph.increment_version(m_out)
     return w_out, m_out

@@ -1,0 +1,28 @@
+"""The learner's operators inside torch: what autograd, forward mode and tracing may rely on, and runs of the operators together
+with the engines that they stand between."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from alphazero_amd import learn
+from alphazero_amd.capi import AzError
+from test_gpu_learn import _cuda, _rows
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_tensor_that_orthogonalize_overwrites_is_a_new_version():
+    """A backward that saved it says so instead of using the new contents."""
+    u = torch.randn(2, 20, 30, device="cuda")
+    out, x = torch.randn(2, 20, 30, device="cuda"), torch.ones(2, 20, 30, device="cuda", requires_grad=True)
+    y = (x * out).sum()
+    before = out._version
+    assert learn.orthogonalize(u, out=out) is out and out._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    w, m = torch.randn(2, 20, 30, device="cuda"), torch.zeros(2, 20, 30, device="cuda")
+    before = w._version, m._version
+    learn.muon_step(w, m, u, lr=0.1)
+    assert w._version > before[0] and m._version > before[1]
+    with torch.inference_mode():
+        assert torch.equal(learn.orthogonalize(u, out=torch.empty_like(u)), learn.orthogonalize(u))
