@@ -12,6 +12,7 @@ is captured into a HIP graph uses policy_loss_grad, which involves no autograd g
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from . import capi
 from .capi import AzError
@@ -35,13 +36,19 @@ def _run(name, args, device):
     capi._chk(getattr(L, "az_%s_dev" % name)(ref, ws.data_ptr(), size, torch.cuda.current_stream(device).cuda_stream))
 
 
+def _dual(t):
+    return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def _on(t, device, what):
     _need(isinstance(t, torch.Tensor) and t.device == device, "%s is not a tensor on %s", what, device)
+    _need(not _dual(t), "%s carries a tangent: there is no forward-mode derivative", what)
 
 
 def _loss_args(features, weight, bias, targets, legal):
     _need(isinstance(features, torch.Tensor) and features.is_cuda and features.dim() == 4, "features: a [B, C, N, N] tensor on the GPU")
     dev = features.device
+    _on(features, dev, "features")
     B, ch, N, N2 = features.shape
     _need(N == N2, "features: board %d x %d is not square", N, N2)
     _need(features.dtype in _DTYPES, "features: %s (float32, float16 or bfloat16)", features.dtype)
@@ -152,6 +159,8 @@ def policy_loss(features, weight, bias, targets, legal=None):
     tgt = (targets,) if isinstance(targets, torch.Tensor) else tuple(targets)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (features, weight, bias)):
         _need(not torch.cuda.is_current_stream_capturing(), "policy_loss with gradients cannot be captured into a graph: policy_loss_grad can")
+        for t in (features, weight, bias) + tgt:
+            _need(not (isinstance(t, torch.Tensor) and _dual(t)), "an argument carries a tangent: there is no forward-mode derivative")
         return _PolicyLoss.apply(features, weight, bias, legal, *tgt)
     return _loss(features, weight, bias, targets, legal)[0]
 
@@ -192,6 +201,7 @@ def orthogonalize(update, scale=1.0, steps=5, coefficients=NEWTON_SCHULZ, eps=1e
     batch may be strided (the convolutions of all blocks in the weight blob), each matrix contiguous.  out: like update,
     apart from it."""
     n, R, K, stride = _batch(update, "update")
+    _on(update, update.device, "update")
     _need(update.dtype in _DTYPES, "update: %s (float32, float16 or bfloat16)", update.dtype)
     if out is None:
         out = torch.empty(update.shape, dtype=update.dtype, device=update.device)
@@ -219,7 +229,7 @@ def muon_step(weight, momentum, grad, lr, beta=0.95, nesterov=True, weight_decay
     a = capi.AzMuonStepArgs()
     w_out = weight if weight_out is None else weight_out
     m_out = momentum if momentum_out is None else momentum_out
-    for t, what in ((momentum, "momentum"), (grad, "grad"), (w_out, "weight_out"), (m_out, "momentum_out")):
+    for t, what in ((weight, "weight"), (momentum, "momentum"), (grad, "grad"), (w_out, "weight_out"), (m_out, "momentum_out")):
         _on(t, weight.device, what)
         _need(t.shape == weight.shape, "%s: shape %s is not the weight's %s", what, t.shape, weight.shape)
     for t, what in ((weight, "weight"), (momentum, "momentum"), (w_out, "weight_out"), (m_out, "momentum_out")):

@@ -26,3 +26,27 @@ def test_a_tensor_that_orthogonalize_overwrites_is_a_new_version():
     assert w._version > before[0] and m._version > before[1]
     with torch.inference_mode():
         assert torch.equal(learn.orthogonalize(u, out=torch.empty_like(u)), learn.orthogonalize(u))
+
+
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_forward_mode_tangents_are_refused(needs_grad):
+    """There is none of these operators' derivatives in it; without the check the result had no tangent, without a word."""
+    p = _rows(2, 5, 16, 2, "f32", seed=1)
+    x, w, b, tgt, _ = _cuda(p)
+    m = torch.randn(1, 16, 20, device="cuda")
+    with forward_ad.dual_level():
+        assert learn.policy_loss(x, w, b, tgt).shape == (2,)                                   # (no tangent among them: fine)
+        for at in range(4):
+            args = [x, w, b, tgt]
+            args[at] = forward_ad.make_dual(args[at].clone().requires_grad_(needs_grad and at < 3), torch.ones_like(args[at]))
+            for call in (learn.policy_loss, learn.policy_loss_grad):
+                with pytest.raises(AzError, match="tangent"):
+                    call(*args)
+        d = forward_ad.make_dual(m.clone(), torch.ones_like(m))
+        with pytest.raises(AzError, match="tangent"):
+            learn.orthogonalize(d)
+        for at in range(3):
+            args = [m.clone(), m.clone(), m.clone()]
+            args[at] = d
+            with pytest.raises(AzError, match="tangent"):
+                learn.muon_step(*args, lr=0.1)
