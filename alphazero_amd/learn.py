@@ -26,6 +26,10 @@ def _need(ok, msg, *a):
         raise AzError(msg % a)
 
 
+def _untraced():
+    _need(not torch.jit.is_tracing(), "torch.jit.trace records torch's own operators, not this call's kernels")
+
+
 def _run(name, args, device):
     L = capi.load()
     ref = C.byref(args)
@@ -46,6 +50,7 @@ def _on(t, device, what):
 
 
 def _loss_args(features, weight, bias, targets, legal):
+    _untraced()
     _need(isinstance(features, torch.Tensor) and features.is_cuda and features.dim() == 4, "features: a [B, C, N, N] tensor on the GPU")
     dev = features.device
     _on(features, dev, "features")
@@ -200,6 +205,7 @@ def orthogonalize(update, scale=1.0, steps=5, coefficients=NEWTON_SCHULZ, eps=1e
     update: [R, K], [n, R, K], a convolution's weight [O, I, kh, kw] or [n, O, I, kh, kw]; float32 / float16 / bfloat16; the
     batch may be strided (the convolutions of all blocks in the weight blob), each matrix contiguous.  out: like update,
     apart from it."""
+    _untraced()
     n, R, K, stride = _batch(update, "update")
     _on(update, update.device, "update")
     _need(update.dtype in _DTYPES, "update: %s (float32, float16 or bfloat16)", update.dtype)
@@ -225,6 +231,7 @@ def muon_step(weight, momentum, grad, lr, beta=0.95, nesterov=True, weight_decay
         weight' = (1 - lr weight_decay) weight - lr orthogonalize(u, scale)
     weight and momentum: float32, shapes as in orthogonalize (views into the weight blob may be strided batches); grad of any
     of the three types.  Without weight_out / momentum_out the step is in place.  Returns (weight', momentum')."""
+    _untraced()
     n, R, K, ws = _batch(weight, "weight")
     a = capi.AzMuonStepArgs()
     w_out = weight if weight_out is None else weight_out

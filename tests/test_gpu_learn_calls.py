@@ -50,3 +50,14 @@ def test_forward_mode_tangents_are_refused(needs_grad):
             args[at] = d
             with pytest.raises(AzError, match="tangent"):
                 learn.muon_step(*args, lr=0.1)
+
+
+def test_tracing_is_refused():
+    """A trace would hold the empty results alone."""
+    p = _rows(2, 5, 16, 2, "f32", seed=1)
+    x, w, b, tgt, _ = _cuda(p)
+    m = torch.randn(1, 16, 20, device="cuda")
+    for call, args in ((lambda x: learn.policy_loss(x, w, b, tgt), x), (lambda x: learn.policy_loss_grad(x, w, b, tgt), x), (learn.orthogonalize, m),
+                       (lambda g: learn.muon_step(m.clone(), m.clone(), g, lr=0.1), m)):
+        with pytest.raises(AzError, match="trace"):
+            torch.jit.trace(call, (args,))
