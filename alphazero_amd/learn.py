@@ -159,9 +159,10 @@ def policy_loss(features, weight, bias, targets, legal=None):
               [B, cap]) as the Blokus rows are drained; they need not sum to 1
     legal     None, or int32 words [B, c_out * N]: bit x of word co * N + y allows action (co, y, x); the softmax runs
               over the allowed actions.  A target outside them makes that board's loss inf; a board without targets has
-              loss 0
+              loss 0.  They get no gradient
     """
     tgt = (targets,) if isinstance(targets, torch.Tensor) else tuple(targets)
+    _need(not (torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tgt)), "targets get no gradient: detach() them")
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (features, weight, bias)):
         _need(not torch.cuda.is_current_stream_capturing(), "policy_loss with gradients cannot be captured into a graph: policy_loss_grad can")
         for t in (features, weight, bias) + tgt:

@@ -61,3 +61,17 @@ def test_tracing_is_refused():
                        (lambda g: learn.muon_step(m.clone(), m.clone(), g, lr=0.1), m)):
         with pytest.raises(AzError, match="trace"):
             torch.jit.trace(call, (args,))
+
+
+@pytest.mark.parametrize("sparse", [False, True], ids=["dense", "sparse"])
+def test_targets_that_require_a_gradient_are_refused(sparse):
+    p = _rows(2, 5, 16, 2, "f32", sparse=sparse, seed=1)
+    x, w, b, tgt, _ = _cuda(p)
+    want = learn.policy_loss(x, w, b, tgt)
+    asks = tgt[:2] + (tgt[2].clone().requires_grad_(),) if sparse else tgt.clone().requires_grad_()
+    for xs in (x, x.clone().requires_grad_()):
+        with pytest.raises(AzError, match="detach"):
+            learn.policy_loss(xs, w, b, asks)
+    with torch.no_grad():
+        assert torch.equal(learn.policy_loss(x, w, b, asks), want)
+    assert torch.equal(learn.policy_loss_grad(x, w, b, asks)[0], want)                         # (its gradients are named)
