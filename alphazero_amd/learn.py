@@ -91,7 +91,7 @@ def _loss_args(features, weight, bias, targets, legal):
         a.counts, a.actions, a.probs, a.cap = counts.data_ptr(), actions.data_ptr(), probs.data_ptr(), actions.shape[1]
     if legal is not None:
         _on(legal, dev, "legal")
-        _need(legal.dtype in (torch.int32, torch.uint32) and legal.is_contiguous() and legal.numel() == B * O * N and legal.shape[0] == B,
+        _need(legal.dtype in (torch.int32, torch.uint32) and legal.is_contiguous() and legal.numel() == B * O * N and legal.dim() > 0 and legal.shape[0] == B,
               "legal: contiguous 32-bit words [%d, %d]", B, O * N)
         a.legal = legal.data_ptr()
     a.scale = 1.0
@@ -161,6 +161,7 @@ def policy_loss(features, weight, bias, targets, legal=None):
               over the allowed actions.  A target outside them makes that board's loss inf; a board without targets has
               loss 0.  They get no gradient
     """
+    _need(isinstance(targets, (torch.Tensor, tuple, list)), "targets: a dense tensor or (counts, actions, probs)")
     tgt = (targets,) if isinstance(targets, torch.Tensor) else tuple(targets)
     _need(not (torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tgt)), "targets get no gradient: detach() them")
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (features, weight, bias)):

@@ -75,3 +75,15 @@ def test_targets_that_require_a_gradient_are_refused(sparse):
     with torch.no_grad():
         assert torch.equal(learn.policy_loss(x, w, b, asks), want)
     assert torch.equal(learn.policy_loss_grad(x, w, b, asks)[0], want)                         # (its gradients are named)
+
+
+def test_words_and_targets_without_a_dimension_are_refused():
+    x, w, b = torch.zeros(1, 4, 1, 1, device="cuda"), torch.zeros(1, 4, device="cuda"), torch.zeros(1, device="cuda")
+    t = torch.ones(1, 1, device="cuda")
+    assert learn.policy_loss(x, w, b, t, legal=torch.ones(1, 1, dtype=torch.int32, device="cuda")).tolist() == [0.0]
+    for kw in (dict(legal=torch.tensor(1, dtype=torch.int32, device="cuda")), dict(legal=t.int()[:0])):
+        with pytest.raises(AzError, match="words"):
+            learn.policy_loss(x, w, b, t, **kw)
+    for bad in (t[0, :0], None, 1.0, (t.int()[0],)):
+        with pytest.raises(AzError, match="targets"):
+            learn.policy_loss(x, w, b, bad)

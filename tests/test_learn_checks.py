@@ -164,3 +164,11 @@ def test_coefficients_that_leave_the_arithmetics_range_are_refused(coef, steps, 
         if not fine:
             rc, msg = _call(name, a)
             assert rc == capi.AZ_E_ARG and "singular values" in msg, msg
+
+
+@pytest.mark.parametrize("targets", [None, 3.0, "abc", {}])
+def test_targets_of_another_kind_are_refused(targets):
+    x, w, b = torch.zeros(2, 8, 3, 3), torch.zeros(1, 8), torch.zeros(1)
+    for call in (learn.policy_loss, learn.policy_loss_grad):
+        with pytest.raises(capi.AzError):
+            call(x, w, b, targets)
