@@ -103,6 +103,7 @@ extern "C" int az_policy_loss_dev(const az_policy_loss_args* p, void* workspace,
         if (!p->target && !p->counts) return lfail(AZ_E_ARG, "null argument: target or counts / actions / probs");
         if (p->target && p->counts) return lfail(AZ_E_ARG, "targets are dense (target) or sparse (counts), not both");
         if (p->counts && (p->cap < 0 || (p->cap > 0 && (!p->actions || !p->probs)))) return lfail(AZ_E_ARG, "null argument: actions / probs (cap %d)", p->cap);
+        if (p->counts && p->cap > 1 << 26) return lfail(AZ_E_ARG, "%d targets a board are too many (2^26)", p->cap);   // (times 16 boards: an int)
         const size_t esz = p->dtype == AZ_F32 ? 4 : 2;
         if (((size_t)p->features | (size_t)p->weight | (size_t)p->bias | (size_t)p->d_features) % esz) return lfail(AZ_E_ARG, "a tensor is not aligned to its element type");
         if (((size_t)p->target | (size_t)p->counts | (size_t)p->actions | (size_t)p->probs | (size_t)p->legal | (size_t)p->row_scale | (size_t)p->loss |

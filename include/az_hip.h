@@ -437,7 +437,7 @@ typedef struct az_policy_loss_args {
     const void* weight;            /* [c_out, C] */
     const void* bias;              /* [c_out] */
     /* targets: dense, f32 [B, c_out * N * N] as az_replay_drain's policy, or sparse as az_blokus_replay_drain's rows:
-     * the first counts[b] (at most cap) of actions i32 / probs f32 [B, cap]; an action named more than once counts with
+     * the first counts[b] (at most cap, itself at most 2^26) of actions i32 / probs f32 [B, cap]; an action named more than once counts with
      * the sum, one outside 0 .. c_out * N * N - 1 is left out */
     const float* target;
     const int32_t* counts;

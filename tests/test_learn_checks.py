@@ -172,3 +172,10 @@ def test_targets_of_another_kind_are_refused(targets):
     for call in (learn.policy_loss, learn.policy_loss_grad):
         with pytest.raises(capi.AzError):
             call(x, w, b, targets)
+
+
+def test_target_lists_beyond_what_an_int_counts_are_refused():
+    """Sixteen small boards' entries are counted together."""
+    for cap, word in (((1 << 26) + 1, "too many"), (1 << 27, "too many"), ((1 << 31) - 1, "too many"), (1 << 26, "workspace")):
+        rc, msg = _call("policy_loss", _policy(N=1, target=None, counts=P, actions=P, probs=P, cap=cap), None)
+        assert rc == capi.AZ_E_ARG and word in msg, msg
