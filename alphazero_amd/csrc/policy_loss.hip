@@ -110,10 +110,22 @@ extern "C" int az_policy_loss_dev(const az_policy_loss_args* p, void* workspace,
              (size_t)p->d_weight | (size_t)p->d_bias) % 4) return lfail(AZ_E_ARG, "a tensor is not aligned to its element type");
     }
     if ((size_t)p->stats % 16) return lfail(AZ_E_ARG, "stats needs 16-byte alignment");
-    if (p->B > 0 && p->d_features) {                                 // (features are read while gradients of other boards are written)
-        const size_t n = (size_t)p->B * p->N * p->N * p->C * (p->dtype == AZ_F32 ? 4 : 2);
-        const char *f = (const char*)p->features, *d = (const char*)p->d_features;
-        if (f < d + n && d < f + n) return lfail(AZ_E_ARG, "d_features overlaps features");
+    if (p->B > 0 && grad) {
+        // Features, targets and statistics are read while gradients of other boards are written; d_weight and d_bias come last.
+        const size_t esz = p->dtype == AZ_F32 ? 4 : 2, B = p->B, cells = (size_t)p->N * p->N, list = B * (p->counts ? p->cap : 0) * 4;
+        const struct { const char* name; const void* at; size_t bytes; } in[] = {
+            {"features", p->features, B * cells * p->C * esz}, {"weight", p->weight, (size_t)p->c_out * p->C * esz}, {"bias", p->bias, p->c_out * esz},
+            {"target", p->target, B * p->c_out * cells * 4}, {"counts", p->counts, B * 4}, {"actions", p->actions, list}, {"probs", p->probs, list},
+            {"legal", p->legal, B * p->c_out * p->N * 4}, {"row_scale", p->row_scale, B * 4}, {"stats", p->stats_given ? p->stats : nullptr, B * 16},
+        }, out[] = {
+            {"d_features", p->d_features, B * cells * p->C * esz}, {"loss", p->loss, B * 4}, {"stats", p->stats_given ? nullptr : p->stats, B * 16},
+            {"d_weight", p->d_weight, (size_t)p->c_out * p->C * 4}, {"d_bias", p->d_bias, (size_t)p->c_out * 4},
+        };
+        const auto meet = [](const auto& a, const auto& b) { return a.at && b.at && (const char*)a.at < (const char*)b.at + b.bytes && (const char*)b.at < (const char*)a.at + a.bytes; };
+        for (int i = 0; i < 5; ++i) {
+            if (i < 3) for (const auto& x : in) if (meet(out[i], x)) return lfail(AZ_E_ARG, "%s overlaps %s", out[i].name, x.name);
+            for (int k = 0; k < i; ++k) if (meet(out[i], out[k])) return lfail(AZ_E_ARG, "%s overlaps %s", out[i].name, out[k].name);
+        }
     }
     const size_t need = az_policy_loss_workspace(p);
     if (!workspace) return lfail(AZ_E_ARG, "null argument: workspace");

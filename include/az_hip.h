@@ -428,7 +428,8 @@ int az_host_env_step(int N, int K, uint8_t* cells, int* to_move, int action, flo
  * d_weight and d_bias in fp32, written, not added to.
  * A board without a target has loss 0 and no gradient; so has one without an allowed action and without a target.  A
  * target on an action that is not allowed makes its board's loss +inf (and that entry's gradient 0).  A NaN among the
- * targets is no target for the loss and makes the board's gradients NaN. */
+ * targets is no target for the loss and makes the board's gradients NaN.
+ * No output may overlap another output, and none but d_weight and d_bias an input. */
 typedef struct az_policy_loss_args {
     int   device;
     int   B, N, C, c_out;          /* boards, 1 <= N <= 32, 1 <= C <= 256, 1 <= c_out <= 128; B may be 0 */

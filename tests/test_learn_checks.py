@@ -179,3 +179,21 @@ def test_target_lists_beyond_what_an_int_counts_are_refused():
     for cap, word in (((1 << 26) + 1, "too many"), (1 << 27, "too many"), ((1 << 31) - 1, "too many"), (1 << 26, "workspace")):
         rc, msg = _call("policy_loss", _policy(N=1, target=None, counts=P, actions=P, probs=P, cap=cap), None)
         assert rc == capi.AZ_E_ARG and word in msg, msg
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(d_features=1 * P), "d_features overlaps features"), (dict(d_features=1 * P + 4 * 81 * 64 * 2 - 2), "d_features overlaps features"), (dict(d_features=2 * P), "d_features overlaps weight"),
+    (dict(d_features=3 * P), "d_features overlaps bias"), (dict(d_features=4 * P + 4 * 3 * 81 * 4 - 2), "d_features overlaps target"), (dict(d_features=6 * P), "d_features overlaps row_scale"),
+    (dict(d_features=7 * P), "d_features overlaps legal"), (dict(loss=1 * P), "loss overlaps features"), (dict(loss=4 * P), "loss overlaps target"), (dict(loss=6 * P), "loss overlaps row_scale"),
+    (dict(loss=8 * P), "loss overlaps d_features"), (dict(stats=9 * P), "d_weight overlaps stats"), (dict(stats=4 * P), "stats overlaps target"), (dict(d_weight=8 * P), "d_weight overlaps d_features"),
+    (dict(d_bias=9 * P + 4 * 3 * 64 - 4), "d_bias overlaps d_weight"), (dict(d_bias=5 * P), "d_bias overlaps loss"), (dict(stats_given=1, stats=8 * P, loss=None), "d_features overlaps stats"),
+    (dict(target=None, counts=8 * P, actions=11 * P, probs=12 * P, cap=5), "d_features overlaps counts"), (dict(target=None, counts=11 * P, actions=8 * P, probs=12 * P, cap=5), "d_features overlaps actions"),
+    (dict(target=None, counts=11 * P, actions=12 * P, probs=8 * P - 4 * 5 * 4 + 4, cap=5), "d_features overlaps probs"),
+    (dict(d_weight=2 * P, d_bias=3 * P), "workspace"), (dict(d_features=1 * P + 4 * 81 * 64 * 2), "workspace"), (dict(), "workspace"),
+], ids=lambda v: "-".join(v) if isinstance(v, dict) else v.replace(" ", "_"))
+def test_policy_loss_gradients_refuse_outputs_that_overlap(kw, word):
+    """The tensors lie P apart; "workspace": everything before was in order (the head in place of its own gradient is)."""
+    v = dict(dtype=capi.AZ_F16, features=1 * P, weight=2 * P, bias=3 * P, target=4 * P, loss=5 * P, row_scale=6 * P, legal=7 * P, d_features=8 * P, d_weight=9 * P, d_bias=10 * P)
+    v.update(kw)
+    rc, msg = _call("policy_loss", _policy(**v), None)
+    assert rc == capi.AZ_E_ARG and word in msg, msg
