@@ -1,12 +1,13 @@
 """The learner's operators inside torch: what autograd, forward mode and tracing may rely on, and runs of the operators together
 with the engines that they stand between."""
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from alphazero_amd import learn
+from alphazero_amd import capi, learn, synth
 from alphazero_amd.capi import AzError
-from test_gpu_learn import _cuda, _rows
+from test_gpu_learn import DT, _check, _cuda, _rows
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +88,85 @@ def test_words_and_targets_without_a_dimension_are_refused():
     for bad in (t[0, :0], None, 1.0, (t.int()[0],)):
         with pytest.raises(AzError, match="targets"):
             learn.policy_loss(x, w, b, bad)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("sparse", [False, True], ids=["dense", "sparse"])
+@pytest.mark.parametrize("B", [4, 90])
+def test_autograd_gives_the_same_gradients_in_16_bits(B, sparse, dtype):
+    """Those of policy_loss_grad, with the weight's and the bias's rounded to their type."""
+    p = _rows(B, 15, 40, 3, dtype, "nhwc", sparse=sparse, legal=0.7, seed=8)
+    x, w, b, tgt, words = _cuda(p)
+    xr, wr, br = x.clone().requires_grad_(), w.view(3, 40, 1, 1).clone().requires_grad_(), b.clone().requires_grad_()
+    g = torch.linspace(-1.0, 2.0, B, device="cuda")
+    loss = learn.policy_loss(xr, wr, br, tgt, legal=words)
+    (loss * g).sum().backward()
+    want, dx, dw, db = learn.policy_loss_grad(x, w, b, tgt, row_scale=g, legal=words)
+    assert torch.equal(loss, want) and torch.equal(xr.grad, dx) and xr.grad.stride() == x.stride()
+    assert torch.equal(wr.grad, dw.view(3, 40, 1, 1).to(DT[dtype])) and torch.equal(br.grad, db.to(DT[dtype]))
+
+
+def test_rows_of_selfplay_through_a_training_step_and_back():
+    """m,n,k rows as az_replay_drain leaves them -> features of a torch convolution, the blob's policy head on them, loss and
+    gradients, the optimiser step inside the blob -> az_load_weights_dev, whose games go on."""
+    N, K, budget, G, Ch = 5, 4, 32, 8, 32
+    eng = capi.Engine(N, K, G, eval_mode=capi.AZ_EVAL_HASH, max_budget=budget, seed=7)
+    eng.selfplay_begin(budget)
+    eng.selfplay_run((2 * budget + 1 + 24 * budget) + 8)
+    cells, tm, pol, _ = eng.replay_drain()
+    eng.close()
+    B = len(tm)
+    assert B >= 40 and (pol.sum(1) > 0).all()
+    blob = torch.from_numpy(synth.make_blob(N, 3, [Ch, Ch], 5)).cuda()
+    off, at = {}, 0
+    for name, shape in synth.blob_layout(N, 3, [Ch, Ch]):
+        off[name] = at, shape
+        at += int(np.prod(shape))
+    part = lambda t, name: t[off[name][0]:off[name][0] + int(np.prod(off[name][1]))].view(off[name][1])       # noqa: E731
+    planes = torch.from_numpy(np.stack([cells == 1, cells == 2, np.repeat(tm[:, None], N * N, 1) == 0], 1).astype(np.float32)).view(B, 3, N, N).cuda()
+    stem = part(blob, "CBlock.conv.weight").clone().requires_grad_()
+    x = torch.relu(torch.nn.functional.conv2d(planes, stem, padding=1))
+    w, b, tgt = part(blob, "PHead.conv.weight"), part(blob, "PHead.conv.bias"), torch.from_numpy(pol).cuda()
+    learn.policy_loss(x, w, b, tgt).mean().backward()
+    loss, dx, dw, db = learn.policy_loss_grad(x.detach(), w, b, tgt, row_scale=1.0 / B)
+    p = dict(x=x.detach().cpu(), w=w.view(1, Ch).cpu(), b=b.cpu(), t=torch.from_numpy(pol).double(), ok=None, B=B, N=N, C=Ch, O=1, dtype="f32")
+    _check(p, (loss, dx, dw, db), torch.full((B,), 1.0 / B, dtype=torch.float32).double())
+    momentum, before = torch.zeros_like(blob), blob.clone()
+    learn.muon_step(part(blob, "CBlock.conv.weight"), part(momentum, "CBlock.conv.weight"), stem.grad, lr=0.02)
+    learn.muon_step(w, part(momentum, "PHead.conv.weight"), dw.view(1, Ch, 1, 1), lr=0.02)
+    b -= 0.02 * db
+    changed = (blob != before).cpu()
+    for name, (o, shape) in off.items():
+        assert changed[o:o + int(np.prod(shape))].any() == (name in ("CBlock.conv.weight", "PHead.conv.weight")), name
+    after = learn.policy_loss(torch.relu(torch.nn.functional.conv2d(planes, part(blob, "CBlock.conv.weight"), padding=1)), w, b, tgt)
+    assert torch.isfinite(after).all()
+    play = capi.Engine(N, K, G, Cs=[Ch, Ch], max_budget=budget, seed=8)
+    play.load_weights_dev(blob.data_ptr(), blob.numel())
+    play.selfplay_begin(budget)
+    play.selfplay_run(4 * budget)
+    play.sync()
+    assert play.stats()["moves"] > 0 and play.stats()["error_games"] == 0
+    play.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("reuse", [False, True], ids=["fresh", "reuse"])
+def test_blokus_rows_as_they_are_drained(reuse, dtype):
+    """Sparse search policies of whole games; with the tree reused a row has room for 4 * budget entries, more than LDS keeps
+    (1 040 here), and most of it is empty."""
+    G, budget, O, N, C, B = 2, 260, 91, 20, 32, 48
+    dev = capi.Blokus(G, seed=3)
+    dev.search_config(max_budget=budget, reuse=reuse)
+    dev.selfplay_config(ring_rows=G * 84, max_budget=budget)
+    dev.selfplay_moves(budget, 86)
+    got = dev.replay_drain(G * 84)
+    dev.close()
+    assert len(got["counts"]) >= B and (got["actions"].shape[1] > 1024) == reuse
+    n, acts, probs = (np.ascontiguousarray(got[k][:B]) for k in ("counts", "actions", "probs"))
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(B, C, N, N, generator=g).relu().to(DT[dtype])
+    w, b = (torch.randn(O, C, generator=g) / 4).to(DT[dtype]), (torch.randn(O, generator=g) * 0.1).to(DT[dtype])
+    t = torch.from_numpy(capi.Blokus.dense_policy(acts, probs, n)).view(B, -1).double()
+    p = dict(x=x, w=w, b=b, t=t, ok=None, tgt=tuple(torch.from_numpy(v) for v in (n, acts, probs)), words=None, B=B, N=N, C=C, O=O, dtype=dtype, layout="nhwc")
+    xg, wg, bg, tg, _ = _cuda(p)
+    _check(p, learn.policy_loss_grad(xg, wg, bg, tg, row_scale=1.0 / B), torch.full((B,), 1.0 / B, dtype=torch.float32).double())
