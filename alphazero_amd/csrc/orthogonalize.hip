@@ -999,6 +999,12 @@ int check_common(int n, int rows, int cols, int steps, float a, float b, float c
     if (!(eps >= 0.f) || std::isinf(eps)) return ofail(AZ_E_ARG, "eps %g", eps);
     return AZ_OK;
 }
+// a launch takes fewer than 2^32 threads
+int check_tiles(const Plan& p) {
+    const long long tiles = (long long)(p.kp / p.apply_tile) * (p.rp / p.apply_tile);
+    if (!p.small && (tiles > p.low ? tiles : p.low) * p.n >= 1 << 24) return ofail(AZ_E_ARG, "%d matrices of %d x %d are too many tiles for one call", p.n, p.rows, p.cols);
+    return AZ_OK;
+}
 int check_ortho(const az_orthogonalize_args* p) {
     if (!p) return ofail(AZ_E_ARG, "null argument: args");
     const int rc = check_common(p->n, p->rows, p->cols, p->steps, p->a, p->b, p->c, p->eps);
@@ -1048,11 +1054,13 @@ int run(const Plan& p, OrthoDev d, int dtype, int steps, unsigned char* ws, hipS
 
 extern "C" size_t az_orthogonalize_workspace(const az_orthogonalize_args* p) {
     if (check_ortho(p) != AZ_OK) return 0;
-    return make_plan(p->n, p->rows, p->cols, p->dtype, p->steps, p->a, p->b, p->c, false).bytes + 256;
+    const Plan plan = make_plan(p->n, p->rows, p->cols, p->dtype, p->steps, p->a, p->b, p->c, false);
+    return check_tiles(plan) == AZ_OK ? plan.bytes + 256 : 0;
 }
 extern "C" size_t az_muon_step_workspace(const az_muon_step_args* p) {
     if (check_muon(p) != AZ_OK) return 0;
-    return make_plan(p->n, p->rows, p->cols, AZ_F32, p->steps, p->a, p->b, p->c, true).bytes + 256;
+    const Plan plan = make_plan(p->n, p->rows, p->cols, AZ_F32, p->steps, p->a, p->b, p->c, true);
+    return check_tiles(plan) == AZ_OK ? plan.bytes + 256 : 0;
 }
 
 extern "C" int az_orthogonalize_dev(const az_orthogonalize_args* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -1068,7 +1076,7 @@ extern "C" int az_orthogonalize_dev(const az_orthogonalize_args* p, void* worksp
     if (meet(span_of(p->update, p->update_stride, p->n, p->rows, p->cols, esz), span_of(p->out, p->out_stride, p->n, p->rows, p->cols, esz)))
         return ofail(AZ_E_ARG, "out overlaps update");
     const Plan plan = make_plan(p->n, p->rows, p->cols, p->dtype, p->steps, p->a, p->b, p->c, false);
-    if ((rc = check_ws(workspace, workspace_bytes, plan.bytes + 256)) != AZ_OK) return rc;
+    if ((rc = check_tiles(plan)) != AZ_OK || (rc = check_ws(workspace, workspace_bytes, plan.bytes + 256)) != AZ_OK) return rc;
     AzDeviceGuard dev(p->device);
     if (!dev.ok) return ofail(AZ_E_HIP, "device %d cannot be used (no HIP device: libazhip has no CPU fallback)", p->device);
     (void)hipGetLastError();                                         // (an earlier call's error is not this one's)
@@ -1115,7 +1123,7 @@ extern "C" int az_muon_step_dev(const az_muon_step_args* p, void* workspace, siz
     if ((meet(w, wo) && !same(w, wo)) || (meet(m, mo) && !same(m, mo)) || meet(wo, mo) || meet(wo, m) || meet(mo, w) || meet(g, wo) || meet(g, mo))
         return ofail(AZ_E_ARG, "an output overlaps another tensor (in place means the same address and stride)");
     const Plan plan = make_plan(p->n, p->rows, p->cols, AZ_F32, p->steps, p->a, p->b, p->c, true);
-    if ((rc = check_ws(workspace, workspace_bytes, plan.bytes + 256)) != AZ_OK) return rc;
+    if ((rc = check_tiles(plan)) != AZ_OK || (rc = check_ws(workspace, workspace_bytes, plan.bytes + 256)) != AZ_OK) return rc;
     AzDeviceGuard dev(p->device);
     if (!dev.ok) return ofail(AZ_E_HIP, "device %d cannot be used (no HIP device: libazhip has no CPU fallback)", p->device);
     (void)hipGetLastError();                                         // (an earlier call's error is not this one's)

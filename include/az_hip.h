@@ -468,7 +468,8 @@ int az_policy_loss_dev(const az_policy_loss_args*, void* workspace, size_t works
  * ResBlocks straight out of the weight blob (az_load_weights).  out may not overlap update. */
 typedef struct az_orthogonalize_args {
     int   device;
-    int   n, rows, cols;           /* n may be 0; the shorter side at most 8192, the longer 2^24 */
+    int   n, rows, cols;           /* n may be 0; the shorter side at most 8192, the longer 2^24, and all matrices' tiles of
+                                      64 x 64 together fewer than 2^24 */
     int   dtype;                   /* of update and out */
     int   steps;                   /* 0..100 */
     float a, b, c, eps, scale;     /* |a| + |b| + |c| <= 32; refused where a singular value of up to 1 would pass 7 ahead of a

@@ -197,3 +197,18 @@ def test_policy_loss_gradients_refuse_outputs_that_overlap(kw, word):
     v.update(kw)
     rc, msg = _call("policy_loss", _policy(**v), None)
     assert rc == capi.AZ_E_ARG and word in msg, msg
+
+
+def test_more_tiles_than_a_launch_takes_are_refused():
+    """Rows of 2^24 elements, 2^18 tiles each: 63 of them are taken, 64 would be 2^32 threads."""
+    L = capi.load()
+    for make, name in ((_ortho, "orthogonalize"), (_muon, "muon_step")):
+        for n, fine in ((63, True), (64, False)):
+            strides = {k: 1 << 24 for k, _ in type(make())._fields_ if k.endswith("_stride")}
+            at = {k: (i + 1) << 40 for i, k in enumerate(("update", "out") if name == "orthogonalize" else ("grad", "weight", "momentum"))}
+            if name == "muon_step":
+                at.update(weight_out=at["weight"], momentum_out=at["momentum"])
+            a = make(n=n, rows=1, cols=1 << 24, **strides, **at)
+            assert (getattr(L, "az_%s_workspace" % name)(C.byref(a)) > 0) == fine
+            rc, msg = _call(name, a, None)
+            assert rc == capi.AZ_E_ARG and ("workspace" if fine else "too many tiles") in msg, msg
