@@ -695,7 +695,8 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
     if (a.C < Cp) for (int i = tid; i < ROWS * ldc; i += NT) ((T*)m.h)[i] = (T)0.f;
     // fp16: dz is r_b (a mean over the batch: 1 / B) times probabilities that may be 1e-5, below what fp16 resolves.  The
     // workgroup's dz carry a power of two that puts the largest of its boards' |r_b| sum |t|, which no dz exceeds, at 2^9 .. 2^10;
-    // it comes off the fp32 sums again.
+    // it comes off the fp32 sums again.  (One power for all: dw sums over them.  A board 2^15 below the largest still has the
+    // precision of its gradients' own rounding.)
     float up = 1.f, down = 1.f;
     if constexpr (DT == 1) {
         const Step last(a, s_hi - 1);

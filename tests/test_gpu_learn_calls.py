@@ -170,3 +170,33 @@ def test_blokus_rows_as_they_are_drained(reuse, dtype):
     p = dict(x=x, w=w, b=b, t=t, ok=None, tgt=tuple(torch.from_numpy(v) for v in (n, acts, probs)), words=None, B=B, N=N, C=C, O=O, dtype=dtype, layout="nhwc")
     xg, wg, bg, tg, _ = _cuda(p)
     _check(p, learn.policy_loss_grad(xg, wg, bg, tg, row_scale=1.0 / B), torch.full((B,), 1.0 / B, dtype=torch.float32).double())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("B,N", [(3, 4), (90, 15)])
+def test_lists_without_room_are_boards_without_targets(B, N, dtype):
+    p = _rows(B, N, 32, 3, dtype, "nhwc", seed=1)
+    x, w, b, _, _ = _cuda(p)
+    none = (torch.full((B,), 5, dtype=torch.int32, device="cuda"), torch.empty(B, 0, dtype=torch.int32, device="cuda"), torch.empty(B, 0, device="cuda"))
+    assert all((v == 0).all() for v in learn.policy_loss_grad(x, w, b, none))
+
+
+def test_calls_at_the_same_time_on_two_streams():
+    """Each has its workspace: results are those of the calls one after the other."""
+    heads = [_cuda(_rows(90, 15, 128, O, "bf16", "nhwc", sparse=True, seed=O)) for O in (3, 91)]
+    mats = [torch.randn(4, 256, 600, device="cuda") for _ in range(2)]
+    call = lambda i: learn.policy_loss_grad(*heads[i][:4]) + (learn.orthogonalize(mats[i]),)                   # noqa: E731
+    want = [call(i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(i))
+    for s in streams:
+        s.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
