@@ -11,14 +11,14 @@
 // small against the largest keeps the absolute precision of A's arithmetic, and the steps enlarge that error as they
 // enlarge the value (a^2 each).  So the products run on pairs of fp16 values, s x = hi + lo (22 bits, s a power of two that
 // keeps lo out of fp16's subnormals where it matters; three MFMA a product, fp32 sums), and for fp32 results X is formed
-// anew after two steps and A from it: for matrices whose largest singular value stands for most of the norm three steps
+// anew after two steps and A from it (16-bit results: after three, make_plan): for matrices whose largest singular value stands for most of the norm three steps
 // leave 6 times fp32's error (64 x 225 with 8 strong directions: 6e-6, two steps 1.1e-6, products in fp32 1.1e-6), two steps
 // at most fp32's.  fp32 matrix instructions would run at 154 TFLOP/s, three fp16 ones at 1.1 / 3 PFLOP/s.
 //
 // Measured on an MI355X that copies 4.9 TB/s and multiplies 1.1 PFLOP/s (fp16): 2 x 4096 x 1024 fp32 655 us (eleven
-// r x r launches of 25 us, X X^T 86 + 59 + 59 us, Q X 70 + 64 + 64 us; the Gram form's operations are 276 us at the rate of
-// a large product); optimiser step of 40 x 256 x 2304 513 us (momentum and norm 65 us at 5.7 TB/s, X X^T 68 + 50, r x r 13
-// launches of 12, Q X 78 + 95 us, the last with weights read and written).  18 x 128 x 1152 bf16 109 us.
+// r x r launches of 25 us, X X^T 75 + 52 + 52 us, Q X 71 + 65 + 65 us; the Gram form's operations are 276 us at the rate of
+// a large product); optimiser step of 40 x 256 x 2304 590 us (momentum and norm 65 us at 5.7 TB/s, X X^T 68 + 50 + 50, r x r 11
+// launches of 12, Q X 78 + 70 + 92 us, the last with weights read and written).  18 x 128 x 1152 bf16 106 us.
 #include "../../include/az_hip.h"
 #include "az_learn.h"
 
@@ -259,9 +259,11 @@ __device__ __forceinline__ void put_symmetric(const OrthoDev& d, short* res, int
 
 // One tile of a product.  Bound by a workgroup's own chain -- loads, LDS, products, barrier: 1.4 us a step of 64 where it
 // has its CU to itself, against 0.2 us of matrix instructions.  X X^T and the r x r products take tiles of 64:
-// 2 x 4096 x 1024 674 us a call, in tiles of 128 803, 16 x 4096 x 1024 3.6 ms either way, 300 x 128 x 1152 bf16 227 and 241 us.  An
-// r x r product of 2 x 1024 rows 25 us; its operands straight from memory to fragments, without LDS, 39.
-// Q X: tiles of 128 where those fill the chip (16 x 4096 x 1024: 3.6 ms a call, in tiles of 64 4.2 ms; 7 x 512 x 512: 244 and 223 us).
+// 2 x 4096 x 1024 674 us a call, in tiles of 128 803, 16 x 4096 x 1024 3.6 ms either way, 300 x 128 x 1152 bf16 (five steps a
+// stage then) 227 and 241 us.  An r x r product of 2 x 1024 rows 25 us; its operands straight from memory to fragments, without LDS, 39.
+// Q X: tiles of 128 where those fill the chip (16 x 4096 x 1024: 3.7 ms a call, in tiles of 64 4.2; 2 x 4096 x 1024 646 and 708 us;
+// 40 x 256 x 2304 585 and 609).  By counters the matrix units work for 36 % of Q X in tiles of 128, LDS bank conflicts of the operand
+// read by columns take 24 %.
 // D[m][n] = sum over the contraction, 4 waves of TILE/2 x TILE/2.  Lane l of a 16 x 16 tile holds rows 4 (l / 16) .. + 3 of
 // column l % 16, so M is the side along which the result is contiguous in memory.
 //   SYM         M = rows of a symmetric matrix, N = rows of another that commutes with it: their product, lower triangle
@@ -462,8 +464,9 @@ __global__ void __launch_bounds__(256) az_ortho_identity_kernel(short* Q, int rp
 
 // All of a stage's steps for matrices of up to R = 64 or 128 rows, one workgroup a matrix: A and P lie in LDS as pairs, Q in
 // registers, A P takes A's place.  Launched one product at a time these cost a launch and a trip to L2 each (5 us) for
-// 1 to 2 us of matrix instructions.  18 matrices of 128 rows, five steps: 58 us, bound by the chain of products of one
-// workgroup and its LDS reads (rows 16 halves longer instead of 8, a two-way conflict: 73 us).  A wave holds 16 columns of Q as operands: the product P Q leaves rows 4 g .. 4 g + 3 of
+// 1 to 2 us of matrix instructions.  18 matrices of 128 rows: two steps 22 us, three 34.  One workgroup's chain of products:
+// by counters its CU's matrix units work for a third of the time, its vector units for a third, LDS bank conflicts take 29 %
+// (rows 16 halves longer instead of 8, a two-way conflict: a quarter more time), and barriers keep them apart.  A wave holds 16 columns of Q as operands: the product P Q leaves rows 4 g .. 4 g + 3 of
 // the tiles 2 s, 2 s + 1 in lane group g, which is a fragment of step s whose contraction runs over those rows in that order,
 // and P's rows are read in the same order.
 template <int R> __global__ void __launch_bounds__(R * 4) az_ortho_iterate_kernel(OrthoDev d, int m) {
@@ -853,7 +856,7 @@ double largest_factor(double a, double b, double c, int steps) {
 // Slices of the contraction of X X^T.  In steps of 64 (1.4 us where a workgroup has its CU to itself; two take 1.7 times as
 // long): what the fullest CU does, two more to begin a workgroup, five for the launch that joins the slices, and the slices'
 // traffic (16 KB a tile written and read).  2 x 4096 x 1024 (272 tiles on 256 CUs, 64 steps): a slice 696 us a call, two 677,
-// four 653; 40 x 256 x 2304 (400 tiles, 36 steps): one 503, two 535; 18 x 128 x 1152 (54 tiles, 18 steps): one 88, four 83.
+// four 653; 40 x 256 x 2304 (400 tiles, 36 steps): one 587, two 613; 18 x 128 x 1152 (54 tiles, 18 steps): one 115, four 107.
 int split_of(long long tiles, int steps) {
     int best = 1;
     double cost = 0.0;

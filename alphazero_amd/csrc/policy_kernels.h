@@ -385,8 +385,10 @@ template <int KT, int KS, int W, bool AHEAD, class F, class S> __device__ __forc
 // once leaves a wave too few registers for four waves a SIMD: 512 boards of 20 x 20, 128 planes bf16 76 us, in halves 40;
 // 91 planes 33 and 30, 64 planes 23.5 and 24).  Sparse targets: the logits pass through LDS, and lanes
 // pick out those that the tile's entries name.
-// 2048 boards of 20 x 20, 128 channels, 91 planes fp16, legal actions only: 86 us, 2.7 TB/s of the features (43 us of copying);
-// bound by the vector instructions of 36 400 exponentials and masks a board.  4096 boards of 15 x 15, one plane bf16: 61 us,
+// 2048 boards of 20 x 20, 128 channels, 91 planes fp16, legal actions only: 88 us, 2.6 TB/s of the features (43 us of copying).
+// By counters the vector units issue for 60 % of that (24 instructions a logit: exponential, mask, maximum, and their share of
+// addresses and conversions), the matrix units work for 10 %; a wave's loads, products and exponentials follow one another, and
+// what four waves a SIMD do not hide of that is the rest.  4096 boards of 15 x 15, one plane bf16: 61 us,
 // 3.9 TB/s, bound by memory.  256 boards of 20 x 20, 256 channels fp32: 91 us, 52 TFLOP/s.
 template <int OT> struct LossTile {
     static constexpr int PASSES = OT >= 4 ? 2 : 1, OTP = OT / PASSES, LDZ = OTP * 16 + 4;
@@ -659,7 +661,7 @@ template <int LD> __device__ __forceinline__ void scatter_targets(const PolicyDe
 // once that has been read.
 // (16-bit features of up to 128 channels and 96 planes have a kernel of their own below for all but the smallest batches.)
 // fp32: bound by the matrix instructions, 32 cycles for the 16 x 16 x 4: 256 boards of 20 x 20, 256 channels, 91 planes
-// 225 us, 64 TFLOP/s (three products: 93 us at the rate of a large one).  256 channels leave no registers to ask for the next
+// 222 us, 65 TFLOP/s (three products: 93 us at the rate of a large one; the matrix units work for half of the time).  256 channels leave no registers to ask for the next
 // step's features early: kept in flight they went to scratch memory and back (367 us).
 template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT, 2) az_policy_grad_kernel(PolicyDev a) {
     typedef Lay<DT, OT, CB> L;
@@ -940,9 +942,10 @@ template <int DT, int OT, int CB, int MODE> __global__ void __launch_bounds__(NT
 // either kind on each SIMD, one barrier a step; each kind holds its shares of w in registers.  Done by the same waves one
 // after the other, neither the vector nor the matrix pipes nor the LDS port were busy half of the time.  LDS: features of
 // three steps, dz (hi and lo) of two, the sparse targets of each row tile.
-// 2048 boards of 20 x 20, 128 channels, 91 planes bf16: 158 us, 361 TFLOP/s of useful products (two of dw's halves counted
-// once), 2.7 TB/s of features and their gradients (86 us of copying); what bounds it is the step's chain of logits, exponentials,
-// LDS and products between two barriers with one workgroup a CU.  4096 boards of 15 x 15, one plane: 93 us, 5.1 TB/s: memory.
+// 2048 boards of 20 x 20, 128 channels, 91 planes bf16: 200 us, 285 TFLOP/s of useful products (the parts of dz counted
+// once), 2.1 TB/s of features and their gradients (86 us of copying); what bounds it is the step's chain of logits, exponentials,
+// LDS and products between two barriers with one workgroup a CU (vector units 38 % of the time, matrix units 28 %; LDS bank
+// conflicts 13 %).  hi alone for dh and two parts for dw took 158.  4096 boards of 15 x 15, one plane: 92 us, 5.1 TB/s: memory.
 template <int DT, int OT> struct PairCfg {
     typedef Lay<DT, OT, 1> L;
     static constexpr int LDP = OT * 16 + 4;
@@ -1252,8 +1255,9 @@ template <int DT, int OT, int MODE> __global__ void __launch_bounds__(NT, OT == 
 constexpr size_t LOSS_STATIC = (size_t)4 * ROWS * 16 + MAX_BOARDS * 4;           // az_policy_loss_kernel's `red` and `negative`
 template <int DT, int OT, int CB, int MODE> hipError_t launch_products(PolicyDev a, bool grad, int& groups, hipStream_t stream) {
     // az_policy_grad16_kernel: 16-bit features of up to 128 channels and 96 planes (with more, w's shares do not fit the
-    // registers), where a workgroup has more than a step.  20 x 20, 91 planes bf16: 2048 boards 228 us a call, with
-    // az_policy_grad_kernel 334; 36 boards (252 steps) 37.7 against 36.6, and 9 x 9, 3 planes fp16 24.7 against 19.8.
+    // registers), where a workgroup has more than a step.  20 x 20, 91 planes bf16: 2048 boards 287 us a call, with
+    // az_policy_grad_kernel 382; 128 boards 47 and 52; at the border, 38 boards (266 steps) 40 and 42.5, 36 (252 steps) 41 and 42;
+    // 9 x 9, 3 planes fp16: 140 boards (280 steps) 30 and 29, 77 boards 28 and 27.
     constexpr bool PAIR = DT != 0 && CB == 1 && OT <= 6;
     const bool pair = PAIR && a.steps > CUS;
     const auto bytes = [&]() -> size_t {
