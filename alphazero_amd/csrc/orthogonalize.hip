@@ -897,7 +897,8 @@ Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b
     size_t o = 0;
     p.off_sq = o; o += up256((size_t)n * p.slices * 8);
     p.off_u = o; if (muon) o += up256((size_t)n * count * 4);
-    p.off_x1 = o; if (p.restart) o += 2 * (p.iter_bytes = up256((size_t)n * 2 * p.rp * p.kp * 2));   // iterates: read one, write the other
+    // iterates: of three stages and more the middle ones read one and write the other
+    p.off_x1 = o; if (p.restart) o += (steps > 2 * p.stage ? 2 : 1) * (p.iter_bytes = up256((size_t)n * 2 * p.rp * p.kp * 2));
     p.off_mat = o; o += 5 * p.pair_bytes;
     p.off_partial = o; if (p.split > 1) o += up256((size_t)n * p.split * p.rp * p.rp * 4);
     p.bytes = o;

@@ -1,5 +1,7 @@
 """The learner's operators inside torch: what autograd, forward mode and tracing may rely on, and runs of the operators together
 with the engines that they stand between."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -43,6 +45,8 @@ def test_forward_mode_tangents_are_refused(needs_grad):
             for call in (learn.policy_loss, learn.policy_loss_grad):
                 with pytest.raises(AzError, match="tangent"):
                     call(*args)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(lambda v: learn.policy_loss(v, w, b, tgt), (x,), (torch.ones_like(x),))
         d = forward_ad.make_dual(m.clone(), torch.ones_like(m))
         with pytest.raises(AzError, match="tangent"):
             learn.orthogonalize(d)
@@ -200,3 +204,61 @@ def test_calls_at_the_same_time_on_two_streams():
     for i in range(2):
         for r in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+@pytest.mark.parametrize("steps", [2, 3, 4, 5, 6, 7, 9, 10])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_no_call_leaves_its_workspace(steps, dtype):
+    """Guards around the workspace and the result of every number of stages, through the C entry."""
+    n, R, K = 3, 130, 200
+    u = torch.randn(n, R, K, device="cuda").to(DT[dtype])
+    a = capi.AzOrthogonalizeArgs()
+    a.device, a.n, a.rows, a.cols, a.dtype, a.steps = u.device.index, n, R, K, {"f32": capi.AZ_F32, "bf16": capi.AZ_BF16}[dtype], steps
+    a.a, a.b, a.c = learn.NEWTON_SCHULZ
+    a.eps, a.scale = 1e-7, 1.0
+    L = capi.load()
+    size, guard = L.az_orthogonalize_workspace(C.byref(a)), 4096
+    ws = torch.full((size + 2 * guard,), 0xA5, dtype=torch.uint8, device="cuda")
+    out = torch.full((n * R * K + 256,), 7.0, dtype=DT[dtype], device="cuda")
+    a.update, a.update_stride, a.out, a.out_stride = u.data_ptr(), R * K, out.data_ptr() + 128 * out.element_size(), R * K
+    capi._chk(L.az_orthogonalize_dev(C.byref(a), ws.data_ptr() + guard, size, torch.cuda.current_stream().cuda_stream))
+    assert (ws[:guard] == 0xA5).all() and (ws[-guard:] == 0xA5).all() and (out[:128] == 7).all() and (out[-128:] == 7).all()
+    assert torch.equal(out[128:-128].view(n, R, K), learn.orthogonalize(u, steps=steps))
+
+
+@pytest.mark.parametrize("case", [(3, 9, 100, 3, "f32"), (2, 20, 250, 91, "f32"), (90, 15, 128, 17, "bf16"), (90, 15, 128, 1, "f16"), (40, 20, 128, 91, "bf16"), (5, 3, 200, 128, "f16")], ids=str)
+@pytest.mark.parametrize("sparse", [False, True], ids=["dense", "sparse"])
+def test_no_loss_leaves_its_workspace_or_outputs(case, sparse):
+    """Guards around everything az_policy_loss_dev writes, and the statistics handed from a call for the losses to one for the
+    gradients."""
+    B, N, ch, O, dtype = case
+    p = _rows(B, N, ch, O, dtype, "nchw", sparse=sparse, seed=B)
+    x, w, b, tgt, _ = _cuda(p)
+    want = learn.policy_loss_grad(x, w, b, tgt, row_scale=0.25)
+    L, a = capi.load(), capi.AzPolicyLossArgs()
+    a.device, a.B, a.N, a.C, a.c_out, a.scale, a.layout = x.device.index, B, N, ch, O, 0.25, capi.AZ_CHANNELS_FIRST
+    a.dtype = {"f32": capi.AZ_F32, "f16": capi.AZ_F16, "bf16": capi.AZ_BF16}[dtype]
+    a.features, a.weight, a.bias = x.data_ptr(), w.data_ptr(), b.data_ptr()
+    if sparse:
+        a.counts, a.actions, a.probs, a.cap = tgt[0].data_ptr(), tgt[1].data_ptr(), tgt[2].data_ptr(), tgt[1].shape[1]
+    else:
+        a.target = tgt.data_ptr()
+    guarded = []
+
+    def room(nbytes):
+        t = torch.full((nbytes + 1024,), 0xA5, dtype=torch.uint8, device="cuda")
+        guarded.append(t)
+        return t[512:-512]
+
+    def call():
+        ws = room(L.az_policy_loss_workspace(C.byref(a)))
+        capi._chk(L.az_policy_loss_dev(C.byref(a), ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
+    loss, stats, dx, dw, db = room(B * 4), room(B * 16), room(x.numel() * x.element_size()), room(O * ch * 4), room(O * 4)
+    a.loss, a.stats = loss.data_ptr(), stats.data_ptr()
+    call()
+    a.loss, a.stats_given, a.d_features, a.d_weight, a.d_bias = None, 1, dx.data_ptr(), dw.data_ptr(), db.data_ptr()
+    call()
+    got = loss.view(torch.float32), dx.view(x.dtype).view(x.shape), dw.view(torch.float32).view(O, ch), db.view(torch.float32)
+    assert all(torch.equal(g, v) for g, v in zip(got, want))
+    for t in guarded:
+        assert (t[:512] == 0xA5).all() and (t[-512:] == 0xA5).all()
