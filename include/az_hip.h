@@ -464,7 +464,8 @@ int az_policy_loss_dev(const az_policy_loss_args*, void* workspace, size_t works
 /* out_i = scale * (update_i with its singular values x taken to what `steps` times x -> a x + b x^3 + c x^5 makes of
  * x / (|update_i|_F + eps)), for n matrices of rows x cols, row-major and contiguous, `stride` elements apart: the
  * orthogonalised update of a convolution's weight [C_out, C_in * 9] (a = 3.4445, b = -4.775, c = 2.0315, 5 steps take
- * singular values between 1/100 and 1 of the norm to about 0.7 .. 1.2).  A strided batch takes the convolutions of all
+ * singular values between 1/100 and 1 of the norm to about 0.7 .. 1.2).  Errors go with singular values of 1: where
+ * |update|_F is far below eps, so that the result is small, they are some 1e-6 of 1, not of the result.  A strided batch takes the convolutions of all
  * ResBlocks straight out of the weight blob (az_load_weights).  out may not overlap update. */
 typedef struct az_orthogonalize_args {
     int   device;

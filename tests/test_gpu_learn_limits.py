@@ -282,3 +282,14 @@ def test_coefficients_that_enlarge(shape, coef, steps, dtype):
         got = learn.orthogonalize(u.to(DT[dtype]).cuda(), steps=steps, coefficients=coef).cpu().double()
         err = torch.linalg.vector_norm((got - u.double() * (x / norm)).flatten(1), dim=1)
         assert (err <= 25 * 3e-5 * most + half * abs(x)).all(), err
+
+
+@pytest.mark.parametrize("norm", [1e-6, 1e-9, 1e-11, 1e-14])
+@pytest.mark.parametrize("shape", [(1, 64, 225), (1, 128, 600), (1, 256, 300)], ids=lambda s: "%dx%dx%d" % s)
+def test_updates_far_smaller_than_eps(shape, norm):
+    """The result shrinks with the update; its error is that of singular values near 1 (3e-5: test_gpu_learn.py)."""
+    u = torch.randn(shape, generator=torch.Generator().manual_seed(2))
+    u = u * (norm / float(u.norm()))
+    want, got = _matrix_exact(u), learn.orthogonalize(u.cuda()).cpu().double()
+    assert torch.linalg.matrix_norm(got - want, 2).max() <= 3e-5 * 1.3
+    assert torch.isfinite(got).all() and float(got.norm()) <= 1.01 * float(want.norm()) + 3e-5 * math.sqrt(min(shape[1:]))
