@@ -176,7 +176,8 @@ def policy_loss(features, weight, bias, targets, legal=None):
 def policy_loss_grad(features, weight, bias, targets, row_scale=None, legal=None):
     """policy_loss and the gradients of sum_b row_scale_b * loss_b in one call: (loss [B], d_features like features,
     d_weight float32 [c_out, C], d_bias float32 [c_out]).  row_scale: None = 1, a number (1 / B for the mean), or float32
-    [B].  For c_out = 1 the bias shifts every logit alike and its gradient is zero."""
+    [B].  For c_out = 1 the bias shifts every logit alike and its gradient is zero (NaN
+    where a board's are)."""
     return _grad(features, weight, bias, targets, legal, row_scale)
 
 
