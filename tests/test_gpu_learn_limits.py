@@ -293,3 +293,14 @@ def test_updates_far_smaller_than_eps(shape, norm):
     want, got = _matrix_exact(u), learn.orthogonalize(u.cuda()).cpu().double()
     assert torch.linalg.matrix_norm(got - want, 2).max() <= 3e-5 * 1.3
     assert torch.isfinite(got).all() and float(got.norm()) <= 1.01 * float(want.norm()) + 3e-5 * math.sqrt(min(shape[1:]))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("case", [(17, 32, 128, 96, 1024, 0.3), (17, 32, 100, 65, 1025, 0.0), (70, 12, 128, 96, 1024, 0.0), (2000, 2, 16, 91, 64, 0.0), (2000, 3, 32, 17, 147, 0.3)],
+                         ids=lambda c: "b%d-n%d-c%d-o%d-cap%d%s" % (c[:5] + ("-legal" if c[5] else "",)))
+def test_lists_that_just_fit_beside_more_than_a_step_a_workgroup(case, dtype):
+    """The largest boards and heads of the paired kernel, with lists at the border of what LDS keeps of a workgroup's boards (1 024)."""
+    B, N, C, O, cap, legal = case
+    p = _rows(B, N, C, O, dtype, "nhwc", sparse=True, legal=legal, seed=cap + N, cap=cap, empty=(0,))
+    x, w, b, tgt, words = _cuda(p)
+    _check(p, learn.policy_loss_grad(x, w, b, tgt, legal=words), torch.ones(B, dtype=torch.float64))
