@@ -887,7 +887,7 @@ Plan make_plan(int n, int rows, int cols, int dtype, int steps, float a, float b
     // with three 493 us a step, with two 579).  16-bit results: three, off by at most 8e-5 where half a step of fp16 is 2e-4 and of bf16
     // 1.7e-3 (relative norms over 128 x 1152 .. 600 x 200, one to eight strong directions a thousand to ten thousand times the
     // rest, where fp32 products are off by as much); all five at once leave 1e-3 to 7e-3 there.  18 x 128 x 1152 bf16: five
-    // 86 us a call, three 109, two 131.  Fewer where the coefficients would take Q out of fp16's range.
+    // 86 us a call, three 106, two 131; 300 x 128 x 1152: five 227, three 390.  Fewer where the coefficients would take Q out of fp16's range.
     p.stage = dtype == AZ_F32 ? 2 : 3;
     const double f = largest_factor(a, b, c, steps);
     while (p.stage > 1 && std::pow(f, p.stage) * SQ > 30000.0) --p.stage;

@@ -207,7 +207,8 @@ def orthogonalize(update, scale=1.0, steps=5, coefficients=NEWTON_SCHULZ, eps=1e
 
     update: [R, K], [n, R, K], a convolution's weight [O, I, kh, kw] or [n, O, I, kh, kw]; float32 / float16 / bfloat16; the
     batch may be strided (the convolutions of all blocks in the weight blob), each matrix contiguous.  out: like update,
-    apart from it."""
+    apart from it.  coefficients that take singular values of up to 1 beyond 7 ahead of a step, or enlarge one more than 200
+    times in a step, are refused."""
     _untraced()
     n, R, K, stride = _batch(update, "update")
     _on(update, update.device, "update")
